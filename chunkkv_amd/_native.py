@@ -17,7 +17,7 @@ import torch  # noqa: F401  (must precede the CDLL load, see module docstring)
 
 LIB_PATH = Path(__file__).resolve().parent / "_lib" / "libchunkkv_amd.so"
 TORCH_OPS_PATH = LIB_PATH.with_name("_torch_ops.so")
-ABI_VERSION = 6
+ABI_VERSION = 7
 
 CKV_OK = 0
 CKV_ERR_INVALID_ARGUMENT = 1
@@ -96,6 +96,24 @@ SIGNATURES = {
         [_p, _p, _i64, _i64, _p, _p, _i64, _p, _i32, _i32, _i32, _i32, _i32, _i32, _f64, _p, _i64, _p, _p],
     ),
     "ckv_attention_workspace_bytes": (_i64, [_i32, _i32, _i32, _i32, _p, _p]),
+    "ckv_quantize_rows": (
+        _i32,
+        [_p, _p, _p, _p, _p, _i64, _i64, _p, _i64, _i64, _i64, _p, _i32, _i32, _i32, _i32, _i32, _i32, _p, _p],
+    ),
+    "ckv_attention_quantized": (
+        _i32,
+        [_p, _p, _i64, _i64, _p, _p, _p, _p, _p, _i32, _i32, _i32, _i32, _i32, _i32, _f64, _p, _i64, _p, _p],
+    ),
+    "ckv_attention_quantized_workspace_bytes": (_i64, [_i32] * 5),
+    "ckv_attention_weights": (
+        _i32,
+        [_p, _p, _p, _i64, _i64, _p, _i64, _p, _i32, _i32, _i32, _i32, _i32, _i32, _f64, _p, _i64, _p, _p],
+    ),
+    "ckv_attention_weights_workspace_bytes": (_i64, [_i32] * 4),
+    "ckv_evict_rows": (
+        _i32,
+        [_p, _i64, _p, _i64, _p, _p, _p, _i64, _p, _i64, _p, _i64, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _p],
+    ),
     "ckv_add_rmsnorm": (_i32, [_p, _p, _p, _p, _p, _i64, _i32, _f32, _i32, _p]),
     "ckv_silu_mul": (_i32, [_p, _i64, _p, _i64, _p, _i64, _i64, _i32, _i32, _p]),
     "ckv_linear": (_i32, [_p, _p, _i64, _p, _p, _i32, _i32, _i32, _i32, _p, _i64, _p]),

@@ -36,11 +36,11 @@ struct AttnMap {
 
 // For x / d as a multiplication (div_by): ceil(2^32 / d) where that is exact for every x <= most
 // (most d < 2^32), 0 elsewhere.
-static uint32_t inverse_of(int64_t most, int64_t d) {
+static inline uint32_t inverse_of(int64_t most, int64_t d) {
   return d > 1 && most * d < (1ll << 32) ? (uint32_t)(((1ll << 32) + d - 1) / d) : 0;
 }
 
-static AttnMap attn_map(int64_t nqb, int Hkv, int group, int64_t splits) {
+static inline AttnMap attn_map(int64_t nqb, int Hkv, int group, int64_t splits) {
   AttnMap m;
   if (kXcds % Hkv != 0) {
     group *= Hkv;
@@ -77,7 +77,7 @@ struct AttnPlan {
 // rows, 224, 157 against 164; 1103 causal rows, 252, 27.8 against 27.1; 1500, 336, 41.1 against
 // 36.5), below two at head_dim 64, where they also hold less work each (14 heads: 3000 causal rows,
 // 336 workgroups, 37.6 against 46.5; 4000, 448, 58.9 against 61.8; 4500, 504, 72.4 against 69.8).
-static bool wave_launch(int n, int Hq, int head_dim) {
+static inline bool wave_launch(int n, int Hq, int head_dim) {
   const int64_t blocks = (int64_t)((n + kAttnBM - 1) / kAttnBM) * Hq;
   return blocks < (head_dim == 128 ? 256 : 450);
 }
@@ -86,20 +86,16 @@ constexpr int kWaveFill = 256;  // workgroups that a split launch aims at: one f
 
 // The most splits a launch takes: a workgroup has at most 32 (token, query head) rows, a split's
 // four wavefronts a chunk each.
-static int64_t most_splits(int n, int N, int Hq, int head_dim) {
+static inline int64_t most_splits(int n, int N, int Hq, int head_dim) {
   const int64_t chunks = (N + kWaveChunk - 1) / kWaveChunk;
   if (!wave_launch(n, Hq, head_dim) || chunks <= 16) return 1;
   return std::max<int64_t>(1, std::min<int64_t>(kWaveFill * 32 / ((int64_t)n * Hq), (chunks + 3) / 4));
 }
 
-// The plan without split 128-query workgroups.
-static AttnPlan attn_base_plan(int n, int N, int Hq, int Hkv, int head_dim, int64_t workspace_bytes) {
+// The plan of attn_wave_kernel.
+static inline AttnPlan attn_wave_plan(int n, int N, int Hq, int Hkv, int head_dim, int64_t workspace_bytes) {
   AttnPlan p;
   const int group = Hq / Hkv;
-  if (!wave_launch(n, Hq, head_dim)) {
-    p.map = attn_map((n + kAttnBM - 1) / kAttnBM, Hkv, group, 1);
-    return p;
-  }
   p.wave = true;
   p.grouped = group > 1 && (int64_t)n * group <= kAttnBM;
   const int rows = p.grouped ? n * group : n, heads = p.grouped ? Hkv : Hq;
@@ -150,13 +146,24 @@ static AttnPlan attn_base_plan(int n, int N, int Hq, int Hkv, int head_dim, int6
   return p;
 }
 
+// The plan without split 128-query workgroups.
+static inline AttnPlan attn_base_plan(int n, int N, int Hq, int Hkv, int head_dim, int64_t workspace_bytes) {
+  AttnPlan p;
+  const int group = Hq / Hkv;
+  if (!wave_launch(n, Hq, head_dim)) {
+    p.map = attn_map((n + kAttnBM - 1) / kAttnBM, Hkv, group, 1);
+    return p;
+  }
+  return attn_wave_plan(n, N, Hq, Hkv, head_dim, workspace_bytes);
+}
+
 // 128-query workgroups over splits of a long cache. Where a launch has few query blocks the small
 // launches' form reads the cache once for every 16 or 32 rows, at half the large kernel's rate, and
 // the large kernel unsplit is a chain of every tile on a part of the CUs. The splits that fill the
 // card once: of q = n / 128 query blocks (a last block of few rows is little work) with positions
 // spread over the cache, split z of s concerns those that reach it, about s (q + 1) / 2 + (q - 1) / 2 of
 // a head's q s workgroups, and 512 (head_dim 64: 768) are resident at once.
-static int64_t large_splits(int n, int N, int Hq, int head_dim) {
+static inline int64_t large_splits(int n, int N, int Hq, int head_dim) {
   const int64_t tiles = (N + kAttnBN - 1) / kAttnBN;
   if (tiles < 80) return 1;  // shorter caches: no form gained enough
   const double q = std::max(1.0, (double)n / kAttnBM), per_head = (head_dim == 128 ? 1024.0 : 1536.0) / Hq;
@@ -168,7 +175,7 @@ static int64_t large_splits(int n, int N, int Hq, int head_dim) {
 // seven head layouts (28 / 4, 32 / 8, 64 / 8, 32 / 32 and 8 / 2 heads of 128, 14 / 2, 32 / 8 and 16 / 16
 // of 64; 3-3000 queries over 1103-32832 rows), within about 10 %: a workgroup's chain of chunks or
 // tiles, or all chunks at the rate of the card, and the partial rows written and read.
-static double base_plan_us(const AttnPlan& p, int n, int N, int Hq, int Hkv, int head_dim) {
+static inline double base_plan_us(const AttnPlan& p, int n, int N, int Hq, int Hkv, int head_dim) {
   const bool d128 = head_dim == 128;
   if (!p.wave) return 4.0 + (d128 ? 1.35 : 0.95) * ((N + kAttnBN - 1) / kAttnBN);
   const int rows = p.grouped ? n * (Hq / Hkv) : n, heads = p.grouped ? Hkv : Hq;
@@ -179,17 +186,17 @@ static double base_plan_us(const AttnPlan& p, int n, int N, int Hq, int Hkv, int
   const double seen = p.grouped ? 1.0 : 0.5;  // half the cache, on average
   return 4.0 + std::max(chain * step, blocks * chunks * seen * work / 256) + (p.splits > 1 ? 4.0 : 0.0);
 }
-static double large_split_us(int n, int N, int Hq, int head_dim, int64_t splits) {
+static inline double large_split_us(int n, int N, int Hq, int head_dim, int64_t splits) {
   const int64_t tiles = (N + kAttnBN - 1) / kAttnBN, chain = (tiles + splits - 1) / splits;
   const double partial_mb = (double)splits * n * Hq * (head_dim + 4) * 4e-6;
   return head_dim == 128 ? 10.0 + 2.1 * chain + 0.31 * partial_mb : 7.0 + 1.6 * chain + 0.45 * partial_mb;
 }
 
 // Bytes of partial rows at the most splits that a launch of this shape may take; 0: it never splits.
-static int64_t attn_most_splits(int n, int N, int Hq, int head_dim) {
+static inline int64_t attn_most_splits(int n, int N, int Hq, int head_dim) {
   return std::max(most_splits(n, N, Hq, head_dim), large_splits(n, N, Hq, head_dim));
 }
-static int64_t attn_workspace_bytes(int n, int N, int Hq, int head_dim) {
+static inline int64_t attn_workspace_bytes(int n, int N, int Hq, int head_dim) {
   const int64_t splits = attn_most_splits(n, N, Hq, head_dim);
   return splits > 1 ? splits * Hq * n * (head_dim + 4) * 4 : 0;
 }
@@ -200,7 +207,7 @@ static int64_t attn_workspace_bytes(int n, int N, int Hq, int head_dim) {
 // of 32832 116 and 44.8, 1153 of 16400 127 and 76.7. Below 64 rows of a KV head the small launches' form
 // stays ahead. Over 1651 shapes of the layouts above 0.90 of the base plan's time in the mean; 11 are
 // more than 3 % slower than it, the worst 1.19 (64 / 8 heads of 128, 180 of 32832 rows, 235 and 279).
-static AttnPlan attn_plan(int n, int N, int Hq, int Hkv, int head_dim, int64_t workspace_bytes) {
+static inline AttnPlan attn_plan(int n, int N, int Hq, int Hkv, int head_dim, int64_t workspace_bytes) {
   AttnPlan p = attn_base_plan(n, N, Hq, Hkv, head_dim, workspace_bytes);
   const int group = Hq / Hkv;
   const int64_t splits = large_splits(n, N, Hq, head_dim);

@@ -20,26 +20,33 @@
 // 14 -> 8.7; 14 heads of 64, 320 causal rows 8.8 -> 5.2, 251 over 1103 16 -> 7.1.
 #pragma once
 
+#include "attention_common.hpp"
+
 namespace ckv {
 
-// Between the stages in which a wavefront's lanes exchange rows through LDS (and before a stage's rows
-// are overwritten): LDS runs one wavefront's operations in order, so this is no instruction, only an
-// order of stores and loads that the compiler has to keep though no lane reads its own bytes.
-__device__ __forceinline__ void wave_lds_stage() {
-  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront", "local");
-  __builtin_amdgcn_wave_barrier();
-  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront", "local");
-}
+// What an 8-bit cache has beside its codes: for head h and 32-row chunk c the scale byte e + 127 of 2^e
+// is at [h * blocks + (c >> chunk_log)], of K and of V.
+struct CacheScales {
+  const uint8_t* k;
+  const uint8_t* v;
+  int blocks, chunk_log;
+};
+struct NoScales {};
 
-template <int D, int QG, int W, bool GROUPED>
+// CODES: the cache holds e4m3 codes. A row's codes become bf16 (exactly: three fraction bits times a
+// power of two) where it is put into LDS, and everything after that is the bf16 cache's.
+template <int D, int QG, int W, bool GROUPED, bool CODES = false>
 __global__ __launch_bounds__(W * 64) void attn_wave_kernel(
     int nqb, int map_group, int xpk_log, int items, uint32_t inv_group, uint32_t inv_nqb,
     const int64_t* __restrict__ pos, int n, int N, const char* __restrict__ kc, const char* __restrict__ vc,
     int64_t kv_hs_b, const char* __restrict__ q, int64_t q_hs_b, int64_t q_ts_b, int Hq, int group, uint32_t inv_gqa,
-    float scale_log2, int split_chunks, char* __restrict__ out, float* __restrict__ ws, int32_t* __restrict__ err) {
+    float scale_log2, int split_chunks, char* __restrict__ out, float* __restrict__ ws, int32_t* __restrict__ err,
+    std::conditional_t<CODES, CacheScales, NoScales> scales) {
   constexpr int DS = D / 32, DT = D / 16, CPR = D / 8, ROWB = D * 2;
   constexpr int ROWS = 16 * QG;               // query rows of the workgroup
-  constexpr int LI = kWaveChunk * CPR / 64;   // 16-byte loads per lane and chunk, of K and of V
+  constexpr int GB = CODES ? D : ROWB;        // bytes of a row in the cache, and 16-byte pieces
+  constexpr int GP = GB / 16;
+  constexpr int LI = kWaveChunk * GP / 64;    // 16-byte loads per lane and chunk, of K and of V
   constexpr int QI = ROWS * CPR / 64;         // of the workgroup's query rows
   constexpr int OP = D + 4;                   // pitch of a partial row in LDS (floats): distinct banks
   constexpr int V_B = W * kWaveChunk * ROWB, O_B = W * ROWS * OP * 4;
@@ -70,10 +77,23 @@ __global__ __launch_bounds__(W * 64) void attn_wave_kernel(
   vec16 kr[LI], vr[LI], qr[QI];
   auto load = [&](vec16(&r)[LI], const char* rows, int c) {  // lane l of load i: piece i 64 + l of the chunk
     c = min(c, (N - 1) / kWaveChunk);
-    const char* base = rows + (int64_t)c * (kWaveChunk * ROWB);
+    const char* base = rows + (int64_t)c * (kWaveChunk * GB);
     const int last = N - 1 - c * kWaveChunk;
 #pragma unroll
-    for (int i = 0; i < LI; ++i) r[i] = ld16(base + min((i * 64 + lane) / CPR, last) * ROWB + (lane % CPR) * 16);
+    for (int i = 0; i < LI; ++i) r[i] = ld16(base + min((i * 64 + lane) / GP, last) * GB + (lane % GP) * 16);
+  };
+  float k_sc = 1.f, v_sc = 1.f;  // scales of the rows in kr and vr
+  auto load_scale = [&](float& s, const uint8_t* of, int c) {
+    c = min(c, (N - 1) / kWaveChunk);
+    if constexpr (CODES) s = __uint_as_float((uint32_t)of[(int64_t)hk * scales.blocks + (c >> scales.chunk_log)] << 23);
+  };
+  auto load_k = [&](int c) {
+    load(kr, kh, c);
+    if constexpr (CODES) load_scale(k_sc, scales.k, c);
+  };
+  auto load_v = [&](int c) {
+    load(vr, vh, c);
+    if constexpr (CODES) load_scale(v_sc, scales.v, c);
   };
 #pragma unroll
   for (int i = 0; i < QI; ++i) {  // absent rows load the last token's query and store nothing
@@ -83,12 +103,13 @@ __global__ __launch_bounds__(W * 64) void attn_wave_kernel(
   }
   const int begin = ws != nullptr ? z * split_chunks : 0;
   int c = begin + wave;
-  load(kr, kh, c);
-  load(vr, vh, c);
+  load_k(c);
+  load_v(c);
   // The operand of matrix step ds for row slot s: logical 16-byte piece 4 ds + g, kept at piece
   // (4 ds + g) ^ swz_k(s) of the slot.
   char* wl = lds + wave * kWaveChunk * ROWB;
-  auto put = [&](int slot, const vec16& v) { *(vec16*)(wl + slot * ROWB + (((lane % CPR) ^ swz_k<CPR>(slot)) * 16)) = v; };
+  auto put_at = [&](int slot, int piece, const vec16& v) { *(vec16*)(wl + slot * ROWB + ((piece ^ swz_k<CPR>(slot)) * 16)) = v; };
+  auto put = [&](int slot, const vec16& v) { put_at(slot, lane % CPR, v); };
   auto operand = [&](int slot, int ds) {
     return *(const bf16x8*)(wl + slot * ROWB + (((4 * ds + g) ^ swz_k<CPR>(slot)) * 16));
   };
@@ -136,10 +157,17 @@ __global__ __launch_bounds__(W * 64) void attn_wave_kernel(
     wave_lds_stage();
 #pragma unroll
     for (int i = 0; i < LI; ++i) {  // K row r = 8 a + 4 t + b to slot 16 t + 4 a + b (kslot_row's inverse)
-      const int r = (i * 64 + lane) / CPR;
-      put(16 * ((r >> 2) & 1) + 4 * (r >> 3) + (r & 3), kr[i]);
+      const int r = (i * 64 + lane) / GP, slot = 16 * ((r >> 2) & 1) + 4 * (r >> 3) + (r & 3);
+      if constexpr (CODES) {
+        vec16 lo, hi;
+        decode16(kr[i], k_sc, lo, hi);
+        put_at(slot, 2 * (lane % GP), lo);
+        put_at(slot, 2 * (lane % GP) + 1, hi);
+      } else {
+        put(slot, kr[i]);
+      }
     }
-    if (c + W < c_end) load(kr, kh, c + W);  // lands while this chunk is worked on
+    if (c + W < c_end) load_k(c + W);  // lands while this chunk is worked on
     wave_lds_stage();
     f32x4 s[QG][2];
 #pragma unroll
@@ -157,11 +185,21 @@ __global__ __launch_bounds__(W * 64) void attn_wave_kernel(
     wave_lds_stage();
 #pragma unroll
     for (int i = 0; i < LI; ++i) {
-      const int slot = (i * 64 + lane) / CPR;
-      const vec16 v = edge && n0 + slot > wmax ? vec16{0, 0, 0, 0} : vr[i];
-      *(vec16*)(wl + slot * ROWB + (((lane % CPR) ^ swz_v<CPR>(slot)) * 16)) = v;
+      const int slot = (i * 64 + lane) / GP;
+      const bool past = edge && n0 + slot > wmax;
+      auto put_v = [&](int piece, const vec16& v) {
+        *(vec16*)(wl + slot * ROWB + ((piece ^ swz_v<CPR>(slot)) * 16)) = past ? vec16{0, 0, 0, 0} : v;
+      };
+      if constexpr (CODES) {
+        vec16 lo, hi;
+        decode16(vr[i], v_sc, lo, hi);
+        put_v(2 * (lane % GP), lo);
+        put_v(2 * (lane % GP) + 1, hi);
+      } else {
+        put_v(lane % CPR, vr[i]);
+      }
     }
-    if (c + W < c_end) load(vr, vh, c + W);
+    if (c + W < c_end) load_v(c + W);
     wave_lds_stage();
 
     const bool need_mask = n0 + kWaveChunk - 1 > wmin;

@@ -53,6 +53,19 @@ __device__ __forceinline__ float canonical_nan(float x) { return x != x ? __uint
 // fp32 -> bf16 bits, round-to-nearest-even, NaN -> 0x7fc0.
 __device__ __forceinline__ uint32_t f32_to_bf16_bits(float f) { return f32x2_to_bf16x2_bits(f, 0.0f) & 0xffffu; }
 
+// 16 e4m3 codes times the power of two `scale`, as 16 bf16 values: exact where the product is a bf16
+// value (three fraction bits always fit; far below 2^-126 it rounds). A scale of byte 255 (here an infinity) gives
+// NaNs, as the e8m0 format has it; checked over all codes and scale bytes.
+__device__ __forceinline__ void decode16(const vec16& c, float scale, vec16& lo, vec16& hi) {
+  auto two = [&](uint32_t w, auto high) {
+    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, scale, decltype(high)::value));
+  };
+  constexpr std::false_type l{};
+  constexpr std::true_type h{};
+  lo = vec16{two(c.x, l), two(c.x, h), two(c.y, l), two(c.y, h)};
+  hi = vec16{two(c.z, l), two(c.z, h), two(c.w, l), two(c.w, h)};
+}
+
 // Element traits: VEC elements per 16-byte vector, unpack to fp32, pack with rounding.
 template <int DTYPE>
 struct Elem;

@@ -9,6 +9,7 @@
 // host for each: attention_active 9.4 us, rope_qkv (k/v into a cache) 10.9, add_rmsnorm 8.0,
 // silu_mul 12.2. The launch itself is 2-3 us of that.
 #include <Python.h>
+#include <c10/core/DeviceGuard.h>
 #include <c10/core/impl/LocalDispatchKeySet.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/Exceptions.h>
@@ -534,7 +535,240 @@ PyObject* extract_chunks(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
   CKV_PY_END
 }
 
+// An 8-bit cache's four tensors of one shape: codes (1, H, N, D), scales (1, H, ceil(N / block)).
+struct CodedCache {
+  const Tensor &k, &v, &ks, &vs;
+  int64_t block, H, N, D;
+};
+CodedCache coded_cache(PyObject* const* a) {
+  const Tensor &k = tensor(a[0]), &v = tensor(a[1]), &ks = tensor(a[2]), &vs = tensor(a[3]);
+  const int64_t block = integer(a[4]);
+  if (block != 32 && block != 64 && block != 128) value_error("block_tokens must be 32, 64 or 128");
+  need_dims(k, 4, "an 8-bit cache's codes");
+  if (k.scalar_type() != at::kFloat8_e4m3fn || v.scalar_type() != at::kFloat8_e4m3fn ||
+      ks.scalar_type() != at::kFloat8_e8m0fnu || vs.scalar_type() != at::kFloat8_e8m0fnu)
+    type_error("an 8-bit cache has float8_e4m3fn codes and float8_e8m0fnu scales");
+  const int64_t H = k.size(1), N = k.size(2), D = k.size(3), blocks = (N + block - 1) / block;
+  if (k.size(0) != 1 || !k.is_contiguous() || !v.is_contiguous() || v.sizes() != k.sizes())
+    value_error("an 8-bit cache's codes must be contiguous (1, Hkv, N, D)");
+  if (ks.sizes() != at::IntArrayRef({1, H, blocks}) || vs.sizes() != ks.sizes() || !ks.is_contiguous() || !vs.is_contiguous())
+    value_error("an 8-bit cache's scales must be contiguous (1, Hkv, ceil(N / block_tokens))");
+  if (N > INT32_MAX) value_error("an 8-bit cache has at most 2^31 - 1 rows");
+  return {k, v, ks, vs, block, H, N, D};
+}
+
+// Head stride (elements) of a (1, H, N, D) cache whose heads each have contiguous rows.
+int64_t head_stride(const Tensor& t, const char* what) {
+  const int64_t N = t.size(2), D = t.size(3);
+  const bool rows = t.stride(3) == 1 && (N <= 1 || t.stride(2) == D);
+  const int64_t hs = t.size(1) > 1 ? t.stride(1) : std::max(t.stride(1), N * D);
+  if (!rows || hs < N * D) value_error(std::string(what) + " must have each head's rows contiguous");
+  return t.size(1) > 1 ? hs : N * D;
+}
+// Stride of dimension d; where there is one element or none, any number serves: the packed one.
+int64_t step(const Tensor& t, int64_t d, int64_t packed) { return t.size(d) > 1 ? t.stride(d) : packed; }
+// An optional device status word.
+int32_t* status_word(const Tensor& err, const Tensor& like) {
+  if (!err.defined()) return nullptr;
+  same_device(like, err);
+  if (err.scalar_type() != at::kInt || err.numel() < 1) value_error("err must be an int32 tensor");
+  return (int32_t*)ptr(err);
+}
+
+// quantize_rows(k codes, v codes, k scales, v scales, block, k, v, start, err)
+PyObject* quantize_rows(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
+  CKV_PY_BEGIN
+  need_args(n_args, 9);
+  const CodedCache c = coded_cache(a);
+  Tensor k = tensor(a[5]), v = tensor(a[6]);
+  const Tensor err = optional_tensor(a[8]);
+  same_device(c.k, c.v, c.ks, c.vs, k, v);
+  need_dims(k, 4, "k");
+  const int64_t n = k.size(2);
+  if (k.size(0) != 1 || k.size(1) != c.H || k.size(3) != c.D || v.sizes() != k.sizes())
+    value_error("rows " + shape_of(k) + " do not match the cache " + shape_of(c.k));
+  if (v.scalar_type() != k.scalar_type()) type_error("k and v must share a dtype");
+  const int code = dtype_code(k);
+  int64_t start = 0;
+  Tensor start_dev;
+  if (THPVariable_Check(a[7])) {
+    start_dev = tensor(a[7]);
+    same_device(c.k, start_dev);
+    if (start_dev.scalar_type() != at::kLong || start_dev.numel() != 1) value_error("start must be an int or one int64 on the device");
+  } else {
+    start = integer(a[7]);
+    if (start < 0 || start > c.N - n)
+      value_error("rows [" + std::to_string(start) + ", " + std::to_string(start + n) + ") outside the cache of " + std::to_string(c.N));
+  }
+  if (n > c.N) value_error("more rows than the cache has");
+  if (n == 0) Py_RETURN_NONE;
+  k = rows_view(k);
+  v = rows_view(v);
+  int32_t* const e = status_word(err, c.k);
+  check(unlocked([&] {
+          const c10::DeviceGuard on(c.k.device());
+          return ckv_quantize_rows(ptr(c.k), ptr(c.v), ptr(c.ks), ptr(c.vs), ptr(k), step(k, 1, n * c.D),
+                                   step(k, 2, c.D), ptr(v), step(v, 1, n * c.D), step(v, 2, c.D), start, (const int64_t*)ptr(start_dev), int32(n), int32(c.N),
+                                   int32(c.H), int32(c.D), int32(c.block), code, e, stream_of(c.k));
+        }),
+        "ckv_quantize_rows");
+  Py_RETURN_NONE;
+  CKV_PY_END
+}
+
+// What attention calls take of their queries: (1, Hq, n, D) bf16, contiguous rows on 16-byte boundaries, int64 positions.
+void query_args(Tensor& q, Tensor& pos, int64_t D, int64_t Hkv) {
+  need_dims(q, 4, "q");
+  if (q.scalar_type() != at::kBFloat16) type_error("q must be bf16");
+  if (q.size(0) != 1 || q.size(3) != D) value_error("q " + shape_of(q) + " must be (1, Hq, n, D) and match the cache's head_dim");
+  if (Hkv <= 0 || q.size(1) <= 0 || q.size(1) % Hkv) value_error("the query heads must be a multiple of the KV heads");
+  q = rows_view(q);
+  if (pos.scalar_type() != at::kLong || pos.numel() != q.size(2)) value_error("positions must be int64 (n,)");
+  pos = pos.contiguous();
+  if (q.size(2) > INT32_MAX || q.size(1) > INT32_MAX) value_error("too many query rows");
+}
+// attention_quantized(q, k codes, v codes, k scales, v scales, block, positions, scale, err, out, split)
+PyObject* attention_quantized(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
+  CKV_PY_BEGIN
+  need_args(n_args, 11);
+  Tensor q = tensor(a[0]), pos = tensor(a[6]);
+  const CodedCache c = coded_cache(a + 1);
+  const Tensor err = optional_tensor(a[8]);
+  Tensor out = optional_tensor(a[9]);
+  same_device(q, c.k, c.v, c.ks, c.vs, pos);
+  query_args(q, pos, c.D, c.H);
+  const int64_t Hq = q.size(1), n = q.size(2);
+  if (!out.defined()) {
+    out = at::empty({1, n, Hq, c.D}, q.options());
+  } else {
+    same_device(q, out);
+    if (out.sizes() != at::IntArrayRef({1, n, Hq, c.D}) || !out.is_contiguous() || out.scalar_type() != q.scalar_type())
+      value_error("out must be contiguous (1, n, Hq, D) bf16");
+  }
+  const double scale = a[7] == Py_None ? 1.0 / std::sqrt((double)c.D) : real(a[7]);
+  const int split = PyObject_IsTrue(a[10]);
+  if (split < 0) throw python_error();
+  const int64_t ws_bytes = split ? ckv_attention_quantized_workspace_bytes(int32(n), int32(c.N), int32(Hq), int32(c.H), int32(c.D)) : 0;
+  Tensor ws;
+  if (ws_bytes > 0) ws = at::empty({(ws_bytes + 3) / 4}, q.options().dtype(at::kFloat));
+  int32_t* const e = status_word(err, q);
+  check(unlocked([&] {
+          const c10::DeviceGuard on(q.device());
+          return ckv_attention_quantized(ptr(out), ptr(q), step(q, 1, n * c.D), step(q, 2, c.D), ptr(c.k), ptr(c.v), ptr(c.ks),
+                                         ptr(c.vs), (const int64_t*)ptr(pos), int32(n), int32(c.N), int32(Hq), int32(c.H),
+                                         int32(c.D), int32(c.block), scale, ptr(ws), ws_bytes, e, stream_of(q));
+        }),
+        "ckv_attention_quantized");
+  return THPVariable_Wrap(out);
+  CKV_PY_END
+}
+
+// attention_weights(q, K, positions, scale, prior, out, err)
+PyObject* attention_weights(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
+  CKV_PY_BEGIN
+  need_args(n_args, 7);
+  Tensor q = tensor(a[0]), pos = tensor(a[2]);
+  const Tensor& K = tensor(a[1]);
+  const Tensor prior = optional_tensor(a[4]), err = optional_tensor(a[6]);
+  Tensor out = optional_tensor(a[5]);
+  same_device(q, K, pos);
+  need_dims(K, 4, "K");
+  if (K.scalar_type() != at::kBFloat16) type_error("K must be bf16");
+  if (K.size(0) != 1) value_error("K must be (1, Hkv, N, D)");
+  const int64_t H = K.size(1), N = K.size(2), D = K.size(3);
+  if (N > INT32_MAX) value_error("K has at most 2^31 - 1 rows");
+  query_args(q, pos, D, H);
+  const int64_t hs = head_stride(K, "K"), Hq = q.size(1), n = q.size(2);
+  auto fits = [&](const Tensor& t, const char* what) {
+    same_device(q, t);
+    if (t.sizes() != at::IntArrayRef({1, H, N}) || !t.is_contiguous() || t.scalar_type() != at::kFloat)
+      value_error(std::string(what) + " must be contiguous (1, Hkv, N) float32");
+  };
+  if (prior.defined()) fits(prior, "prior");
+  if (!out.defined()) out = at::empty({1, H, N}, q.options().dtype(at::kFloat));
+  else fits(out, "out");
+  const double scale = a[3] == Py_None ? 1.0 / std::sqrt((double)D) : real(a[3]);
+  const int64_t ws_bytes = ckv_attention_weights_workspace_bytes(int32(n), int32(N), int32(Hq), int32(H));
+  Tensor ws;
+  if (ws_bytes > 0) ws = at::empty({(ws_bytes + 3) / 4}, q.options().dtype(at::kFloat));
+  int32_t* const e = status_word(err, q);
+  check(unlocked([&] {
+          const c10::DeviceGuard on(q.device());
+          return ckv_attention_weights((float*)ptr(out), (const float*)ptr(prior), ptr(q), step(q, 1, n * D), step(q, 2, D), ptr(K),
+                                       hs, (const int64_t*)ptr(pos), int32(n), int32(N), int32(Hq), int32(H), int32(D),
+                                       CKV_DTYPE_BF16, scale, ptr(ws), ws_bytes, e, stream_of(q));
+        }),
+        "ckv_attention_weights");
+  return THPVariable_Wrap(out);
+  CKV_PY_END
+}
+
+// Whether the bytes that two caches' heads span have any in common.
+bool overlap(const Tensor& a, int64_t a_hs, const Tensor& b, int64_t b_hs) {
+  auto span = [](const Tensor& t, int64_t hs) {
+    const uintptr_t p = (uintptr_t)t.data_ptr();
+    return std::make_pair(p, p + (uintptr_t)(((t.size(1) - 1) * hs + t.size(2) * t.size(3)) * t.element_size()));
+  };
+  const auto x = span(a, a_hs), y = span(b, b_hs);
+  return x.first < y.second && y.first < x.second;
+}
+
+// evict_rows(K, V, weights, n_keep, n_sink, n_recent, k_out, v_out): (K, V, rows, weights) of the kept rows
+PyObject* evict_rows(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
+  CKV_PY_BEGIN
+  need_args(n_args, 8);
+  const Tensor &K = tensor(a[0]), &V = tensor(a[1]), &w = tensor(a[2]);
+  const int64_t keep = integer(a[3]), sink = integer(a[4]), recent = integer(a[5]);
+  Tensor ko = optional_tensor(a[6]), vo = optional_tensor(a[7]);
+  same_device(K, V, w);
+  need_dims(K, 4, "K");
+  const int64_t H = K.size(1), N = K.size(2), D = K.size(3);
+  if (K.size(0) != 1 || V.sizes() != K.sizes()) value_error("K/V must be (1, Hkv, N, D) of one shape");
+  if (V.scalar_type() != K.scalar_type()) type_error("K and V must share a dtype");
+  if (N > INT32_MAX || H <= 0) value_error("K/V have 1 to 2^31 - 1 rows and a head at least");
+  const int64_t khs = head_stride(K, "K"), vhs = head_stride(V, "V");
+  if (w.sizes() != at::IntArrayRef({1, H, N}) || w.scalar_type() != at::kFloat || (N > 1 && w.stride(2) != 1))
+    value_error("weights must be (1, Hkv, N) float32 with contiguous rows");
+  const int64_t whs = H > 1 ? w.stride(1) : N;
+  if (sink < 0 || recent < 0 || keep < 0 || keep > N || sink > keep || recent > keep - sink)
+    value_error("n_sink + n_recent <= n_keep <= N must hold: got " + std::to_string(sink) + " + " + std::to_string(recent) +
+                ", " + std::to_string(keep) + ", " + std::to_string(N));
+  const int code = dtype_code(K);
+  auto to = [&](Tensor& t, const char* what) {
+    if (!t.defined()) {
+      t = at::empty({1, H, keep, D}, K.options());
+      return;
+    }
+    same_device(K, t);
+    if (t.sizes() != at::IntArrayRef({1, H, keep, D}) || t.scalar_type() != K.scalar_type())
+      value_error(std::string(what) + " must be (1, Hkv, n_keep, D) of K's dtype");
+  };
+  const bool given = ko.defined() || vo.defined();
+  to(ko, "k_out");
+  to(vo, "v_out");
+  const int64_t kohs = head_stride(ko, "k_out"), vohs = head_stride(vo, "v_out");
+  const Tensor rows = at::empty({1, H, keep}, K.options().dtype(at::kLong)), wo = at::empty({1, H, keep}, w.options());
+  if (keep > 0) {
+    if (given && (overlap(ko, kohs, K, khs) || overlap(ko, kohs, V, vhs) || overlap(vo, vohs, K, khs) || overlap(vo, vohs, V, vhs) ||
+                  overlap(ko, kohs, vo, vohs)))
+      value_error("k_out and v_out must overlap neither K, V nor each other");
+    check(unlocked([&] {
+            const c10::DeviceGuard on(K.device());
+            return ckv_evict_rows(ptr(ko), kohs, ptr(vo), vohs, (int64_t*)ptr(rows), (float*)ptr(wo), ptr(K), khs, ptr(V), vhs,
+                                  (const float*)ptr(w), whs, int32(N), int32(keep), int32(sink), int32(recent), int32(H),
+                                  int32(D), code, stream_of(K));
+          }),
+          "ckv_evict_rows");
+  }
+  return Py_BuildValue("(NNNN)", THPVariable_Wrap(ko), THPVariable_Wrap(vo), THPVariable_Wrap(rows), THPVariable_Wrap(wo));
+  CKV_PY_END
+}
+
 PyMethodDef kMethods[] = {
+    {"quantize_rows", (PyCFunction)(void (*)(void))quantize_rows, METH_FASTCALL, nullptr},
+    {"attention_quantized", (PyCFunction)(void (*)(void))attention_quantized, METH_FASTCALL, nullptr},
+    {"attention_weights", (PyCFunction)(void (*)(void))attention_weights, METH_FASTCALL, nullptr},
+    {"evict_rows", (PyCFunction)(void (*)(void))evict_rows, METH_FASTCALL, nullptr},
     {"attention_active", (PyCFunction)(void (*)(void))attention_active, METH_FASTCALL, nullptr},
     {"rope_qkv", (PyCFunction)(void (*)(void))rope_qkv, METH_FASTCALL, nullptr},
     {"add_rmsnorm", (PyCFunction)(void (*)(void))add_rmsnorm, METH_FASTCALL, nullptr},

@@ -635,6 +635,120 @@ def attention_active(
     return _native.torch_ops().attention_active(q, K, V, positions, scale, err, out, split)
 
 
+@dataclass
+class QuantizedCache:
+    """One layer's K/V cache in 8 bits: a row's values are code * scale, with one power-of-two scale for each head and
+    block of `block_tokens` rows, K and V apart (quantize_rows says which)."""
+
+    k: torch.Tensor  # float8_e4m3fn (1, Hkv, N, D), contiguous
+    v: torch.Tensor
+    k_scale: torch.Tensor  # float8_e8m0fnu (1, Hkv, ceil(N / block_tokens)), contiguous
+    v_scale: torch.Tensor
+    block_tokens: int = 64
+
+
+def quantized_cache(n_kv_heads: int, n_tokens: int, head_dim: int, device, block_tokens: int = 64) -> QuantizedCache:
+    """A cache of n_tokens rows for quantize_rows to fill; nothing in it is initialised."""
+    if int(block_tokens) not in (32, 64, 128):
+        raise ValueError("block_tokens must be 32, 64 or 128")
+    blocks = -(-int(n_tokens) // int(block_tokens))
+
+    def empty(n, dtype):
+        return torch.empty((1, int(n_kv_heads), *n), dtype=torch.uint8, device=device).view(dtype)
+
+    code, scale = torch.float8_e4m3fn, torch.float8_e8m0fnu
+    rows = (int(n_tokens), int(head_dim))
+    return QuantizedCache(empty(rows, code), empty(rows, code), empty((blocks,), scale), empty((blocks,), scale),
+                          int(block_tokens))
+
+
+def quantize_rows(
+    cache: QuantizedCache,
+    k: torch.Tensor,
+    v: torch.Tensor,
+    start: int | torch.Tensor = 0,
+    err: torch.Tensor | None = None,
+) -> None:
+    """Write k/v (1, Hkv, n, D), bf16 or float32, into rows [start, start + n) of an 8-bit cache, one launch: a whole
+    prefill's rows, or a decoded token's appended to its block.
+
+    A block's scale is the least power of two 2^e that brings its largest |x| to at most 448 2^e, a code
+    e4m3(x / scale) to nearest even. Rows in front of start keep their values (their codes follow where their block's
+    scale grows; only codes that become subnormal lose bits); rows behind start + n hold nothing any more. An infinity
+    or a NaN makes its block NaN. start: an int, or an int64 tensor of one element on the device, which a captured
+    decode step reads on each replay (out of range: nothing is written, and err is set).
+    """
+    _native.torch_ops().quantize_rows(cache.k, cache.v, cache.k_scale, cache.v_scale, cache.block_tokens, k, v, start, err)
+
+
+def attention_quantized(
+    q: torch.Tensor,
+    cache: QuantizedCache,
+    positions: torch.Tensor,
+    scale: float | None = None,
+    err: torch.Tensor | None = None,
+    out: torch.Tensor | None = None,
+    split: bool = True,
+) -> torch.Tensor:
+    """attention_active over an 8-bit cache: the same function, with the same roundings, of the rows that its codes and
+    scales stand for. q, positions, scale, err and out as there; rows past the largest position may hold anything,
+    rows up to it are finite.
+    split: let launches use a workspace (allocated here): partial results where the cache range is split, and the cache as
+    bf16 where many queries read it."""
+    return _native.torch_ops().attention_quantized(q, cache.k, cache.v, cache.k_scale, cache.v_scale, cache.block_tokens,
+                                                   positions, scale, err, out, split)
+
+
+def attention_weights(
+    q: torch.Tensor,
+    K: torch.Tensor,
+    positions: torch.Tensor,
+    scale: float | None = None,
+    *,
+    prior: torch.Tensor | None = None,
+    out: torch.Tensor | None = None,
+    err: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """The attention weight each cached row received: (1, Hkv, N) float32, prior (or 0) plus, for each row, the softmax
+    weights that the query rows and the query heads of its KV head give it, query i seeing positions <= positions[i].
+
+    q: (1, Hq, n, D) bf16 with contiguous rows; K: (1, Hkv, N, D) bf16, a head's rows contiguous (e.g. a [:, :, :N] view of
+    a longer cache), rows past the largest position anything, rows up to it finite. prior and out: float32 (1, Hkv, N) contiguous, and may be
+    one tensor (weights that grow over decode steps). Sums are fp32 in a fixed order.
+    """
+    return _native.torch_ops().attention_weights(q, K, positions, scale, prior, out, err)
+
+
+@dataclass
+class Evicted:
+    K: torch.Tensor  # (1, Hkv, n_keep, D): the kept rows, in order
+    V: torch.Tensor
+    rows: torch.Tensor  # int64 (1, Hkv, n_keep): the row each was, ascending
+    weights: torch.Tensor  # float32 (1, Hkv, n_keep): its weight
+
+
+def evict_rows(
+    K: torch.Tensor,
+    V: torch.Tensor,
+    weights: torch.Tensor,
+    n_keep: int,
+    n_sink: int = 0,
+    n_recent: int = 0,
+    *,
+    k_out: torch.Tensor | None = None,
+    v_out: torch.Tensor | None = None,
+) -> Evicted:
+    """Cut a layer's cache (1, Hkv, N, D) to n_keep rows per KV head: the first n_sink, the last n_recent, and of the
+    others those of the largest weights (1, Hkv, N) float32 (attention_weights), the lower row first among equals, a NaN
+    below every number. Keys keep the rotation of their positions: later queries attend over the n_keep rows with
+    positions counted in them, as rows are appended behind.
+
+    K/V: bf16 or float32, a head's rows contiguous (views of longer caches too). k_out/v_out: where the kept rows go,
+    (1, Hkv, n_keep, D) likewise (new tensors by default); they must not overlap K or V.
+    """
+    return Evicted(*_native.torch_ops().evict_rows(K, V, weights, int(n_keep), int(n_sink), int(n_recent), k_out, v_out))
+
+
 def rope_qkv(
     q_in: torch.Tensor | None,
     k_in: torch.Tensor,

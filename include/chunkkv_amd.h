@@ -30,7 +30,7 @@
 extern "C" {
 #endif
 
-#define CKV_ABI_VERSION 6
+#define CKV_ABI_VERSION 7
 
 typedef enum ckv_status {
   CKV_OK = 0,
@@ -553,6 +553,87 @@ int32_t ckv_attention_active(void* out, const void* q, int64_t q_head_stride, in
  */
 int64_t ckv_attention_workspace_bytes(int32_t n_queries, int32_t n_tokens, int32_t n_q_heads,
                                       int32_t head_dim, int32_t* splits, int32_t* split_tiles);
+
+/*
+ * Write rows [start, start + n_rows) of an 8-bit K/V cache. Such a cache holds, for K and for V, e4m3 codes
+ * (OCP, one byte an element: (n_heads, n_tokens, head_dim) contiguous) and a scale for each head and block of
+ * block_tokens rows, a power of two as its exponent byte e + 127 (OCP e8m0, 255 = NaN;
+ * (n_heads, ceil(n_tokens / block_tokens))); a row's values are code * scale.
+ *   scale of a block = 2^e, e the least integer >= -126 with max |x| <= 448 * 2^e over the block's rows
+ *   code             = e4m3(x / scale), to nearest even
+ * Rows of the first block in front of `start` are kept: the block's scale is the larger of theirs and the new
+ * rows', and where it grows their codes are rescaled (exactly, but for codes that become subnormal). Rows
+ * behind start + n_rows keep their bytes but not their scale: they hold nothing any more. An infinity or a
+ * NaN among the new rows makes its block's rows and scale NaN.
+ *   k, v          the rows, (n_heads, n_rows, head_dim) with the given strides (elements; rows contiguous, 16-byte
+ *                 aligned), bf16 or f32
+ *   start_dev     optional device word that is read in place of `start` (a captured decode step's
+ *                 position); a start outside [0, n_tokens - n_rows] writes nothing and is flagged in *err
+ * head_dim 64 or 128; block_tokens 32, 64 or 128. One launch. No counterpart in the reference.
+ */
+int32_t ckv_quantize_rows(void* k_codes, void* v_codes, void* k_scales, void* v_scales, const void* k,
+                          int64_t k_head_stride, int64_t k_token_stride, const void* v, int64_t v_head_stride,
+                          int64_t v_token_stride, int64_t start, const int64_t* start_dev, int32_t n_rows,
+                          int32_t n_tokens, int32_t n_heads, int32_t head_dim, int32_t block_tokens, int32_t dtype,
+                          int32_t* err, void* stream);
+
+/*
+ * ckv_attention_active over an 8-bit cache (ckv_quantize_rows): the same function of the rows that codes and scales
+ * stand for, which are bf16 values, with the same roundings. q, out, positions, scale and err as there. Rows past
+ * the largest position may hold anything, as may the scales of blocks past its block; rows up to it are finite.
+ *   workspace  optional device buffer of workspace_bytes >= ckv_attention_quantized_workspace_bytes(...)
+ *              (16-byte aligned): partial rows of split launches and, for launches of many queries, the cache as
+ *              bf16. With less, or none, they run without (slower; the same up to the order of fp32 sums).
+ * No counterpart in the reference.
+ */
+int32_t ckv_attention_quantized(void* out, const void* q, int64_t q_head_stride, int64_t q_token_stride,
+                                const void* k_codes, const void* v_codes, const void* k_scales,
+                                const void* v_scales, const int64_t* positions, int32_t n_queries,
+                                int32_t n_tokens, int32_t n_q_heads, int32_t n_kv_heads, int32_t head_dim,
+                                int32_t block_tokens, double scale, void* workspace, int64_t workspace_bytes,
+                                int32_t* err, void* stream);
+
+/* Bytes of workspace that ckv_attention_quantized uses for this shape (0: none). Host-only. */
+int64_t ckv_attention_quantized_workspace_bytes(int32_t n_queries, int32_t n_tokens, int32_t n_q_heads,
+                                                int32_t n_kv_heads, int32_t head_dim);
+
+/*
+ * The attention weight that each cached row received, over all query rows and the query heads of its KV head:
+ *   out[hk, j] = prior[hk, j] + sum over i and over h in group hk of w[h, i, j],
+ *   w[h, i, :] = softmax over j in [0, positions[i]] of scale * q[h, i, :] . K[hk, j, :]   (0 past it).
+ * prior (NULL: zeros) and out are (n_kv_heads, n_tokens) fp32 contiguous and may be the same. q, k_cache, positions,
+ * scale and err as in ckv_attention_active (bf16, head_dim 64 or 128, k_head_stride at least n_tokens * head_dim);
+ * rows past the largest position may hold anything, rows up to it are finite. Scores, weights and sums are fp32, added in a fixed order.
+ *   workspace  device buffer of workspace_bytes >= ckv_attention_weights_workspace_bytes(...), 16-byte aligned
+ * No counterpart in the reference.
+ */
+int32_t ckv_attention_weights(float* out, const float* prior, const void* q, int64_t q_head_stride,
+                              int64_t q_token_stride, const void* k_cache, int64_t k_head_stride,
+                              const int64_t* positions, int32_t n_queries, int32_t n_tokens, int32_t n_q_heads,
+                              int32_t n_kv_heads, int32_t head_dim, int32_t dtype, double scale, void* workspace,
+                              int64_t workspace_bytes, int32_t* err, void* stream);
+
+/* Bytes of workspace that ckv_attention_weights needs for this shape. Host-only. */
+int64_t ckv_attention_weights_workspace_bytes(int32_t n_queries, int32_t n_tokens, int32_t n_q_heads,
+                                              int32_t n_kv_heads);
+
+/*
+ * Cut a layer's cache to n_keep rows per KV head: the first n_sink rows, the last n_recent, and of the others those
+ * of the largest weights[h, row] until n_keep stay, the lower row first among equal weights (-0 equals 0, a NaN ranks
+ * below every number):
+ *   rows_out[h, i]    = the i-th kept row of head h, ascending         (n_heads, n_keep) contiguous
+ *   weights_out[h, i] = weights[h, rows_out[h, i]]                     (n_heads, n_keep) contiguous
+ *   k_out[h, i, :]    = k_cache[h, rows_out[h, i], :], v_out likewise  bit copies
+ * Caches are (n_heads, rows, head_dim) with contiguous rows and the given head strides (elements, 16-byte multiples);
+ * weights' head stride is weights_head_stride. The outputs overlap none of the inputs.
+ * n_sink + n_recent <= n_keep <= n_tokens (CKV_ERR_OUT_OF_RANGE otherwise); head_dim 64, 128 or 256; bf16 or f32.
+ * No counterpart in the reference.
+ */
+int32_t ckv_evict_rows(void* k_out, int64_t ko_head_stride, void* v_out, int64_t vo_head_stride, int64_t* rows_out,
+                       float* weights_out, const void* k_cache, int64_t k_head_stride, const void* v_cache,
+                       int64_t v_head_stride, const float* weights, int64_t weights_head_stride, int32_t n_tokens,
+                       int32_t n_keep, int32_t n_sink, int32_t n_recent, int32_t n_heads, int32_t head_dim,
+                       int32_t dtype, void* stream);
 
 /*
  * Residual add and RMSNorm of each row, the elementwise steps around a decoder layer's GEMMs:
