@@ -109,7 +109,7 @@ SIGNATURES = {
         _i32,
         [_p, _p, _p, _i64, _i64, _p, _i64, _p, _i32, _i32, _i32, _i32, _i32, _i32, _f64, _p, _i64, _p, _p],
     ),
-    "ckv_attention_weights_workspace_bytes": (_i64, [_i32] * 4),
+    "ckv_attention_weights_workspace_bytes": (_i64, [_i32] * 5),
     "ckv_evict_rows": (
         _i32,
         [_p, _i64, _p, _i64, _p, _p, _p, _i64, _p, _i64, _p, _i64, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _p],

@@ -38,6 +38,14 @@ __global__ __launch_bounds__(256) void decode_rows_kernel(char* __restrict__ k_o
 static bool decode_first(int n, int N, int Hq, int Hkv, int head_dim) {
   return !attn_plan(n, N, Hq, Hkv, head_dim, attn_workspace_bytes(n, N, Hq, head_dim)).wave;
 }
+#ifndef FILL
+#define FILL 512
+#endif
+static int wave_fill(int N) { return N >= 4096 ? FILL : kWaveFill; }
+static int64_t wave_workspace_bytes(int n, int N, int Hq, int head_dim) {
+  const int64_t splits = most_splits(n, N, Hq, head_dim, wave_fill(N));
+  return splits > 1 ? splits * Hq * n * (head_dim + 4) * 4 : 0;
+}
 static int64_t decoded_bytes(int N, int Hkv, int head_dim) { return (int64_t)Hkv * N * head_dim * 4; }
 
 }  // namespace ckv
@@ -46,8 +54,9 @@ extern "C" int64_t ckv_attention_quantized_workspace_bytes(int32_t n_queries, in
                                                            int32_t n_kv_heads, int32_t head_dim) {
   using namespace ckv;
   if (n_queries <= 0 || n_tokens <= 0 || n_q_heads <= 0 || n_kv_heads <= 0 || head_dim <= 0 || n_q_heads % n_kv_heads) return 0;
-  return attn_workspace_bytes(n_queries, n_tokens, n_q_heads, head_dim) +
-         (decode_first(n_queries, n_tokens, n_q_heads, n_kv_heads, head_dim) ? decoded_bytes(n_tokens, n_kv_heads, head_dim) : 0);
+  return decode_first(n_queries, n_tokens, n_q_heads, n_kv_heads, head_dim)
+             ? decoded_bytes(n_tokens, n_kv_heads, head_dim) + attn_workspace_bytes(n_queries, n_tokens, n_q_heads, head_dim)
+             : wave_workspace_bytes(n_queries, n_tokens, n_q_heads, head_dim);
 }
 
 extern "C" int32_t ckv_attention_quantized(void* out, const void* q, int64_t q_head_stride, int64_t q_token_stride,
@@ -94,7 +103,7 @@ extern "C" int32_t ckv_attention_quantized(void* out, const void* q, int64_t q_h
 
   const float scale_log2 = (float)(scale * 1.4426950408889634);  // exp(x) = exp2(x log2 e)
   const int group = n_q_heads / n_kv_heads;
-  const AttnPlan plan = attn_wave_plan(n_queries, n_tokens, n_q_heads, n_kv_heads, head_dim, workspace_bytes);
+  const AttnPlan plan = attn_wave_plan(n_queries, n_tokens, n_q_heads, n_kv_heads, head_dim, workspace_bytes, wave_fill(n_tokens));
   const AttnMap& map = plan.map;
   float* ws = plan.splits > 1 ? (float*)workspace : nullptr;
   const CacheScales scales = {(const uint8_t*)k_scales, (const uint8_t*)v_scales, blocks, block_log - 5};

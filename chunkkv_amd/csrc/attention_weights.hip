@@ -20,8 +20,11 @@
 namespace ckv {
 
 constexpr int kWtThreads = 256;
-constexpr int kWtRows = 128;   // query rows of a workgroup of the first pass, cache rows of one of the second
 constexpr int kWtTile = 64;    // cache rows of a tile of the first pass, query rows of one of the second
+constexpr int kWtQG = 2;       // 16-row groups of a wavefront of the first pass, and of the second's cache rows
+constexpr int kWtKG = 2;
+constexpr int kWtFewRows = 16;  // query rows of a KV head up to which scores go through memory
+constexpr int kWtMostParts = 128;  // splits of the cache there
 
 // A query row's normaliser and position, as the second pass reads it.
 struct RowStat {
@@ -33,14 +36,14 @@ typedef __attribute__((address_space(1))) void wt_gvoid;
 typedef __attribute__((address_space(3))) void wt_lvoid;
 
 // SPLIT: split z of the cache's tiles; (max, sum) of a row's split to part[z].
-template <int D, bool SPLIT>
+template <int D, int QG, bool SPLIT>
 __global__ __launch_bounds__(kWtThreads) void weights_lse_kernel(
     int nqb, int map_group, int xpk_log, int items, uint32_t inv_group, uint32_t inv_nqb,
     const int64_t* __restrict__ pos, int N, int rows, int group, uint32_t inv_gqa, const char* __restrict__ kc,
     int64_t k_hs_b, const char* __restrict__ q, int64_t q_hs_b, int64_t q_ts_b, float scale_log2,
-    RowStat* __restrict__ stat, float2* __restrict__ part, int64_t part_stride, int split_tiles,
+    RowStat* __restrict__ stat, char* __restrict__ packed, int stat_rows, float2* __restrict__ part, int64_t part_stride, int split_tiles,
     int32_t* __restrict__ err) {
-  constexpr int DS = D / 32, CPR = D / 8, ROWB = D * 2, QG = 2, KI = kWtTile * CPR / kWtThreads;
+  constexpr int DS = D / 32, CPR = D / 8, ROWB = D * 2, KI = kWtTile * CPR / kWtThreads, BR = 64 * QG;
   __shared__ __attribute__((aligned(1024))) char lds0[kWtTile * ROWB];
   __shared__ __attribute__((aligned(1024))) char lds1[kWtTile * ROWB];
   __shared__ int blk_max_s[kWtThreads / 64];
@@ -53,7 +56,7 @@ __global__ __launch_bounds__(kWtThreads) void weights_lse_kernel(
   bf16x8 qf[QG][DS];
 #pragma unroll
   for (int qg = 0; qg < QG; ++qg) {
-    const int r = rb * kWtRows + wave * 32 + qg * 16 + lm;
+    const int r = rb * BR + (wave * QG + qg) * 16 + lm;
     const int rc = min(r, rows - 1), t = div_by(rc, group, inv_gqa), gh = rc - t * group;
     const int64_t p64 = pos[t];
     int p = p64 < 0 ? 0 : p64 >= N ? N - 1 : (int)p64;
@@ -71,6 +74,15 @@ __global__ __launch_bounds__(kWtThreads) void weights_lse_kernel(
   }
   wmax = __builtin_amdgcn_readfirstlane(row16_reduce(wmax, [](int a, int b) { return max(a, b); }));
   wmin = __builtin_amdgcn_readfirstlane(row16_reduce(wmin, [](int a, int b) { return min(a, b); }));
+  if (!SPLIT || z == 0) {  // the rows packed, for the second pass
+#pragma unroll
+    for (int qg = 0; qg < QG; ++qg) {
+      const int r = rb * BR + (wave * QG + qg) * 16 + lm;
+#pragma unroll
+      for (int s = 0; s < DS; ++s)
+        if (r < stat_rows) st16(packed + ((int64_t)hk * stat_rows + r) * ROWB + (32 * s + 8 * g) * 2, __builtin_bit_cast(vec16, qf[qg][s]));
+    }
+  }
   if (lane == 0) blk_max_s[wave] = wmax;
   __syncthreads();
   int bmax = blk_max_s[0];
@@ -82,10 +94,11 @@ __global__ __launch_bounds__(kWtThreads) void weights_lse_kernel(
   if (SPLIT) n_tiles = min(n_tiles, tile_begin + split_tiles);
 
   // A lane's own maximum and sum over the cache rows that it gets.
-  float m_run[QG], l_run[QG];
+  float m_run[QG], m_sub[QG], l_run[QG];
 #pragma unroll
   for (int qg = 0; qg < QG; ++qg) {
     m_run[qg] = -INFINITY;
+    m_sub[qg] = 0.f;
     l_run[qg] = 0.f;
   }
   const char* kh = kc + (int64_t)hk * k_hs_b;
@@ -97,11 +110,16 @@ __global__ __launch_bounds__(kWtThreads) void weights_lse_kernel(
   }
   auto issue = [&](int n0, char* kb) {
     const char* kt = kh + (int64_t)n0 * ROWB;
-    const int last = bmax - n0;  // rows past every position load the last one's
-#pragma unroll
-    for (int i = 0; i < KI; ++i) {
-      const int o = min(off[i] / ROWB, last) * ROWB + off[i] % ROWB;
+    const int last = bmax - n0;
+    auto load = [&](int i, int o) {
       __builtin_amdgcn_global_load_lds((wt_gvoid*)(kt + (uint32_t)o), (wt_lvoid*)(kb + (wave * KI + i) * 1024), 16, 0, 0);
+    };
+    if (last >= kWtTile - 1) {  // uniform: a whole tile
+#pragma unroll
+      for (int i = 0; i < KI; ++i) load(i, off[i]);
+    } else {  // rows past every position load the last one's
+#pragma unroll
+      for (int i = 0; i < KI; ++i) load(i, min(off[i] / ROWB, last) * ROWB + off[i] % ROWB);
     }
   };
   int k_rd[DS];
@@ -115,45 +133,58 @@ __global__ __launch_bounds__(kWtThreads) void weights_lse_kernel(
     if (tile + 1 < n_tiles) issue(n0 + kWtTile, nxt);
     if (n0 > wmax) return;  // uniform per wavefront
     const bool need_mask = n0 + kWtTile - 1 > wmin;
-    constexpr int T = kWtTile / 16;
-    f32x4 s[QG][T];  // lane (g, lm): query lm, cache rows n0 + 16 t + 4 g + e
+    constexpr int T = 2;  // 32 cache rows at a time
 #pragma unroll
-    for (int t = 0; t < T; ++t)
+    for (int half = 0; half < kWtTile / (16 * T); ++half) {
+      f32x4 s[QG][T];  // lane (g, lm): query lm, cache rows n0 + 32 half + 16 t + 4 g + e
 #pragma unroll
-      for (int ds = 0; ds < DS; ++ds) {
-        const bf16x8 a = *(const bf16x8*)(cur + t * 16 * ROWB + k_rd[ds]);
+      for (int ds = 0; ds < DS; ++ds)  // dependent products four apart
 #pragma unroll
-        for (int qg = 0; qg < QG; ++qg)
-          s[qg][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, qf[qg][ds], ds == 0 ? f32x4{0.f, 0.f, 0.f, 0.f} : s[qg][t], 0, 0, 0);
+        for (int t = 0; t < T; ++t) {
+          const bf16x8 a = *(const bf16x8*)(cur + (half * T + t) * 16 * ROWB + k_rd[ds]);
+#pragma unroll
+          for (int qg = 0; qg < QG; ++qg)
+            s[qg][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, qf[qg][ds], ds == 0 ? f32x4{0.f, 0.f, 0.f, 0.f} : s[qg][t], 0, 0, 0);
+        }
+      if (need_mask) {
+#pragma unroll
+        for (int qg = 0; qg < QG; ++qg) {
+          const int lim = my_pos[qg] - n0 - 16 * T * half - 4 * g;
+#pragma unroll
+          for (int t = 0; t < T; ++t)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (16 * t + e > lim) s[qg][t][e] = -INFINITY;
+        }
+      }
+      float bm[QG];
+      bool raise = false;
+#pragma unroll
+      for (int qg = 0; qg < QG; ++qg) {
+        bm[qg] = s[qg][0][0];
+#pragma unroll
+        for (int t = 0; t < T; ++t)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) bm[qg] = fmaxf(bm[qg], s[qg][t][e]);
+        bm[qg] *= scale_log2;  // > 0: max commutes
+        raise = raise || bm[qg] > m_run[qg] + 8.f;  // a sum's fp32 range takes weights up to 2^8
+      }
+      if (__builtin_amdgcn_ballot_w64(raise)) {
+#pragma unroll
+        for (int qg = 0; qg < QG; ++qg) {
+          const float m_new = bm[qg] > m_run[qg] + 8.f ? bm[qg] : m_run[qg];
+          l_run[qg] *= m_run[qg] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m_run[qg] - m_new);
+          m_run[qg] = m_new;
+          m_sub[qg] = m_new == -INFINITY ? 0.f : m_new;
+        }
       }
 #pragma unroll
-    for (int qg = 0; qg < QG; ++qg) {
-      if (need_mask) {
-        const int lim = my_pos[qg] - n0 - 4 * g;
+      for (int qg = 0; qg < QG; ++qg)
 #pragma unroll
         for (int t = 0; t < T; ++t)
 #pragma unroll
           for (int e = 0; e < 4; ++e)
-            if (16 * t + e > lim) s[qg][t][e] = -INFINITY;
-      }
-      float bm = -INFINITY;
-#pragma unroll
-      for (int t = 0; t < T; ++t)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) bm = fmaxf(bm, s[qg][t][e]);
-      bm *= scale_log2;  // > 0: max commutes
-      // raised only by more than 2^8, which the sum's fp32 range takes
-      if (__builtin_amdgcn_ballot_w64(bm > m_run[qg] + 8.f)) {
-        const float m_new = bm > m_run[qg] + 8.f ? bm : m_run[qg];
-        l_run[qg] *= m_run[qg] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m_run[qg] - m_new);
-        m_run[qg] = m_new;
-      }
-      const float sub = m_run[qg] == -INFINITY ? 0.f : m_run[qg];
-#pragma unroll
-      for (int t = 0; t < T; ++t)
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          l_run[qg] += __builtin_amdgcn_exp2f(__builtin_fmaf(s[qg][t][e], scale_log2, -sub));
+            l_run[qg] += __builtin_amdgcn_exp2f(__builtin_fmaf(s[qg][t][e], scale_log2, -m_sub[qg]));
     }
   };
   for (int tile = tile_begin; tile < n_tiles; tile += 2) {
@@ -167,40 +198,39 @@ __global__ __launch_bounds__(kWtThreads) void weights_lse_kernel(
     float l = m_run[qg] == -INFINITY ? 0.f : l_run[qg] * __builtin_amdgcn_exp2f(m_run[qg] - m);
     l += __shfl_xor(l, 16);
     l += __shfl_xor(l, 32);
-    const int r = rb * kWtRows + wave * 32 + qg * 16 + lm;
-    if (r >= rows || g != 0) continue;
-    const int64_t at = (int64_t)hk * rows + r;
+    const int r = rb * BR + (wave * QG + qg) * 16 + lm;
+    if (r >= stat_rows || g != 0) continue;
+    const int64_t at = (int64_t)hk * stat_rows + r;
     if (SPLIT) part[z * part_stride + at] = make_float2(m, l);
-    else stat[at] = RowStat{m + __builtin_amdgcn_logf(l), my_pos[qg]};
+    else stat[at] = r < rows ? RowStat{m + __builtin_amdgcn_logf(l), my_pos[qg]} : RowStat{INFINITY, -1};
   }
 }
 
-// Joins the splits of the first pass, a row a thread.
+// Joins the splits (at most 64) of the first pass: a row a wavefront, a split a lane.
 __global__ __launch_bounds__(256) void weights_join_kernel(const float2* __restrict__ part, int64_t stride, int splits,
                                                            const int64_t* __restrict__ pos, int N, int rows, int group,
-                                                           RowStat* __restrict__ stat, int64_t total) {
-  const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x;
+                                                           RowStat* __restrict__ stat, int stat_rows, int64_t total) {
+  const int64_t at = (int64_t)blockIdx.x * 4 + threadIdx.x / 64;
+  const int lane = threadIdx.x % 64;
   if (at >= total) return;
-  float m = -INFINITY, l = 0.f;
-  for (int z = 0; z < splits; ++z) {
-    const float2 p = part[z * stride + at];
-    if (p.x == -INFINITY) continue;
-    const float mn = fmaxf(m, p.x);
-    l = l * __builtin_amdgcn_exp2f(m - mn) + p.y * __builtin_amdgcn_exp2f(p.x - mn);
-    m = mn;
-  }
-  const int64_t p64 = pos[(int)(at % rows) / group];
-  stat[at] = RowStat{m + __builtin_amdgcn_logf(l), p64 < 0 ? 0 : p64 >= N ? N - 1 : (int)p64};
+  const float2 p = part[min(lane, splits - 1) * stride + at];
+  const int row = (int)(at % stat_rows);
+  const int64_t p64 = pos[min(row, rows - 1) / group];
+  float m = lane < splits ? p.x : -INFINITY;
+  const float mine = m;
+  for (int d = 32; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor(m, d));
+  const float l = wave_butterfly_sum(mine == -INFINITY ? 0.f : p.y * __builtin_amdgcn_exp2f(mine - m));
+  if (lane == 0)
+    stat[at] = row < rows ? RowStat{m + __builtin_amdgcn_logf(l), p64 < 0 ? 0 : p64 >= N ? N - 1 : (int)p64} : RowStat{INFINITY, -1};
 }
 
 // PARTS: part z of the query rows; sums to ws[z], else prior + sum to out.
-template <int D, bool PARTS>
-__global__ __launch_bounds__(kWtThreads) void weights_sum_kernel(
-    int nkb, int map_group, int xpk_log, int items, uint32_t inv_group, uint32_t inv_nkb, int N, int rows, int group,
-    uint32_t inv_gqa, const char* __restrict__ kc, int64_t k_hs_b, const char* __restrict__ q, int64_t q_hs_b,
-    int64_t q_ts_b, float scale_log2, const RowStat* __restrict__ stat, const float* prior, float* out,
-    int64_t part_stride, int part_tiles) {
-  constexpr int DS = D / 32, CPR = D / 8, ROWB = D * 2, KG = 2, KI = kWtTile * CPR / kWtThreads, QT = kWtTile / 16;
+template <int D, int KG, bool PARTS>
+__global__ __launch_bounds__(kWtThreads, 4) void weights_sum_kernel(
+    int nkb, int map_group, int xpk_log, int items, uint32_t inv_group, uint32_t inv_nkb, int N, int stat_rows,
+    const char* __restrict__ kc, int64_t k_hs_b, const char* __restrict__ packed, float scale_log2,
+    const RowStat* __restrict__ stat, const float* prior, float* out, int64_t part_stride, int part_tiles) {
+  constexpr int DS = D / 32, CPR = D / 8, ROWB = D * 2, KI = kWtTile * CPR / kWtThreads, QT = kWtTile / 16;
   __shared__ __attribute__((aligned(1024))) char lds0[kWtTile * ROWB];
   __shared__ __attribute__((aligned(1024))) char lds1[kWtTile * ROWB];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x % 64;
@@ -208,16 +238,15 @@ __global__ __launch_bounds__(kWtThreads) void weights_sum_kernel(
   int kb, hk, z;
   if (!attn_work_item(nkb, map_group, xpk_log, items, inv_group, inv_nkb, kb, hk, z)) return;
   kb = nkb - 1 - kb;  // the first cache rows, which the most queries see, first
-  const RowStat* st = stat + (int64_t)hk * rows;
-  const int tile_begin = PARTS ? z * part_tiles : 0;
-  const int tiles = (rows + kWtTile - 1) / kWtTile;
+  const RowStat* st = stat + (int64_t)hk * stat_rows;
+  const int tile_begin = PARTS ? z * part_tiles : 0, tiles = stat_rows / kWtTile;
   const int tile_end = PARTS ? min(tiles, tile_begin + part_tiles) : tiles;
-  const int k0 = kb * kWtRows + wave * 32;  // this wavefront's cache rows
+  const int k0 = (kb * (kWtThreads / 64) + wave) * (16 * KG);  // this wavefront's cache rows
 
   // does any query row of the part see these cache rows?
   int seen = -1;
-  for (int r = tile_begin * kWtTile + (int)threadIdx.x; r < min(tile_end * kWtTile, rows); r += kWtThreads) seen = max(seen, st[r].pos);
-  const bool any = __syncthreads_or(seen >= kb * kWtRows);
+  for (int r = tile_begin * kWtTile + (int)threadIdx.x; r < tile_end * kWtTile; r += kWtThreads) seen = max(seen, st[r].pos);
+  const bool any = __syncthreads_or(seen >= kb * (kWtThreads / 64) * 16 * KG);
 
   f32x4 acc[KG];
 #pragma unroll
@@ -230,34 +259,31 @@ __global__ __launch_bounds__(kWtThreads) void weights_sum_kernel(
 #pragma unroll
       for (int ds = 0; ds < DS; ++ds)
         kf[kg][ds] = __builtin_bit_cast(bf16x8, ld16(kh + (int64_t)min(k0 + 16 * kg + lm, N - 1) * ROWB + (32 * ds + 8 * g) * 2));
-    const char* qh = q + (int64_t)hk * group * q_hs_b;
-    RowStat nx[QT];
-    auto issue = [&](int tile, char* qb) {
+    const char* qh = packed + (int64_t)hk * stat_rows * ROWB;
+    int off[KI];
 #pragma unroll
-      for (int i = 0; i < KI; ++i) {
-        const int P = (wave * KI + i) * 64 + lane, slot = P / CPR;
-        const int r = min(tile * kWtTile + slot, rows - 1), t = div_by(r, group, inv_gqa);
-        const char* src = qh + (int64_t)(r - t * group) * q_hs_b + (int64_t)t * q_ts_b + ((P % CPR) ^ swz_k<CPR>(slot)) * 16;
-        __builtin_amdgcn_global_load_lds((wt_gvoid*)src, (wt_lvoid*)(qb + (wave * KI + i) * 1024), 16, 0, 0);
-      }
+    for (int i = 0; i < KI; ++i) {
+      const int P = (wave * KI + i) * 64 + lane, slot = P / CPR;
+      off[i] = slot * ROWB + ((P % CPR) ^ swz_k<CPR>(slot)) * 16;
+    }
+    auto issue = [&](int tile, char* qb, RowStat(&s)[QT]) {
+      const char* qt = qh + (int64_t)tile * (kWtTile * ROWB);
 #pragma unroll
-      for (int t = 0; t < QT; ++t) {
-        const int r = tile * kWtTile + t * 16 + lm;
-        nx[t] = st[min(r, rows - 1)];
-        if (r >= rows) nx[t].pos = -1;
-      }
+      for (int i = 0; i < KI; ++i)
+        __builtin_amdgcn_global_load_lds((wt_gvoid*)(qt + (uint32_t)off[i]), (wt_lvoid*)(qb + (wave * KI + i) * 1024), 16, 0, 0);
+      const RowStat* sr = st + (int64_t)tile * kWtTile;
+#pragma unroll
+      for (int t = 0; t < QT; ++t) s[t] = sr[(uint32_t)(t * 16 + lm)];
     };
     int q_rd[DS];
 #pragma unroll
     for (int ds = 0; ds < DS; ++ds) q_rd[ds] = lm * ROWB + (((4 * ds + g) ^ swz_k<CPR>(lm)) * 16);
-    issue(tile_begin, lds0);
-    auto body = [&](int tile, const char* cur, char* nxt) {
+    RowStat st0[QT], st1[QT];
+    issue(tile_begin, lds0, st0);
+    auto body = [&](int tile, const char* cur, char* nxt, const RowStat(&now)[QT], RowStat(&next)[QT]) {
       __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
       __syncthreads();
-      RowStat now[QT];
-#pragma unroll
-      for (int t = 0; t < QT; ++t) now[t] = nx[t];
-      if (tile + 1 < tile_end) issue(tile + 1, nxt);
+      if (tile + 1 < tile_end) issue(tile + 1, nxt, next);
       int top = now[0].pos, low = now[0].pos;
 #pragma unroll
       for (int t = 1; t < QT; ++t) {
@@ -265,35 +291,43 @@ __global__ __launch_bounds__(kWtThreads) void weights_sum_kernel(
         low = min(low, now[t].pos);
       }
       if (!__builtin_amdgcn_ballot_w64(top >= k0)) return;  // uniform per wavefront
-      const bool need_mask = __builtin_amdgcn_ballot_w64(low < k0 + 31);
+      const bool need_mask = __builtin_amdgcn_ballot_w64(low < k0 + 16 * KG - 1);
+      constexpr int U = 2;  // query groups at a time: dependent products U KG apart
 #pragma unroll
-      for (int t = 0; t < QT; ++t) {
-        f32x4 s[KG];
+      for (int t0 = 0; t0 < QT; t0 += U) {
+        f32x4 s[U][KG];
 #pragma unroll
-        for (int ds = 0; ds < DS; ++ds) {
-          const bf16x8 b = *(const bf16x8*)(cur + t * 16 * ROWB + q_rd[ds]);
+        for (int ds = 0; ds < DS; ++ds)
 #pragma unroll
-          for (int kg = 0; kg < KG; ++kg)
-            s[kg] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[kg][ds], b, ds == 0 ? f32x4{0.f, 0.f, 0.f, 0.f} : s[kg], 0, 0, 0);
-        }
+          for (int u = 0; u < U; ++u) {
+            const bf16x8 b = *(const bf16x8*)(cur + (t0 + u) * 16 * ROWB + q_rd[ds]);
+#pragma unroll
+            for (int kg = 0; kg < KG; ++kg)
+              s[u][kg] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[kg][ds], b, ds == 0 ? f32x4{0.f, 0.f, 0.f, 0.f} : s[u][kg], 0, 0, 0);
+          }
         if (need_mask) {
-          const int lim = now[t].pos - k0 - 4 * g;
+#pragma unroll
+          for (int u = 0; u < U; ++u) {
+            const int lim = now[t0 + u].pos - k0 - 4 * g;
+#pragma unroll
+            for (int kg = 0; kg < KG; ++kg)
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                if (16 * kg + e > lim) s[u][kg][e] = -INFINITY;
+          }
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u)
 #pragma unroll
           for (int kg = 0; kg < KG; ++kg)
 #pragma unroll
             for (int e = 0; e < 4; ++e)
-              if (16 * kg + e > lim) s[kg][e] = -INFINITY;
-        }
-#pragma unroll
-        for (int kg = 0; kg < KG; ++kg)
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            acc[kg][e] += __builtin_amdgcn_exp2f(__builtin_fmaf(s[kg][e], scale_log2, -now[t].lse));
+              acc[kg][e] += __builtin_amdgcn_exp2f(__builtin_fmaf(s[u][kg][e], scale_log2, -now[t0 + u].lse));
       }
     };
     for (int tile = tile_begin; tile < tile_end; tile += 2) {
-      body(tile, lds0, lds1);
-      if (tile + 1 < tile_end) body(tile + 1, lds1, lds0);
+      body(tile, lds0, lds1, st0, st1);
+      if (tile + 1 < tile_end) body(tile + 1, lds1, lds0, st1, st0);
     }
   }
 #pragma unroll
@@ -314,29 +348,191 @@ __global__ __launch_bounds__(256) void weights_reduce_kernel(const float* __rest
   const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (at >= total) return;
   float sum = 0.f;
-  for (int z = 0; z < parts; ++z) sum += part[z * stride + at];
+  for (int z = 0; z < parts; z += 8) {  // eight loads in flight
+    float p[8];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) p[u] = part[min(z + u, parts - 1) * stride + at];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) sum += z + u < parts ? p[u] : 0.f;
+  }
   out[at] = prior != nullptr ? prior[at] + sum : sum;
 }
 
+// ---- few rows (one token's heads) ----------------------------------------------------------------------
+// Up to 16 query rows of a KV head are one matrix tile: weights_scores_kernel streams K once, a wavefront its own 32-row
+// chunks (whole-row loads into its part of LDS, the next chunk's in flight), leaves the scores in the workspace, a
+// fraction of K's bytes, and each split's maxima and sums; weights_from_scores_kernel joins those and adds up.
+template <int D>
+__global__ __launch_bounds__(kWtThreads) void weights_scores_kernel(
+    const int64_t* __restrict__ pos, int N, int rows, int group, const char* __restrict__ kc, int64_t k_hs_b,
+    const char* __restrict__ q, int64_t q_hs_b, int64_t q_ts_b, float scale_log2, int split_chunks, int splits,
+    float* __restrict__ scores, int64_t score_stride, float2* __restrict__ part, int32_t* __restrict__ err) {
+  constexpr int DS = D / 32, CPR = D / 8, ROWB = D * 2, CH = 32, W = kWtThreads / 64, LI = CH * CPR / 64;
+  __shared__ __attribute__((aligned(1024))) char lds[W * CH * ROWB];
+  __shared__ float2 s_ml[W][16];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x % 64;
+  const int g = lane / 16, lm = lane % 16;
+  const int z = blockIdx.x, hk = blockIdx.y;
+  const char* kh = kc + (int64_t)hk * k_hs_b;
+  vec16 kr[LI];
+  auto load = [&](int c) {  // rows past the cache load its last one
+    c = min(c, (N - 1) / CH);
+    const char* base = kh + (int64_t)c * (CH * ROWB);
+    const int last = N - 1 - c * CH;
+#pragma unroll
+    for (int i = 0; i < LI; ++i) kr[i] = ld16(base + min((i * 64 + lane) / CPR, last) * ROWB + (lane % CPR) * 16);
+  };
+  const int begin = z * split_chunks;
+  int c = begin + wave;
+  load(c);
+  const int r = min(lm, rows - 1), t = r / group;
+  const char* qr = q + (int64_t)(hk * group + r - t * group) * q_hs_b + (int64_t)t * q_ts_b;
+  bf16x8 qf[DS];
+#pragma unroll
+  for (int ds = 0; ds < DS; ++ds) qf[ds] = __builtin_bit_cast(bf16x8, ld16(qr + (32 * ds + 8 * g) * 2));
+  const int64_t p64 = pos[t];
+  const int p = p64 < 0 ? 0 : p64 >= N ? N - 1 : (int)p64;
+  if (p != p64 && lm < rows) flag_error(err, CKV_DEVICE_ERR_RANGE);
+  const int wmax = __builtin_amdgcn_readfirstlane(row16_reduce(p, [](int a, int b) { return max(a, b); }));
+  const int wmin = __builtin_amdgcn_readfirstlane(row16_reduce(p, [](int a, int b) { return min(a, b); }));
+  const int c_end = min(wmax / CH + 1, begin + split_chunks);
+  char* wl = lds + wave * CH * ROWB;
+  float m_run = -INFINITY, l_run = 0.f;
+  float* srow = scores + (int64_t)(hk * rows + r) * score_stride;
+  for (; c < c_end; c += W) {
+    wave_lds_stage();
+#pragma unroll
+    for (int i = 0; i < LI; ++i) {
+      const int slot = (i * 64 + lane) / CPR;
+      *(vec16*)(wl + slot * ROWB + (((lane % CPR) ^ swz_k<CPR>(slot)) * 16)) = kr[i];
+    }
+    if (c + W < c_end) load(c + W);  // lands while this chunk is worked on
+    wave_lds_stage();
+    const int n0 = c * CH;
+    f32x4 s[2];
+#pragma unroll
+    for (int ds = 0; ds < DS; ++ds)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int slot = 16 * h + lm;
+        const bf16x8 a = *(const bf16x8*)(wl + slot * ROWB + (((4 * ds + g) ^ swz_k<CPR>(slot)) * 16));
+        s[h] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, qf[ds], ds == 0 ? f32x4{0.f, 0.f, 0.f, 0.f} : s[h], 0, 0, 0);
+      }
+    // lane (g, lm): row lm, cache rows n0 + 16 h + 4 g + e
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      s[h] *= scale_log2;
+      if (lm < rows) *(f32x4*)(srow + n0 + 16 * h + 4 * g) = s[h];
+    }
+    if (n0 + CH - 1 > wmin) {
+      const int lim = p - n0 - 4 * g;
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (16 * h + e > lim) s[h][e] = -INFINITY;
+    }
+    float bm = s[0][0];
+#pragma unroll
+    for (int j = 1; j < 8; ++j) bm = fmaxf(bm, s[j / 4][j % 4]);
+    const float m_new = fmaxf(m_run, bm), sub = m_new == -INFINITY ? 0.f : m_new;
+    l_run *= __builtin_amdgcn_exp2f(m_run - sub);  // 0 while m_run is -inf
+#pragma unroll
+    for (int j = 0; j < 8; ++j) l_run += __builtin_amdgcn_exp2f(s[j / 4][j % 4] - sub);
+    m_run = m_new;
+  }
+  // a row's four lanes, then the wavefronts
+  const float m = group_max(m_run);
+  float l = m_run == -INFINITY ? 0.f : l_run * __builtin_amdgcn_exp2f(m_run - m);
+  l += __shfl_xor(l, 16);
+  l += __shfl_xor(l, 32);
+  if (g == 0) s_ml[wave][lm] = make_float2(m, l);
+  __syncthreads();
+  if ((int)threadIdx.x < rows) {
+    float mx = -INFINITY, sum = 0.f;
+#pragma unroll
+    for (int w = 0; w < W; ++w) mx = fmaxf(mx, s_ml[w][lm].x);
+#pragma unroll
+    for (int w = 0; w < W; ++w) sum += s_ml[w][lm].x == -INFINITY ? 0.f : s_ml[w][lm].y * __builtin_amdgcn_exp2f(s_ml[w][lm].x - mx);
+    part[(int64_t)(hk * rows + lm) * splits + z] = make_float2(mx, sum);
+  }
+}
+
+__global__ __launch_bounds__(kWtThreads) void weights_from_scores_kernel(
+    const int64_t* __restrict__ pos, int N, int rows, int group, const float* __restrict__ scores, int64_t score_stride,
+    const float2* __restrict__ part, int splits, const float* prior, float* out) {
+  __shared__ float s_lse[kWtFewRows];
+  __shared__ int s_pos[kWtFewRows];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x % 64, hk = blockIdx.y;
+  const int j = blockIdx.x * kWtThreads + threadIdx.x;
+  float s[kWtFewRows];
+  const float* sc = scores + (int64_t)hk * rows * score_stride + min(j, N - 1);
+#pragma unroll
+  for (int r = 0; r < kWtFewRows; ++r)
+    if (r < rows) s[r] = sc[r * score_stride];
+  const float before = prior != nullptr && j < N ? prior[(int64_t)hk * N + j] : 0.f;
+  for (int r = wave; r < rows; r += kWtThreads / 64) {
+    const float2* pr = part + (int64_t)(hk * rows + r) * splits;
+    static_assert(kWtMostParts == 128, "two splits a lane");
+    const float2 none = make_float2(-INFINITY, 0.f);
+    const float2 a = lane < splits ? pr[lane] : none, b = lane + 64 < splits ? pr[lane + 64] : none;
+    float m = fmaxf(a.x, b.x);
+    for (int d = 32; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor(m, d));
+    const float l = wave_butterfly_sum((a.x == -INFINITY ? 0.f : a.y * __builtin_amdgcn_exp2f(a.x - m)) +
+                                       (b.x == -INFINITY ? 0.f : b.y * __builtin_amdgcn_exp2f(b.x - m)));
+    if (lane == 0) {
+      const int64_t p64 = pos[r / group];
+      s_lse[r] = m + __builtin_amdgcn_logf(l);
+      s_pos[r] = p64 < 0 ? 0 : p64 >= N ? N - 1 : (int)p64;
+    }
+  }
+  __syncthreads();
+  if (j >= N) return;
+  float sum = 0.f;
+#pragma unroll
+  for (int r = 0; r < kWtFewRows; ++r)
+    if (r < rows) sum += j <= s_pos[r] ? __builtin_amdgcn_exp2f(s[r] - s_lse[r]) : 0.f;
+  out[(int64_t)hk * N + j] = before + sum;
+}
+
+struct FewPlan {
+  int rows, splits, split_chunks;
+  int64_t score_stride, score_bytes, bytes;
+};
+static FewPlan few_plan(int rows, int N, int Hkv) {
+  const int chunks = (N + 31) / 32;
+  const int64_t splits = std::max<int64_t>(1, std::min<int64_t>({512 / Hkv, (chunks + 3) / 4, kWtMostParts}));
+  FewPlan p;
+  p.rows = rows;
+  p.split_chunks = (int)((chunks + splits - 1) / splits);
+  p.splits = (chunks + p.split_chunks - 1) / p.split_chunks;
+  p.score_stride = (int64_t)chunks * 32;
+  p.score_bytes = (int64_t)Hkv * rows * p.score_stride * 4;
+  p.bytes = p.score_bytes + (int64_t)Hkv * rows * p.splits * 8;
+  return p;
+}
+
 struct WeightsPlan {
-  int rows = 0, row_blocks = 0, splits = 1, split_tiles = 0, key_blocks = 0, parts = 1, part_tiles = 0;
+  int rows = 0, stat_rows = 0, row_blocks = 0,  // stat_rows: rows in whole tiles
+      splits = 1, split_tiles = 0, key_blocks = 0, parts = 1, part_tiles = 0;
   int64_t stat_bytes = 0, part_bytes = 0, sum_bytes = 0;
 };
 
 static WeightsPlan weights_plan(int n, int N, int Hq, int Hkv) {
   WeightsPlan p;
   p.rows = n * (Hq / Hkv);
-  p.row_blocks = (p.rows + kWtRows - 1) / kWtRows;
+  p.row_blocks = (p.rows + 64 * kWtQG - 1) / (64 * kWtQG);
   const int tiles = (N + kWtTile - 1) / kWtTile, row_tiles = (p.rows + kWtTile - 1) / kWtTile;
-  p.key_blocks = (N + kWtRows - 1) / kWtRows;
+  p.key_blocks = (N + 64 * kWtKG - 1) / (64 * kWtKG);
   const int64_t lse_blocks = (int64_t)p.row_blocks * Hkv, sum_blocks = (int64_t)p.key_blocks * Hkv;
-  int64_t splits = std::max<int64_t>(1, std::min<int64_t>({512 / lse_blocks, tiles / 2, 64}));
+  int64_t splits = std::max<int64_t>(1, std::min<int64_t>({1024 / lse_blocks, tiles / 2, 64}));
   p.split_tiles = (int)((tiles + splits - 1) / splits);
   p.splits = (tiles + p.split_tiles - 1) / p.split_tiles;
-  const int64_t parts = std::max<int64_t>(1, std::min<int64_t>(2048 / sum_blocks, row_tiles / 4));
+  const int64_t parts = std::max<int64_t>(1, std::min<int64_t>(8192 / sum_blocks, row_tiles / 4));
   p.part_tiles = (int)((row_tiles + parts - 1) / parts);
   p.parts = (row_tiles + p.part_tiles - 1) / p.part_tiles;
-  const int64_t total = (int64_t)Hkv * p.rows;
+  p.stat_rows = row_tiles * kWtTile;
+  const int64_t total = (int64_t)Hkv * p.stat_rows;
   p.stat_bytes = (total * (int64_t)sizeof(RowStat) + 15) / 16 * 16;
   p.part_bytes = p.splits > 1 ? (total * 8 * p.splits + 15) / 16 * 16 : 0;
   p.sum_bytes = p.parts > 1 ? (int64_t)Hkv * N * 4 * p.parts : 0;
@@ -346,13 +542,14 @@ static WeightsPlan weights_plan(int n, int N, int Hq, int Hkv) {
 }  // namespace ckv
 
 extern "C" int64_t ckv_attention_weights_workspace_bytes(int32_t n_queries, int32_t n_tokens, int32_t n_q_heads,
-                                                         int32_t n_kv_heads) {
+                                                         int32_t n_kv_heads, int32_t head_dim) {
   using namespace ckv;
-  if (n_queries <= 0 || n_tokens <= 0 || n_kv_heads <= 0 || n_q_heads <= 0 || n_q_heads % n_kv_heads ||
+  if (n_queries <= 0 || n_tokens <= 0 || n_kv_heads <= 0 || n_q_heads <= 0 || head_dim <= 0 || n_q_heads % n_kv_heads ||
       (int64_t)n_queries * (n_q_heads / n_kv_heads) > INT32_MAX / 2)
     return 0;
+  if (n_queries * (n_q_heads / n_kv_heads) <= kWtFewRows) return few_plan(n_queries * (n_q_heads / n_kv_heads), n_tokens, n_kv_heads).bytes;
   const WeightsPlan p = weights_plan(n_queries, n_tokens, n_q_heads, n_kv_heads);
-  return p.stat_bytes + std::max(p.part_bytes, p.sum_bytes);
+  return p.stat_bytes + (int64_t)n_kv_heads * p.stat_rows * head_dim * 2 + std::max(p.part_bytes, p.sum_bytes);
 }
 
 extern "C" int32_t ckv_attention_weights(float* out, const float* prior, const void* q, int64_t q_head_stride,
@@ -380,43 +577,62 @@ extern "C" int32_t ckv_attention_weights(float* out, const float* prior, const v
   if (q_token_stride % 8 || q_head_stride % 8 || k_head_stride % 8) return CKV_ERR_INVALID_ARGUMENT;  // 16-byte rows
   if (((uintptr_t)q | (uintptr_t)k_cache) % 16) return CKV_ERR_INVALID_ARGUMENT;
   if (q_token_stride < head_dim || k_head_stride < (int64_t)n_tokens * head_dim) return CKV_ERR_OUT_OF_RANGE;
-  if ((int64_t)n_queries * group > INT32_MAX / 2) return CKV_ERR_TOO_LARGE;
+  if ((int64_t)n_queries * group > INT32_MAX / 2 || n_kv_heads > 65535) return CKV_ERR_TOO_LARGE;
   if (workspace == nullptr || (uintptr_t)workspace % 16 ||
-      workspace_bytes < ckv_attention_weights_workspace_bytes(n_queries, n_tokens, n_q_heads, n_kv_heads))
+      workspace_bytes < ckv_attention_weights_workspace_bytes(n_queries, n_tokens, n_q_heads, n_kv_heads, head_dim))
     return CKV_ERR_INVALID_ARGUMENT;
-  const WeightsPlan p = weights_plan(n_queries, n_tokens, n_q_heads, n_kv_heads);
   const float scale_log2 = (float)(scale * 1.4426950408889634);  // exp(x) = exp2(x log2 e)
+  if (n_queries * group <= kWtFewRows) {
+    const FewPlan p = few_plan(n_queries * group, n_tokens, n_kv_heads);
+    float* scores = (float*)workspace;
+    float2* part = (float2*)((char*)workspace + p.score_bytes);
+    auto launch = [&](auto kernel) {
+      hipLaunchKernelGGL(kernel, dim3((unsigned)p.splits, (unsigned)n_kv_heads), dim3(kWtThreads), 0, s, positions, n_tokens, p.rows,
+                         group, (const char*)k_cache, k_head_stride * 2, (const char*)q, q_head_stride * 2, q_token_stride * 2,
+                         scale_log2, p.split_chunks, p.splits, scores, p.score_stride, part, err);
+    };
+    if (head_dim == 128) launch(weights_scores_kernel<128>);
+    else launch(weights_scores_kernel<64>);
+    CKV_RETURN_IF_LAUNCH_FAILED();
+    hipLaunchKernelGGL(weights_from_scores_kernel, dim3((unsigned)((n_tokens + kWtThreads - 1) / kWtThreads), (unsigned)n_kv_heads),
+                       dim3(kWtThreads), 0, s, positions, n_tokens, p.rows, group, (const float*)scores, p.score_stride,
+                       (const float2*)part, p.splits, prior, out);
+    CKV_RETURN_IF_LAUNCH_FAILED();
+    return CKV_OK;
+  }
+  const WeightsPlan p = weights_plan(n_queries, n_tokens, n_q_heads, n_kv_heads);
   const uint32_t inv_gqa = inverse_of(p.rows, group);
   RowStat* stat = (RowStat*)workspace;
-  float* scratch = (float*)((char*)workspace + p.stat_bytes);  // the splits' rows, then the parts' sums
-  const int64_t rows_total = (int64_t)n_kv_heads * p.rows;
+  char* packed = (char*)workspace + p.stat_bytes;
+  float* scratch = (float*)(packed + (int64_t)n_kv_heads * p.stat_rows * head_dim * 2);  // the splits' rows, then the parts' sums
+  const int64_t rows_total = (int64_t)n_kv_heads * p.stat_rows;
   {
     const AttnMap m = attn_map(p.row_blocks, n_kv_heads, 1, p.splits);
     auto launch = [&](auto kernel) {
       hipLaunchKernelGGL(kernel, dim3(m.blocks), dim3(kWtThreads), 0, s, m.nqb, m.group, m.xpk_log, m.items, m.inv_group,
                          m.inv_nqb, positions, n_tokens, p.rows, group, inv_gqa, (const char*)k_cache, k_head_stride * 2,
-                         (const char*)q, q_head_stride * 2, q_token_stride * 2, scale_log2, stat, (float2*)scratch,
+                         (const char*)q, q_head_stride * 2, q_token_stride * 2, scale_log2, stat, packed, p.stat_rows, (float2*)scratch,
                          rows_total, p.split_tiles, err);
     };
-    if (head_dim == 128) p.splits > 1 ? launch(weights_lse_kernel<128, true>) : launch(weights_lse_kernel<128, false>);
-    else p.splits > 1 ? launch(weights_lse_kernel<64, true>) : launch(weights_lse_kernel<64, false>);
+    if (head_dim == 128) p.splits > 1 ? launch(weights_lse_kernel<128, kWtQG, true>) : launch(weights_lse_kernel<128, kWtQG, false>);
+    else p.splits > 1 ? launch(weights_lse_kernel<64, kWtQG, true>) : launch(weights_lse_kernel<64, kWtQG, false>);
     CKV_RETURN_IF_LAUNCH_FAILED();
   }
   if (p.splits > 1) {
-    hipLaunchKernelGGL(weights_join_kernel, dim3((unsigned)((rows_total + 255) / 256)), dim3(256), 0, s, (const float2*)scratch,
-                       rows_total, p.splits, positions, n_tokens, p.rows, group, stat, rows_total);
+    hipLaunchKernelGGL(weights_join_kernel, dim3((unsigned)((rows_total + 3) / 4)), dim3(256), 0, s, (const float2*)scratch,
+                       rows_total, p.splits, positions, n_tokens, p.rows, group, stat, p.stat_rows, rows_total);
     CKV_RETURN_IF_LAUNCH_FAILED();
   }
   {
     const AttnMap m = attn_map(p.key_blocks, n_kv_heads, 1, p.parts);
     auto launch = [&](auto kernel) {
       hipLaunchKernelGGL(kernel, dim3(m.blocks), dim3(kWtThreads), 0, s, m.nqb, m.group, m.xpk_log, m.items, m.inv_group,
-                         m.inv_nqb, n_tokens, p.rows, group, inv_gqa, (const char*)k_cache, k_head_stride * 2, (const char*)q,
-                         q_head_stride * 2, q_token_stride * 2, scale_log2, (const RowStat*)stat, prior,
+                         m.inv_nqb, n_tokens, p.stat_rows, (const char*)k_cache, k_head_stride * 2, (const char*)packed, scale_log2,
+                         (const RowStat*)stat, prior,
                          p.parts > 1 ? scratch : out, total, p.part_tiles);
     };
-    if (head_dim == 128) p.parts > 1 ? launch(weights_sum_kernel<128, true>) : launch(weights_sum_kernel<128, false>);
-    else p.parts > 1 ? launch(weights_sum_kernel<64, true>) : launch(weights_sum_kernel<64, false>);
+    if (head_dim == 128) p.parts > 1 ? launch(weights_sum_kernel<128, kWtKG, true>) : launch(weights_sum_kernel<128, kWtKG, false>);
+    else p.parts > 1 ? launch(weights_sum_kernel<64, kWtKG, true>) : launch(weights_sum_kernel<64, kWtKG, false>);
     CKV_RETURN_IF_LAUNCH_FAILED();
   }
   if (p.parts > 1) {

@@ -688,7 +688,7 @@ PyObject* attention_weights(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
   if (!out.defined()) out = at::empty({1, H, N}, q.options().dtype(at::kFloat));
   else fits(out, "out");
   const double scale = a[3] == Py_None ? 1.0 / std::sqrt((double)D) : real(a[3]);
-  const int64_t ws_bytes = ckv_attention_weights_workspace_bytes(int32(n), int32(N), int32(Hq), int32(H));
+  const int64_t ws_bytes = ckv_attention_weights_workspace_bytes(int32(n), int32(N), int32(Hq), int32(H), int32(D));
   Tensor ws;
   if (ws_bytes > 0) ws = at::empty({(ws_bytes + 3) / 4}, q.options().dtype(at::kFloat));
   int32_t* const e = status_word(err, q);

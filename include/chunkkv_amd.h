@@ -615,7 +615,7 @@ int32_t ckv_attention_weights(float* out, const float* prior, const void* q, int
 
 /* Bytes of workspace that ckv_attention_weights needs for this shape. Host-only. */
 int64_t ckv_attention_weights_workspace_bytes(int32_t n_queries, int32_t n_tokens, int32_t n_q_heads,
-                                              int32_t n_kv_heads);
+                                              int32_t n_kv_heads, int32_t head_dim);
 
 /*
  * Cut a layer's cache to n_keep rows per KV head: the first n_sink rows, the last n_recent, and of the others those

@@ -71,8 +71,8 @@ def test_workspace_sizes_are_host_only():
     assert attn(2976, 8256, 28, 4, 128) >= 2 * 2 * 4 * 8256 * 128  # the cache as bf16
     assert attn(0, 100, 28, 4, 128) == attn(1, 0, 28, 4, 128) == attn(1, 100, 28, 3, 128) == attn(1, 100, 28, 0, 128) == 0
     w = lib.ckv_attention_weights_workspace_bytes
-    assert w(1, 1, 4, 4) > 0 and w(0, 100, 28, 4) == w(1, 100, 28, 3) == 0
-    assert w(2**31 - 1, 100, 64, 1) == 0  # refused by the call
+    assert w(1, 1, 4, 4, 64) > 0 and w(0, 100, 28, 4, 64) == w(1, 100, 28, 3, 64) == 0
+    assert w(2**31 - 1, 100, 64, 1, 64) == 0  # refused by the call
 
 
 def test_every_wave_plan_can_be_launched(tmp_path):
