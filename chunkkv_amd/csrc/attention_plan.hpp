@@ -86,15 +86,14 @@ constexpr int kWaveFill = 256;  // workgroups that a split launch aims at: one f
 
 // The most splits a launch takes: a workgroup has at most 32 (token, query head) rows, a split's
 // four wavefronts a chunk each.
-static inline int64_t most_splits(int n, int N, int Hq, int head_dim, int fill = kWaveFill) {
+static inline int64_t most_splits(int n, int N, int Hq, int head_dim) {
   const int64_t chunks = (N + kWaveChunk - 1) / kWaveChunk;
   if (!wave_launch(n, Hq, head_dim) || chunks <= 16) return 1;
-  return std::max<int64_t>(1, std::min<int64_t>((int64_t)fill * 32 / ((int64_t)n * Hq), (chunks + 3) / 4));
+  return std::max<int64_t>(1, std::min<int64_t>(kWaveFill * 32 / ((int64_t)n * Hq), (chunks + 3) / 4));
 }
 
 // The plan of attn_wave_kernel.
-static inline AttnPlan attn_wave_plan(int n, int N, int Hq, int Hkv, int head_dim, int64_t workspace_bytes,
-                                      int fill = kWaveFill) {
+static inline AttnPlan attn_wave_plan(int n, int N, int Hq, int Hkv, int head_dim, int64_t workspace_bytes) {
   AttnPlan p;
   const int group = Hq / Hkv;
   p.wave = true;
@@ -118,9 +117,9 @@ static inline AttnPlan attn_wave_plan(int n, int N, int Hq, int Hkv, int head_di
   // (5 queries of 28 heads over 1103 rows 13.9 us, over 1600 17.9), so 16 rows by four wavefronts,
   // split (8.8, 8.9); the three microseconds of the merge are not worth it at head_dim 64 (7.1 whole).
   const int64_t row_b = (int64_t)Hq * n * (head_dim + 4) * 4;
-  const int64_t can = std::min<int64_t>(most_splits(n, N, Hq, head_dim, fill), workspace_bytes / row_b);
+  const int64_t can = std::min<int64_t>(most_splits(n, N, Hq, head_dim), workspace_bytes / row_b);
   if (head_dim == 128 && rows > 16 && lng && chunks < 64) {
-    const int64_t splits = std::min<int64_t>(std::min<int64_t>(can, fill / b16), chunks / 4);
+    const int64_t splits = std::min<int64_t>(std::min<int64_t>(can, kWaveFill / b16), chunks / 4);
     if (splits > 1) {
       p.qg = 1;
       p.waves = 4;
@@ -137,7 +136,7 @@ static inline AttnPlan attn_wave_plan(int n, int N, int Hq, int Hkv, int head_di
   // Splits cost the merge launch, about 3 us: taken for one token's rows from 17 chunks on (28
   // heads, 700 rows 7.1 against 8.5 us, 8288 rows 8.7 against 45), else where eight wavefronts
   // would have eight chunks each (150 of 1500 rows, 47 chunks, 8.5 us whole and 9.5 in two).
-  int64_t splits = std::min<int64_t>(can, fill / std::max(blocks, 1));
+  int64_t splits = std::min<int64_t>(can, kWaveFill / std::max(blocks, 1));
   if (rows > 16 && chunks < 64) splits = 1;
   if (rows <= 16) p.waves = splits > 1 ? 4 : 8;
   splits = std::max<int64_t>(1, std::min<int64_t>(splits, (chunks + p.waves - 1) / p.waves));
