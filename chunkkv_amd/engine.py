@@ -40,6 +40,11 @@ kernels:
   mask + SDPA (:157, :68-72)                         ckv_attention_active: matrix-core
                                                        attention masked by the active positions
                                                        (bf16, head_dim 64/128)
+  decode's torch.cat caches (:180-198)               preallocated caches; generate(keep=..., cache_bits=8):
+                                                       cut by the attention weights of prefill(observe=...)
+                                                       and held in 8 bits (ckv_attention_weights,
+                                                       ckv_evict_rows, ckv_quantize_rows,
+                                                       ckv_attention_quantized)
 All layers' caches live in one (L, 1, H, N, D) slab; PrefillResult.keys/values are its views.
 
 Attention: the reference calls SDPA with enable_gqa and an explicit boolean (n_active x N) mask,
@@ -421,7 +426,8 @@ class HipEngine(DecoderPieces):
     # -- decode ---------------------------------------------------------------------------
 
     @torch.inference_mode()
-    def generate(self, result: PrefillResult, max_tokens: int = 32) -> list[int]:
+    def generate(self, result: PrefillResult, max_tokens: int = 32, *, cache_bits: int = 16, keep: int | None = None,
+                 keep_sink: int = 4, keep_recent: int = 32) -> list[int]:
         """Greedy decode continuing a prefill (torch_engine.py:180-198) on preallocated caches.
 
         The reference appends each new token with a torch.cat of every layer's whole cache
@@ -431,23 +437,54 @@ class HipEngine(DecoderPieces):
         position as the mask (rows past pos are never read). With the positions-masked attention
         kernel a step reads its token and position from device tensors and writes the next greedy
         token back, so after the first (eager) step every step is one HIP graph replay; the host
-        only reads the token, for the EOS test."""
+        only reads the token, for the EOS test.
+
+        keep: decode over the keep heaviest rows of each layer and KV head (ops.evict_rows on result.weights, from
+        prefill(observe=...)): the first keep_sink and the last keep_recent always among them. A prompt of
+        keep rows or fewer is not cut. cache_bits=8: the decode caches are 8-bit (ops.quantize_rows: e4m3 codes, a
+        scale for each 64 rows and head), half the bytes that a step reads. Both need the positions-masked attention
+        kernel (bf16 caches with head_dim 64 or 128)."""
+        device_loop = self._native_attention and self.attention in ("fused", "sdpa")
+        if cache_bits not in (8, 16):
+            raise ValueError("cache_bits must be 8 or 16")
+        if (cache_bits == 8 or keep is not None) and not device_loop:
+            raise ValueError("cache_bits=8 and keep need the attention kernel: bf16, head_dim 64 or 128, attention 'fused' or 'sdpa'")
+        N = result.keys[0].shape[2]
+        if keep is not None:
+            if keep < 1 or min(keep_sink, keep_recent) < 0 or keep_sink + keep_recent > keep:
+                raise ValueError("keep must be at least 1 and hold keep_sink + keep_recent rows")
+            if keep >= N:
+                keep = None
+            elif result.weights is None:
+                raise ValueError("keep needs the weights of prefill(observe=...)")
         out: list[int] = []
         nxt = int(result.logits[-1].argmax().item())
         if max_tokens <= 0 or nxt in self.eos:
             return out
         dev, H, D, L = self.device, self.n_kv, self.head_dim, len(self.layers)
-        N = result.keys[0].shape[2]
-        cap = N + max_tokens
-        Ks = torch.empty((L, 1, H, cap, D), dtype=self.kv_dtype, device=dev)
-        Vs = torch.empty_like(Ks)
+        M = N if keep is None else keep  # prompt rows in the decode caches
+        cap = M + max_tokens
+        Ks = Vs = coded = None
+        if cache_bits == 16:
+            Ks = torch.empty((L, 1, H, cap, D), dtype=self.kv_dtype, device=dev)
+            Vs = torch.empty_like(Ks)
+        else:
+            coded = [ops.quantized_cache(H, cap, D, dev) for _ in range(L)]
         for li in range(L):
-            Ks[li, :, :, :N].copy_(result.keys[li])
-            Vs[li, :, :, :N].copy_(result.values[li])
+            K, V = result.keys[li], result.values[li]
+            if keep is not None:
+                cut = {} if Ks is None else dict(k_out=Ks[li, :, :, :M], v_out=Vs[li, :, :, :M])
+                e = ops.evict_rows(K, V, result.weights[li], keep, keep_sink, keep_recent, **cut)
+                K, V = e.K, e.V
+            elif Ks is not None:
+                Ks[li, :, :, :N].copy_(K)
+                Vs[li, :, :, :N].copy_(V)
+            if coded is not None:
+                ops.quantize_rows(coded[li], K, V)
         err = torch.zeros(1, dtype=torch.int32, device=dev)
-        device_loop = self._native_attention and self.attention in ("fused", "sdpa")
         tok = torch.tensor([[nxt]], dtype=torch.int64, device=dev)
         where = torch.tensor([N], dtype=torch.int64, device=dev)
+        row = where if M == N else torch.tensor([M], dtype=torch.int64, device=dev)
         graph = None
         while len(out) < max_tokens and nxt not in self.eos:
             out.append(nxt)
@@ -456,30 +493,40 @@ class HipEngine(DecoderPieces):
             elif graph is not None:
                 graph.replay()
             else:
-                self._decode_step(tok, where, Ks, Vs, err)  # also the warm-up of the capture
+                self._decode_step(tok, where, Ks, Vs, err, row, coded)  # also the warm-up of the capture
                 if max_tokens - len(out) >= 2 and self.decode_graphs:
                     graph = torch.cuda.CUDAGraph()
                     with torch.cuda.graph(graph):
-                        self._decode_step(tok, where, Ks, Vs, err)
+                        self._decode_step(tok, where, Ks, Vs, err, row, coded)
             nxt = int(tok.item())
         if int(err.item()) != 0:
             raise RuntimeError("a decode kernel reported an out-of-range position")
         return out
 
-    def _decode_step(self, tok, where, Ks, Vs, err) -> None:
+    def _decode_step(self, tok, where, Ks, Vs, err, row=None, coded=None) -> None:
         """One token (tok: (1, 1) int64 at position where: (1,) int64) through every layer; writes
-        the next greedy token into tok and advances where. No host values are read."""
+        the next greedy token into tok and advances where. No host values are read. row: the cache row it takes, where
+        that is not its position (caches cut to fewer rows); advanced too. coded: the layers' 8-bit caches, in the place of
+        Ks/Vs."""
         H, D = self.n_kv, self.head_dim
+        row = where if row is None else row
         h, pending = self.inner.embed_tokens(tok), None
         for li, layer in enumerate(self.layers):
             h, x = self._norm(li, layer, h, pending)
             q_in, k_in, v_in = self._project(li, x)
-            q, _ = ops.rope_qkv(q_in, k_in, v_in, where, self.n_heads, H, D, self.theta, k_out=Ks[li], v_out=Vs[li],
-                                rows=where, err=err)
-            o = ops.attention_active(q.transpose(1, 2), Ks[li], Vs[li], where, err=err)
+            if coded is None:
+                q, _ = ops.rope_qkv(q_in, k_in, v_in, where, self.n_heads, H, D, self.theta, k_out=Ks[li], v_out=Vs[li],
+                                    rows=row, err=err)
+                o = ops.attention_active(q.transpose(1, 2), Ks[li], Vs[li], row, err=err)
+            else:
+                q, k = ops.rope_qkv(q_in, k_in, None, where, self.n_heads, H, D, self.theta, err=err)
+                ops.quantize_rows(coded[li], k, v_in.view(1, 1, H, D).transpose(1, 2), row, err)
+                o = ops.attention_quantized(q.transpose(1, 2), coded[li], row, err=err)
             h, pending = self._mlp(li, layer, h, layer.self_attn.o_proj(o.view(1, 1, -1)))
         tok.copy_(self._final_logits(h, pending)[0, -1].argmax().view(1, 1))
         where.add_(1)
+        if row is not where:
+            row.add_(1)
 
     def _decode_step_sdpa(self, tok, pos: int, Ks, Vs, err) -> None:
         """_decode_step for models outside the attention kernel's range (SDPA over rows <= pos)."""
@@ -499,7 +546,12 @@ class HipEngine(DecoderPieces):
     # -- main entry -----------------------------------------------------------------------
 
     @torch.inference_mode()
-    def prefill(self, tokens, placements=None, config=None, logits_from=None) -> PrefillResult:
+    def prefill(self, tokens, placements=None, config=None, logits_from=None, *, observe: int = 0) -> PrefillResult:
+        """torch_engine.py:80-178. observe: also return, in result.weights, the attention weight that each cached row of each
+        layer and KV head received from the last `observe` rows computed there (ops.attention_weights), for
+        generate(keep=...); needs bf16 caches with head_dim 64 or 128."""
+        if observe < 0 or observe and not self._native_attention:
+            raise ValueError("observe must be >= 0, and needs bf16 caches with head_dim 64 or 128")
         placements = placements or []
         config = config or BlendConfig()
         N = len(tokens)
@@ -542,6 +594,7 @@ class HipEngine(DecoderPieces):
         k_slab = torch.empty((n_layers, 1, H, N, D), dtype=self.kv_dtype, device=dev)
         v_slab = torch.empty_like(k_slab)
         err = torch.zeros(1, dtype=torch.int32, device=dev)
+        weights = torch.empty((n_layers, 1, H, N), dtype=torch.float32, device=dev) if observe else None
         keys_out = list(k_slab.unbind(0))
         values_out = list(v_slab.unbind(0))
 
@@ -627,6 +680,8 @@ class HipEngine(DecoderPieces):
                                     rows=active, err=err)
                 if ready.get(li) is not None:
                     torch.cuda.current_stream(dev).wait_event(ready[li])
+            if observe:
+                ops.attention_weights(q[:, -observe:].transpose(1, 2), K, active[-observe:], out=weights[li], err=err)
             h, pending = self._attend_active(li, layer, h, q, K, V, active, ar, masks, err)
 
         n_want = N - logits_from
@@ -662,4 +717,5 @@ class HipEngine(DecoderPieces):
         layer0 = len(plan.layer0_idx) if config.full_first_layer else N - plan.n_cached
         stats = stats_dict(N, plan.n_cached, n_layers, layer0, selected_cached, chunk_stats)
         return PrefillResult(logits, torch.arange(logits_from, N), keys_out, values_out, stats,
-                             copy=lambda t: t.contiguous(), extract=lambda spans: ops.extract_chunks(k_slab, v_slab, spans))
+                             copy=lambda t: t.contiguous(), extract=lambda spans: ops.extract_chunks(k_slab, v_slab, spans),
+                             weights=None if weights is None else list(weights.unbind(0)))

@@ -60,6 +60,9 @@ class PrefillResult:
     # Batched extraction hook (spans -> one (2, L, 1, H, len, D) buffer per span); set by HipEngine
     # to its one-launch kernel. None: the per-layer `copy` path of the reference.
     extract: Callable[[list], list] | None = None
+    # With HipEngine.prefill(observe=n): per layer the (1, H, N) float32 attention weight that each cached row received from
+    # the last n rows computed, which HipEngine.generate(keep=...) cuts the caches by.
+    weights: Any = None
 
     def chunk(self, start: int, end: int) -> ChunkKV:
         return self.chunks([(start, end)])[0]
