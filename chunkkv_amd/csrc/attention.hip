@@ -359,7 +359,7 @@ extern "C" int32_t ckv_attention_active(void* out, const void* q, int64_t q_head
       hipLaunchKernelGGL(kernel, dim3(map.blocks), dim3(waves * 64), 0, st, map.nqb, map.group, map.xpk_log, map.items,
                          map.inv_group, map.inv_nqb, positions, n_queries, n_tokens, (const char*)k_cache,
                          (const char*)v_cache, kv_head_stride * 2, (const char*)q, q_head_stride * 2, q_token_stride * 2,
-                         n_q_heads, group, inv_gqa, scale_log2, plan.split_chunks, (char*)out, ws, err, NoScales{});
+                         n_q_heads, group, inv_gqa, scale_log2, plan.split_chunks, (char*)out, ws, err);
     };
 #define CKV_WAVE(HD, QG, W, GR) \
   else if (head_dim == HD && plan.qg == QG && plan.waves == W && plan.grouped == GR) \

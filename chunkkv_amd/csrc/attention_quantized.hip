@@ -432,7 +432,7 @@ extern "C" int32_t ckv_attention_quantized(void* out, const void* q, int64_t q_h
   };
 #define CKV_WAVE(HD, QG, W, GR) \
   else if (head_dim == HD && plan.qg == QG && plan.waves == W && plan.grouped == GR) \
-    launch(attn_wave_kernel<HD, QG, W, GR, true>, W);
+    launch(attn_wave_kernel<HD, QG, W, GR, CacheScales>, W);
   if (false) {
   }
   CKV_WAVE_FORMS(CKV_WAVE)

@@ -31,17 +31,17 @@ struct CacheScales {
   const uint8_t* v;
   int blocks, chunk_log;
 };
-struct NoScales {};
 
-// CODES: the cache holds e4m3 codes. A row's codes become bf16 (exactly: three fraction bits times a
+// With a CacheScales argument at the end the cache holds e4m3 codes. A row's codes become bf16 (exactly: three fraction bits times a
 // power of two) where it is put into LDS, and everything after that is the bf16 cache's.
-template <int D, int QG, int W, bool GROUPED, bool CODES = false>
+template <int D, int QG, int W, bool GROUPED, typename... Scales>
 __global__ __launch_bounds__(W * 64) void attn_wave_kernel(
     int nqb, int map_group, int xpk_log, int items, uint32_t inv_group, uint32_t inv_nqb,
     const int64_t* __restrict__ pos, int n, int N, const char* __restrict__ kc, const char* __restrict__ vc,
     int64_t kv_hs_b, const char* __restrict__ q, int64_t q_hs_b, int64_t q_ts_b, int Hq, int group, uint32_t inv_gqa,
     float scale_log2, int split_chunks, char* __restrict__ out, float* __restrict__ ws, int32_t* __restrict__ err,
-    std::conditional_t<CODES, CacheScales, NoScales> scales) {
+    Scales... scales) {
+  constexpr bool CODES = sizeof...(Scales) == 1;
   constexpr int DS = D / 32, DT = D / 16, CPR = D / 8, ROWB = D * 2;
   constexpr int ROWS = 16 * QG;               // query rows of the workgroup
   constexpr int GB = CODES ? D : ROWB;        // bytes of a row in the cache, and 16-byte pieces
@@ -82,18 +82,10 @@ __global__ __launch_bounds__(W * 64) void attn_wave_kernel(
 #pragma unroll
     for (int i = 0; i < LI; ++i) r[i] = ld16(base + min((i * 64 + lane) / GP, last) * GB + (lane % GP) * 16);
   };
-  float k_sc = 1.f, v_sc = 1.f;  // scales of the rows in kr and vr
-  auto load_scale = [&](float& s, const uint8_t* of, int c) {
+  [[maybe_unused]] float k_sc = 1.f, v_sc = 1.f;  // scales of the rows in kr and vr
+  [[maybe_unused]] auto load_scales = [&](int c, const uint8_t* of, float& s, int blocks, int chunk_log) {
     c = min(c, (N - 1) / kWaveChunk);
-    if constexpr (CODES) s = __uint_as_float((uint32_t)of[(int64_t)hk * scales.blocks + (c >> scales.chunk_log)] << 23);
-  };
-  auto load_k = [&](int c) {
-    load(kr, kh, c);
-    if constexpr (CODES) load_scale(k_sc, scales.k, c);
-  };
-  auto load_v = [&](int c) {
-    load(vr, vh, c);
-    if constexpr (CODES) load_scale(v_sc, scales.v, c);
+    s = __uint_as_float((uint32_t)of[(int64_t)hk * blocks + (c >> chunk_log)] << 23);
   };
 #pragma unroll
   for (int i = 0; i < QI; ++i) {  // absent rows load the last token's query and store nothing
@@ -103,13 +95,22 @@ __global__ __launch_bounds__(W * 64) void attn_wave_kernel(
   }
   const int begin = ws != nullptr ? z * split_chunks : 0;
   int c = begin + wave;
-  load_k(c);
-  load_v(c);
+  load(kr, kh, c);
+  load(vr, vh, c);
+  (load_scales(c, scales.k, k_sc, scales.blocks, scales.chunk_log), ...);
+  (load_scales(c, scales.v, v_sc, scales.blocks, scales.chunk_log), ...);
   // The operand of matrix step ds for row slot s: logical 16-byte piece 4 ds + g, kept at piece
   // (4 ds + g) ^ swz_k(s) of the slot.
   char* wl = lds + wave * kWaveChunk * ROWB;
-  auto put_at = [&](int slot, int piece, const vec16& v) { *(vec16*)(wl + slot * ROWB + ((piece ^ swz_k<CPR>(slot)) * 16)) = v; };
-  auto put = [&](int slot, const vec16& v) { put_at(slot, lane % CPR, v); };
+  auto put = [&](int slot, const vec16& v) { *(vec16*)(wl + slot * ROWB + (((lane % CPR) ^ swz_k<CPR>(slot)) * 16)) = v; };
+  // codes: a lane's piece is the row's 16-byte places 2 p and 2 p + 1, p = lane % GP
+  auto put_two = [&](int slot, int swz, const vec16& c, float scale) {
+    vec16 lo, hi;
+    decode16(c, scale, lo, hi);
+    char* to = wl + slot * ROWB;
+    *(vec16*)(to + ((2 * (lane % GP)) ^ swz) * 16) = lo;
+    *(vec16*)(to + ((2 * (lane % GP) + 1) ^ swz) * 16) = hi;
+  };
   auto operand = [&](int slot, int ds) {
     return *(const bf16x8*)(wl + slot * ROWB + (((4 * ds + g) ^ swz_k<CPR>(slot)) * 16));
   };
@@ -157,17 +158,18 @@ __global__ __launch_bounds__(W * 64) void attn_wave_kernel(
     wave_lds_stage();
 #pragma unroll
     for (int i = 0; i < LI; ++i) {  // K row r = 8 a + 4 t + b to slot 16 t + 4 a + b (kslot_row's inverse)
-      const int r = (i * 64 + lane) / GP, slot = 16 * ((r >> 2) & 1) + 4 * (r >> 3) + (r & 3);
+      const int r = (i * 64 + lane) / GP;
       if constexpr (CODES) {
-        vec16 lo, hi;
-        decode16(kr[i], k_sc, lo, hi);
-        put_at(slot, 2 * (lane % GP), lo);
-        put_at(slot, 2 * (lane % GP) + 1, hi);
+        const int slot = 16 * ((r >> 2) & 1) + 4 * (r >> 3) + (r & 3);
+        put_two(slot, swz_k<CPR>(slot), kr[i], k_sc);
       } else {
-        put(slot, kr[i]);
+        put(16 * ((r >> 2) & 1) + 4 * (r >> 3) + (r & 3), kr[i]);
       }
     }
-    if (c + W < c_end) load_k(c + W);  // lands while this chunk is worked on
+    if (c + W < c_end) {  // lands while this chunk is worked on
+      load(kr, kh, c + W);
+      (load_scales(c + W, scales.k, k_sc, scales.blocks, scales.chunk_log), ...);
+    }
     wave_lds_stage();
     f32x4 s[QG][2];
 #pragma unroll
@@ -186,20 +188,14 @@ __global__ __launch_bounds__(W * 64) void attn_wave_kernel(
 #pragma unroll
     for (int i = 0; i < LI; ++i) {
       const int slot = (i * 64 + lane) / GP;
-      const bool past = edge && n0 + slot > wmax;
-      auto put_v = [&](int piece, const vec16& v) {
-        *(vec16*)(wl + slot * ROWB + ((piece ^ swz_v<CPR>(slot)) * 16)) = past ? vec16{0, 0, 0, 0} : v;
-      };
-      if constexpr (CODES) {
-        vec16 lo, hi;
-        decode16(vr[i], v_sc, lo, hi);
-        put_v(2 * (lane % GP), lo);
-        put_v(2 * (lane % GP) + 1, hi);
-      } else {
-        put_v(lane % CPR, vr[i]);
-      }
+      const vec16 v = edge && n0 + slot > wmax ? vec16{0, 0, 0, 0} : vr[i];
+      if constexpr (CODES) put_two(slot, swz_v<CPR>(slot), v, v_sc);
+      else *(vec16*)(wl + slot * ROWB + (((lane % CPR) ^ swz_v<CPR>(slot)) * 16)) = v;
     }
-    if (c + W < c_end) load_v(c + W);
+    if (c + W < c_end) {
+      load(vr, vh, c + W);
+      (load_scales(c + W, scales.v, v_sc, scales.blocks, scales.chunk_log), ...);
+    }
     wave_lds_stage();
 
     const bool need_mask = n0 + kWaveChunk - 1 > wmin;
