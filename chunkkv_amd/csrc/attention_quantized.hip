@@ -6,7 +6,8 @@
 //  - Few query rows (some tokens, short prompts): attention_wave.hpp's kernel reads the codes and makes them bf16
 //    on their way into LDS, a wavefront its own 32 rows.
 //  - Many: one pass writes the cache as bf16 into the workspace and attention.hip runs on it. There every
-//    row is read by many workgroups of 128 queries, and each would convert it again.
+//    row is read by many workgroups of 128 queries, and each would convert it again: about a third more vector
+//    instructions in a kernel that they bound, against 7 of 191 us (2976 queries over 8256 rows, 28 / 4 heads of 128).
 #include "attention_common.hpp"
 #include "attention_wave.hpp"
 

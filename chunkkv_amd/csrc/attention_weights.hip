@@ -1,18 +1,25 @@
 // The attention weight that each cached row received, summed over query rows and the query heads of its KV head:
 //   out[hk, j] = prior[hk, j] + sum over i, h in group hk of softmax_j(scale * q[h, i] . K[hk, j]),  j <= pos[i],
 // what a cache's rows are ranked by before the light ones are dropped (evict.hip). Neither the scores nor the
-// weights go to memory.
+// weights go to memory (but for one token's scores, below).
 //
 // Design: the n x group (token, query head) pairs of a KV head are its rows. A weight needs its row's maximum
 // and sum before it can be formed, so the product with K^T runs twice:
 //  1. weights_lse_kernel: 128 rows a workgroup walk the cache in 64-row tiles (attention.hip's first half, with the
 //     maximum and the sum kept per lane); with few row blocks, in splits of the cache. Leaves L = max + log2(sum) and the
 //     position of each row (weights_join_kernel joins the splits).
-//  2. weights_sum_kernel: 128 cache rows a workgroup hold their operands in registers while the query rows pass
-//     through LDS: S = K Q^T gives a lane four cache rows of one query row, and 2^(s scale - L) adds up in
+//  2. weights_sum_kernel: 128 cache rows a workgroup hold their operands in registers while the query rows (packed by the
+//     first pass: a tile's loads then need no addresses) pass through LDS: S = K Q^T gives a lane four cache rows of one query row, and 2^(s scale - L) adds up in
 //     registers over all query rows; the 16 lanes of a cache row meet once, at the end. With few cache blocks the
 //     query rows are split, and weights_reduce_kernel adds the parts in order (no atomics: the same sums every time).
 // Scores and sums are fp32 throughout, products bf16 x bf16 (exact) accumulated in fp32 on the matrix cores.
+//
+// Bound: the issue of a SIMD. A score costs a matrix instruction a quarter and, to stay in fp32, a product, an exponential and
+// an addition (the first pass: half a maximum too); alone these take 16.3 and 17.0 cycles for four scores a lane, both
+// together 28.3, whichever way the two are interleaved (within a wavefront, across wavefronts, by priority), so they
+// hardly overlap. Measured (us, kernels traced, 28 / 4 heads of 128): 8256 causal rows 251 + 258 + 4, of which 175 each is that
+// issue at 2.4 GHz and the clock was near 2.0; 64 rows over 32832 24 + 20 and 4 for the join; one row over 8257 4.6 + 4.4.
+// Slower: 64 rows a wavefront (275 and 320 us: two wavefronts a SIMD), exponentials one step behind the products (266, 283).
 #include <algorithm>
 
 #include "attention_common.hpp"
@@ -21,8 +28,8 @@ namespace ckv {
 
 constexpr int kWtThreads = 256;
 constexpr int kWtTile = 64;    // cache rows of a tile of the first pass, query rows of one of the second
-constexpr int kWtQG = 2;       // 16-row groups of a wavefront of the first pass, and of the second's cache rows
-constexpr int kWtKG = 2;
+constexpr int kWtQG = 2;       // 16-row groups of a wavefront of the first pass
+constexpr int kWtKG = 2;       // and of the second's cache rows
 constexpr int kWtFewRows = 16;  // query rows of a KV head up to which scores go through memory
 constexpr int kWtMostParts = 128;  // splits of the cache there
 
@@ -51,6 +58,29 @@ __global__ __launch_bounds__(kWtThreads) void weights_lse_kernel(
   const int g = lane / 16, lm = lane % 16;
   int rb, hk, z;
   if (!attn_work_item(nqb, map_group, xpk_log, items, inv_group, inv_nqb, rb, hk, z)) return;
+  const char* kh = kc + (int64_t)hk * k_hs_b;
+  int off[KI];
+#pragma unroll
+  for (int i = 0; i < KI; ++i) {
+    const int P = (wave * KI + i) * 64 + lane, slot = P / CPR;
+    off[i] = slot * ROWB + ((P % CPR) ^ swz_k<CPR>(slot)) * 16;
+  }
+  auto issue = [&](int n0, char* kb) {
+    const char* kt = kh + (int64_t)n0 * ROWB;
+    const int last = N - 1 - n0;
+    auto load = [&](int i, int o) {
+      __builtin_amdgcn_global_load_lds((wt_gvoid*)(kt + (uint32_t)o), (wt_lvoid*)(kb + (wave * KI + i) * 1024), 16, 0, 0);
+    };
+    if (last >= kWtTile - 1) {  // uniform: a whole tile
+#pragma unroll
+      for (int i = 0; i < KI; ++i) load(i, off[i]);
+    } else {  // rows past the cache load its last one; those past every position are masked
+#pragma unroll
+      for (int i = 0; i < KI; ++i) load(i, min(off[i] / ROWB, last) * ROWB + off[i] % ROWB);
+    }
+  };
+  const int tile_begin = SPLIT ? z * split_tiles : 0;
+  issue(tile_begin * kWtTile, lds0);  // known before the positions are
   int my_pos[QG];
   int wmax = -1, wmin = N;
   bf16x8 qf[QG][DS];
@@ -90,8 +120,9 @@ __global__ __launch_bounds__(kWtThreads) void weights_lse_kernel(
   for (int w = 1; w < kWtThreads / 64; ++w) bmax = max(bmax, blk_max_s[w]);
   bmax = __builtin_amdgcn_readfirstlane(bmax);
   int n_tiles = bmax / kWtTile + 1;  // a block has a row: bmax >= 0
-  const int tile_begin = SPLIT ? z * split_tiles : 0;
   if (SPLIT) n_tiles = min(n_tiles, tile_begin + split_tiles);
+  // a split past every position: its loads into LDS land before the workgroup ends
+  if (tile_begin >= n_tiles) __builtin_amdgcn_s_waitcnt(0x0F70);
 
   // A lane's own maximum and sum over the cache rows that it gets.
   float m_run[QG], m_sub[QG], l_run[QG];
@@ -101,31 +132,9 @@ __global__ __launch_bounds__(kWtThreads) void weights_lse_kernel(
     m_sub[qg] = 0.f;
     l_run[qg] = 0.f;
   }
-  const char* kh = kc + (int64_t)hk * k_hs_b;
-  int off[KI];
-#pragma unroll
-  for (int i = 0; i < KI; ++i) {
-    const int P = (wave * KI + i) * 64 + lane, slot = P / CPR;
-    off[i] = slot * ROWB + ((P % CPR) ^ swz_k<CPR>(slot)) * 16;
-  }
-  auto issue = [&](int n0, char* kb) {
-    const char* kt = kh + (int64_t)n0 * ROWB;
-    const int last = bmax - n0;
-    auto load = [&](int i, int o) {
-      __builtin_amdgcn_global_load_lds((wt_gvoid*)(kt + (uint32_t)o), (wt_lvoid*)(kb + (wave * KI + i) * 1024), 16, 0, 0);
-    };
-    if (last >= kWtTile - 1) {  // uniform: a whole tile
-#pragma unroll
-      for (int i = 0; i < KI; ++i) load(i, off[i]);
-    } else {  // rows past every position load the last one's
-#pragma unroll
-      for (int i = 0; i < KI; ++i) load(i, min(off[i] / ROWB, last) * ROWB + off[i] % ROWB);
-    }
-  };
   int k_rd[DS];
 #pragma unroll
   for (int ds = 0; ds < DS; ++ds) k_rd[ds] = lm * ROWB + (((4 * ds + g) ^ swz_k<CPR>(lm)) * 16);
-  if (tile_begin < n_tiles) issue(tile_begin * kWtTile, lds0);
   auto body = [&](int tile, const char* cur, char* nxt) {
     const int n0 = tile * kWtTile;
     __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): this wavefront's loads of the tile landed
@@ -244,21 +253,18 @@ __global__ __launch_bounds__(kWtThreads, 4) void weights_sum_kernel(
   const int k0 = (kb * (kWtThreads / 64) + wave) * (16 * KG);  // this wavefront's cache rows
 
   // does any query row of the part see these cache rows?
-  int seen = -1;
-  for (int r = tile_begin * kWtTile + (int)threadIdx.x; r < tile_end * kWtTile; r += kWtThreads) seen = max(seen, st[r].pos);
-  const bool any = __syncthreads_or(seen >= kb * (kWtThreads / 64) * 16 * KG);
+  bool any = true;
+  if constexpr (PARTS) {
+    int seen = -1;
+    for (int r = tile_begin * kWtTile + (int)threadIdx.x; r < tile_end * kWtTile; r += kWtThreads) seen = max(seen, st[r].pos);
+    any = __syncthreads_or(seen >= kb * (kWtThreads / 64) * 16 * KG);
+  }
 
   f32x4 acc[KG];
 #pragma unroll
   for (int kg = 0; kg < KG; ++kg) acc[kg] = f32x4{0.f, 0.f, 0.f, 0.f};
   if (any) {
     const char* kh = kc + (int64_t)hk * k_hs_b;
-    bf16x8 kf[KG][DS];
-#pragma unroll
-    for (int kg = 0; kg < KG; ++kg)
-#pragma unroll
-      for (int ds = 0; ds < DS; ++ds)
-        kf[kg][ds] = __builtin_bit_cast(bf16x8, ld16(kh + (int64_t)min(k0 + 16 * kg + lm, N - 1) * ROWB + (32 * ds + 8 * g) * 2));
     const char* qh = packed + (int64_t)hk * stat_rows * ROWB;
     int off[KI];
 #pragma unroll
@@ -280,6 +286,12 @@ __global__ __launch_bounds__(kWtThreads, 4) void weights_sum_kernel(
     for (int ds = 0; ds < DS; ++ds) q_rd[ds] = lm * ROWB + (((4 * ds + g) ^ swz_k<CPR>(lm)) * 16);
     RowStat st0[QT], st1[QT];
     issue(tile_begin, lds0, st0);
+    bf16x8 kf[KG][DS];
+#pragma unroll
+    for (int kg = 0; kg < KG; ++kg)
+#pragma unroll
+      for (int ds = 0; ds < DS; ++ds)
+        kf[kg][ds] = __builtin_bit_cast(bf16x8, ld16(kh + (int64_t)min(k0 + 16 * kg + lm, N - 1) * ROWB + (32 * ds + 8 * g) * 2));
     auto body = [&](int tile, const char* cur, char* nxt, const RowStat(&now)[QT], RowStat(&next)[QT]) {
       __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
       __syncthreads();
@@ -361,7 +373,8 @@ __global__ __launch_bounds__(256) void weights_reduce_kernel(const float* __rest
 // ---- few rows (one token's heads) ----------------------------------------------------------------------
 // Up to 16 query rows of a KV head are one matrix tile: weights_scores_kernel streams K once, a wavefront its own 32-row
 // chunks (whole-row loads into its part of LDS, the next chunk's in flight), leaves the scores in the workspace, a
-// fraction of K's bytes, and each split's maxima and sums; weights_from_scores_kernel joins those and adds up.
+// fraction of K's bytes, and each split's maxima and sums; weights_from_scores_kernel joins those and adds up. One row of 28 / 4
+// heads of 128 over 8257: 8.4 us in the place of 28 by the passes above.
 template <int D>
 __global__ __launch_bounds__(kWtThreads) void weights_scores_kernel(
     const int64_t* __restrict__ pos, int N, int rows, int group, const char* __restrict__ kc, int64_t k_hs_b,
@@ -518,6 +531,9 @@ struct WeightsPlan {
   int64_t stat_bytes = 0, part_bytes = 0, sum_bytes = 0;
 };
 
+// Splits of the first pass until its workgroups are all that the card holds at once (1024; half as many took 28 us where
+// these take 24); parts of the second until eight times that (its work is the lower triangle: parts that see nothing return at
+// once), of four tiles of query rows at least.
 static WeightsPlan weights_plan(int n, int N, int Hq, int Hkv) {
   WeightsPlan p;
   p.rows = n * (Hq / Hkv);

@@ -4,12 +4,15 @@
 //
 // Design: a row becomes an integer that orders as its weight does, above all of them for a row that stays anyway, and
 // the n_keep-th largest (with how many of its equals stay) comes out of a radix histogram in LDS of 11, 11 and 10 bits.
-// Up to 34,816 rows one launch does everything: the integers of a head's rows stay in LDS (in registers they
-// unroll every pass, for the same time), a wavefront has a run of
-// consecutive rows, so that the places of kept rows are ballots and a scan over 16 wavefronts. Many workgroups a head
+// Up to 34,816 rows one launch does everything: the integers of a head's rows stay in LDS (in registers they unroll every pass,
+// for the same time), a wavefront has a run of consecutive rows, so that the places of kept rows are ballots and a scan over
+// 16 wavefronts. Many workgroups a head
 // find the same threshold, each for a slice of the kept rows that it then copies: the selection is the latency of
 // one CU whatever is done, and this way no launch waits for it. Longer caches: one workgroup a head reads the weights
 // again for each pass, and evict_gather_kernel copies.
+// Bound: the issue of the CU that selects: 32832 rows of 4 heads of 128 cut to 4104 take 20 us, by phase, us: loads 3, first pass 4,
+// the other two 4, count 2, list and copy 2, launch; 1103 fp32 rows of 2 heads of 64 cut to 300 take 7.7, mostly the passes'
+// scans and barriers. One workgroup a head with a copy launch behind it took 46 and 11.4.
 #include <algorithm>
 
 #include "ckv_common.hpp"
