@@ -322,7 +322,9 @@ struct CodesPlan {
 // to read: 28 / 4 heads of 128 over 32832 rows 16.8 us, one 12.4), a chunk at least for each wavefront.
 static CodesPlan codes_plan(int n, int N, int Hq, int Hkv, int head_dim, int64_t workspace_bytes) {
   const int64_t chunks = (N + kWaveChunk - 1) / kWaveChunk, row_b = (int64_t)Hq * n * (head_dim + 4) * 4;
-  int64_t splits = chunks <= 16 ? 1 : std::min<int64_t>(kWaveFill / Hkv, (chunks + kCodeWaves - 1) / kCodeWaves);
+  // whole up to 1024 rows of 128 and 1536 of 64: the join is a launch (us, eager calls, whole and split: 28 / 4 heads of 128, 1000
+  // rows 7.8 and 9.6, 1400 rows 9.2 and 9.5 but 7.2 in a graph; 14 / 2 heads of 64, 1500 rows 7.5 and 9.6)
+  int64_t splits = chunks <= (head_dim == 128 ? 32 : 48) ? 1 : std::min<int64_t>(kWaveFill / Hkv, (chunks + kCodeWaves - 1) / kCodeWaves);
   splits = std::max<int64_t>(1, std::min(splits, workspace_bytes / row_b));
   CodesPlan p;
   p.split_chunks = (int)((chunks + splits - 1) / splits);

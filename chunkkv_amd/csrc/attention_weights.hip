@@ -32,6 +32,8 @@ constexpr int kWtQG = 2;       // 16-row groups of a wavefront of the first pass
 constexpr int kWtKG = 2;       // and of the second's cache rows
 constexpr int kWtFewRows = 16;  // query rows of a KV head up to which scores go through memory
 constexpr int kWtMostParts = 128;  // splits of the cache there
+constexpr int kWtWholeRows = 1024;  // cache rows up to which one workgroup a head does all of it
+constexpr int kWtWholeWaves = 8;
 
 // A query row's normaliser and position, as the second pass reads it.
 struct RowStat {
@@ -374,14 +376,22 @@ __global__ __launch_bounds__(256) void weights_reduce_kernel(const float* __rest
 // Up to 16 query rows of a KV head are one matrix tile: weights_scores_kernel streams K once, a wavefront its own 32-row
 // chunks (whole-row loads into its part of LDS, the next chunk's in flight), leaves the scores in the workspace, a
 // fraction of K's bytes, and each split's maxima and sums; weights_from_scores_kernel joins those and adds up. One row of 28 / 4
-// heads of 128 over 8257: 8.4 us in the place of 28 by the passes above.
-template <int D>
-__global__ __launch_bounds__(kWtThreads) void weights_scores_kernel(
+// heads of 128 over 8257: 8.4 us in the place of 28 by the passes above. Up to 1024 cache rows one workgroup a head keeps its
+// scores in LDS and is the whole call (eager calls, which the host's launches bound: 9.3 -> 4.9 us, 7.9 at 1000 rows).
+// WHOLE: one workgroup of W wavefronts takes a head's whole cache, of at most kWtWholeRows rows: the scores stay in LDS and it
+// adds them up itself.
+template <int D, int W, bool WHOLE>
+__global__ __launch_bounds__(W * 64) void weights_scores_kernel(
     const int64_t* __restrict__ pos, int N, int rows, int group, const char* __restrict__ kc, int64_t k_hs_b,
     const char* __restrict__ q, int64_t q_hs_b, int64_t q_ts_b, float scale_log2, int split_chunks, int splits,
-    float* __restrict__ scores, int64_t score_stride, float2* __restrict__ part, int32_t* __restrict__ err) {
-  constexpr int DS = D / 32, CPR = D / 8, ROWB = D * 2, CH = 32, W = kWtThreads / 64, LI = CH * CPR / 64;
+    float* __restrict__ scores, int64_t score_stride, float2* __restrict__ part, const float* prior, float* out,
+    int32_t* __restrict__ err) {
+  constexpr int DS = D / 32, CPR = D / 8, ROWB = D * 2, CH = 32, LI = CH * CPR / 64;
+  constexpr int PITCH = kWtWholeRows + 4;  // of a row's scores in LDS
   __shared__ __attribute__((aligned(1024))) char lds[W * CH * ROWB];
+  __shared__ __attribute__((aligned(16))) float s_scores[WHOLE ? kWtFewRows * PITCH : 4];
+  __shared__ float s_lse[kWtFewRows];
+  __shared__ int s_pos[kWtFewRows];
   __shared__ float2 s_ml[W][16];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x % 64;
   const int g = lane / 16, lm = lane % 16;
@@ -411,7 +421,7 @@ __global__ __launch_bounds__(kWtThreads) void weights_scores_kernel(
   const int c_end = min(wmax / CH + 1, begin + split_chunks);
   char* wl = lds + wave * CH * ROWB;
   float m_run = -INFINITY, l_run = 0.f;
-  float* srow = scores + (int64_t)(hk * rows + r) * score_stride;
+  float* srow = WHOLE ? s_scores + lm * PITCH : scores + (int64_t)(hk * rows + r) * score_stride;
   for (; c < c_end; c += W) {
     wave_lds_stage();
 #pragma unroll
@@ -467,9 +477,24 @@ __global__ __launch_bounds__(kWtThreads) void weights_scores_kernel(
     for (int w = 0; w < W; ++w) mx = fmaxf(mx, s_ml[w][lm].x);
 #pragma unroll
     for (int w = 0; w < W; ++w) sum += s_ml[w][lm].x == -INFINITY ? 0.f : s_ml[w][lm].y * __builtin_amdgcn_exp2f(s_ml[w][lm].x - mx);
-    part[(int64_t)(hk * rows + lm) * splits + z] = make_float2(mx, sum);
+    if constexpr (WHOLE) {
+      s_lse[lm] = mx + __builtin_amdgcn_logf(sum);
+      s_pos[lm] = p;
+    } else {
+      part[(int64_t)(hk * rows + lm) * splits + z] = make_float2(mx, sum);
+    }
+  }
+  if constexpr (WHOLE) {
+    __syncthreads();
+    for (int j = threadIdx.x; j < N; j += W * 64) {
+      const int64_t at = (int64_t)hk * N + j;
+      float total = 0.f;
+      for (int r = 0; r < rows; ++r) total += j <= s_pos[r] ? __builtin_amdgcn_exp2f(s_scores[r * PITCH + j] - s_lse[r]) : 0.f;
+      out[at] = prior != nullptr ? prior[at] + total : total;
+    }
   }
 }
+
 
 __global__ __launch_bounds__(kWtThreads) void weights_from_scores_kernel(
     const int64_t* __restrict__ pos, int N, int rows, int group, const float* __restrict__ scores, int64_t score_stride,
@@ -509,7 +534,7 @@ __global__ __launch_bounds__(kWtThreads) void weights_from_scores_kernel(
 }
 
 struct FewPlan {
-  int rows, splits, split_chunks;
+  int rows, chunks, splits, split_chunks;
   int64_t score_stride, score_bytes, bytes;
 };
 static FewPlan few_plan(int rows, int N, int Hkv) {
@@ -517,6 +542,7 @@ static FewPlan few_plan(int rows, int N, int Hkv) {
   const int64_t splits = std::max<int64_t>(1, std::min<int64_t>({512 / Hkv, (chunks + 3) / 4, kWtMostParts}));
   FewPlan p;
   p.rows = rows;
+  p.chunks = chunks;
   p.split_chunks = (int)((chunks + splits - 1) / splits);
   p.splits = (chunks + p.split_chunks - 1) / p.split_chunks;
   p.score_stride = (int64_t)chunks * 32;
@@ -563,6 +589,7 @@ extern "C" int64_t ckv_attention_weights_workspace_bytes(int32_t n_queries, int3
   if (n_queries <= 0 || n_tokens <= 0 || n_kv_heads <= 0 || n_q_heads <= 0 || head_dim <= 0 || n_q_heads % n_kv_heads ||
       (int64_t)n_queries * (n_q_heads / n_kv_heads) > INT32_MAX / 2)
     return 0;
+  if (n_queries * (n_q_heads / n_kv_heads) <= kWtFewRows && n_tokens <= kWtWholeRows) return 0;
   if (n_queries * (n_q_heads / n_kv_heads) <= kWtFewRows) return few_plan(n_queries * (n_q_heads / n_kv_heads), n_tokens, n_kv_heads).bytes;
   const WeightsPlan p = weights_plan(n_queries, n_tokens, n_q_heads, n_kv_heads);
   return p.stat_bytes + (int64_t)n_kv_heads * p.stat_rows * head_dim * 2 + std::max(p.part_bytes, p.sum_bytes);
@@ -594,21 +621,27 @@ extern "C" int32_t ckv_attention_weights(float* out, const float* prior, const v
   if (((uintptr_t)q | (uintptr_t)k_cache) % 16) return CKV_ERR_INVALID_ARGUMENT;
   if (q_token_stride < head_dim || k_head_stride < (int64_t)n_tokens * head_dim) return CKV_ERR_OUT_OF_RANGE;
   if ((int64_t)n_queries * group > INT32_MAX / 2 || n_kv_heads > 65535) return CKV_ERR_TOO_LARGE;
-  if (workspace == nullptr || (uintptr_t)workspace % 16 ||
-      workspace_bytes < ckv_attention_weights_workspace_bytes(n_queries, n_tokens, n_q_heads, n_kv_heads, head_dim))
-    return CKV_ERR_INVALID_ARGUMENT;
+  const int64_t need = ckv_attention_weights_workspace_bytes(n_queries, n_tokens, n_q_heads, n_kv_heads, head_dim);
+  if (need > 0 && (workspace == nullptr || (uintptr_t)workspace % 16 || workspace_bytes < need)) return CKV_ERR_INVALID_ARGUMENT;
   const float scale_log2 = (float)(scale * 1.4426950408889634);  // exp(x) = exp2(x log2 e)
   if (n_queries * group <= kWtFewRows) {
+    const bool whole = n_tokens <= kWtWholeRows;
     const FewPlan p = few_plan(n_queries * group, n_tokens, n_kv_heads);
     float* scores = (float*)workspace;
     float2* part = (float2*)((char*)workspace + p.score_bytes);
-    auto launch = [&](auto kernel) {
-      hipLaunchKernelGGL(kernel, dim3((unsigned)p.splits, (unsigned)n_kv_heads), dim3(kWtThreads), 0, s, positions, n_tokens, p.rows,
+    auto launch = [&](auto kernel, int splits, int waves) {
+      hipLaunchKernelGGL(kernel, dim3((unsigned)splits, (unsigned)n_kv_heads), dim3(waves * 64), 0, s, positions, n_tokens, p.rows,
                          group, (const char*)k_cache, k_head_stride * 2, (const char*)q, q_head_stride * 2, q_token_stride * 2,
-                         scale_log2, p.split_chunks, p.splits, scores, p.score_stride, part, err);
+                         scale_log2, whole ? p.chunks : p.split_chunks, p.splits, scores, p.score_stride, part, prior, out, err);
     };
-    if (head_dim == 128) launch(weights_scores_kernel<128>);
-    else launch(weights_scores_kernel<64>);
+    if (whole) {
+      if (head_dim == 128) launch(weights_scores_kernel<128, kWtWholeWaves, true>, 1, kWtWholeWaves);
+      else launch(weights_scores_kernel<64, kWtWholeWaves, true>, 1, kWtWholeWaves);
+      CKV_RETURN_IF_LAUNCH_FAILED();
+      return CKV_OK;
+    }
+    if (head_dim == 128) launch(weights_scores_kernel<128, 4, false>, p.splits, 4);
+    else launch(weights_scores_kernel<64, 4, false>, p.splits, 4);
     CKV_RETURN_IF_LAUNCH_FAILED();
     hipLaunchKernelGGL(weights_from_scores_kernel, dim3((unsigned)((n_tokens + kWtThreads - 1) / kWtThreads), (unsigned)n_kv_heads),
                        dim3(kWtThreads), 0, s, positions, n_tokens, p.rows, group, (const float*)scores, p.score_stride,

@@ -561,7 +561,7 @@ int64_t ckv_attention_workspace_bytes(int32_t n_queries, int32_t n_tokens, int32
  * (n_heads, ceil(n_tokens / block_tokens))); a row's values are code * scale.
  *   scale of a block = 2^e, e the least integer >= -126 with max |x| <= 448 * 2^e over the block's rows
  *   code             = e4m3(x / scale), to nearest even
- * Rows of the first block in front of `start` are kept: the block's scale is the larger of theirs and the new
+ * Rows of the first block in front of `start` (written by earlier calls) are kept: the block's scale is the larger of theirs and the new
  * rows', and where it grows their codes are rescaled (exactly, but for codes that become subnormal). Rows
  * behind start + n_rows keep their bytes but not their scale: they hold nothing any more. An infinity or a
  * NaN among the new rows makes its block's rows and scale NaN.
@@ -613,7 +613,7 @@ int32_t ckv_attention_weights(float* out, const float* prior, const void* q, int
                               int32_t n_kv_heads, int32_t head_dim, int32_t dtype, double scale, void* workspace,
                               int64_t workspace_bytes, int32_t* err, void* stream);
 
-/* Bytes of workspace that ckv_attention_weights needs for this shape. Host-only. */
+/* Bytes of workspace that ckv_attention_weights needs for this shape (0: none). Host-only. */
 int64_t ckv_attention_weights_workspace_bytes(int32_t n_queries, int32_t n_tokens, int32_t n_q_heads,
                                               int32_t n_kv_heads, int32_t head_dim);
 

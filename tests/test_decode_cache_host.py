@@ -49,8 +49,8 @@ EVICT = [("ko", 16), ("ko_hs", 640), ("vo", 16), ("vo_hs", 640), ("rows", 16), (
     ("ckv_attention_weights", WEIGHTS, [
         (dict(out=None), INVALID), (dict(q=None), INVALID), (dict(k=None), INVALID), (dict(pos=None), INVALID), (dict(k=8), INVALID),
         (dict(dtype=0), INVALID), (dict(D=256), INVALID), (dict(Hq=3), INVALID), (dict(N=0), INVALID), (dict(n=-1), INVALID),
-        (dict(scale=-1.0), INVALID), (dict(q_hs=68), INVALID), (dict(q_ts=56), RANGE), (dict(k_hs=6392), RANGE), (dict(ws=None), INVALID),
-        (dict(wsb=16), INVALID), (dict(ws=8), INVALID), (dict(n=1 << 30), LARGE), (dict(n=0, q=None, k=None, pos=None, prior=16), OK)]),
+        (dict(scale=-1.0), INVALID), (dict(q_hs=68), INVALID), (dict(q_ts=56), RANGE), (dict(k_hs=6392), RANGE), (dict(ws=None, n=40), INVALID),
+        (dict(wsb=16, n=40), INVALID), (dict(ws=8, n=40), INVALID), (dict(n=1 << 30), LARGE), (dict(n=0, q=None, k=None, pos=None, prior=16), OK)]),
     ("ckv_evict_rows", EVICT, [
         (dict(ko=None), INVALID), (dict(rows=None), INVALID), (dict(w=None), INVALID), (dict(vo=8), INVALID), (dict(k=8), INVALID),
         (dict(ko_hs=644), INVALID), (dict(D=96), INVALID), (dict(dtype=2), INVALID), (dict(N=0), INVALID), (dict(sink=-1), INVALID),
@@ -72,7 +72,7 @@ def test_workspace_sizes_are_host_only():
     assert attn(2976, 8256, 28, 4, 128) >= 2 * 2 * 4 * 8256 * 128  # the cache as bf16
     assert attn(0, 100, 28, 4, 128) == attn(1, 0, 28, 4, 128) == attn(1, 100, 28, 3, 128) == attn(1, 100, 28, 0, 128) == 0
     w = lib.ckv_attention_weights_workspace_bytes
-    assert w(1, 1, 4, 4, 64) > 0 and w(0, 100, 28, 4, 64) == w(1, 100, 28, 3, 64) == 0
+    assert w(40, 100, 4, 4, 64) > 0 and w(1, 100, 4, 4, 64) == 0 and w(1, 2000, 4, 4, 64) > 0 and w(0, 100, 28, 4, 64) == w(1, 100, 28, 3, 64) == 0
     assert w(2**31 - 1, 100, 64, 1, 64) == 0  # refused by the call
 
 
