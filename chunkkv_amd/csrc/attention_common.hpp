@@ -7,6 +7,14 @@
 
 namespace ckv {
 
+// What an 8-bit cache has beside its codes: for head h and 32-row chunk c the scale byte e + 127 of 2^e
+// is at [h * blocks + (c >> chunk_log)], of K and of V.
+struct CacheScales {
+  const uint8_t* k;
+  const uint8_t* v;
+  int blocks, chunk_log;
+};
+
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 

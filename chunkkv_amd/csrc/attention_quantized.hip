@@ -5,10 +5,11 @@
 //  - One token's rows: attn_codes_kernel below.
 //  - Few query rows (some tokens, short prompts): attention_wave.hpp's kernel reads the codes and makes them bf16
 //    on their way into LDS, a wavefront its own 32 rows.
-//  - Many: one pass writes the cache as bf16 into the workspace and attention.hip runs on it. There every
-//    row is read by many workgroups of 128 queries, and each would convert it again: about a third more vector
-//    instructions in a kernel that they bound, against 7 of 191 us (2976 queries over 8256 rows, 28 / 4 heads of 128).
-#include "attention_common.hpp"
+//  - More, as attention_plan.hpp decides for bf16 rows: attention_large.hpp's workgroups of 128 queries, which convert a tile on
+//    its way into LDS. Every workgroup that reads a row converts it again, about a tenth of the kernel's time,
+//  - so launches of many rows first write the cache as bf16 into the workspace, one pass, and attention.hip runs on that
+//    (kDecodeRows has both sides).
+#include "attention_large.hpp"
 #include "attention_wave.hpp"
 
 namespace ckv {
@@ -332,13 +333,14 @@ static CodesPlan codes_plan(int n, int N, int Hq, int Hkv, int head_dim, int64_t
   return p;
 }
 static bool few_rows(int n, int Hq, int Hkv) { return (int64_t)n * (Hq / Hkv) <= kCodeRows; }
-// Whether a launch converts the cache first.
+// (token, query head) rows of a KV head from which a launch converts the cache first. That pass is the cache's bytes, the
+// conversion inside the kernel grows with the rows (us, converting inside and first: 28 / 4 heads of 128 over 28787 rows 128
+// queries 67 and 80, 500 175 and 176, 800 311 and 298; 14 / 2 heads of 64 over 65536, 128 57 and 65, 800 199 and 194; 16 / 16 of
+// 64 over 28787, 128 25 and 42, 2976 166 and 170). Cache lengths move the crossing little: both costs grow with them.
+constexpr int kDecodeRows = 3500;
 static bool decode_first(int n, int N, int Hq, int Hkv, int head_dim) {
-  return !few_rows(n, Hq, Hkv) && !attn_plan(n, N, Hq, Hkv, head_dim, attn_workspace_bytes(n, N, Hq, head_dim)).wave;
-}
-static int64_t wave_workspace_bytes(int n, int N, int Hq, int Hkv, int head_dim) {
-  const int64_t splits = few_rows(n, Hq, Hkv) ? codes_plan(n, N, Hq, Hkv, head_dim, INT64_MAX).splits : most_splits(n, N, Hq, head_dim);
-  return splits > 1 ? splits * Hq * n * (head_dim + 4) * 4 : 0;
+  return (int64_t)n * (Hq / Hkv) > kDecodeRows &&
+         !attn_plan(n, N, Hq, Hkv, head_dim, attn_workspace_bytes(n, N, Hq, head_dim)).wave;
 }
 static int64_t decoded_bytes(int N, int Hkv, int head_dim) { return (int64_t)Hkv * N * head_dim * 4; }
 
@@ -348,9 +350,12 @@ extern "C" int64_t ckv_attention_quantized_workspace_bytes(int32_t n_queries, in
                                                            int32_t n_kv_heads, int32_t head_dim) {
   using namespace ckv;
   if (n_queries <= 0 || n_tokens <= 0 || n_q_heads <= 0 || n_kv_heads <= 0 || head_dim <= 0 || n_q_heads % n_kv_heads) return 0;
-  return decode_first(n_queries, n_tokens, n_q_heads, n_kv_heads, head_dim)
-             ? decoded_bytes(n_tokens, n_kv_heads, head_dim) + attn_workspace_bytes(n_queries, n_tokens, n_q_heads, head_dim)
-             : wave_workspace_bytes(n_queries, n_tokens, n_q_heads, n_kv_heads, head_dim);
+  if (few_rows(n_queries, n_q_heads, n_kv_heads)) {
+    const int splits = codes_plan(n_queries, n_tokens, n_q_heads, n_kv_heads, head_dim, INT64_MAX).splits;
+    return splits > 1 ? (int64_t)splits * n_q_heads * n_queries * (head_dim + 4) * 4 : 0;
+  }
+  return attn_workspace_bytes(n_queries, n_tokens, n_q_heads, head_dim) +
+         (decode_first(n_queries, n_tokens, n_q_heads, n_kv_heads, head_dim) ? decoded_bytes(n_tokens, n_kv_heads, head_dim) : 0);
 }
 
 extern "C" int32_t ckv_attention_quantized(void* out, const void* q, int64_t q_head_stride, int64_t q_token_stride,
@@ -423,24 +428,36 @@ extern "C" int32_t ckv_attention_quantized(void* out, const void* q, int64_t q_h
     }
     return CKV_OK;
   }
-  const AttnPlan plan = attn_wave_plan(n_queries, n_tokens, n_q_heads, n_kv_heads, head_dim, workspace_bytes);
+  const AttnPlan plan = attn_plan(n_queries, n_tokens, n_q_heads, n_kv_heads, head_dim, workspace_bytes);
   const AttnMap& map = plan.map;
   float* ws = plan.splits > 1 ? (float*)workspace : nullptr;
-  const uint32_t inv_gqa = inverse_of((int64_t)n_queries * group, group);
-  auto launch = [&](auto kernel, int waves) {
-    hipLaunchKernelGGL(kernel, dim3(map.blocks), dim3(waves * 64), 0, st, map.nqb, map.group, map.xpk_log, map.items,
-                       map.inv_group, map.inv_nqb, positions, n_queries, n_tokens, (const char*)k_codes,
-                       (const char*)v_codes, (int64_t)n_tokens * head_dim, (const char*)q, q_head_stride * 2,
-                       q_token_stride * 2, n_q_heads, group, inv_gqa, scale_log2, plan.split_chunks, (char*)out, ws, err, scales);
-  };
+  if (plan.wave) {
+    const uint32_t inv_gqa = inverse_of((int64_t)n_queries * group, group);
+    auto launch = [&](auto kernel, int waves) {
+      hipLaunchKernelGGL(kernel, dim3(map.blocks), dim3(waves * 64), 0, st, map.nqb, map.group, map.xpk_log, map.items,
+                         map.inv_group, map.inv_nqb, positions, n_queries, n_tokens, (const char*)k_codes,
+                         (const char*)v_codes, (int64_t)n_tokens * head_dim, (const char*)q, q_head_stride * 2,
+                         q_token_stride * 2, n_q_heads, group, inv_gqa, scale_log2, plan.split_chunks, (char*)out, ws, err, scales);
+    };
 #define CKV_WAVE(HD, QG, W, GR) \
   else if (head_dim == HD && plan.qg == QG && plan.waves == W && plan.grouped == GR) \
     launch(attn_wave_kernel<HD, QG, W, GR, CacheScales>, W);
-  if (false) {
-  }
-  CKV_WAVE_FORMS(CKV_WAVE)
-  else return CKV_ERR_INVALID_ARGUMENT;  // a plan outside the list
+    if (false) {
+    }
+    CKV_WAVE_FORMS(CKV_WAVE)
+    else return CKV_ERR_INVALID_ARGUMENT;  // a plan outside the list
 #undef CKV_WAVE
+  } else {
+    auto launch = [&](auto kernel) {
+      hipLaunchKernelGGL(kernel, dim3(map.blocks), dim3(kAttnWaves * 64), 0, st, map.nqb, map.group, map.xpk_log, map.items,
+                         map.inv_group, map.inv_nqb, positions, n_queries, n_tokens, (const char*)k_codes,
+                         (const char*)v_codes, (int64_t)n_tokens * head_dim, (const char*)q, q_head_stride * 2,
+                         q_token_stride * 2, n_q_heads, group, scale_log2, (char*)out, err, ws,
+                         plan.split_chunks / (kAttnBN / kWaveChunk), scales);
+    };
+    if (head_dim == 128) ws != nullptr ? launch(attn_active_kernel<128, true, CacheScales>) : launch(attn_active_kernel<128, false, CacheScales>);
+    else ws != nullptr ? launch(attn_active_kernel<64, true, CacheScales>) : launch(attn_active_kernel<64, false, CacheScales>);
+  }
   CKV_RETURN_IF_LAUNCH_FAILED();
   if (ws != nullptr) {
     join(ws, plan.splits);

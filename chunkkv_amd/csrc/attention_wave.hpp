@@ -24,14 +24,6 @@
 
 namespace ckv {
 
-// What an 8-bit cache has beside its codes: for head h and 32-row chunk c the scale byte e + 127 of 2^e
-// is at [h * blocks + (c >> chunk_log)], of K and of V.
-struct CacheScales {
-  const uint8_t* k;
-  const uint8_t* v;
-  int blocks, chunk_log;
-};
-
 // With a CacheScales argument at the end the cache holds e4m3 codes. A row's codes become bf16 (exactly: three fraction bits times a
 // power of two) where it is put into LDS, and everything after that is the bf16 cache's.
 template <int D, int QG, int W, bool GROUPED, typename... Scales>

@@ -1,5 +1,4 @@
-// Walks attn_wave_plan, the plan of launches that take attn_wave_kernel whatever their size (an 8-bit cache without a
-// workspace to convert it in): its form exists, its splits cover the cache, none empty, and fit the workspace, its work items
+// Walks attn_wave_plan, attn_wave_kernel's plan, over launches of any size (attn_plan asks it for small ones): its form exists, its splits cover the cache, none empty, and fit the workspace, its work items
 // cover every (query block, head, split) once. Prints the plans checked and the bad ones.
 #include "attention_plan.hpp"
 

@@ -42,6 +42,11 @@ def _check(q, K, pos, prior=None, scale=None, out=None):
         (6, 3, 64, 129, 65),  # heads that do not divide 8
         (64, 1, 128, 130, 9),  # a group of 64
         (4, 4, 128, 64, 17),
+        (28, 4, 128, 1024, 2),  # up to 16 rows of a KV head: whole, and split from 1025 cached rows on
+        (28, 4, 128, 1025, 2),
+        (16, 1, 64, 1024, 1),
+        (17, 1, 64, 1024, 1),  # 17 rows
+        (4, 4, 64, 1023, 16),
     ],
 )
 def test_weights_match_the_plain_form(Hq, Hkv, D, N, n):

@@ -211,7 +211,17 @@ def _attends(q, c, pos, rows, scale=None, **kw):
         (8, 8, 64, 333, 333, 333, 64),  # no shared heads, causal, ragged
         (14, 2, 64, 1103, 1103, 251, 32),
         (28, 4, 128, 1500, 1500, 1500, 64),  # 128-query workgroups: the cache read as bf16
-        (28, 4, 128, 8256, 8250, 130, 128),  # the same in splits
+        (28, 4, 128, 8256, 8250, 130, 128),  # the same in splits, the codes converted by each
+        (28, 4, 128, 6001, 5985, 500, 32),  # at the change between these
+        (28, 4, 128, 6001, 5985, 501, 32),
+        (14, 2, 64, 16390, 16385, 65, 64),
+        (16, 16, 64, 5700, 5633, 130, 128),
+        (32, 32, 128, 1100, 1090, 1000, 32),  # no shared heads: the codes converted, unsplit
+        (64, 64, 64, 1000, 993, 910, 64),
+        (28, 4, 128, 1100, 1024, 1, 32),  # one token, whole and split
+        (28, 4, 128, 1025, 1025, 1, 32),
+        (14, 2, 64, 1536, 1536, 2, 64),
+        (14, 2, 64, 1600, 1537, 1, 128),
         (6, 3, 64, 130, 129, 100, 32),  # heads that do not divide 8
         (64, 1, 128, 700, 700, 3, 64),  # a group of 64
     ],
