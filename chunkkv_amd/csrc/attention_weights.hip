@@ -5,7 +5,7 @@
 //
 // Design: the n x group (token, query head) pairs of a KV head are its rows. A weight needs its row's maximum
 // and sum before it can be formed, so the product with K^T runs twice:
-//  1. weights_lse_kernel: 128 rows a workgroup walk the cache in 64-row tiles (attention.hip's first half, with the
+//  1. weights_lse_kernel: 128 rows a workgroup (64 in small launches, as in the second pass) walk the cache in 64-row tiles (attention.hip's first half, with the
 //     maximum and the sum kept per lane); with few row blocks, in splits of the cache. Leaves L = max + log2(sum) and the
 //     position of each row (weights_join_kernel joins the splits).
 //  2. weights_sum_kernel: 128 cache rows a workgroup hold their operands in registers while the query rows (packed by the
@@ -28,8 +28,6 @@ namespace ckv {
 
 constexpr int kWtThreads = 256;
 constexpr int kWtTile = 64;    // cache rows of a tile of the first pass, query rows of one of the second
-constexpr int kWtQG = 2;       // 16-row groups of a wavefront of the first pass
-constexpr int kWtKG = 2;       // and of the second's cache rows
 constexpr int kWtFewRows = 16;  // query rows of a KV head up to which scores go through memory
 constexpr int kWtMostParts = 128;  // splits of the cache there
 constexpr int kWtWholeRows = 1024;  // cache rows up to which one workgroup a head does all of it
@@ -306,7 +304,7 @@ __global__ __launch_bounds__(kWtThreads, 4) void weights_sum_kernel(
       }
       if (!__builtin_amdgcn_ballot_w64(top >= k0)) return;  // uniform per wavefront
       const bool need_mask = __builtin_amdgcn_ballot_w64(low < k0 + 16 * KG - 1);
-      constexpr int U = 2;  // query groups at a time: dependent products U KG apart
+      constexpr int U = 4 / KG;  // query groups at a time: dependent products four apart
 #pragma unroll
       for (int t0 = 0; t0 < QT; t0 += U) {
         f32x4 s[U][KG];
@@ -551,26 +549,42 @@ static FewPlan few_plan(int rows, int N, int Hkv) {
   return p;
 }
 
+template <int I>
+using Int = std::integral_constant<int, I>;
+
 struct WeightsPlan {
   int rows = 0, stat_rows = 0, row_blocks = 0,  // stat_rows: rows in whole tiles
-      splits = 1, split_tiles = 0, key_blocks = 0, parts = 1, part_tiles = 0;
+      splits = 1, split_tiles = 0, key_blocks = 0, parts = 1, part_tiles = 0,
+      qg = 2, kg = 2;  // 16-row groups of a wavefront: query rows of the first pass, cache rows of the second
   int64_t stat_bytes = 0, part_bytes = 0, sum_bytes = 0;
 };
 
 // Splits of the first pass until its workgroups are all that the card holds at once (1024; half as many took 28 us where
 // these take 24); parts of the second until eight times that (its work is the lower triangle: parts that see nothing return at
 // once), of four tiles of query rows at least.
-static WeightsPlan weights_plan(int n, int N, int Hq, int Hkv) {
+static WeightsPlan weights_plan(int n, int N, int Hq, int Hkv, int head_dim) {
   WeightsPlan p;
   p.rows = n * (Hq / Hkv);
-  p.row_blocks = (p.rows + 64 * kWtQG - 1) / (64 * kWtQG);
   const int tiles = (N + kWtTile - 1) / kWtTile, row_tiles = (p.rows + kWtTile - 1) / kWtTile;
-  p.key_blocks = (N + 64 * kWtKG - 1) / (64 * kWtKG);
-  const int64_t lse_blocks = (int64_t)p.row_blocks * Hkv, sum_blocks = (int64_t)p.key_blocks * Hkv;
+  // 64 rows a workgroup of the first pass in the place of 128 where there is little work (a wavefront's chain over a tile is half as
+  // long, every K row is read twice as often): 28 / 4 heads of 128 (us, 128 rows and 64), 30 queries over 1103 16.0 and 14.1, 128 over
+  // 8302 36.4 and 34.2, 128 over 16400 51.6 and 51.1, 251 84.9 and 87.8; over 65536 17 queries 37.8 and 40.2, but 8, which 64 rows
+  // hold, 33.8 and 28.9. 14 / 2 heads of 64, 251 over 16400 40.5 and 39.3, 500 over 32832 106 and 109.
+  const bool short_rows = (int64_t)((p.rows + 127) / 128) * tiles * Hkv <= 8300 && (int64_t)N * head_dim <= 5 << 20;
+  p.qg = p.rows <= 64 || short_rows ? 1 : 2;
+  p.row_blocks = (p.rows + 64 * p.qg - 1) / (64 * p.qg);
+  const int64_t lse_blocks = (int64_t)p.row_blocks * Hkv;
   int64_t splits = std::max<int64_t>(1, std::min<int64_t>({1024 / lse_blocks, tiles / 2, 64}));
   p.split_tiles = (int)((tiles + splits - 1) / splits);
   p.splits = (tiles + p.split_tiles - 1) / p.split_tiles;
-  const int64_t parts = std::max<int64_t>(1, std::min<int64_t>(8192 / sum_blocks, row_tiles / 4));
+  auto parts_of = [&](int64_t blocks) { return std::max<int64_t>(1, std::min<int64_t>(8192 / blocks, row_tiles / 4)); };
+  // The same in the second pass, 64 cache rows a workgroup for 128, while two of these a CU do not fill the card: 28 / 4 heads of 128
+  // (us, 128 cache rows and 64), 64 queries over 1103 19.1 and 16.5, over 8302 26.9 and 24.3, 251 over 2048 27.7 and 27.8, 128 over 8302
+  // 36.4 and 37.3.
+  const int64_t wide = (int64_t)((N + 127) / 128) * Hkv;
+  p.kg = wide * parts_of(wide) <= 512 ? 1 : 2;
+  p.key_blocks = (N + 64 * p.kg - 1) / (64 * p.kg);
+  const int64_t parts = parts_of((int64_t)p.key_blocks * Hkv);
   p.part_tiles = (int)((row_tiles + parts - 1) / parts);
   p.parts = (row_tiles + p.part_tiles - 1) / p.part_tiles;
   p.stat_rows = row_tiles * kWtTile;
@@ -591,7 +605,7 @@ extern "C" int64_t ckv_attention_weights_workspace_bytes(int32_t n_queries, int3
     return 0;
   if (n_queries * (n_q_heads / n_kv_heads) <= kWtFewRows && n_tokens <= kWtWholeRows) return 0;
   if (n_queries * (n_q_heads / n_kv_heads) <= kWtFewRows) return few_plan(n_queries * (n_q_heads / n_kv_heads), n_tokens, n_kv_heads).bytes;
-  const WeightsPlan p = weights_plan(n_queries, n_tokens, n_q_heads, n_kv_heads);
+  const WeightsPlan p = weights_plan(n_queries, n_tokens, n_q_heads, n_kv_heads, head_dim);
   return p.stat_bytes + (int64_t)n_kv_heads * p.stat_rows * head_dim * 2 + std::max(p.part_bytes, p.sum_bytes);
 }
 
@@ -649,7 +663,7 @@ extern "C" int32_t ckv_attention_weights(float* out, const float* prior, const v
     CKV_RETURN_IF_LAUNCH_FAILED();
     return CKV_OK;
   }
-  const WeightsPlan p = weights_plan(n_queries, n_tokens, n_q_heads, n_kv_heads);
+  const WeightsPlan p = weights_plan(n_queries, n_tokens, n_q_heads, n_kv_heads, head_dim);
   const uint32_t inv_gqa = inverse_of(p.rows, group);
   RowStat* stat = (RowStat*)workspace;
   char* packed = (char*)workspace + p.stat_bytes;
@@ -663,8 +677,12 @@ extern "C" int32_t ckv_attention_weights(float* out, const float* prior, const v
                          (const char*)q, q_head_stride * 2, q_token_stride * 2, scale_log2, stat, packed, p.stat_rows, (float2*)scratch,
                          rows_total, p.split_tiles, err);
     };
-    if (head_dim == 128) p.splits > 1 ? launch(weights_lse_kernel<128, kWtQG, true>) : launch(weights_lse_kernel<128, kWtQG, false>);
-    else p.splits > 1 ? launch(weights_lse_kernel<64, kWtQG, true>) : launch(weights_lse_kernel<64, kWtQG, false>);
+    auto form = [&](auto dim, auto qg) {
+      constexpr int D = decltype(dim)::value, QG = decltype(qg)::value;
+      p.splits > 1 ? launch(weights_lse_kernel<D, QG, true>) : launch(weights_lse_kernel<D, QG, false>);
+    };
+    if (head_dim == 128) p.qg == 1 ? form(Int<128>{}, Int<1>{}) : form(Int<128>{}, Int<2>{});
+    else p.qg == 1 ? form(Int<64>{}, Int<1>{}) : form(Int<64>{}, Int<2>{});
     CKV_RETURN_IF_LAUNCH_FAILED();
   }
   if (p.splits > 1) {
@@ -680,8 +698,12 @@ extern "C" int32_t ckv_attention_weights(float* out, const float* prior, const v
                          (const RowStat*)stat, prior,
                          p.parts > 1 ? scratch : out, total, p.part_tiles);
     };
-    if (head_dim == 128) p.parts > 1 ? launch(weights_sum_kernel<128, kWtKG, true>) : launch(weights_sum_kernel<128, kWtKG, false>);
-    else p.parts > 1 ? launch(weights_sum_kernel<64, kWtKG, true>) : launch(weights_sum_kernel<64, kWtKG, false>);
+    auto form = [&](auto dim, auto kg) {
+      constexpr int D = decltype(dim)::value, KG = decltype(kg)::value;
+      p.parts > 1 ? launch(weights_sum_kernel<D, KG, true>) : launch(weights_sum_kernel<D, KG, false>);
+    };
+    if (head_dim == 128) p.kg == 1 ? form(Int<128>{}, Int<1>{}) : form(Int<128>{}, Int<2>{});
+    else p.kg == 1 ? form(Int<64>{}, Int<1>{}) : form(Int<64>{}, Int<2>{});
     CKV_RETURN_IF_LAUNCH_FAILED();
   }
   if (p.parts > 1) {
