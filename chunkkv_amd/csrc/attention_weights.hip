@@ -32,6 +32,8 @@ constexpr int kWtFewRows = 16;  // query rows of a KV head up to which scores go
 constexpr int kWtMostParts = 128;  // splits of the cache there
 constexpr int kWtWholeRows = 1024;  // cache rows up to which one workgroup a head does all of it
 constexpr int kWtWholeWaves = 8;
+constexpr int kWtJoinSplits = 16;   // splits of the first pass, and query rows of a part of the second, that the second joins
+constexpr int kWtJoinRows = 512;
 
 // A query row's normaliser and position, as the second pass reads it.
 struct RowStat {
@@ -233,12 +235,22 @@ __global__ __launch_bounds__(256) void weights_join_kernel(const float2* __restr
     stat[at] = row < rows ? RowStat{m + __builtin_amdgcn_logf(l), p64 < 0 ? 0 : p64 >= N ? N - 1 : (int)p64} : RowStat{INFINITY, -1};
 }
 
-// PARTS: part z of the query rows; sums to ws[z], else prior + sum to out.
-template <int D, int KG, bool PARTS>
+// What a second pass that joins the first's splits itself reads (as weights_join_kernel does).
+struct WeightsJoin {
+  const float2* part;
+  int64_t stride;
+  int splits;
+  const int64_t* pos;
+  int rows, group;
+};
+
+// PARTS: part z of the query rows; sums to ws[z], else prior + sum to out. JOIN: at most kWtJoinRows rows a part, whose normalisers
+// every workgroup makes for itself.
+template <int D, int KG, bool PARTS, bool JOIN>
 __global__ __launch_bounds__(kWtThreads, 4) void weights_sum_kernel(
     int nkb, int map_group, int xpk_log, int items, uint32_t inv_group, uint32_t inv_nkb, int N, int stat_rows,
     const char* __restrict__ kc, int64_t k_hs_b, const char* __restrict__ packed, float scale_log2,
-    const RowStat* __restrict__ stat, const float* prior, float* out, int64_t part_stride, int part_tiles) {
+    const RowStat* __restrict__ stat, const float* prior, float* out, int64_t part_stride, int part_tiles, WeightsJoin join) {
   constexpr int DS = D / 32, CPR = D / 8, ROWB = D * 2, KI = kWtTile * CPR / kWtThreads, QT = kWtTile / 16;
   __shared__ __attribute__((aligned(1024))) char lds0[kWtTile * ROWB];
   __shared__ __attribute__((aligned(1024))) char lds1[kWtTile * ROWB];
@@ -252,11 +264,36 @@ __global__ __launch_bounds__(kWtThreads, 4) void weights_sum_kernel(
   const int tile_end = PARTS ? min(tiles, tile_begin + part_tiles) : tiles;
   const int k0 = (kb * (kWtThreads / 64) + wave) * (16 * KG);  // this wavefront's cache rows
 
+  __shared__ RowStat s_stat[JOIN ? kWtJoinRows : 1];
   // does any query row of the part see these cache rows?
   bool any = true;
-  if constexpr (PARTS) {
+  if constexpr (PARTS || JOIN) {
     int seen = -1;
-    for (int r = tile_begin * kWtTile + (int)threadIdx.x; r < tile_end * kWtTile; r += kWtThreads) seen = max(seen, st[r].pos);
+    for (int r = tile_begin * kWtTile + (int)threadIdx.x; r < tile_end * kWtTile; r += kWtThreads) {
+      if constexpr (JOIN) {
+        const float2* pr = join.part + (int64_t)hk * stat_rows + r;
+        const int64_t p64 = join.pos[min(r, join.rows - 1) / join.group];
+        float2 p[kWtJoinSplits];
+#pragma unroll
+        for (int z = 0; z < kWtJoinSplits; ++z) {
+          p[z] = make_float2(-INFINITY, 0.f);
+          if (z < kWtJoinSplits / 2 || join.splits > kWtJoinSplits / 2)  // uniform
+            p[z] = pr[min(z, join.splits - 1) * join.stride];
+        }
+        float m = -INFINITY, l = 0.f;
+#pragma unroll
+        for (int z = 0; z < kWtJoinSplits; ++z) m = fmaxf(m, p[z].x);
+#pragma unroll
+        for (int z = 0; z < kWtJoinSplits; ++z)
+          l += z < join.splits && p[z].x != -INFINITY ? p[z].y * __builtin_amdgcn_exp2f(p[z].x - m) : 0.f;
+        const RowStat own = r < join.rows ? RowStat{m + __builtin_amdgcn_logf(l), p64 < 0 ? 0 : p64 >= N ? N - 1 : (int)p64}
+                                          : RowStat{INFINITY, -1};
+        s_stat[r - tile_begin * kWtTile] = own;
+        seen = max(seen, own.pos);
+      } else {
+        seen = max(seen, st[r].pos);
+      }
+    }
     any = __syncthreads_or(seen >= kb * (kWtThreads / 64) * 16 * KG);
   }
 
@@ -277,7 +314,7 @@ __global__ __launch_bounds__(kWtThreads, 4) void weights_sum_kernel(
 #pragma unroll
       for (int i = 0; i < KI; ++i)
         __builtin_amdgcn_global_load_lds((wt_gvoid*)(qt + (uint32_t)off[i]), (wt_lvoid*)(qb + (wave * KI + i) * 1024), 16, 0, 0);
-      const RowStat* sr = st + (int64_t)tile * kWtTile;
+      const RowStat* sr = JOIN ? s_stat + (tile - tile_begin) * kWtTile : st + (int64_t)tile * kWtTile;
 #pragma unroll
       for (int t = 0; t < QT; ++t) s[t] = sr[(uint32_t)(t * 16 + lm)];
     };
@@ -556,12 +593,14 @@ struct WeightsPlan {
   int rows = 0, stat_rows = 0, row_blocks = 0,  // stat_rows: rows in whole tiles
       splits = 1, split_tiles = 0, key_blocks = 0, parts = 1, part_tiles = 0,
       qg = 2, kg = 2;  // 16-row groups of a wavefront: query rows of the first pass, cache rows of the second
+  bool join = false;  // the second pass joins the first's splits
   int64_t stat_bytes = 0, part_bytes = 0, sum_bytes = 0;
 };
 
 // Splits of the first pass until its workgroups are all that the card holds at once (1024; half as many took 28 us where
 // these take 24); parts of the second until eight times that (its work is the lower triangle: parts that see nothing return at
-// once), of four tiles of query rows at least.
+// once), of four tiles of query rows or a few more (parts of four, 256 rows: 128 queries of 28 / 4 heads over 1103 15.6 us, in parts of
+// five 18.4). Up to 80 tiles no more splits than the second pass joins (30 over 4100 14.3 -> 13.7; over 8302 17.5 -> 18.1).
 static WeightsPlan weights_plan(int n, int N, int Hq, int Hkv, int head_dim) {
   WeightsPlan p;
   p.rows = n * (Hq / Hkv);
@@ -574,10 +613,10 @@ static WeightsPlan weights_plan(int n, int N, int Hq, int Hkv, int head_dim) {
   p.qg = p.rows <= 64 || short_rows ? 1 : 2;
   p.row_blocks = (p.rows + 64 * p.qg - 1) / (64 * p.qg);
   const int64_t lse_blocks = (int64_t)p.row_blocks * Hkv;
-  int64_t splits = std::max<int64_t>(1, std::min<int64_t>({1024 / lse_blocks, tiles / 2, 64}));
+  int64_t splits = std::max<int64_t>(1, std::min<int64_t>({1024 / lse_blocks, tiles / 2, tiles <= 80 ? kWtJoinSplits : 64}));
   p.split_tiles = (int)((tiles + splits - 1) / splits);
   p.splits = (tiles + p.split_tiles - 1) / p.split_tiles;
-  auto parts_of = [&](int64_t blocks) { return std::max<int64_t>(1, std::min<int64_t>(8192 / blocks, row_tiles / 4)); };
+  auto parts_of = [&](int64_t blocks) { return std::max<int64_t>(1, std::min<int64_t>(8192 / blocks, row_tiles < 8 ? 1 : (row_tiles + 3) / 4)); };
   // The same in the second pass, 64 cache rows a workgroup for 128, while two of these a CU do not fill the card: 28 / 4 heads of 128
   // (us, 128 cache rows and 64), 64 queries over 1103 19.1 and 16.5, over 8302 26.9 and 24.3, 251 over 2048 27.7 and 27.8, 128 over 8302
   // 36.4 and 37.3.
@@ -588,6 +627,11 @@ static WeightsPlan weights_plan(int n, int N, int Hq, int Hkv, int head_dim) {
   p.part_tiles = (int)((row_tiles + parts - 1) / parts);
   p.parts = (row_tiles + p.part_tiles - 1) / p.part_tiles;
   p.stat_rows = row_tiles * kWtTile;
+  // A launch less where each workgroup of the second pass finds its rows' normalisers as fast itself, 256 rows at a time, from at
+  // most 16 splits in all: 28 / 4 heads of 128 (us, eager, joined by a launch and so), 17 queries over 1103 12.6 and 11.1, 251
+  // 21.2 and 19.6, 1000 40.1 and 35.1; but 64 over 2048, 448 rows and 16 splits, 15.6 and 17.6.
+  p.join = p.splits > 1 && p.part_tiles * kWtTile <= kWtJoinRows &&
+           p.splits * ((p.part_tiles * kWtTile + kWtThreads - 1) / kWtThreads) <= kWtJoinSplits;
   const int64_t total = (int64_t)Hkv * p.stat_rows;
   p.stat_bytes = (total * (int64_t)sizeof(RowStat) + 15) / 16 * 16;
   p.part_bytes = p.splits > 1 ? (total * 8 * p.splits + 15) / 16 * 16 : 0;
@@ -606,7 +650,8 @@ extern "C" int64_t ckv_attention_weights_workspace_bytes(int32_t n_queries, int3
   if (n_queries * (n_q_heads / n_kv_heads) <= kWtFewRows && n_tokens <= kWtWholeRows) return 0;
   if (n_queries * (n_q_heads / n_kv_heads) <= kWtFewRows) return few_plan(n_queries * (n_q_heads / n_kv_heads), n_tokens, n_kv_heads).bytes;
   const WeightsPlan p = weights_plan(n_queries, n_tokens, n_q_heads, n_kv_heads, head_dim);
-  return p.stat_bytes + (int64_t)n_kv_heads * p.stat_rows * head_dim * 2 + std::max(p.part_bytes, p.sum_bytes);
+  return p.stat_bytes + (int64_t)n_kv_heads * p.stat_rows * head_dim * 2 +
+         (p.join ? p.part_bytes + p.sum_bytes : std::max(p.part_bytes, p.sum_bytes));
 }
 
 extern "C" int32_t ckv_attention_weights(float* out, const float* prior, const void* q, int64_t q_head_stride,
@@ -668,6 +713,7 @@ extern "C" int32_t ckv_attention_weights(float* out, const float* prior, const v
   RowStat* stat = (RowStat*)workspace;
   char* packed = (char*)workspace + p.stat_bytes;
   float* scratch = (float*)(packed + (int64_t)n_kv_heads * p.stat_rows * head_dim * 2);  // the splits' rows, then the parts' sums
+  float* sums = scratch + (p.join ? p.part_bytes / 4 : 0);  // the joined splits are read while the sums are written
   const int64_t rows_total = (int64_t)n_kv_heads * p.stat_rows;
   {
     const AttnMap m = attn_map(p.row_blocks, n_kv_heads, 1, p.splits);
@@ -685,7 +731,7 @@ extern "C" int32_t ckv_attention_weights(float* out, const float* prior, const v
     else p.qg == 1 ? form(Int<64>{}, Int<1>{}) : form(Int<64>{}, Int<2>{});
     CKV_RETURN_IF_LAUNCH_FAILED();
   }
-  if (p.splits > 1) {
+  if (p.splits > 1 && !p.join) {
     hipLaunchKernelGGL(weights_join_kernel, dim3((unsigned)((rows_total + 3) / 4)), dim3(256), 0, s, (const float2*)scratch,
                        rows_total, p.splits, positions, n_tokens, p.rows, group, stat, p.stat_rows, rows_total);
     CKV_RETURN_IF_LAUNCH_FAILED();
@@ -696,18 +742,20 @@ extern "C" int32_t ckv_attention_weights(float* out, const float* prior, const v
       hipLaunchKernelGGL(kernel, dim3(m.blocks), dim3(kWtThreads), 0, s, m.nqb, m.group, m.xpk_log, m.items, m.inv_group,
                          m.inv_nqb, n_tokens, p.stat_rows, (const char*)k_cache, k_head_stride * 2, (const char*)packed, scale_log2,
                          (const RowStat*)stat, prior,
-                         p.parts > 1 ? scratch : out, total, p.part_tiles);
+                         p.parts > 1 ? sums : out, total, p.part_tiles,
+                         WeightsJoin{(const float2*)scratch, rows_total, p.splits, positions, p.rows, group});
     };
     auto form = [&](auto dim, auto kg) {
       constexpr int D = decltype(dim)::value, KG = decltype(kg)::value;
-      p.parts > 1 ? launch(weights_sum_kernel<D, KG, true>) : launch(weights_sum_kernel<D, KG, false>);
+      if (p.join) p.parts > 1 ? launch(weights_sum_kernel<D, KG, true, true>) : launch(weights_sum_kernel<D, KG, false, true>);
+      else p.parts > 1 ? launch(weights_sum_kernel<D, KG, true, false>) : launch(weights_sum_kernel<D, KG, false, false>);
     };
     if (head_dim == 128) p.kg == 1 ? form(Int<128>{}, Int<1>{}) : form(Int<128>{}, Int<2>{});
     else p.kg == 1 ? form(Int<64>{}, Int<1>{}) : form(Int<64>{}, Int<2>{});
     CKV_RETURN_IF_LAUNCH_FAILED();
   }
   if (p.parts > 1) {
-    hipLaunchKernelGGL(weights_reduce_kernel, dim3(total_blocks), dim3(256), 0, s, (const float*)scratch, total, p.parts, prior, out, total);
+    hipLaunchKernelGGL(weights_reduce_kernel, dim3(total_blocks), dim3(256), 0, s, sums, total, p.parts, prior, out, total);
     CKV_RETURN_IF_LAUNCH_FAILED();
   }
   return CKV_OK;

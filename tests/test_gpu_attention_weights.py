@@ -47,6 +47,14 @@ def _check(q, K, pos, prior=None, scale=None, out=None):
         (16, 1, 64, 1024, 1),
         (17, 1, 64, 1024, 1),  # 17 rows
         (4, 4, 64, 1023, 16),
+        (28, 4, 128, 2050, 18),  # 64 rows a workgroup, a split joined by the second pass
+        (28, 4, 128, 1103, 128),  # in parts too
+        (28, 4, 128, 2050, 64),  # 448 rows and 16 splits: joined by a launch
+        (28, 4, 128, 5185, 3),
+        (14, 2, 64, 16500, 300),  # 128 rows a workgroup in the first pass, and in both
+        (14, 2, 64, 40000, 90),
+        (16, 16, 64, 650, 250),
+        (1, 1, 128, 300, 257),
     ],
 )
 def test_weights_match_the_plain_form(Hq, Hkv, D, N, n):
