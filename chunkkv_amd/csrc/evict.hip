@@ -65,7 +65,7 @@ __global__ __launch_bounds__(kEvictThreads) void evict_kernel(const float* __res
   __shared__ uint32_t wave_tot[3][kEvictWaves];
   __shared__ uint32_t wave_gt[kEvictWaves], wave_eq[kEvictWaves];
   __shared__ uint32_t step_count[kEvictWaves][PER > 0 ? PER : 1];
-  __shared__ uint32_t found[3][2];
+  __shared__ uint32_t found[3][3];  // the bin, the kept keys in it, its keys
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / kWave), lane = tid % kWave;
   const int h = blockIdx.y;
   const float* w = weights + (int64_t)h * w_hs;
@@ -134,6 +134,7 @@ __global__ __launch_bounds__(kEvictThreads) void evict_kernel(const float* __res
   __syncthreads();
 
   uint32_t need = (uint32_t)n_keep, prefix = 0;  // kept among the keys that start with the bits found
+  bool whole = false;                             // all of them are: the bits behind need not be known
   auto pass = [&](int p, int bits, uint32_t a, uint32_t b) {
     // the bin, from the top, in which the need-th key lies: two bins (a, then b) a thread
     const int top = (1 << bits) - 1 - 2 * tid;
@@ -146,13 +147,20 @@ __global__ __launch_bounds__(kEvictThreads) void evict_kernel(const float* __res
     if (before < need && need <= before + a) {
       found[p][0] = (uint32_t)top;
       found[p][1] = need - before;
+      found[p][2] = a;
     } else if (before + a < need && need <= before + a + b) {
       found[p][0] = (uint32_t)(top - 1);
       found[p][1] = need - before - a;
+      found[p][2] = b;
     }
     __syncthreads();
     prefix = (prefix << bits) | (uint32_t)__builtin_amdgcn_readfirstlane((int)found[p][0]);
     need = (uint32_t)__builtin_amdgcn_readfirstlane((int)found[p][1]);
+    whole = need == (uint32_t)__builtin_amdgcn_readfirstlane((int)found[p][2]) && prefix != 0;  // (0: among keys of no row)
+    if (whole && p < 2) {  // then the keys above the bin's last predecessor stay, and none of that
+      prefix = (prefix << (p == 0 ? 21 : 10)) - 1u;
+      need = 0;
+    }
   };
   {
     uint32_t* mine = hist0 + (lane % kEvictCopies) * kEvictPitch;
@@ -172,7 +180,7 @@ __global__ __launch_bounds__(kEvictThreads) void evict_kernel(const float* __res
     pass(0, 11, a, b);
   }
 #pragma unroll 1
-  for (int p = 1; p < 3; ++p) {
+  for (int p = 1; p < 3 && !whole; ++p) {
     const int bits = p == 1 ? 11 : 10, shift = p == 1 ? 21 : 10, next = p == 1 ? 10 : 0;
     const uint32_t low = prefix << shift, span = 1u << shift;
     uint32_t* bins = hist0 + (p - 1) * kEvictPitch;
