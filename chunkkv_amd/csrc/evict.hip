@@ -10,9 +10,11 @@
 // find the same threshold, each for a slice of the kept rows that it then copies: the selection is the latency of
 // one CU whatever is done, and this way no launch waits for it. Longer caches: one workgroup a head reads the weights
 // again for each pass, and evict_gather_kernel copies.
-// Bound: the issue of the CU that selects: 32832 rows of 4 heads of 128 cut to 4104 take 20 us, by phase, us: loads 3, first pass 4,
-// the other two 4, count 2, list and copy 2, launch; 1103 fp32 rows of 2 heads of 64 cut to 300 take 7.7, mostly the passes'
-// scans and barriers. One workgroup a head with a copy launch behind it took 46 and 11.4.
+// The first histogram counts a row as it arrives (32832 rows of 4 heads of 128 cut to 4104 20.1 -> 19.1 us), and a bin that stays whole
+// needs no further pass (20.9 -> 20.1; 60000 to 4000, where each pass reads the weights again, 52 -> 49).
+// Bound: the issue of the CU that selects. Those 19 us by phase, about: rows and first pass 6, the other two 3, count 2, list and
+// copy 2, the rest start and launch; 1103 fp32 rows of 2 heads of 64 cut to 300 take 7.5-7.8, mostly the passes' scans and barriers.
+// One workgroup a head with a copy launch behind it took 46 and 11.4.
 #include <algorithm>
 
 #include "ckv_common.hpp"
@@ -95,12 +97,21 @@ __global__ __launch_bounds__(kEvictThreads) void evict_kernel(const float* __res
       }
     }
   };
-  for (int b = tid; b < kEvictCopies * kEvictPitch; b += kEvictThreads) hist0[b] = 0;
+  uint32_t* mine = hist0 + (lane % kEvictCopies) * kEvictPitch;
+  auto count4 = [&](const uint32_t(&k)[4]) {  // the first pass; key 0 counts below every row's
+#pragma unroll
+    for (int j = 0; j < 4; ++j) atomicAdd(&mine[k[j] >> 21], 1u);
+  };
+  auto clear = [&] {
+    for (int b = tid; b < kEvictCopies * kEvictPitch; b += kEvictThreads) hist0[b] = 0;
+    lds_barrier();  // loads stay in flight
+  };
   if constexpr (PER > 0) {
     float x[PER][4];
 #pragma unroll
     for (int i = 0; i < PER; ++i)
       if (i < steps) load4(i, x[i]);
+    clear();
 #pragma unroll
     for (int i = 0; i < PER; ++i)
       if (i < steps) {
@@ -108,7 +119,10 @@ __global__ __launch_bounds__(kEvictThreads) void evict_kernel(const float* __res
         keys4(i, x[i], k);
         const int at = (wave * run_steps + i) * STEP + 4 * lane;  // only this wavefront reads them
         *(vec16*)(keys + at) = vec16{k[0], k[1], k[2], k[3]};
+        count4(k);
       }
+  } else {
+    clear();
   }
   // f(step, keys) for each of this thread's steps (key 0: no row)
   auto each = [&](auto f) {
@@ -131,7 +145,6 @@ __global__ __launch_bounds__(kEvictThreads) void evict_kernel(const float* __res
       }
     }
   };
-  __syncthreads();
 
   uint32_t need = (uint32_t)n_keep, prefix = 0;  // kept among the keys that start with the bits found
   bool whole = false;                             // all of them are: the bits behind need not be known
@@ -163,11 +176,7 @@ __global__ __launch_bounds__(kEvictThreads) void evict_kernel(const float* __res
     }
   };
   {
-    uint32_t* mine = hist0 + (lane % kEvictCopies) * kEvictPitch;
-    each([&](int, const uint32_t(&k)[4]) {
-#pragma unroll
-      for (int j = 0; j < 4; ++j) atomicAdd(&mine[k[j] >> 21], 1u);  // key 0 counts below every row's
-    });
+    if constexpr (PER == 0) each([&](int, const uint32_t(&k)[4]) { count4(k); });
     __syncthreads();
     const int top = kEvictBins - 1 - 2 * tid;
     uint32_t a = 0, b = 0;
