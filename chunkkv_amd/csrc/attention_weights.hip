@@ -7,7 +7,7 @@
 // and sum before it can be formed, so the product with K^T runs twice:
 //  1. weights_lse_kernel: 128 rows a workgroup (64 in small launches, as in the second pass) walk the cache in 64-row tiles (attention.hip's first half, with the
 //     maximum and the sum kept per lane); with few row blocks, in splits of the cache. Leaves L = max + log2(sum) and the
-//     position of each row (weights_join_kernel joins the splits).
+//     position of each row (weights_join_kernel joins the splits, or, of few, each workgroup of the second pass for its rows).
 //  2. weights_sum_kernel: 128 cache rows a workgroup hold their operands in registers while the query rows (packed by the
 //     first pass: a tile's loads then need no addresses) pass through LDS: S = K Q^T gives a lane four cache rows of one query row, and 2^(s scale - L) adds up in
 //     registers over all query rows; the 16 lanes of a cache row meet once, at the end. With few cache blocks the
@@ -18,7 +18,7 @@
 // an addition (the first pass: half a maximum too); alone these take 16.3 and 17.0 cycles for four scores a lane, both
 // together 28.3, whichever way the two are interleaved (within a wavefront, across wavefronts, by priority), so they
 // hardly overlap. Measured (us, kernels traced, 28 / 4 heads of 128): 8256 causal rows 251 + 258 + 4, of which 175 each is that
-// issue at 2.4 GHz and the clock was near 2.0; 64 rows over 32832 24 + 20 and 4 for the join; one row over 8257 4.6 + 4.4.
+// issue at 2.4 GHz and the clock was near 2.0; 64 rows over 32832 21 + 20 and 4 for the join; one row over 8257 4.6 + 4.4.
 // Slower: 64 rows a wavefront (275 and 320 us: two wavefronts a SIMD), exponentials one step behind the products (266, 283).
 #include <algorithm>
 
