@@ -669,6 +669,10 @@ extern "C" int32_t ckv_attention_weights(float* out, const float* prior, const v
   hipStream_t s = (hipStream_t)stream;
   const int64_t total = (int64_t)n_kv_heads * n_tokens;
   const unsigned total_blocks = (unsigned)((total + 255) / 256);
+  if (prior != nullptr && prior != out) {  // one buffer or two: a workgroup's sums would meet another's prior
+    const intptr_t apart = (intptr_t)prior - (intptr_t)out;
+    if ((apart < 0 ? -apart : apart) < total * 4) return CKV_ERR_INVALID_ARGUMENT;
+  }
   if (n_queries == 0) {  // no query: prior, or zeros
     if (prior == out) return CKV_OK;
     hipLaunchKernelGGL(weights_reduce_kernel, dim3(total_blocks), dim3(256), 0, s, (const float*)nullptr, (int64_t)0, 0, prior, out, total);

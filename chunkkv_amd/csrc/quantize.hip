@@ -167,7 +167,7 @@ extern "C" int32_t ckv_quantize_rows(void* k_codes, void* v_codes, void* k_scale
   const int blocks = (int)(((int64_t)n_tokens + block_tokens - 1) >> log);
   // blocks that n_rows rows touch: from a known start, or at most
   const int64_t grid = start_dev == nullptr ? ((start + n_rows - 1) >> log) - (start >> log) + 1
-                                            : std::min<int64_t>((n_rows + block_tokens - 2) / block_tokens + 1, blocks);
+                                            : std::min<int64_t>(((int64_t)n_rows + block_tokens - 2) / block_tokens + 1, blocks);
   const int eb = dtype == CKV_DTYPE_BF16 ? 2 : 4;
   const QuantTensor kt = {(char*)k_codes, (uint8_t*)k_scales, (const char*)k, k_head_stride * eb, k_token_stride * eb};
   const QuantTensor vt = {(char*)v_codes, (uint8_t*)v_scales, (const char*)v, v_head_stride * eb, v_token_stride * eb};

@@ -714,7 +714,7 @@ def attention_weights(
 
     q: (1, Hq, n, D) bf16 with contiguous rows; K: (1, Hkv, N, D) bf16, a head's rows contiguous (e.g. a [:, :, :N] view of
     a longer cache), rows past the largest position anything, rows up to it finite. prior and out: float32 (1, Hkv, N) contiguous, and may be
-    one tensor (weights that grow over decode steps). Sums are fp32 in a fixed order.
+    one tensor (weights that grow over decode steps), else apart. Sums are fp32 in a fixed order.
     """
     return _native.torch_ops().attention_weights(q, K, positions, scale, prior, out, err)
 

@@ -601,7 +601,7 @@ int64_t ckv_attention_quantized_workspace_bytes(int32_t n_queries, int32_t n_tok
  * The attention weight that each cached row received, over all query rows and the query heads of its KV head:
  *   out[hk, j] = prior[hk, j] + sum over i and over h in group hk of w[h, i, j],
  *   w[h, i, :] = softmax over j in [0, positions[i]] of scale * q[h, i, :] . K[hk, j, :]   (0 past it).
- * prior (NULL: zeros) and out are (n_kv_heads, n_tokens) fp32 contiguous and may be the same. q, k_cache, positions,
+ * prior (NULL: zeros) and out are (n_kv_heads, n_tokens) fp32 contiguous, the same or apart. q, k_cache, positions,
  * scale and err as in ckv_attention_active (bf16, head_dim 64 or 128, k_head_stride at least n_tokens * head_dim);
  * rows past the largest position may hold anything, rows up to it are finite. Scores, weights and sums are fp32, added in a fixed order.
  *   workspace  device buffer of workspace_bytes >= ckv_attention_weights_workspace_bytes(...), 16-byte aligned

@@ -50,7 +50,8 @@ EVICT = [("ko", 16), ("ko_hs", 640), ("vo", 16), ("vo_hs", 640), ("rows", 16), (
         (dict(out=None), INVALID), (dict(q=None), INVALID), (dict(k=None), INVALID), (dict(pos=None), INVALID), (dict(k=8), INVALID),
         (dict(dtype=0), INVALID), (dict(D=256), INVALID), (dict(Hq=3), INVALID), (dict(N=0), INVALID), (dict(n=-1), INVALID),
         (dict(scale=-1.0), INVALID), (dict(q_hs=68), INVALID), (dict(q_ts=56), RANGE), (dict(k_hs=6392), RANGE), (dict(ws=None, n=40), INVALID),
-        (dict(wsb=16, n=40), INVALID), (dict(ws=8, n=40), INVALID), (dict(n=1 << 30), LARGE), (dict(n=0, q=None, k=None, pos=None, prior=16), OK)]),
+        (dict(wsb=16, n=40), INVALID), (dict(ws=8, n=40), INVALID), (dict(n=1 << 30), LARGE),
+        (dict(out=4096, prior=4096 + 796), INVALID), (dict(out=4096, prior=4096 - 4), INVALID), (dict(out=4096, prior=4100, n=0), INVALID), (dict(n=0, q=None, k=None, pos=None, prior=16), OK)]),
     ("ckv_evict_rows", EVICT, [
         (dict(ko=None), INVALID), (dict(rows=None), INVALID), (dict(w=None), INVALID), (dict(vo=8), INVALID), (dict(k=8), INVALID),
         (dict(ko_hs=644), INVALID), (dict(D=96), INVALID), (dict(dtype=2), INVALID), (dict(N=0), INVALID), (dict(sink=-1), INVALID),

@@ -155,6 +155,9 @@ def test_refusals():
                      ((_randn((1, 4, 2, 96), 1), _randn((1, 2, 100, 96), 2), pos), {})):
         with pytest.raises(ValueError):
             ops.attention_weights(*args, **kw)
+    buf = f(201)  # out moved by one row against prior
+    with pytest.raises(ValueError):
+        ops.attention_weights(q, K, pos, prior=buf[:200].view(1, 2, 100), out=buf[1:].view(1, 2, 100))
     with pytest.raises(TypeError):
         ops.attention_weights(q.float(), K, pos)
     with pytest.raises(TypeError):
