@@ -1,7 +1,7 @@
 // The attention weight that each cached row received, summed over query rows and the query heads of its KV head:
 //   out[hk, j] = prior[hk, j] + sum over i, h in group hk of softmax_j(scale * q[h, i] . K[hk, j]),  j <= pos[i],
 // what a cache's rows are ranked by before the light ones are dropped (evict.hip). Neither the scores nor the
-// weights go to memory (but for one token's scores, below).
+// weights go to memory (but for one token's scores, below). Short caches have a kernel of their own (weights_short_kernel).
 //
 // Design: the n x group (token, query head) pairs of a KV head are its rows. A weight needs its row's maximum
 // and sum before it can be formed, so the product with K^T runs twice:
@@ -32,6 +32,7 @@ constexpr int kWtFewRows = 16;  // query rows of a KV head up to which scores go
 constexpr int kWtMostParts = 128;  // splits of the cache there
 constexpr int kWtWholeRows = 1024;  // cache rows up to which one workgroup a head does all of it
 constexpr int kWtWholeWaves = 8;
+constexpr int kWtShortWaves = 8;
 constexpr int kWtJoinSplits = 16;   // splits of the first pass, and query rows of a part of the second, that the second joins
 constexpr int kWtJoinRows = 512;
 
@@ -568,6 +569,115 @@ __global__ __launch_bounds__(kWtThreads) void weights_from_scores_kernel(
   out[(int64_t)hk * N + j] = before + sum;
 }
 
+// ---- short caches -----------------------------------------------------------------------------------------
+// Up to 16 T cache rows one workgroup a KV head is the whole call: K in LDS, a wavefront 16 query rows at a time with all their
+// scores in registers (lane (g, lm): row lm, cache rows 16 t + 4 g + e), so a weight is formed from the exponential that its row's sum
+// took, and adds up in place over the wavefront's rows; lanes and wavefronts meet once, at the end.
+template <int D, int T>
+__global__ __launch_bounds__(kWtShortWaves * 64) void weights_short_kernel(
+    const int64_t* __restrict__ pos, int N, int rows, int group, uint32_t inv_gqa, const char* __restrict__ kc, int64_t k_hs_b,
+    const char* __restrict__ q, int64_t q_hs_b, int64_t q_ts_b, float scale_log2, const float* prior, float* out,
+    int32_t* __restrict__ err) {
+  constexpr int W = kWtShortWaves, DS = D / 32, CPR = D / 8, ROWB = D * 2, LI = T * 16 * CPR / (W * 64);
+  static_assert(LI >= 1 && T * 16 * CPR % (W * 64) == 0 && T % 4 == 0, "whole loads");
+  __shared__ __attribute__((aligned(1024))) char lds[T * 16 * ROWB];
+  __shared__ float s_part[W][T * 16];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x % 64;
+  const int g = lane / 16, lm = lane % 16, hk = blockIdx.x;
+  const char* kh = kc + (int64_t)hk * k_hs_b;
+#pragma unroll
+  for (int i = 0; i < LI; ++i) {
+    const int P = (wave * LI + i) * 64 + lane, slot = P / CPR;
+    const uint32_t off = (uint32_t)(min(slot, N - 1) * ROWB + ((P % CPR) ^ swz_k<CPR>(slot)) * 16);
+    __builtin_amdgcn_global_load_lds((wt_gvoid*)(kh + off), (wt_lvoid*)(lds + (wave * LI + i) * 1024), 16, 0, 0);
+  }
+  bf16x8 qf[DS];
+  int my_pos;
+  auto load_rows = [&](int r0) {
+    const int r = r0 + lm, rc = min(r, rows - 1), t = div_by(rc, group, inv_gqa), gh = rc - t * group;
+    const char* qr = q + (int64_t)(hk * group + gh) * q_hs_b + (int64_t)t * q_ts_b;
+#pragma unroll
+    for (int ds = 0; ds < DS; ++ds) qf[ds] = __builtin_bit_cast(bf16x8, ld16(qr + (32 * ds + 8 * g) * 2));
+    const int64_t p64 = pos[t];
+    const int p = p64 < 0 ? 0 : p64 >= N ? N - 1 : (int)p64;
+    if (r < rows && p != p64) flag_error(err, CKV_DEVICE_ERR_RANGE);
+    my_pos = r < rows ? p : -1;
+  };
+  load_rows(wave * 16);
+  int k_rd[DS];
+#pragma unroll
+  for (int ds = 0; ds < DS; ++ds) k_rd[ds] = lm * ROWB + (((4 * ds + g) ^ swz_k<CPR>(lm)) * 16);
+  f32x4 acc[T];
+#pragma unroll
+  for (int t = 0; t < T; ++t) acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+  __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): this wavefront's part of K landed
+  __syncthreads();
+  for (int r0 = wave * 16; r0 < rows; r0 += W * 16) {
+    f32x4 s[T];
+    float m = -INFINITY;
+#pragma unroll
+    for (int u = 0; u < T; u += 4) {
+      if (16 * u >= N) continue;  // uniform
+#pragma unroll
+      for (int ds = 0; ds < DS; ++ds)  // dependent products four apart
+#pragma unroll
+        for (int t = u; t < u + 4; ++t)
+          s[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(*(const bf16x8*)(lds + t * 16 * ROWB + k_rd[ds]), qf[ds],
+                                                         ds == 0 ? f32x4{0.f, 0.f, 0.f, 0.f} : s[t], 0, 0, 0);
+#pragma unroll
+      for (int t = u; t < u + 4; ++t)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          if (16 * t + 4 * g + e > my_pos) s[t][e] = -INFINITY;
+          m = fmaxf(m, s[t][e]);
+        }
+    }
+    if (r0 + W * 16 < rows) load_rows(r0 + W * 16);
+    m = group_max(m) * scale_log2;  // > 0: max commutes
+    const float sub = m == -INFINITY ? 0.f : m;  // no such row
+    float l = 0.f;
+#pragma unroll
+    for (int u = 0; u < T; u += 4) {
+      if (16 * u >= N) continue;
+#pragma unroll
+      for (int t = u; t < u + 4; ++t)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          s[t][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][e], scale_log2, -sub));
+          l += s[t][e];
+        }
+    }
+    l += __shfl_xor(l, 16);
+    l += __shfl_xor(l, 32);
+    const float inv = l > 0.f ? 1.f / l : 0.f;
+#pragma unroll
+    for (int u = 0; u < T; u += 4) {
+      if (16 * u >= N) continue;
+#pragma unroll
+      for (int t = u; t < u + 4; ++t)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[t][e] = __builtin_fmaf(s[t][e], inv, acc[t][e]);
+    }
+  }
+#pragma unroll
+  for (int t = 0; t < T; ++t) {
+    if (16 * t >= N) continue;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float sum = row16_reduce(acc[t][e], [](float a, float b) { return a + b; });
+      if (lm == 0) s_part[wave][16 * t + 4 * g + e] = sum;
+    }
+  }
+  __syncthreads();
+  for (int j = threadIdx.x; j < N; j += W * 64) {
+    float total = 0.f;
+#pragma unroll
+    for (int w = 0; w < W; ++w) total += s_part[w][j];
+    const int64_t at = (int64_t)hk * N + j;
+    out[at] = prior != nullptr ? prior[at] + total : total;
+  }
+}
+
 struct FewPlan {
   int rows, chunks, splits, split_chunks;
   int64_t score_stride, score_bytes, bytes;
@@ -588,6 +698,12 @@ static FewPlan few_plan(int rows, int N, int Hkv) {
 
 template <int I>
 using Int = std::integral_constant<int, I>;
+
+// Whether a launch of more than kWtFewRows rows takes weights_short_kernel: while its chain, 128 rows at a time over 64 cache rows, is
+// shorter than two launches. us (eager, two launches or three and one), 28 / 4 heads of 128: 17 queries over 64 8.4 and 4.8, 64 over 64
+// 11.0 and 7.4, 50 over 128 11.0 and 10.1, 91 over 128 12.4 and 14.2, 17 over 256 10.0 and 8.8, 30 over 256 11.2 and 12.1; 14 / 2 of 64,
+// 30 over 190 8.6 and 8.3, 50 over 190 9.5 and 10.4.
+static bool short_cache(int rows, int N) { return N <= 256 && (int64_t)rows * ((N + 63) / 64 * 64) <= 50000; }
 
 struct WeightsPlan {
   int rows = 0, stat_rows = 0, row_blocks = 0,  // stat_rows: rows in whole tiles
@@ -649,6 +765,7 @@ extern "C" int64_t ckv_attention_weights_workspace_bytes(int32_t n_queries, int3
     return 0;
   if (n_queries * (n_q_heads / n_kv_heads) <= kWtFewRows && n_tokens <= kWtWholeRows) return 0;
   if (n_queries * (n_q_heads / n_kv_heads) <= kWtFewRows) return few_plan(n_queries * (n_q_heads / n_kv_heads), n_tokens, n_kv_heads).bytes;
+  if (short_cache(n_queries * (n_q_heads / n_kv_heads), n_tokens)) return 0;
   const WeightsPlan p = weights_plan(n_queries, n_tokens, n_q_heads, n_kv_heads, head_dim);
   return p.stat_bytes + (int64_t)n_kv_heads * p.stat_rows * head_dim * 2 +
          (p.join ? p.part_bytes + p.sum_bytes : std::max(p.part_bytes, p.sum_bytes));
@@ -709,6 +826,18 @@ extern "C" int32_t ckv_attention_weights(float* out, const float* prior, const v
     hipLaunchKernelGGL(weights_from_scores_kernel, dim3((unsigned)((n_tokens + kWtThreads - 1) / kWtThreads), (unsigned)n_kv_heads),
                        dim3(kWtThreads), 0, s, positions, n_tokens, p.rows, group, (const float*)scores, p.score_stride,
                        (const float2*)part, p.splits, prior, out);
+    CKV_RETURN_IF_LAUNCH_FAILED();
+    return CKV_OK;
+  }
+  if (short_cache(n_queries * group, n_tokens)) {
+    const int rows = n_queries * group;
+    auto launch = [&](auto kernel) {
+      hipLaunchKernelGGL(kernel, dim3((unsigned)n_kv_heads), dim3(kWtShortWaves * 64), 0, s, positions, n_tokens, rows, group,
+                         inverse_of(rows, group), (const char*)k_cache, k_head_stride * 2, (const char*)q, q_head_stride * 2,
+                         q_token_stride * 2, scale_log2, prior, out, err);
+    };
+    if (head_dim == 128) n_tokens <= 64 ? launch(weights_short_kernel<128, 4>) : launch(weights_short_kernel<128, 16>);
+    else n_tokens <= 64 ? launch(weights_short_kernel<64, 4>) : launch(weights_short_kernel<64, 16>);
     CKV_RETURN_IF_LAUNCH_FAILED();
     return CKV_OK;
   }

@@ -77,14 +77,16 @@ def attention(q, K, V, pos, scale):
 
 def weights(q, K, pos, scale, prior=None):
     """(1, Hkv, N) weights and the most each may be off: a weight by its scores' and normaliser's error, the sum over R rows
-    by a chain of R / 16 + 68 additions (16 lanes a row of the cache, 64 parts, the lanes' tree)."""
+    by a chain of R / 16 + 68 additions (16 lanes a row of the cache, 64 parts, the lanes' tree). An exponential below 2^-126
+    is 0 on the device, whichever way its weight is normalised: each of the R weights may be off by that (R of 100 rows, sum
+    3.9e-38: 1.61 * 2^-126)."""
     p, e_s = softmax_rows(q, K, pos, scale)
     H, group = K.shape[1], len(p) // K.shape[1]
     got = torch.stack([sum(p[h].sum(0) for h in range(k * group, (k + 1) * group)) for k in range(H)])[None]
     rows = group * pos.numel()
     per = 4 * e_s + (K.shape[2] / 64 + 80) * F32_STEP + (rows / 16 + 68) * F32_STEP
     base = torch.zeros_like(got) if prior is None else prior.double().cpu()
-    return base + got, per * got + 2 * F32_STEP * (base.abs() + got) + 2.0 ** -126
+    return base + got, per * got + 2 * F32_STEP * (base.abs() + got) + rows * 2.0 ** -126
 
 
 def kept_rows(w: np.ndarray, keep: int, sink: int, recent: int) -> list[int]:

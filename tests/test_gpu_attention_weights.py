@@ -47,6 +47,13 @@ def _check(q, K, pos, prior=None, scale=None, out=None):
         (16, 1, 64, 1024, 1),
         (17, 1, 64, 1024, 1),  # 17 rows
         (4, 4, 64, 1023, 16),
+        (28, 4, 128, 64, 64),  # a short cache: one launch
+        (28, 4, 128, 256, 27),
+        (28, 4, 128, 256, 28),  # and three
+        (14, 2, 64, 257, 3),
+        (14, 2, 64, 33, 33),
+        (16, 16, 64, 193, 190),
+        (40, 2, 128, 2, 2),
         (28, 4, 128, 2050, 18),  # 64 rows a workgroup, a split joined by the second pass
         (28, 4, 128, 1103, 128),  # in parts too
         (28, 4, 128, 2050, 64),  # 448 rows and 16 splits: joined by a launch
@@ -80,10 +87,32 @@ def test_rows_behind_the_positions_and_views_of_longer_caches():
     _check(_randn((1, 14, 8, 64), 4), slab[:, :, :400], pos)
 
 
+@pytest.mark.parametrize("Hq,Hkv,D,N,last,n", [(28, 4, 128, 200, 130, 12), (14, 2, 64, 60, 0, 40), (28, 4, 128, 1103, 700, 128),
+                                               (14, 2, 64, 9000, 8200, 100), (28, 4, 128, 4100, 65, 40), (28, 4, 128, 900, 777, 1)])
+def test_rows_behind_the_positions_in_every_form(Hq, Hkv, D, N, last, n):
+    K = _randn((1, Hkv, N, D), 3)
+    K[:, :, last + 1 :] = float("nan")
+    pos = torch.randint(0, last + 1, (n,), generator=torch.Generator().manual_seed(N))
+    pos[n // 2] = last
+    _check(_randn((1, Hq, n, D), 4), K, pos, torch.rand((1, Hkv, N), device=DEV))
+
+
+@pytest.mark.parametrize("Hq,Hkv,D,N,n", [(28, 4, 128, 100, 20), (14, 2, 64, 600, 300), (28, 4, 128, 5000, 40)])
+def test_positions_outside_in_every_form(Hq, Hkv, D, N, n):
+    q, K, err = _randn((1, Hq, n, D), 1), _randn((1, Hkv, N, D), 2), torch.zeros(1, dtype=torch.int32, device=DEV)
+    pos = torch.randint(0, N, (n,), generator=torch.Generator().manual_seed(n)).to(DEV)
+    wild = pos.clone()
+    pos[0], pos[n - 1], wild[0], wild[n - 1] = 0, N - 1, -(2**40), N
+    got = ops.attention_weights(q, K, wild, err=err)
+    assert int(err) == 1
+    assert torch.equal(got, ops.attention_weights(q, K, pos))
+
+
 def test_rows_of_very_different_scores():
     """Scores from -600 to 600: sums that start far below a later maximum, weights that vanish."""
     K = _randn((1, 2, 777, 64), 5, 30.0)
     _check(_randn((1, 4, 50, 64), 6, 4.0), K, torch.arange(727, 777))
+    _check(_randn((1, 4, 50, 64), 6, 4.0), K[:, :, :200], torch.arange(150, 200))
     _check(_randn((1, 4, 1, 64), 6, 0.0), K, torch.tensor([776]))  # all scores 0: 1 / 777 each
 
 
