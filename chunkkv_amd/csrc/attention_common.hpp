@@ -14,6 +14,10 @@ struct CacheScales {
   const uint8_t* v;
   int blocks, chunk_log;
 };
+// The same for a launch whose query rows are the (token, query head) pairs of a KV head; inv_gqa: for div_by of its heads.
+struct GroupedCacheScales : CacheScales {
+  uint32_t inv_gqa;
+};
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));

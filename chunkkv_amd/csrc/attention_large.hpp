@@ -17,7 +17,7 @@ __global__ __launch_bounds__(kAttnWaves * 64) void attn_active_kernel(
     const int64_t* __restrict__ pos, int n, int N, const char* __restrict__ kc, const char* __restrict__ vc,
     int64_t kv_hs_b, const char* __restrict__ q, int64_t q_hs_b, int64_t q_ts_b, int Hq, int group, float scale_log2,
     char* __restrict__ out, int32_t* __restrict__ err, float* __restrict__ ws, int split_tiles, Scales... scales) {
-  constexpr bool CODES = sizeof...(Scales) == 1;
+  constexpr bool CODES = sizeof...(Scales) == 1, GROUPED = (std::is_same_v<Scales, GroupedCacheScales> || ...);
   constexpr int DS = D / 32;          // k-steps of S^T = K Q^T
   constexpr int DT = D / 16;          // 16-row tiles of O^T
   constexpr int CPR = D / 8;          // 16-byte chunks per cache row
@@ -38,7 +38,13 @@ __global__ __launch_bounds__(kAttnWaves * 64) void attn_active_kernel(
   const int g = lane / 16, lm = lane % 16;
   int qb, hq, z;
   if (!attn_work_item(nqb, map_group, xpk_log, items, inv_group, inv_nqb, qb, hq, z)) return;
-  const int hk = hq / group;
+  const int hk = GROUPED ? hq : hq / group;
+  const int rows = GROUPED ? n * group : n;
+  auto token_of = [&](int m) {  // of row m
+    if constexpr (GROUPED) return div_by(m, group, (scales.inv_gqa, ...));
+    else return m;
+  };
+  auto head_of = [&](int m, int t) { return GROUPED ? hk * group + m - t * group : hq; };
   const int q0 = qb * kAttnBM + wave * kAttnQG * 16;
   // Positions of this lane's queries (-1 = no query); out-of-range positions are flagged and
   // clamped so that every read stays inside the cache.
@@ -48,8 +54,8 @@ __global__ __launch_bounds__(kAttnWaves * 64) void attn_active_kernel(
   for (int qg = 0; qg < kAttnQG; ++qg) {
     const int m = q0 + qg * 16 + lm;
     int p = -1;
-    if (m < n) {
-      const int64_t p64 = pos[m];
+    if (m < rows) {
+      const int64_t p64 = pos[token_of(m)];
       if (p64 < 0 || p64 >= N) {
         flag_error(err, CKV_DEVICE_ERR_RANGE);
         p = p64 < 0 ? 0 : N - 1;
@@ -81,7 +87,10 @@ __global__ __launch_bounds__(kAttnWaves * 64) void attn_active_kernel(
 #pragma unroll
     for (int s = 0; s < DS; ++s) {
       vec16 v = {0, 0, 0, 0};
-      if (m < n) v = ld16(q + (int64_t)hq * q_hs_b + (int64_t)m * q_ts_b + (32 * s + 8 * g) * 2);
+      if (m < rows) {
+        const int t = token_of(m);
+        v = ld16(q + (int64_t)head_of(m, t) * q_hs_b + (int64_t)t * q_ts_b + (32 * s + 8 * g) * 2);
+      }
       qf[qg][s] = __builtin_bit_cast(bf16x8, v);
     }
   }
@@ -311,9 +320,10 @@ __global__ __launch_bounds__(kAttnWaves * 64) void attn_active_kernel(
   for (int qg = 0; qg < kAttnQG; ++qg) {
     const float l = l_acc[qg][0];
     const int m = q0 + qg * 16 + lm;
-    if (m >= n) continue;
+    if (m >= rows) continue;
+    const int t = token_of(m), h = head_of(m, t);
     if (SPLIT) {
-      float* prow = ws + (((int64_t)z * Hq + hq) * n + m) * (D + 4);  // 16-byte aligned rows
+      float* prow = ws + (((int64_t)z * Hq + h) * n + t) * (D + 4);  // 16-byte aligned rows
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt) *(f32x4*)(prow + dt * 16 + 4 * g) = o[qg][dt];
       if (g == 0) {
@@ -323,7 +333,7 @@ __global__ __launch_bounds__(kAttnWaves * 64) void attn_active_kernel(
       continue;
     }
     const float inv = 1.f / l;
-    char* orow = out + ((int64_t)m * Hq + hq) * (D * 2);
+    char* orow = out + ((int64_t)t * Hq + h) * (D * 2);
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) {
       unsigned w[2];

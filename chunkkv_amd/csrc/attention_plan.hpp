@@ -224,4 +224,44 @@ static inline AttnPlan attn_plan(int n, int N, int Hq, int Hkv, int head_dim, in
   return p;
 }
 
+// 128-query workgroups of an 8-bit cache whose rows are the (token, query head) pairs of a KV head, over splits of the cache
+// (splits >= 2, else the launch takes attn_plan's form). A block then holds the heads of few neighbouring tokens: full where there are
+// few tokens, and near in position, so that it stops early; every row it loads and converts serves all of them.
+// us, attn_plan's form and this: 28 / 4 heads of 128 over 28787 rows, 33 queries 64.9 and 32, 84 64.1 and 49, 160 117 and 68, 300 177 and
+// 105, 800 295 and 229, 1100 294 and 316; over 8302, 25 queries 18.2 and 18.9, 33 25.3 and 21, 251 51.9 and 43.5; 32 / 8 heads of 128 over
+// 28787, 160 132 and 75, 500 192 and 170; 14 / 2 heads of 64 over 28787, 25 20.6 and 17.4, 500 72 and 59, 1500 128 and 127, 2000 164 and
+// 169; over 5000, 400 24.5 and 27.9. Behind it: heads in pairs, 8 / 4 of 64, whose 251 queries fill attn_plan's blocks (33.9 and 36.5).
+struct GroupedPlan {
+  int splits = 0, split_tiles = 0;
+  AttnMap map;
+};
+static inline GroupedPlan attn_grouped_plan(int n, int N, int Hq, int Hkv, int head_dim, int64_t workspace_bytes) {
+  GroupedPlan p;
+  const bool d128 = head_dim == 128;
+  const int64_t group = Hq / Hkv, rows = n * group;
+  if (group == 1 || rows <= kAttnBM || rows > (d128 ? 6400 : 11000) || N < (d128 ? 6000 : 8000) || rows * N < (d128 ? 1900000 : 3800000)) return p;
+  const int64_t tiles = (N + kAttnBN - 1) / kAttnBN, q = (rows + kAttnBM - 1) / kAttnBM;
+  // Of positions spread over the cache a head's q blocks have s (q + 1) / 2 + (q - 1) / 2 splits with work. As many splits as
+  // keep those somewhat below the head's share of the 512 (head_dim 64: 768) workgroups that are resident at once: where a part of
+  // them waits, most of what shorter splits save is lost (28 / 4 heads of 128, 128 places a head, 84 queries over 28787: 110
+  // workgroups with work 48.6 us, 122 58.3; 500 queries, 115 152 us, 130 185). Of five splits or fewer one more saves more than
+  // that (32 / 8 heads, 64 places, 800 queries: three splits and 51 workgroups 315 us, four and 64 251).
+  const double places = (d128 ? 512.0 : 768.0) / Hkv;
+  int64_t fill = std::max<int64_t>(0, (int64_t)((2 * 0.87 * places - (double)(q - 1)) / (double)(q + 1) + 0.4));
+  if (fill <= 4 && (double)(fill + 1) * (double)(q + 1) + (double)(q - 1) <= 2.5 * places) ++fill;
+  // and no more than the partial rows cost: a split's chain falls by as much as writing and reading its rows takes
+  const double chain_us = (double)tiles * (d128 ? 1.5 : 0.9), part_us = (double)n * Hq * (head_dim + 4) * 4e-6 * (d128 ? 0.31 : 0.45);
+  const int64_t row_b = (int64_t)Hq * n * (head_dim + 4) * 4;
+  int64_t splits = std::min<int64_t>({fill, tiles / 4, 64, workspace_bytes / row_b});
+  while (splits > 2 && (double)splits * splits * part_us > chain_us) --splits;
+  if (splits < 2) return p;
+  p.split_tiles = (int)((tiles + splits - 1) / splits);
+  p.splits = (int)((tiles + p.split_tiles - 1) / p.split_tiles);
+  // An odd count of blocks, with one of no rows if need be: workgroups go round-robin to the 32 CUs of an XCD, and with an even
+  // one the latest blocks, which every split concerns, would always meet the same CUs (32 / 8 heads of 128 over 28787, 128 queries 92
+  // and 67 us, 251 147 and 102). Of two or three blocks of head_dim 64 there are too few for that (25 queries of 14 / 2 heads 17.4 and 20.4).
+  p.map = attn_map(d128 || q > 3 ? q | 1 : q, Hkv, 1, p.splits);
+  return p;
+}
+
 }  // namespace ckv

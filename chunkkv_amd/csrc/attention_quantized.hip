@@ -6,9 +6,9 @@
 //  - Few query rows (some tokens, short prompts): attention_wave.hpp's kernel reads the codes and makes them bf16
 //    on their way into LDS, a wavefront its own 32 rows.
 //  - More, as attention_plan.hpp decides for bf16 rows: attention_large.hpp's workgroups of 128 queries, which convert a tile on
-//    its way into LDS. Every workgroup that reads a row converts it again, about a tenth of the kernel's time,
-//  - so launches of many rows first write the cache as bf16 into the workspace, one pass, and attention.hip runs on that
-//    (kDecodeRows has both sides).
+//    its way into LDS. Over a long cache (attn_grouped_plan) a workgroup has 128 of the (token, query head) rows of a KV head instead.
+//  - Every workgroup that reads a row converts it again, about a tenth of the kernel's time, so launches of many rows first write
+//    the cache as bf16 into the workspace, one pass, and attention.hip runs on that (kDecodeRows has both sides).
 #include "attention_large.hpp"
 #include "attention_wave.hpp"
 
@@ -354,6 +354,8 @@ extern "C" int64_t ckv_attention_quantized_workspace_bytes(int32_t n_queries, in
     const int splits = codes_plan(n_queries, n_tokens, n_q_heads, n_kv_heads, head_dim, INT64_MAX).splits;
     return splits > 1 ? (int64_t)splits * n_q_heads * n_queries * (head_dim + 4) * 4 : 0;
   }
+  if (const GroupedPlan p = attn_grouped_plan(n_queries, n_tokens, n_q_heads, n_kv_heads, head_dim, INT64_MAX); p.splits > 0)
+    return (int64_t)p.splits * n_q_heads * n_queries * (head_dim + 4) * 4;
   return attn_workspace_bytes(n_queries, n_tokens, n_q_heads, head_dim) +
          (decode_first(n_queries, n_tokens, n_q_heads, n_kv_heads, head_dim) ? decoded_bytes(n_tokens, n_kv_heads, head_dim) : 0);
 }
@@ -381,24 +383,6 @@ extern "C" int32_t ckv_attention_quantized(void* out, const void* q, int64_t q_h
   const int blocks = (int)(((int64_t)n_tokens + block_tokens - 1) >> block_log);
   hipStream_t st = (hipStream_t)stream;
   if (workspace == nullptr || (uintptr_t)workspace % 16) workspace_bytes = 0;
-
-  const int64_t decoded = decoded_bytes(n_tokens, n_kv_heads, head_dim);
-  if (workspace_bytes >= decoded && decode_first(n_queries, n_tokens, n_q_heads, n_kv_heads, head_dim)) {
-    char* kd = (char*)workspace;
-    char* vd = kd + decoded / 2;
-    const int64_t pieces = (int64_t)n_tokens * (head_dim / 16);
-    const dim3 grid((unsigned)((pieces + 255) / 256), (unsigned)n_kv_heads, 2);
-    auto decode = [&](auto kernel) {
-      hipLaunchKernelGGL(kernel, grid, dim3(256), 0, st, kd, vd, (const char*)k_codes, (const char*)v_codes,
-                         (const uint8_t*)k_scales, (const uint8_t*)v_scales, n_tokens, blocks, block_log);
-    };
-    if (head_dim == 128) decode(decode_rows_kernel<128>);
-    else decode(decode_rows_kernel<64>);
-    CKV_RETURN_IF_LAUNCH_FAILED();
-    return ckv_attention_active(out, q, q_head_stride, q_token_stride, kd, vd, (int64_t)n_tokens * head_dim, positions,
-                                n_queries, n_tokens, n_q_heads, n_kv_heads, head_dim, CKV_DTYPE_BF16, scale,
-                                vd + decoded / 2, workspace_bytes - decoded, err, stream);
-  }
 
   const float scale_log2 = (float)(scale * 1.4426950408889634);  // exp(x) = exp2(x log2 e)
   const int group = n_q_heads / n_kv_heads;
@@ -428,6 +412,40 @@ extern "C" int32_t ckv_attention_quantized(void* out, const void* q, int64_t q_h
     }
     return CKV_OK;
   }
+  if (const GroupedPlan p = attn_grouped_plan(n_queries, n_tokens, n_q_heads, n_kv_heads, head_dim, workspace_bytes); p.splits > 0) {
+    float* ws = (float*)workspace;
+    const GroupedCacheScales gs = {scales, inverse_of((int64_t)n_queries * group, group)};
+    auto launch = [&](auto kernel) {
+      hipLaunchKernelGGL(kernel, dim3(p.map.blocks), dim3(kAttnWaves * 64), 0, st, p.map.nqb, p.map.group, p.map.xpk_log,
+                         p.map.items, p.map.inv_group, p.map.inv_nqb, positions, n_queries, n_tokens, (const char*)k_codes,
+                         (const char*)v_codes, (int64_t)n_tokens * head_dim, (const char*)q, q_head_stride * 2,
+                         q_token_stride * 2, n_q_heads, group, scale_log2, (char*)out, err, ws, p.split_tiles, gs);
+    };
+    if (head_dim == 128) launch(attn_active_kernel<128, true, GroupedCacheScales>);
+    else launch(attn_active_kernel<64, true, GroupedCacheScales>);
+    CKV_RETURN_IF_LAUNCH_FAILED();
+    join(ws, p.splits);
+    CKV_RETURN_IF_LAUNCH_FAILED();
+    return CKV_OK;
+  }
+  const int64_t decoded = decoded_bytes(n_tokens, n_kv_heads, head_dim);
+  if (workspace_bytes >= decoded && decode_first(n_queries, n_tokens, n_q_heads, n_kv_heads, head_dim)) {
+    char* kd = (char*)workspace;
+    char* vd = kd + decoded / 2;
+    const int64_t pieces = (int64_t)n_tokens * (head_dim / 16);
+    const dim3 grid((unsigned)((pieces + 255) / 256), (unsigned)n_kv_heads, 2);
+    auto decode = [&](auto kernel) {
+      hipLaunchKernelGGL(kernel, grid, dim3(256), 0, st, kd, vd, (const char*)k_codes, (const char*)v_codes,
+                         (const uint8_t*)k_scales, (const uint8_t*)v_scales, n_tokens, blocks, block_log);
+    };
+    if (head_dim == 128) decode(decode_rows_kernel<128>);
+    else decode(decode_rows_kernel<64>);
+    CKV_RETURN_IF_LAUNCH_FAILED();
+    return ckv_attention_active(out, q, q_head_stride, q_token_stride, kd, vd, (int64_t)n_tokens * head_dim, positions,
+                                n_queries, n_tokens, n_q_heads, n_kv_heads, head_dim, CKV_DTYPE_BF16, scale,
+                                vd + decoded / 2, workspace_bytes - decoded, err, stream);
+  }
+
   const AttnPlan plan = attn_plan(n_queries, n_tokens, n_q_heads, n_kv_heads, head_dim, workspace_bytes);
   const AttnMap& map = plan.map;
   float* ws = plan.splits > 1 ? (float*)workspace : nullptr;

@@ -49,8 +49,8 @@ EVICT = [("ko", 16), ("ko_hs", 640), ("vo", 16), ("vo_hs", 640), ("rows", 16), (
     ("ckv_attention_weights", WEIGHTS, [
         (dict(out=None), INVALID), (dict(q=None), INVALID), (dict(k=None), INVALID), (dict(pos=None), INVALID), (dict(k=8), INVALID),
         (dict(dtype=0), INVALID), (dict(D=256), INVALID), (dict(Hq=3), INVALID), (dict(N=0), INVALID), (dict(n=-1), INVALID),
-        (dict(scale=-1.0), INVALID), (dict(q_hs=68), INVALID), (dict(q_ts=56), RANGE), (dict(k_hs=6392), RANGE), (dict(ws=None, n=40), INVALID),
-        (dict(wsb=16, n=40), INVALID), (dict(ws=8, n=40), INVALID), (dict(n=1 << 30), LARGE),
+        (dict(scale=-1.0), INVALID), (dict(q_hs=68), INVALID), (dict(q_ts=56), RANGE), (dict(k_hs=6392), RANGE), (dict(ws=None, n=400), INVALID),
+        (dict(wsb=16, n=400), INVALID), (dict(ws=8, n=400), INVALID), (dict(n=1 << 30), LARGE),
         (dict(out=4096, prior=4096 + 796), INVALID), (dict(out=4096, prior=4096 - 4), INVALID), (dict(out=4096, prior=4100, n=0), INVALID), (dict(n=0, q=None, k=None, pos=None, prior=16), OK)]),
     ("ckv_evict_rows", EVICT, [
         (dict(ko=None), INVALID), (dict(rows=None), INVALID), (dict(w=None), INVALID), (dict(vo=8), INVALID), (dict(k=8), INVALID),
@@ -70,10 +70,12 @@ def test_workspace_sizes_are_host_only():
     assert attn(1, 100, 28, 4, 128) == 0  # one launch
     row = 28 * 132 * 4  # a partial row per query head: 128 values, its maximum and sum
     assert attn(1, 8256, 28, 4, 128) > row and attn(1, 8256, 28, 4, 128) % row == 0
+    mid = attn(160, 8256, 28, 4, 128)  # splits of grouped rows, no bf16 copy
+    assert 0 < mid <= 64 * 160 * row and mid % (160 * row) == 0
     assert attn(2976, 8256, 28, 4, 128) >= 2 * 2 * 4 * 8256 * 128  # the cache as bf16
     assert attn(0, 100, 28, 4, 128) == attn(1, 0, 28, 4, 128) == attn(1, 100, 28, 3, 128) == attn(1, 100, 28, 0, 128) == 0
     w = lib.ckv_attention_weights_workspace_bytes
-    assert w(40, 100, 4, 4, 64) > 0 and w(1, 100, 4, 4, 64) == 0 and w(1, 2000, 4, 4, 64) > 0 and w(0, 100, 28, 4, 64) == w(1, 100, 28, 3, 64) == 0
+    assert w(400, 100, 4, 4, 64) > 0 and w(40, 300, 4, 4, 64) > 0 and w(1, 100, 4, 4, 64) == w(40, 100, 4, 4, 64) == 0 and w(1, 2000, 4, 4, 64) > 0 and w(0, 100, 28, 4, 64) == w(1, 100, 28, 3, 64) == 0
     assert w(2**31 - 1, 100, 64, 1, 64) == 0  # refused by the call
 
 
@@ -87,6 +89,18 @@ def test_every_wave_plan_can_be_launched(tmp_path):
     out = subprocess.run([str(exe)], check=True, capture_output=True, text=True, timeout=300).stdout
     checked, bad = map(int, out.splitlines()[-1].split())
     assert checked > 40_000 and bad == 0, out
+
+
+def test_every_grouped_plan_can_be_launched(tmp_path):
+    gxx = shutil.which("g++")
+    if gxx is None:
+        pytest.skip("g++ not available")
+    exe = tmp_path / "attention_grouped_plan_walk"
+    subprocess.run([gxx, "-O2", "-std=c++17", f"-I{ROOT / 'chunkkv_amd' / 'csrc'}",
+                    str(ROOT / "tests" / "native" / "attention_grouped_plan_walk.cpp"), "-o", str(exe)], check=True)
+    out = subprocess.run([str(exe)], check=True, capture_output=True, text=True, timeout=300).stdout
+    checked, taken, bad = map(int, out.splitlines()[-1].split())
+    assert checked > 40_000 and taken > 2_000 and bad == 0, out
 
 
 def test_host_tensors_and_block_sizes_are_refused():

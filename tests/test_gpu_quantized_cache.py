@@ -218,6 +218,13 @@ def _attends(q, c, pos, rows, scale=None, **kw):
         (16, 16, 64, 5700, 5633, 130, 128),
         (32, 32, 128, 1100, 1090, 1000, 32),  # no shared heads: the codes converted, unsplit
         (64, 64, 64, 1000, 993, 910, 64),
+        (28, 4, 128, 8256, 8250, 33, 64),  # a head's (token, query head) rows in one block after another: two blocks
+        (28, 4, 128, 8300, 8290, 251, 32),  # fourteen, and one of no rows
+        (32, 8, 128, 9000, 8999, 100, 128),
+        (14, 2, 64, 16390, 16385, 40, 32),
+        (14, 2, 64, 9000, 8901, 700, 64),
+        (10, 2, 128, 12000, 11000, 66, 64),
+        (6, 3, 64, 33000, 32990, 65, 128),
         (28, 4, 128, 1100, 1024, 1, 32),  # one token, whole and split
         (28, 4, 128, 1025, 1025, 1, 32),
         (14, 2, 64, 1536, 1536, 2, 64),
