@@ -98,7 +98,7 @@ def _build_torch_ops(verbose: bool) -> None:
           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", f"-I{INCLUDE}",
           "-isystem", str(t / "include"), "-isystem", str(t / "include/torch/csrc/api/include"),
           "-isystem", f"{rocm}/include", "-isystem", sysconfig.get_paths()["include"], str(CSRC / TORCH_SOURCE),
-          "-o", str(tmp), f"-L{t / 'lib'}", "-ltorch_python", "-ltorch_cpu", "-lc10", "-lc10_hip",
+          "-o", str(tmp), f"-L{t / 'lib'}", "-ltorch_python", "-ltorch_cpu", "-ltorch_hip", "-lc10", "-lc10_hip",
           f"-L{LIB_DIR}", f"-l:{LIB_NAME}", "-Wl,-rpath,$ORIGIN"], verbose)
     os.replace(tmp, out)
 

@@ -13,7 +13,8 @@
 // The first histogram counts a row as it arrives (32832 rows of 4 heads of 128 cut to 4104 20.1 -> 19.1 us), and a bin that stays whole
 // needs no further pass (20.9 -> 20.1; 60000 to 4000, where each pass reads the weights again, 52 -> 49).
 // Bound: the issue of the CU that selects. Those 19 us by phase, about: rows and first pass 6, the other two 3, count 2, list and
-// copy 2, the rest start and launch; 1103 fp32 rows of 2 heads of 64 cut to 300 take 7.5-7.8, mostly the passes' scans and barriers.
+// copy 2, the rest start and launch; 1103 fp32 rows of 2 heads of 64 cut to 300 take 5.5 (eager calls 6.4, the host's time), mostly the
+// passes' scans and barriers.
 // One workgroup a head with a copy launch behind it took 46 and 11.4.
 #include <algorithm>
 

@@ -9,6 +9,7 @@
 // host for each: attention_active 9.4 us, rope_qkv (k/v into a cache) 10.9, add_rmsnorm 8.0,
 // silu_mul 12.2. The launch itself is 2-3 us of that.
 #include <Python.h>
+#include <ATen/hip/EmptyTensor.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/core/impl/LocalDispatchKeySet.h>
 #include <c10/hip/HIPStream.h>
@@ -535,6 +536,11 @@ PyObject* extract_chunks(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
   CKV_PY_END
 }
 
+// A new tensor beside `like`, without the dispatcher's round.
+Tensor new_tensor(at::IntArrayRef sizes, at::ScalarType type, const Tensor& like) {
+  return at::detail::empty_cuda(sizes, type, like.device(), std::nullopt);
+}
+
 // An 8-bit cache's four tensors of one shape: codes (1, H, N, D), scales (1, H, ceil(N / block)).
 struct CodedCache {
   const Tensor &k, &v, &ks, &vs;
@@ -639,7 +645,7 @@ PyObject* attention_quantized(PyObject*, PyObject* const* a, Py_ssize_t n_args) 
   query_args(q, pos, c.D, c.H);
   const int64_t Hq = q.size(1), n = q.size(2);
   if (!out.defined()) {
-    out = at::empty({1, n, Hq, c.D}, q.options());
+    out = new_tensor({1, n, Hq, c.D}, q.scalar_type(), q);
   } else {
     same_device(q, out);
     if (out.sizes() != at::IntArrayRef({1, n, Hq, c.D}) || !out.is_contiguous() || out.scalar_type() != q.scalar_type())
@@ -650,7 +656,7 @@ PyObject* attention_quantized(PyObject*, PyObject* const* a, Py_ssize_t n_args) 
   if (split < 0) throw python_error();
   const int64_t ws_bytes = split ? ckv_attention_quantized_workspace_bytes(int32(n), int32(c.N), int32(Hq), int32(c.H), int32(c.D)) : 0;
   Tensor ws;
-  if (ws_bytes > 0) ws = at::empty({(ws_bytes + 3) / 4}, q.options().dtype(at::kFloat));
+  if (ws_bytes > 0) ws = new_tensor({(ws_bytes + 3) / 4}, at::kFloat, q);
   int32_t* const e = status_word(err, q);
   check(unlocked([&] {
           const c10::DeviceGuard on(q.device());
@@ -685,12 +691,12 @@ PyObject* attention_weights(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
       value_error(std::string(what) + " must be contiguous (1, Hkv, N) float32");
   };
   if (prior.defined()) fits(prior, "prior");
-  if (!out.defined()) out = at::empty({1, H, N}, q.options().dtype(at::kFloat));
+  if (!out.defined()) out = new_tensor({1, H, N}, at::kFloat, q);
   else fits(out, "out");
   const double scale = a[3] == Py_None ? 1.0 / std::sqrt((double)D) : real(a[3]);
   const int64_t ws_bytes = ckv_attention_weights_workspace_bytes(int32(n), int32(N), int32(Hq), int32(H), int32(D));
   Tensor ws;
-  if (ws_bytes > 0) ws = at::empty({(ws_bytes + 3) / 4}, q.options().dtype(at::kFloat));
+  if (ws_bytes > 0) ws = new_tensor({(ws_bytes + 3) / 4}, at::kFloat, q);
   int32_t* const e = status_word(err, q);
   check(unlocked([&] {
           const c10::DeviceGuard on(q.device());
@@ -736,7 +742,7 @@ PyObject* evict_rows(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
   const int code = dtype_code(K);
   auto to = [&](Tensor& t, const char* what) {
     if (!t.defined()) {
-      t = at::empty({1, H, keep, D}, K.options());
+      t = new_tensor({1, H, keep, D}, K.scalar_type(), K);
       return;
     }
     same_device(K, t);
@@ -747,7 +753,7 @@ PyObject* evict_rows(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
   to(ko, "k_out");
   to(vo, "v_out");
   const int64_t kohs = head_stride(ko, "k_out"), vohs = head_stride(vo, "v_out");
-  const Tensor rows = at::empty({1, H, keep}, K.options().dtype(at::kLong)), wo = at::empty({1, H, keep}, w.options());
+  const Tensor rows = new_tensor({1, H, keep}, at::kLong, K), wo = new_tensor({1, H, keep}, at::kFloat, K);
   if (keep > 0) {
     if (given && (overlap(ko, kohs, K, khs) || overlap(ko, kohs, V, vhs) || overlap(vo, vohs, K, khs) || overlap(vo, vohs, V, vhs) ||
                   overlap(ko, kohs, vo, vohs)))
