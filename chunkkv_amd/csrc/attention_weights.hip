@@ -725,11 +725,16 @@ static WeightsPlan weights_plan(int n, int N, int Hq, int Hkv, int head_dim) {
   // long, every K row is read twice as often): 28 / 4 heads of 128 (us, 128 rows and 64), 30 queries over 1103 16.0 and 14.1, 128 over
   // 8302 36.4 and 34.2, 128 over 16400 51.6 and 51.1, 251 84.9 and 87.8; over 65536 17 queries 37.8 and 40.2, but 8, which 64 rows
   // hold, 33.8 and 28.9. 14 / 2 heads of 64, 251 over 16400 40.5 and 39.3, 500 over 32832 106 and 109.
-  const bool short_rows = (int64_t)((p.rows + 127) / 128) * tiles * Hkv <= 8300 && (int64_t)N * head_dim <= 5 << 20;
+  const int64_t work = (int64_t)((p.rows + 127) / 128) * tiles * Hkv;
+  const bool short_rows = work <= 8300 && (int64_t)N * head_dim <= 5 << 20;
   p.qg = p.rows <= 64 || short_rows ? 1 : 2;
   p.row_blocks = (p.rows + 64 * p.qg - 1) / (64 * p.qg);
   const int64_t lse_blocks = (int64_t)p.row_blocks * Hkv;
-  int64_t splits = std::max<int64_t>(1, std::min<int64_t>({1024 / lse_blocks, tiles / 2, tiles <= 80 ? kWtJoinSplits : 64}));
+  // With much work over a long cache two or four times as many even out what the blocks see of it (us, positions spread over it, 1024
+  // workgroups and more: 14 / 2 heads of 64, 750 queries over 21000 92 and 78; 28 / 4 of 128, 1750 over 32832 532 and 483, but 1000 over
+  // 8302 102 and 106), unless the blocks alone are about as many as the card holds (5000 over 13000 518 and 551).
+  const int64_t most = N < 12000 || work < 10000 || lse_blocks > 700 ? 1024 : work < 50000 ? 2048 : 4096;
+  int64_t splits = std::max<int64_t>(1, std::min<int64_t>({most / lse_blocks, tiles / 2, tiles <= 80 ? kWtJoinSplits : 64}));
   p.split_tiles = (int)((tiles + splits - 1) / splits);
   p.splits = (tiles + p.split_tiles - 1) / p.split_tiles;
   auto parts_of = [&](int64_t blocks) { return std::max<int64_t>(1, std::min<int64_t>(8192 / blocks, row_tiles < 8 ? 1 : (row_tiles + 3) / 4)); };

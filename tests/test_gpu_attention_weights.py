@@ -54,6 +54,7 @@ def _check(q, K, pos, prior=None, scale=None, out=None):
         (14, 2, 64, 33, 33),
         (16, 16, 64, 193, 190),
         (40, 2, 128, 2, 2),
+        (14, 2, 64, 13000, 520),  # more splits over a long cache
         (28, 4, 128, 2050, 18),  # 64 rows a workgroup, a split joined by the second pass
         (28, 4, 128, 1103, 128),  # in parts too
         (28, 4, 128, 2050, 64),  # 448 rows and 16 splits: joined by a launch
