@@ -308,16 +308,6 @@ __device__ __forceinline__ void rotate_pairs(const vec16& a16, const vec16& b16,
   y2_16 = E::pack(y2);
 }
 
-// Workgroup barrier that orders LDS only: waits for this wavefront's LDS operations (lgkmcnt 0),
-// not for its global loads and stores, which __syncthreads() would also drain. Values loaded
-// from global memory are still waited for where they are used.
-__device__ __forceinline__ void lds_barrier() {
-  asm volatile("" ::: "memory");
-  __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0); vmcnt and expcnt at their maxima (no wait)
-  __builtin_amdgcn_s_barrier();
-  asm volatile("" ::: "memory");
-}
-
 }  // namespace ckv
 
 // Host-side status helper shared by the entry points.

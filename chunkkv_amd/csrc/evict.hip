@@ -45,6 +45,14 @@ __device__ __forceinline__ uint32_t bits_below(uint64_t mask, uint32_t more) {
   return __builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mask, more));
 }
 
+// A workgroup barrier behind which LDS writes are seen; global loads stay in flight.
+__device__ __forceinline__ void lds_barrier() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0)
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
 struct EvictCopy {
   const char *k, *v;
   char *ko, *vo;
@@ -105,7 +113,7 @@ __global__ __launch_bounds__(kEvictThreads) void evict_kernel(const float* __res
   };
   auto clear = [&] {
     for (int b = tid; b < kEvictCopies * kEvictPitch; b += kEvictThreads) hist0[b] = 0;
-    lds_barrier();  // loads stay in flight
+    lds_barrier();
   };
   if constexpr (PER > 0) {
     float x[PER][4];

@@ -120,6 +120,16 @@ __device__ __forceinline__ uint32_t top_bin_prefix(uint32_t b) { return kTopLo +
 
 __device__ __forceinline__ bool bit_of(const uint32_t* w, int p) { return (w[p >> 5] >> (p & 31)) & 1u; }
 
+// Workgroup barrier that orders LDS only: waits for this wavefront's LDS operations (lgkmcnt 0),
+// not for its global loads and stores, which __syncthreads() would also drain. Values loaded
+// from global memory are still waited for where they are used.
+__device__ __forceinline__ void lds_barrier() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0); vmcnt and expcnt at their maxima (no wait)
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
 // Exclusive prefix count of `pred` over the workgroup in thread order, plus the total.
 __device__ __forceinline__ int block_excl_count(bool pred, int* wave_tot, int& total) {
   const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
