@@ -10,10 +10,11 @@
 // find the same threshold, each for a slice of the kept rows that it then copies: the selection is the latency of
 // one CU whatever is done, and this way no launch waits for it. Longer caches: one workgroup a head reads the weights
 // again for each pass, and evict_gather_kernel copies.
-// The first histogram counts a row as it arrives (32832 rows of 4 heads of 128 cut to 4104 20.1 -> 19.1 us), and a bin that stays whole
+// Weights of 0, as rows that no query reached have, are counted by ballots: atomics on one address queue (a fifth of 32832 rows at 0
+// 19.1 -> 17.6 us). The first histogram counts a row as it arrives (32832 rows of 4 heads of 128 cut to 4104 20.1 -> 19.1 us), and a bin that stays whole
 // needs no further pass (20.9 -> 20.1; 60000 to 4000, where each pass reads the weights again, 52 -> 49).
-// Bound: the issue of the CU that selects. Those 19 us by phase, about: rows and first pass 6, the other two 3, count 2, list and
-// copy 2, the rest start and launch; 1103 fp32 rows of 2 heads of 64 cut to 300 take 5.5 (eager calls 6.4, the host's time), mostly the
+// Bound: the issue of the CU that selects. Those 17.6 us by phase, about: rows and first pass 5, the other two 3, count 2, list
+// and copy 2, the rest start and launch; 1103 fp32 rows of 2 heads of 64 cut to 300 take 5.5 (eager calls 6.4, the host's time), mostly the
 // passes' scans and barriers.
 // One workgroup a head with a copy launch behind it took 46 and 11.4.
 #include <algorithm>
@@ -29,6 +30,7 @@ constexpr int kEvictCopies = 2;                 // of the first histogram: a lan
 constexpr int kEvictPitch = kEvictBins + 16;    // copies of a bin on banks of their own
 constexpr int kEvictList = 2048;                // kept rows that a workgroup lists at a time
 constexpr int kEvictKeys = 34 * 1024;           // rows whose integers LDS holds, at most
+constexpr uint32_t kKeyZero = 0x80000000u;   // of the weight 0
 constexpr uint32_t kKeyFixed = 0xffffffffu;     // a row that stays, above every weight's key
 
 // An integer that orders as the weight does: 1 for a NaN, below -infinity's; 0 is no row's.
@@ -107,9 +109,14 @@ __global__ __launch_bounds__(kEvictThreads) void evict_kernel(const float* __res
     }
   };
   uint32_t* mine = hist0 + (lane % kEvictCopies) * kEvictPitch;
+  uint32_t zeros = 0;  // of this wavefront
   auto count4 = [&](const uint32_t(&k)[4]) {  // the first pass; key 0 counts below every row's
 #pragma unroll
-    for (int j = 0; j < 4; ++j) atomicAdd(&mine[k[j] >> 21], 1u);
+    for (int j = 0; j < 4; ++j) {
+      const bool zero = k[j] == kKeyZero;
+      zeros += (uint32_t)__popcll(__builtin_amdgcn_ballot_w64(zero));
+      if (!zero) atomicAdd(&mine[k[j] >> 21], 1u);
+    }
   };
   auto clear = [&] {
     for (int b = tid; b < kEvictCopies * kEvictPitch; b += kEvictThreads) hist0[b] = 0;
@@ -186,6 +193,7 @@ __global__ __launch_bounds__(kEvictThreads) void evict_kernel(const float* __res
   };
   {
     if constexpr (PER == 0) each([&](int, const uint32_t(&k)[4]) { count4(k); });
+    if (lane == 0) atomicAdd(&mine[kKeyZero >> 21], zeros);
     __syncthreads();
     const int top = kEvictBins - 1 - 2 * tid;
     uint32_t a = 0, b = 0;
