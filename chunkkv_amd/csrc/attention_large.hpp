@@ -322,6 +322,9 @@ __global__ __launch_bounds__(kAttnWaves * 64) void attn_active_kernel(
     const int m = q0 + qg * 16 + lm;
     if (m >= rows) continue;
     const int t = token_of(m), h = head_of(m, t);
+    if constexpr (GROUPED && SPLIT) {
+      if (my_pos[qg] < tile_begin * kAttnBN) continue;  // nothing of this split: its row is not read
+    }
     if (SPLIT) {
       float* prow = ws + (((int64_t)z * Hq + h) * n + t) * (D + 4);  // 16-byte aligned rows
 #pragma unroll

@@ -316,6 +316,62 @@ __global__ __launch_bounds__(kCodeWaves * 64) void attn_codes_kernel(
   }
 }
 
+// ---- the splits of (token, query head) rows joined ---------------------------------------------------------------
+// attn_combine_kernel's merge for launches of many rows: a row a wavefront, D / 4 lanes a partial row (16-byte loads) and 64 / (D / 4)
+// partials side by side, four of each in flight. Only the splits that begin at or before the row's position are written and
+// read: half of them where positions are spread over the cache.
+template <int D>
+__global__ __launch_bounds__(256) void join_rows_kernel(char* __restrict__ out, const float* __restrict__ ws,
+                                                        const int64_t* __restrict__ pos, int n, int N, int Hq, int splits,
+                                                        int split_rows) {
+  constexpr int LR = D / 4, P = 64 / LR, U = 4;
+  const int lane = threadIdx.x % 64, sub = lane / LR, col = lane % LR * 4;
+  const int64_t row = (int64_t)blockIdx.x * 4 + threadIdx.x / 64;
+  if (row >= (int64_t)n * Hq) return;  // uniform
+  const int h = (int)(row / n), m = (int)(row - (int64_t)h * n);
+  const int64_t p64 = pos[m], stride = (int64_t)Hq * n * (D + 4);
+  const int p = p64 < 0 ? 0 : p64 >= N ? N - 1 : (int)p64;
+  const int live = __builtin_amdgcn_readfirstlane(min(splits, p / split_rows + 1));
+  const float* base = ws + row * (D + 4);
+  float M = -INFINITY, L = 0.f;
+  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+  for (int z0 = 0; z0 < live; z0 += P * U) {
+    f32x4 o[U];
+    float2 ml[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const float* pz = base + (int64_t)min(z0 + u * P + sub, live - 1) * stride;
+      o[u] = *(const f32x4*)(pz + col);
+      ml[u] = *(const float2*)(pz + D);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const bool mine = z0 + u * P + sub < live;
+      const float mz = mine ? ml[u].x : -INFINITY, mn = fmaxf(M, mz), ref = mn == -INFINITY ? 0.f : mn;
+      const float a = __builtin_amdgcn_exp2f(M - ref), b = __builtin_amdgcn_exp2f(mz - ref);  // 0 of -inf
+      L = L * a + (mine ? ml[u].y : 0.f) * b;
+      acc = acc * a + o[u] * b;
+      M = mn;
+    }
+  }
+  float mx = M;
+#pragma unroll
+  for (int d = LR; d < 64; d *= 2) mx = fmaxf(mx, __shfl_xor(mx, d));
+  const float s = __builtin_amdgcn_exp2f(M - mx);  // the first split has a visible row
+  L *= s;
+  acc *= s;
+#pragma unroll
+  for (int d = LR; d < 64; d *= 2) {
+    L += __shfl_xor(L, d);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) acc[e] += __shfl_xor(acc[e], d);
+  }
+  const float inv = 1.f / L;
+  if (sub == 0)
+    *(uint2*)(out + ((int64_t)m * Hq + h) * (D * 2) + col * 2) =
+        uint2{f32x2_to_bf16x2_bits(acc[0] * inv, acc[1] * inv), f32x2_to_bf16x2_bits(acc[2] * inv, acc[3] * inv)};
+}
+
 struct CodesPlan {
   int splits, split_chunks;
 };
@@ -424,7 +480,13 @@ extern "C" int32_t ckv_attention_quantized(void* out, const void* q, int64_t q_h
     if (head_dim == 128) launch(attn_active_kernel<128, true, GroupedCacheScales>);
     else launch(attn_active_kernel<64, true, GroupedCacheScales>);
     CKV_RETURN_IF_LAUNCH_FAILED();
-    join(ws, p.splits);
+    const dim3 grid((unsigned)(((int64_t)n_queries * n_q_heads + 3) / 4));
+    auto merge = [&](auto kernel) {
+      hipLaunchKernelGGL(kernel, grid, dim3(256), 0, st, (char*)out, (const float*)ws, positions, n_queries, n_tokens, n_q_heads, p.splits,
+                         p.split_tiles * kAttnBN);
+    };
+    if (head_dim == 128) merge(join_rows_kernel<128>);
+    else merge(join_rows_kernel<64>);
     CKV_RETURN_IF_LAUNCH_FAILED();
     return CKV_OK;
   }
