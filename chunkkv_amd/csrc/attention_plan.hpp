@@ -227,10 +227,10 @@ static inline AttnPlan attn_plan(int n, int N, int Hq, int Hkv, int head_dim, in
 // 128-query workgroups of an 8-bit cache whose rows are the (token, query head) pairs of a KV head, over splits of the cache
 // (splits >= 2, else the launch takes attn_plan's form). A block then holds the heads of few neighbouring tokens: full where there are
 // few tokens, and near in position, so that it stops early; every row it loads and converts serves all of them.
-// us, attn_plan's form and this: 28 / 4 heads of 128 over 28787 rows, 33 queries 64.9 and 32, 84 64.1 and 49, 160 117 and 68, 300 177 and
-// 105, 800 295 and 229, 1100 294 and 316; over 8302, 25 queries 18.2 and 18.9, 33 25.3 and 21, 251 51.9 and 43.5; 32 / 8 heads of 128 over
-// 28787, 160 132 and 75, 500 192 and 170; 14 / 2 heads of 64 over 28787, 25 20.6 and 17.4, 500 72 and 59, 1500 128 and 127, 2000 164 and
-// 169; over 5000, 400 24.5 and 27.9. Behind it: heads in pairs, 8 / 4 of 64, whose 251 queries fill attn_plan's blocks (33.9 and 36.5).
+// us, attn_plan's form and this: 28 / 4 heads of 128 over 28787 rows, 33 queries 64.9 and 32, 84 64.1 and 43, 160 117 and 62, 300 177 and
+// 100, 800 295 and 222, 1100 294 and 316; over 8302, 25 queries 18.2 and 18.9, 33 25.3 and 21, 251 51.9 and 39; 32 / 8 heads of 128 over
+// 28787, 160 132 and 68, 500 192 and 166; 14 / 2 heads of 64 over 28787, 25 20.6 and 17.5, 500 72 and 53, 1500 128 and 127, 2000 164 and
+// 169; over 5000, 400 24.5 and 27.9.
 struct GroupedPlan {
   int splits = 0, split_tiles = 0;
   AttnMap map;
@@ -250,7 +250,7 @@ static inline GroupedPlan attn_grouped_plan(int n, int N, int Hq, int Hkv, int h
   int64_t fill = std::max<int64_t>(0, (int64_t)((2 * 0.87 * places - (double)(q - 1)) / (double)(q + 1) + 0.4));
   if (fill <= 4 && (double)(fill + 1) * (double)(q + 1) + (double)(q - 1) <= 2.5 * places) ++fill;
   // and no more than the partial rows cost: a split's chain falls by as much as writing and reading its rows takes
-  const double chain_us = (double)tiles * (d128 ? 1.5 : 0.9), part_us = (double)n * Hq * (head_dim + 4) * 4e-6 * (d128 ? 0.31 : 0.45);
+  const double chain_us = (double)tiles * (d128 ? 1.5 : 0.9), part_us = (double)n * Hq * (head_dim + 4) * 4e-6 * (d128 ? 0.18 : 0.25);
   const int64_t row_b = (int64_t)Hq * n * (head_dim + 4) * 4;
   int64_t splits = std::min<int64_t>({fill, tiles / 4, 64, workspace_bytes / row_b});
   while (splits > 2 && (double)splits * splits * part_us > chain_us) --splits;

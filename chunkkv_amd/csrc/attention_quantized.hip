@@ -340,6 +340,9 @@ __global__ __launch_bounds__(256) void join_rows_kernel(char* __restrict__ out, 
     float2 ml[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
+      o[u] = f32x4{0.f, 0.f, 0.f, 0.f};
+      ml[u] = make_float2(-INFINITY, 0.f);
+      if (z0 + u * P >= live) continue;  // uniform
       const float* pz = base + (int64_t)min(z0 + u * P + sub, live - 1) * stride;
       o[u] = *(const f32x4*)(pz + col);
       ml[u] = *(const float2*)(pz + D);
