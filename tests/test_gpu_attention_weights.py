@@ -136,6 +136,21 @@ def test_weights_that_grow_in_place_over_a_captured_step():
         assert torch.equal(w, eager)
 
 
+@pytest.mark.parametrize("Hq,Hkv,D,N,n", [(28, 4, 128, 64, 20), (28, 4, 128, 2050, 64), (28, 4, 128, 1103, 128), (14, 2, 64, 9000, 1)])
+def test_graph_replays_match_eager(Hq, Hkv, D, N, n):
+    K, q, pos = _randn((1, Hkv, N, D), 1), _randn((1, Hq, n, D), 2), torch.arange(N - n, N, device=DEV)
+    prior = torch.rand((1, Hkv, N), device=DEV)
+    ops.attention_weights(q, K, pos, prior=prior)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = ops.attention_weights(q, K, pos, prior=prior)
+    for step in range(5):
+        q.copy_(_randn((1, Hq, n, D), 20 + step))
+        pos.copy_(torch.randint(0, N, (n,), generator=torch.Generator().manual_seed(step)))
+        graph.replay()
+        assert torch.equal(out, ops.attention_weights(q, K, pos, prior=prior))
+
+
 def test_two_calls_give_the_same_bits_and_streams_do_not_mix():
     q, K, pos = _randn((1, 28, 100, 128), 9), _randn((1, 4, 3000, 128), 10), torch.arange(2900, 3000, device=DEV)
     want = ops.attention_weights(q, K, pos)

@@ -242,10 +242,35 @@ def test_attention_matches_the_plain_form(Hq, Hkv, D, N, rows, n, block, split):
     _attends(_q(Hq, n, D, rows, token_major=n % 2 == 0), c, pos, rows, split=split)
 
 
+@pytest.mark.parametrize("Hq,Hkv,D,N,n", [(28, 4, 128, 8256, 60), (14, 2, 64, 16390, 40), (28, 4, 128, 8256, 1), (28, 4, 128, 6000, 500)])
+def test_a_workspace_may_hold_anything(Hq, Hkv, D, N, n):
+    """The allocator hands out memory full of NaN; positions from the first row to the last, the first half near the front."""
+    c = _filled(Hkv, N, D, 64, N, n)
+    pos = torch.cat([torch.arange(n // 2), torch.arange(N - (n - n // 2), N)])
+    q = _q(Hq, n, D, 7)
+    for mb in (4, 32, 128):
+        torch.full((mb << 18,), float("nan"), device=DEV)
+    _attends(q, c, pos, N)
+
+
 def test_attention_of_unsorted_and_repeated_positions_and_another_scale():
     c = _filled(2, 300, 64, 32, 300, 3)
     pos = torch.tensor([299, 0, 5, 5, 120, 64, 31, 32, 33, 0])
     _attends(_q(14, 10, 64, 4), c, pos, 300, scale=0.31)
+    c = _filled(2, 16500, 64, 32, 16500, 3)  # over a long cache, blocks of rows in any order
+    pos = torch.randint(0, 16500, (60,), generator=torch.Generator().manual_seed(1))
+    _attends(_q(14, 60, 64, 4), c, pos, 16500, scale=0.31)
+
+
+def test_positions_outside_over_a_long_cache():
+    c = _filled(4, 8400, 128, 64, 8400, 3)
+    q, err = _q(28, 60, 128, 5), torch.zeros(1, dtype=torch.int32, device=DEV)
+    pos = torch.arange(8340, 8400, device=DEV)
+    wild = pos.clone()
+    wild[3], pos[3], wild[59] = -7, 0, 2**40
+    got = ops.attention_quantized(q, c, wild, err=err)
+    assert int(err) == 1
+    assert torch.equal(got, ops.attention_quantized(q, c, pos))
 
 
 def test_attention_clamps_and_flags_positions_outside():
@@ -302,6 +327,24 @@ def test_decode_graph_replays_match_eager():
         ops.quantize_rows(eager, k[:, :, i : i + 1], v[:, :, i : i + 1], i)
         want = ops.attention_quantized(q[:, :, i : i + 1], eager, torch.tensor([i], device=DEV))
         assert torch.equal(out, want)
+
+
+@pytest.mark.parametrize("Hq,Hkv,D,N,n", [(28, 4, 128, 8256, 60), (14, 2, 64, 1103, 251), (28, 4, 128, 1500, 1500)])
+def test_prompt_graph_replays_match_eager(Hq, Hkv, D, N, n):
+    """Two graphs of one call each, replayed in turn with eager calls between, positions and queries changed every time."""
+    c, bufs, graphs, outs = _filled(Hkv, N, D, 32, N, 5), [], [], []
+    for i in range(2):
+        bufs.append((_q(Hq, n, D, i), torch.arange(N - n, N, device=DEV)))
+        ops.attention_quantized(bufs[i][0], c, bufs[i][1])
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[i]):
+            outs.append(ops.attention_quantized(bufs[i][0], c, bufs[i][1]))
+    for step in range(6):
+        i = step % 2
+        bufs[i][0].copy_(_q(Hq, n, D, 10 + step))
+        bufs[i][1].copy_(torch.randint(0, N, (n,), generator=torch.Generator().manual_seed(step)).sort().values)
+        graphs[i].replay()
+        assert torch.equal(outs[i], ops.attention_quantized(bufs[i][0], c, bufs[i][1]))
 
 
 def test_calls_on_two_streams_at_once():
