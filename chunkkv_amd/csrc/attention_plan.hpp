@@ -228,9 +228,10 @@ static inline AttnPlan attn_plan(int n, int N, int Hq, int Hkv, int head_dim, in
 // (splits >= 2, else the launch takes attn_plan's form). A block then holds the heads of few neighbouring tokens: full where there are
 // few tokens, and near in position, so that it stops early; every row it loads and converts serves all of them.
 // us, attn_plan's form and this: 28 / 4 heads of 128 over 28787 rows, 33 queries 64.9 and 32, 84 64.1 and 43, 160 117 and 62, 300 177 and
-// 100, 800 295 and 222, 1100 294 and 316; over 8302, 25 queries 18.2 and 18.9, 33 25.3 and 21, 251 51.9 and 39; 32 / 8 heads of 128 over
+// 100, 800 295 and 222, 1100 294 and 316; over 8302, 25 queries 18.2 and 18.9, 33 25.3 and 21, 251 51.9 and 39; over 4100, 33 18.2 and 17.0, 128
+// 25.6 and 27.4, 160 35.3 and 28.2; over 3000, 251 28.3 and 28.1; 32 / 8 heads of 128 over
 // 28787, 160 132 and 68, 500 192 and 166; 14 / 2 heads of 64 over 28787, 25 20.6 and 17.5, 500 72 and 53, 1500 128 and 127, 2000 164 and
-// 169; over 5000, 400 24.5 and 27.9.
+// 169; over 4100, 160 19.2 and 14.3, 800 24.0 and 30.4.
 struct GroupedPlan {
   int splits = 0, split_tiles = 0;
   AttnMap map;
@@ -239,7 +240,8 @@ static inline GroupedPlan attn_grouped_plan(int n, int N, int Hq, int Hkv, int h
   GroupedPlan p;
   const bool d128 = head_dim == 128;
   const int64_t group = Hq / Hkv, rows = n * group;
-  if (group == 1 || rows <= kAttnBM || rows > (d128 ? 6400 : 11000) || N < (d128 ? 6000 : 8000) || rows * N < (d128 ? 1900000 : 3800000)) return p;
+  if (group == 1 || rows <= kAttnBM || rows > (d128 ? 6400 : 11000) || N < 4000 || rows * N < (d128 ? 1300000 : 2400000)) return p;
+  if (!d128 && N < 7000 && rows > N / 2) return p;
   const int64_t tiles = (N + kAttnBN - 1) / kAttnBN, q = (rows + kAttnBM - 1) / kAttnBM;
   // Of positions spread over the cache a head's q blocks have s (q + 1) / 2 + (q - 1) / 2 splits with work. As many splits as
   // keep those somewhat below the head's share of the 512 (head_dim 64: 768) workgroups that are resident at once: where a part of

@@ -18,7 +18,7 @@ int main() {
     for (int hkv : {1, 2, 3, 4, 5, 8, 16, 64, 600})
       for (int group : {1, 2, 3, 7, 8, 16, 64})
         for (int n : {1, 3, 17, 25, 33, 64, 84, 128, 129, 251, 300, 500, 915, 1100, 2000, 2976, 8256})
-          for (int N : {1, 33, 1103, 5999, 6000, 8256, 8302, 28787, 65536, 131072, 1000000, 2147483647})
+          for (int N : {1, 33, 1103, 3999, 4000, 6999, 7000, 8256, 8302, 28787, 65536, 131072, 1000000, 2147483647})
             for (int share : {0, 1, 2, 3}) {
               const int Hq = hkv * group;
               const int64_t row_b = (int64_t)Hq * n * (D + 4) * 4, ws = share == 3 ? INT64_MAX : row_b * share * 2;
