@@ -231,7 +231,8 @@ static inline AttnPlan attn_plan(int n, int N, int Hq, int Hkv, int head_dim, in
 // 100, 800 295 and 222, 1100 294 and 316; over 8302, 25 queries 18.2 and 18.9, 33 25.3 and 21, 251 51.9 and 39; over 4100, 33 18.2 and 17.0, 128
 // 25.6 and 27.4, 160 35.3 and 28.2; over 3000, 251 28.3 and 28.1; 32 / 8 heads of 128 over
 // 28787, 160 132 and 68, 500 192 and 166; 14 / 2 heads of 64 over 28787, 25 20.6 and 17.5, 500 72 and 53, 1500 128 and 127, 2000 164 and
-// 169; over 4100, 160 19.2 and 14.3, 800 24.0 and 30.4.
+// 169; over 4100, 160 19.2 and 14.3, 800 24.0 and 30.4; 16 / 16 heads of 64 over 41741, 288 51.9 and 41, 1000 100 and 80, 4000 270 and 241; 32 / 32
+// of 128, 130 171 and 179, 1000 671 and 460.
 struct GroupedPlan {
   int splits = 0, split_tiles = 0;
   AttnMap map;
@@ -240,17 +241,20 @@ static inline GroupedPlan attn_grouped_plan(int n, int N, int Hq, int Hkv, int h
   GroupedPlan p;
   const bool d128 = head_dim == 128;
   const int64_t group = Hq / Hkv, rows = n * group;
-  if (group == 1 || rows <= kAttnBM || rows > (d128 ? 6400 : 11000) || N < 4000 || rows * N < (d128 ? 1300000 : 2400000)) return p;
+  if (rows <= kAttnBM || rows > (d128 ? 6400 : 11000) || N < 4000 || rows * N < (d128 ? 1300000 : 2400000)) return p;
   if (!d128 && N < 7000 && rows > N / 2) return p;
   const int64_t tiles = (N + kAttnBN - 1) / kAttnBN, q = (rows + kAttnBM - 1) / kAttnBM;
   // Of positions spread over the cache a head's q blocks have s (q + 1) / 2 + (q - 1) / 2 splits with work. As many splits as
   // keep those somewhat below the head's share of the 512 (head_dim 64: 768) workgroups that are resident at once: where a part of
   // them waits, most of what shorter splits save is lost (28 / 4 heads of 128, 128 places a head, 84 queries over 28787: 110
-  // workgroups with work 48.6 us, 122 58.3; 500 queries, 115 152 us, 130 185). Of five splits or fewer one more saves more than
-  // that (32 / 8 heads, 64 places, 800 queries: three splits and 51 workgroups 315 us, four and 64 251).
-  const double places = (d128 ? 512.0 : 768.0) / Hkv;
-  int64_t fill = std::max<int64_t>(0, (int64_t)((2 * 0.87 * places - (double)(q - 1)) / (double)(q + 1) + 0.4));
-  if (fill <= 4 && (double)(fill + 1) * (double)(q + 1) + (double)(q - 1) <= 2.5 * places) ++fill;
+  // workgroups with work 48.6 us, 122 58.3; 500 queries, 115 152 us, 130 185). Of four or five splits or fewer one more saves
+  // more than that (32 / 8 heads, 64 places, 800 queries: three splits and 51 workgroups 315 us, four and 64 251).
+  // Of eight heads or more at head_dim 128, each on one XCD or all over all of them, less room serves for what is uneven (32 / 8, 400
+  // queries 147 and 132 us). A second block of a few rows is little work (32 / 32 heads, 130 queries over 41741 232 and 179).
+  const bool even = d128 && Hkv >= 8;
+  const double places = (d128 ? 512.0 : 768.0) / Hkv, b = rows <= kAttnBM + 24 ? (double)rows / kAttnBM : (double)q;
+  int64_t fill = std::max<int64_t>(0, (int64_t)((2 * (even ? 0.93 : 0.87) * places - (b - 1)) / (b + 1) + 0.4));
+  if (fill <= (even ? 3 : 4) && (double)(fill + 1) * (b + 1) + (b - 1) <= 2.5 * places) ++fill;
   // and no more than the partial rows cost: a split's chain falls by as much as writing and reading its rows takes
   const double chain_us = (double)tiles * (d128 ? 1.5 : 0.9), part_us = (double)n * Hq * (head_dim + 4) * 4e-6 * (d128 ? 0.18 : 0.25);
   const int64_t row_b = (int64_t)Hq * n * (head_dim + 4) * 4;

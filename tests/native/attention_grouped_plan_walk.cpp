@@ -28,7 +28,7 @@ int main() {
               ++taken_form;
               const int64_t tiles = ((int64_t)N + kAttnBN - 1) / kAttnBN, rows = (int64_t)n * group;
               const AttnMap& m = p.map;
-              bool ok = group > 1 && p.splits >= 2 && (int64_t)m.nqb * kAttnBM >= rows && (int64_t)p.splits * p.split_tiles >= tiles &&
+              bool ok = p.splits >= 2 && (int64_t)m.nqb * kAttnBM >= rows && (int64_t)p.splits * p.split_tiles >= tiles &&
                         (int64_t)(p.splits - 1) * p.split_tiles < tiles && p.splits * row_b <= ws;
               std::vector<char> taken((size_t)hkv * m.nqb * p.splits, 0);
               size_t count = 0;

@@ -221,6 +221,8 @@ def _attends(q, c, pos, rows, scale=None, **kw):
         (28, 4, 128, 8256, 8250, 33, 64),  # a head's (token, query head) rows in one block after another: two blocks
         (28, 4, 128, 8300, 8290, 251, 32),  # fourteen, and one of no rows
         (28, 4, 128, 4000, 3990, 160, 32),
+        (16, 16, 64, 8300, 8258, 300, 32),  # no shared heads
+        (8, 8, 128, 10500, 10433, 130, 64),
         (14, 2, 64, 4100, 4033, 251, 64),
         (32, 8, 128, 9000, 8999, 100, 128),
         (14, 2, 64, 16390, 16385, 40, 32),
