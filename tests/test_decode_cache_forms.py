@@ -1,0 +1,47 @@
+"""The kernel forms that the decode cache's launches can take, walked on the host, and whether the GPU tests' shapes leave one out."""
+
+import shutil
+import subprocess
+from pathlib import Path
+
+import pytest
+
+from tests import test_gpu_attention_weights as weights_tests
+from tests import test_gpu_attention_weights_forms as weights_forms
+
+ROOT = Path(__file__).resolve().parents[1]
+
+
+def _shapes(test, names):
+    """The parametrised shapes of a test."""
+    return next(m.args[1] for m in test.pytestmark if m.name == "parametrize" and m.args[0] == names)
+
+
+def _walker(tmp_path, name):
+    gxx = shutil.which("g++")
+    if gxx is None:
+        pytest.skip("g++ not available")
+    exe = tmp_path / name
+    subprocess.run([gxx, "-O2", "-std=c++17", f"-I{ROOT / 'chunkkv_amd' / 'csrc'}", str(ROOT / "tests" / "native" / f"{name}.cpp"), "-o", str(exe)],
+                   check=True)
+
+    def run(shapes=()):
+        text = "".join(" ".join(map(str, s)) + "\n" for s in shapes)
+        return subprocess.run([str(exe)], input=text, check=True, capture_output=True, text=True, timeout=300).stdout.splitlines()
+
+    return run
+
+
+def _forms(run, shapes):
+    lines = run(shapes)
+    assert len(lines) == len(shapes)
+    return {f for line in lines for f in line.split("; ")}
+
+
+def test_every_form_of_the_attention_weights_is_tested(tmp_path):
+    run = _walker(tmp_path, "attention_weights_forms")
+    *every, counts = run()
+    walked, bad = map(int, counts.split())
+    assert walked > 100_000 and bad == 0, every
+    shapes = _shapes(weights_tests.test_weights_match_the_plain_form, "Hq,Hkv,D,N,n") + weights_forms.SHAPES
+    assert set(every) - _forms(run, shapes) == set()

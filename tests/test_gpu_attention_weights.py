@@ -57,10 +57,10 @@ def _check(q, K, pos, prior=None, scale=None, out=None):
         (14, 2, 64, 13000, 520),  # more splits over a long cache
         (28, 4, 128, 2050, 18),  # 64 rows a workgroup, a split joined by the second pass
         (28, 4, 128, 1103, 128),  # in parts too
-        (28, 4, 128, 2050, 64),  # 448 rows and 16 splits: joined by a launch
+        (28, 4, 128, 2050, 64),  # 448 rows and 11 splits: joined by a launch
         (28, 4, 128, 5185, 3),
-        (14, 2, 64, 16500, 300),  # 128 rows a workgroup in the first pass, and in both
-        (14, 2, 64, 40000, 90),
+        (14, 2, 64, 16500, 300),  # 128 rows a workgroup in both passes
+        (14, 2, 64, 40000, 90),  # in the second only
         (16, 16, 64, 650, 250),
         (1, 1, 128, 300, 257),
     ],
