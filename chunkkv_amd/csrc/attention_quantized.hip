@@ -10,6 +10,7 @@
 //  - Every workgroup that reads a row converts it again, about a tenth of the kernel's time, so launches of many rows first write
 //    the cache as bf16 into the workspace, one pass, and attention.hip runs on that (kDecodeRows has both sides).
 #include "attention_large.hpp"
+#include "attention_quantized_plan.hpp"
 #include "attention_wave.hpp"
 
 namespace ckv {
@@ -45,9 +46,6 @@ __global__ __launch_bounds__(256) void decode_rows_kernel(char* __restrict__ k_o
 // the loop. Bound: from about 30 MB of codes their bytes, below the two launches. Measured (us, 28 / 4 heads of 128, one row,
 // with attention_wave.hpp's kernel on codes before): over 131072 rows 41.3 -> 29.8 (134 MB; reading as much and nothing else
 // takes 25), 65536 20.6 -> 17.0, 32832 15.2 -> 12.4, 8302 9.4 and 9.5; 8 heads of 64 over 65536 21.7 -> 15.7.
-constexpr int kCodeWaves = 4;
-constexpr int kCodeRows = 16;
-
 // LDS rows of D code bytes, PP = D / 16 pieces of 16: piece p of row r is at p ^ swz_code(r). The 16 rows that one S^T
 // operand reads, 8 a + 4 t + b (a, b < 4), and the 16 that two lane groups of a transposing read name, r and r + 1 .. + 15,
 // fall on distinct 16-byte places of 256 bytes.
@@ -374,34 +372,6 @@ __global__ __launch_bounds__(256) void join_rows_kernel(char* __restrict__ out, 
     *(uint2*)(out + ((int64_t)m * Hq + h) * (D * 2) + col * 2) =
         uint2{f32x2_to_bf16x2_bits(acc[0] * inv, acc[1] * inv), f32x2_to_bf16x2_bits(acc[2] * inv, acc[3] * inv)};
 }
-
-struct CodesPlan {
-  int splits, split_chunks;
-};
-// Splits of a launch of up to kCodeRows rows a KV head: a workgroup for each CU (two were slower to join and no faster
-// to read: 28 / 4 heads of 128 over 32832 rows 16.8 us, one 12.4), a chunk at least for each wavefront.
-static CodesPlan codes_plan(int n, int N, int Hq, int Hkv, int head_dim, int64_t workspace_bytes) {
-  const int64_t chunks = (N + kWaveChunk - 1) / kWaveChunk, row_b = (int64_t)Hq * n * (head_dim + 4) * 4;
-  // whole up to 1024 rows of 128 and 1536 of 64: the join is a launch (us, eager calls, whole and split: 28 / 4 heads of 128, 1000
-  // rows 7.8 and 9.6, 1400 rows 9.2 and 9.5 but 7.2 in a graph; 14 / 2 heads of 64, 1500 rows 7.5 and 9.6)
-  int64_t splits = chunks <= (head_dim == 128 ? 32 : 48) ? 1 : std::min<int64_t>(kWaveFill / Hkv, (chunks + kCodeWaves - 1) / kCodeWaves);
-  splits = std::max<int64_t>(1, std::min(splits, workspace_bytes / row_b));
-  CodesPlan p;
-  p.split_chunks = (int)((chunks + splits - 1) / splits);
-  p.splits = (int)((chunks + p.split_chunks - 1) / p.split_chunks);
-  return p;
-}
-static bool few_rows(int n, int Hq, int Hkv) { return (int64_t)n * (Hq / Hkv) <= kCodeRows; }
-// (token, query head) rows of a KV head from which a launch converts the cache first. That pass is the cache's bytes, the
-// conversion inside the kernel grows with the rows (us, converting inside and first: 28 / 4 heads of 128 over 28787 rows 128
-// queries 67 and 80, 500 175 and 176, 800 311 and 298; 14 / 2 heads of 64 over 65536, 128 57 and 65, 800 199 and 194; 16 / 16 of
-// 64 over 28787, 128 25 and 42, 2976 166 and 170). Cache lengths move the crossing little: both costs grow with them.
-constexpr int kDecodeRows = 3500;
-static bool decode_first(int n, int N, int Hq, int Hkv, int head_dim) {
-  return (int64_t)n * (Hq / Hkv) > kDecodeRows &&
-         !attn_plan(n, N, Hq, Hkv, head_dim, attn_workspace_bytes(n, N, Hq, head_dim)).wave;
-}
-static int64_t decoded_bytes(int N, int Hkv, int head_dim) { return (int64_t)Hkv * N * head_dim * 4; }
 
 }  // namespace ckv
 

@@ -8,6 +8,8 @@ import pytest
 
 from tests import test_gpu_attention_weights as weights_tests
 from tests import test_gpu_attention_weights_forms as weights_forms
+from tests import test_gpu_quantized_attention_forms as quantized_forms
+from tests import test_gpu_quantized_cache as quantized_tests
 
 ROOT = Path(__file__).resolve().parents[1]
 
@@ -44,4 +46,15 @@ def test_every_form_of_the_attention_weights_is_tested(tmp_path):
     walked, bad = map(int, counts.split())
     assert walked > 100_000 and bad == 0, every
     shapes = _shapes(weights_tests.test_weights_match_the_plain_form, "Hq,Hkv,D,N,n") + weights_forms.SHAPES
+    assert set(every) - _forms(run, shapes) == set()
+
+
+def test_every_form_of_attention_over_an_8_bit_cache_is_tested(tmp_path):
+    run = _walker(tmp_path, "attention_quantized_forms")
+    *every, counts = run()
+    walked, bad = map(int, counts.split())
+    assert walked > 100_000 and bad == 0, every
+    both = _shapes(quantized_tests.test_attention_matches_the_plain_form, "Hq,Hkv,D,N,rows,n,block")  # with and without a workspace
+    shapes = [(hq, hkv, d, N, n, ws) for hq, hkv, d, N, _, n, _ in both for ws in (0, 1)]
+    shapes += [(hq, hkv, d, N, n, 1) for hq, hkv, d, N, _, n, _ in quantized_forms.SHAPES]
     assert set(every) - _forms(run, shapes) == set()

@@ -211,11 +211,11 @@ def _attends(q, c, pos, rows, scale=None, **kw):
         (8, 8, 64, 333, 333, 333, 64),  # no shared heads, causal, ragged
         (14, 2, 64, 1103, 1103, 251, 32),
         (28, 4, 128, 1500, 1500, 1500, 64),  # 128-query workgroups: the cache read as bf16
-        (28, 4, 128, 8256, 8250, 130, 128),  # the same in splits, the codes converted by each
-        (28, 4, 128, 6001, 5985, 500, 32),  # at the change between these
+        (28, 4, 128, 8256, 8250, 130, 128),  # a head's (token, query head) rows, in splits of the cache
+        (28, 4, 128, 6001, 5985, 500, 32),
         (28, 4, 128, 6001, 5985, 501, 32),
         (14, 2, 64, 16390, 16385, 65, 64),
-        (16, 16, 64, 5700, 5633, 130, 128),
+        (16, 16, 64, 5700, 5633, 130, 128),  # 128-query workgroups in splits, the codes converted by each
         (32, 32, 128, 1100, 1090, 1000, 32),  # no shared heads: the codes converted, unsplit
         (64, 64, 64, 1000, 993, 910, 64),
         (28, 4, 128, 8256, 8250, 33, 64),  # a head's (token, query head) rows in one block after another: two blocks
