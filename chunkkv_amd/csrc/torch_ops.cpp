@@ -709,14 +709,24 @@ PyObject* attention_weights(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
   CKV_PY_END
 }
 
-// Whether the bytes that two caches' heads span have any in common.
-bool overlap(const Tensor& a, int64_t a_hs, const Tensor& b, int64_t b_hs) {
-  auto span = [](const Tensor& t, int64_t hs) {
-    const uintptr_t p = (uintptr_t)t.data_ptr();
-    return std::make_pair(p, p + (uintptr_t)(((t.size(1) - 1) * hs + t.size(2) * t.size(3)) * t.element_size()));
-  };
-  const auto x = span(a, a_hs), y = span(b, b_hs);
-  return x.first < y.second && y.first < x.second;
+// The bytes of a cache (1, H, rows, D): `count` heads of `size` each, `step` apart.
+struct HeadBytes {
+  uintptr_t at;
+  int64_t size, step, count;
+};
+HeadBytes head_bytes(const Tensor& t, int64_t head_stride) {
+  const int64_t e = t.element_size(), heads = t.size(1);
+  return {(uintptr_t)t.data_ptr(), heads > 0 ? t.numel() / heads * e : 0, head_stride * e, heads};
+}
+// Whether two caches have a byte in common. Caches whose heads take turns in one buffer have none. Heads ascend, so of two that do
+// not meet the lower one meets no later one either.
+bool overlap(const HeadBytes& a, const HeadBytes& b) {
+  for (int64_t i = 0, j = 0; i < a.count && j < b.count;) {
+    const uintptr_t x = a.at + i * a.step, y = b.at + j * b.step;
+    if (x < y + b.size && y < x + a.size) return true;
+    x < y ? ++i : ++j;
+  }
+  return false;
 }
 
 // evict_rows(K, V, weights, n_keep, n_sink, n_recent, k_out, v_out): (K, V, rows, weights) of the kept rows
@@ -755,9 +765,11 @@ PyObject* evict_rows(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
   const int64_t kohs = head_stride(ko, "k_out"), vohs = head_stride(vo, "v_out");
   const Tensor rows = new_tensor({1, H, keep}, at::kLong, K), wo = new_tensor({1, H, keep}, at::kFloat, K);
   if (keep > 0) {
-    if (given && (overlap(ko, kohs, K, khs) || overlap(ko, kohs, V, vhs) || overlap(vo, vohs, K, khs) || overlap(vo, vohs, V, vhs) ||
-                  overlap(ko, kohs, vo, vohs)))
-      value_error("k_out and v_out must overlap neither K, V nor each other");
+    if (given) {
+      const HeadBytes kb = head_bytes(K, khs), vb = head_bytes(V, vhs), kob = head_bytes(ko, kohs), vob = head_bytes(vo, vohs);
+      if (overlap(kob, kb) || overlap(kob, vb) || overlap(vob, kb) || overlap(vob, vb) || overlap(kob, vob))
+        value_error("k_out and v_out must overlap neither K, V nor each other");
+    }
     check(unlocked([&] {
             const c10::DeviceGuard on(K.device());
             return ckv_evict_rows(ptr(ko), kohs, ptr(vo), vohs, (int64_t*)ptr(rows), (float*)ptr(wo), ptr(K), khs, ptr(V), vhs,

@@ -44,3 +44,23 @@ def test_replays_match_eager(N):
         want = ops.evict_rows(K, V, w, 4000, 4, 32)
         assert torch.equal(e.rows, want.rows) and torch.equal(e.K, want.K) and torch.equal(e.V, want.V)
         assert torch.equal(e.weights.view(torch.int32), want.weights.view(torch.int32))
+
+
+def test_outputs_whose_heads_take_turns_with_others():
+    """Disjoint caches that share a buffer: K's and V's kept rows head by head in one, and behind the rows of the caches
+    that are cut."""
+    H, N, D, keep = 4, 700, 64, 150
+    K, V = E._caches(H, N, D, BF, 1)
+    w = E._weights(H, N, "spread", 2)
+    both = torch.zeros((1, H, 2, keep, D), dtype=BF, device=DEV)
+    E._check(K, V, w, keep, 4, 16, k_out=both[:, :, 0], v_out=both[:, :, 1])
+    assert both.any(-1).all()
+    slabs = E._caches(H, N + 200, D, BF, 3)
+    before = [t.clone() for t in slabs]
+    k, v = (t[:, :, :N] for t in slabs)
+    E._check(k, v, w, keep, 4, 16, k_out=slabs[0][:, :, N : N + keep], v_out=slabs[1][:, :, N : N + keep])
+    for t, b in zip(slabs, before):
+        assert torch.equal(t[:, :, :N], b[:, :, :N]) and torch.equal(t[:, :, N + keep :], b[:, :, N + keep :])
+    for bad in (slabs[0][:, :, N - 1 : N - 1 + keep], slabs[1][:, :, 3 : 3 + keep]):  # the last row of each head, and inside V
+        with pytest.raises(ValueError):
+            ops.evict_rows(k, v, w, keep, k_out=bad)
