@@ -709,7 +709,7 @@ PyObject* attention_weights(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
   CKV_PY_END
 }
 
-// The bytes of a cache (1, H, rows, D): `count` heads of `size` each, `step` apart.
+// The bytes of a tensor (1, H, ...): `count` heads of `size` each, `step` apart.
 struct HeadBytes {
   uintptr_t at;
   int64_t size, step, count;
@@ -767,8 +767,9 @@ PyObject* evict_rows(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
   if (keep > 0) {
     if (given) {
       const HeadBytes kb = head_bytes(K, khs), vb = head_bytes(V, vhs), kob = head_bytes(ko, kohs), vob = head_bytes(vo, vohs);
-      if (overlap(kob, kb) || overlap(kob, vb) || overlap(vob, kb) || overlap(vob, vb) || overlap(kob, vob))
-        value_error("k_out and v_out must overlap neither K, V nor each other");
+      const HeadBytes wb = head_bytes(w, whs);  // every workgroup reads all of a head's, others write by then
+      if (overlap(kob, kb) || overlap(kob, vb) || overlap(vob, kb) || overlap(vob, vb) || overlap(kob, vob) || overlap(kob, wb) || overlap(vob, wb))
+        value_error("k_out and v_out must overlap none of K, V, weights and each other");
     }
     check(unlocked([&] {
             const c10::DeviceGuard on(K.device());

@@ -744,7 +744,7 @@ def evict_rows(
     positions counted in them, as rows are appended behind.
 
     K/V: bf16 or float32, a head's rows contiguous (views of longer caches too). k_out/v_out: where the kept rows go,
-    (1, Hkv, n_keep, D) likewise (new tensors by default); they must not overlap K or V.
+    (1, Hkv, n_keep, D) likewise (new tensors by default); they must not overlap K, V, weights or each other.
     """
     return Evicted(*_native.torch_ops().evict_rows(K, V, weights, int(n_keep), int(n_sink), int(n_recent), k_out, v_out))
 

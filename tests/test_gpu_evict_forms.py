@@ -64,3 +64,15 @@ def test_outputs_whose_heads_take_turns_with_others():
     for bad in (slabs[0][:, :, N - 1 : N - 1 + keep], slabs[1][:, :, 3 : 3 + keep]):  # the last row of each head, and inside V
         with pytest.raises(ValueError):
             ops.evict_rows(k, v, w, keep, k_out=bad)
+
+
+def test_outputs_over_the_weights_are_refused():
+    """fp32 caches: an output in the weights' buffer would be written while other workgroups still rank by it."""
+    K, V = E._caches(2, 50, 64, F32, 1)
+    flat = torch.rand(3000, device=DEV)
+    w, keep = flat[: 2 * 50].view(1, 2, 50), 10
+    out = lambda at: flat[at : at + 2 * keep * 64].view(1, 2, keep, 64)  # noqa: E731
+    for kw in (dict(k_out=out(0)), dict(v_out=out(96)), dict(k_out=out(200), v_out=out(0))):
+        with pytest.raises(ValueError, match="overlap"):
+            ops.evict_rows(K, V, w, keep, **kw)
+    E._check(K, V, w, keep, 0, 0, k_out=out(100), v_out=out(100 + 2 * keep * 64))
