@@ -16,6 +16,13 @@ constexpr int kAttnBM = kAttnWaves * kAttnQG * 16;  // queries per workgroup
 constexpr int kAttnBN = 64;                         // cache rows per tile
 constexpr int kWaveChunk = 32;                      // cache rows per step of attn_wave_kernel's wavefronts
 
+// scale * log2(e), with which the kernels form exp(scale x) = exp2(x scale log2 e); 0 (no scale) where that is no normal fp32
+// number: a masked score, -infinity, times 0 is a NaN, and so is a score of 0 times infinity.
+static inline float log2_scale(double scale) {
+  const double s = scale * 1.4426950408889634;
+  return s >= 0x1p-126 && s < 0x1p128 * (1 - 0x1p-25) ? (float)s : 0.f;
+}
+
 constexpr int kXcds = 8;  // MI355X: workgroups go round-robin to 8 XCDs, each with its own L2
 
 // Which work item (query block qb, head h, cache split z) a workgroup takes. The hardware hands

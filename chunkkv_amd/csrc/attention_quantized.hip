@@ -398,7 +398,7 @@ extern "C" int32_t ckv_attention_quantized(void* out, const void* q, int64_t q_h
   using namespace ckv;
   if (head_dim != 64 && head_dim != 128) return CKV_ERR_INVALID_ARGUMENT;
   if (block_tokens != 32 && block_tokens != 64 && block_tokens != 128) return CKV_ERR_INVALID_ARGUMENT;
-  if (n_queries < 0 || n_tokens <= 0 || n_q_heads <= 0 || n_kv_heads <= 0 || n_q_heads % n_kv_heads != 0 || !(scale > 0.0))
+  if (n_queries < 0 || n_tokens <= 0 || n_q_heads <= 0 || n_kv_heads <= 0 || n_q_heads % n_kv_heads != 0 || log2_scale(scale) == 0.f)
     return CKV_ERR_INVALID_ARGUMENT;
   if (n_queries == 0) return CKV_OK;
   if (out == nullptr || q == nullptr || k_codes == nullptr || v_codes == nullptr || k_scales == nullptr ||
@@ -413,7 +413,7 @@ extern "C" int32_t ckv_attention_quantized(void* out, const void* q, int64_t q_h
   hipStream_t st = (hipStream_t)stream;
   if (workspace == nullptr || (uintptr_t)workspace % 16) workspace_bytes = 0;
 
-  const float scale_log2 = (float)(scale * 1.4426950408889634);  // exp(x) = exp2(x log2 e)
+  const float scale_log2 = log2_scale(scale);
   const int group = n_q_heads / n_kv_heads;
   const CacheScales scales = {(const uint8_t*)k_scales, (const uint8_t*)v_scales, blocks, block_log - 5};
   static_assert(kWaveChunk == 32, "a chunk has one scale");

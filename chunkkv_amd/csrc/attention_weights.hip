@@ -694,7 +694,7 @@ extern "C" int32_t ckv_attention_weights(float* out, const float* prior, const v
   using namespace ckv;
   if (out == nullptr) return CKV_ERR_INVALID_ARGUMENT;
   if (dtype != CKV_DTYPE_BF16 || (head_dim != 64 && head_dim != 128)) return CKV_ERR_INVALID_ARGUMENT;
-  if (n_queries < 0 || n_tokens <= 0 || n_q_heads <= 0 || n_kv_heads <= 0 || n_q_heads % n_kv_heads != 0 || !(scale > 0.0))
+  if (n_queries < 0 || n_tokens <= 0 || n_q_heads <= 0 || n_kv_heads <= 0 || n_q_heads % n_kv_heads != 0 || log2_scale(scale) == 0.f)
     return CKV_ERR_INVALID_ARGUMENT;
   const int group = n_q_heads / n_kv_heads;
   hipStream_t s = (hipStream_t)stream;
@@ -717,7 +717,7 @@ extern "C" int32_t ckv_attention_weights(float* out, const float* prior, const v
   if ((int64_t)n_queries * group > INT32_MAX / 2 || n_kv_heads > 65535) return CKV_ERR_TOO_LARGE;
   const int64_t need = ckv_attention_weights_workspace_bytes(n_queries, n_tokens, n_q_heads, n_kv_heads, head_dim);
   if (need > 0 && (workspace == nullptr || (uintptr_t)workspace % 16 || workspace_bytes < need)) return CKV_ERR_INVALID_ARGUMENT;
-  const float scale_log2 = (float)(scale * 1.4426950408889634);  // exp(x) = exp2(x log2 e)
+  const float scale_log2 = log2_scale(scale);
   if (n_queries * group <= kWtFewRows) {
     const bool whole = n_tokens <= kWtWholeRows;
     const FewPlan p = few_plan(n_queries * group, n_tokens, n_kv_heads);

@@ -579,7 +579,8 @@ int32_t ckv_quantize_rows(void* k_codes, void* v_codes, void* k_scales, void* v_
 
 /*
  * ckv_attention_active over an 8-bit cache (ckv_quantize_rows): the same function of the rows that codes and scales
- * stand for, which are bf16 values, with the same roundings. q, out, positions, scale and err as there. Rows past
+ * stand for, which are bf16 values, with the same roundings. q, out, positions, scale and err as there, and scale is within
+ * the normal fp32 numbers' range (CKV_ERR_INVALID_ARGUMENT otherwise). Rows past
  * the largest position may hold anything, as may the scales of blocks past its block; rows up to it are finite.
  *   workspace  optional device buffer of workspace_bytes >= ckv_attention_quantized_workspace_bytes(...)
  *              (16-byte aligned): partial rows of split launches and, for launches of many queries, the cache as
@@ -602,7 +603,7 @@ int64_t ckv_attention_quantized_workspace_bytes(int32_t n_queries, int32_t n_tok
  *   out[hk, j] = prior[hk, j] + sum over i and over h in group hk of w[h, i, j],
  *   w[h, i, :] = softmax over j in [0, positions[i]] of scale * q[h, i, :] . K[hk, j, :]   (0 past it).
  * prior (NULL: zeros) and out are (n_kv_heads, n_tokens) fp32 contiguous, the same or apart. q, k_cache, positions,
- * scale and err as in ckv_attention_active (bf16, head_dim 64 or 128, k_head_stride at least n_tokens * head_dim);
+ * scale and err as in ckv_attention_quantized (bf16, head_dim 64 or 128, k_head_stride at least n_tokens * head_dim);
  * rows past the largest position may hold anything, rows up to it are finite. Scores, weights and sums are fp32, added in a fixed order.
  *   workspace  device buffer of workspace_bytes >= ckv_attention_weights_workspace_bytes(...), 16-byte aligned
  * No counterpart in the reference.

@@ -159,3 +159,12 @@ print("alive")
     r = subprocess.run([sys.executable, "-c", PRELUDE + body], cwd=ROOT, env=env, capture_output=True, text=True, timeout=300)
     assert r.returncode == 0, (r.returncode, r.stdout[-2000:], r.stderr[-2000:])
     assert r.stdout.splitlines()[-1] == "alive"
+
+
+@pytest.mark.parametrize("scale", [1e-39, 1e-60, 5e-324, 3e38, 1e300, float("inf"), -float("inf")])
+def test_scales_that_fp32_cannot_hold_are_refused(scale):
+    """Their product with log2(e) is 0, subnormal or infinite there, and a masked score times it a NaN."""
+    assert _native.lib().ckv_attention_quantized(*_with(ATTN, scale=scale)) == INVALID
+    assert _native.lib().ckv_attention_weights(*_with(WEIGHTS, scale=scale)) == INVALID
+    assert _native.lib().ckv_attention_quantized(*_with(ATTN, scale=1e-37, n=0)) == OK
+    assert _native.lib().ckv_attention_weights(*_with(WEIGHTS, scale=2e38, n=0, prior=16)) == OK
