@@ -6,7 +6,8 @@
 // A power of two because e4m3 is a floating type, which gains nothing from a finer scale, while this one makes
 // every step but the rounding exact: x / s, code * s (a bf16 value), and a kept row's new codes when a row that
 // is appended to its block raises s (codes move by whole exponents; only those that fall below 2^-6 lose bits).
-// So a cache that grew row by row has the scales of one written at once.
+// So a cache that grew row by row has the scales of one written at once (unless rows were dropped and written again from the
+// middle of a block: its stored scale stands, which the dropped ones may have raised).
 //
 // Design: one workgroup per block, head and tensor holds the block's new rows in registers between the
 // maximum and the codes: each element is read once and written once. Bound: HBM for a prefill's rows (32832 bf16 rows of 4

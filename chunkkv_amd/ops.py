@@ -675,7 +675,8 @@ def quantize_rows(
     A block's scale is the least power of two 2^e that brings its largest |x| to at most 448 2^e, a code
     e4m3(x / scale) to nearest even. Rows in front of start, written by earlier calls, keep their values (their codes follow
     where their block's scale grows; only codes that become subnormal lose bits); rows behind start + n hold nothing any more. An infinity
-    or a NaN makes its block NaN. start: an int, or an int64 tensor of one element on the device, which a captured
+    or a NaN makes its block NaN. Writing again over dropped rows from the middle of a block keeps the scale that they may have
+    raised, from a block's first row on not. start: an int, or an int64 tensor of one element on the device, which a captured
     decode step reads on each replay (out of range: nothing is written, and err is set).
     """
     _native.torch_ops().quantize_rows(cache.k, cache.v, cache.k_scale, cache.v_scale, cache.block_tokens, k, v, start, err)

@@ -561,9 +561,11 @@ int64_t ckv_attention_workspace_bytes(int32_t n_queries, int32_t n_tokens, int32
  * (n_heads, ceil(n_tokens / block_tokens))); a row's values are code * scale.
  *   scale of a block = 2^e, e the least integer >= -126 with max |x| <= 448 * 2^e over the block's rows
  *   code             = e4m3(x / scale), to nearest even
- * Rows of the first block in front of `start` (written by earlier calls) are kept: the block's scale is the larger of theirs and the new
- * rows', and where it grows their codes are rescaled (exactly, but for codes that become subnormal). Rows
- * behind start + n_rows keep their bytes but not their scale: they hold nothing any more. An infinity or a
+ * Rows of the first block in front of `start` (written by earlier calls) are kept: the block's scale is the larger of the stored one and
+ * the new rows', and where it grows the kept codes are rescaled (exactly, but for codes that become subnormal). Rows
+ * behind start + n_rows keep their bytes but not their scale: they hold nothing any more. Where rows are dropped in this way and
+ * written again from the middle of a block, the stored scale may be one that the dropped rows raised (the kept codes
+ * follow it), NaN among them; from a block's first row on it is the new rows' alone. An infinity or a
  * NaN among the new rows makes its block's rows and scale NaN.
  *   k, v          the rows, (n_heads, n_rows, head_dim) with the given strides (elements; rows contiguous, 16-byte
  *                 aligned), bf16 or f32
