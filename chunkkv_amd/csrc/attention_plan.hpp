@@ -240,6 +240,11 @@ static inline AttnPlan attn_plan(int n, int N, int Hq, int Hkv, int head_dim, in
 // 28787, 160 132 and 68, 500 192 and 166; 14 / 2 heads of 64 over 28787, 25 20.6 and 17.5, 500 72 and 53, 1500 128 and 127, 2000 164 and
 // 169; over 4100, 160 19.2 and 14.3, 800 24.0 and 30.4; 16 / 16 heads of 64 over 41741, 288 51.9 and 41, 1000 100 and 80, 4000 270 and 241; 32 / 32
 // of 128, 130 171 and 179, 1000 671 and 460.
+// Those are of positions spread over the cache, which the splits below are counted for. Of query rows at its end, as a follow-up question
+// has them, every block has work in every split, 700 to 880 workgroups for the 512 places; the same, in graph replays: 28 / 4 heads of 128 over
+// 28787, 33 queries 65 and 36, 84 62 and 64, 160 126 and 92, 251 139 and 136, 500 254 and 256, 800 390 and 368; over 8302, 33 25.6 and 26.6, 84 31.7
+// and 37.9, 160 52.8 and 47.8, 251 57.7 and 56.6, 500 123 and 89; over 4100, 160 35.3 and 32.0, 500 65.8 and 58.1; 32 / 8 of 128 over 28787, 160 131 and 98, 500
+// 258 and 257; 14 / 2 of 64 over 28787, 40 27.0 and 23.9, 160 47.8 and 41.1, 500 84.2 and 79.7; 32 / 32 of 128 over 41741, 130 180 and 185, 1000 676 and 705.
 struct GroupedPlan {
   int splits = 0, split_tiles = 0;
   AttnMap map;

@@ -27,9 +27,13 @@ static inline CodesPlan codes_plan(int n, int N, int Hq, int Hkv, int head_dim, 
 }
 static inline bool few_rows(int n, int Hq, int Hkv) { return (int64_t)n * (Hq / Hkv) <= kCodeRows; }
 // (token, query head) rows of a KV head from which a launch converts the cache first. That pass is the cache's bytes, the
-// conversion inside the kernel grows with the rows (us, converting inside and first: 28 / 4 heads of 128 over 28787 rows 128
-// queries 67 and 80, 500 175 and 176, 800 311 and 298; 14 / 2 heads of 64 over 65536, 128 57 and 65, 800 199 and 194; 16 / 16 of
-// 64 over 28787, 128 25 and 42, 2976 166 and 170). Cache lengths move the crossing little: both costs grow with them.
+// conversion inside the kernel grows with the rows. Most launches near the bound take grouped rows (attn_grouped_plan); it decides
+// over caches of fewer than 4000 rows, and far behind it the launches of more rows than those take. us in graph replays, converting
+// inside and first, positions spread over the cache (at its end): 64 / 8 heads of 128 over 3900 rows, 3496 rows of a KV head 88.4 and 91.7 (89.3
+// and 92.7), 4800 92.9 and 95.4 (114.0 and 111.5), 16000 154.7 and 147.9 (189.7 and 182.6); 28 / 4 of 128 over 3900, 8400 88.6 and 89.2 (97.5 and
+// 93.8), 21000 99.6 and 98.1 (130.5 and 124.2); over 8302, 7000 107.8 and 101.7 (152 and 146); over 28787, 7000 318 and 290 (483 and 453), 20832 682
+// and 631 (1319 and 1196); 14 / 2 of 64 over 28787, 11900 148 and 141 (222 and 211). Without shared heads a row of the cache serves
+// one head and converting inside stays ahead over such a cache: 32 / 32 of 128, 3900 142.0 and 147.3, 16 / 16 of 64, 3900 60.0 and 70.8.
 constexpr int kDecodeRows = 3500;
 static inline bool decode_first(int n, int N, int Hq, int Hkv, int head_dim) {
   return (int64_t)n * (Hq / Hkv) > kDecodeRows &&

@@ -14,11 +14,12 @@
 //     query rows are split, and weights_reduce_kernel adds the parts in order (no atomics: the same sums every time).
 // Scores and sums are fp32 throughout, products bf16 x bf16 (exact) accumulated in fp32 on the matrix cores.
 //
-// Bound: the issue of a SIMD. A score costs a matrix instruction a quarter and, to stay in fp32, a product, an exponential and
-// an addition (the first pass: half a maximum too); alone these take 16.3 and 17.0 cycles for four scores a lane, both
-// together 28.3, whichever way the two are interleaved (within a wavefront, across wavefronts, by priority), so they
+// Bound: the issue of a SIMD. A wavefront's score a lane costs one matrix instruction at head_dim 128 (four make four) and, to stay in
+// fp32, a product, an exponential and an addition (the first pass: half a maximum too); alone these take 16.3 and 17.0 cycles for one
+// score a lane, both together 28.3, whichever way the two are interleaved (within a wavefront, across wavefronts, by priority), so they
 // hardly overlap. Measured (us, kernels traced, 28 / 4 heads of 128): 8256 causal rows 251 + 258 + 4, of which 175 each is that
-// issue at 2.4 GHz and the clock was near 2.0; 64 rows over 32832 21 + 20 and 4 for the join; one row over 8257 4.6 + 4.4.
+// issue at 2.4 GHz and the clock was near 2.0; 64 rows, spread over 32832, 21 + 20 and 4 for the join
+// (the last 64 rows, twice the work, 25 + 27 and 4); one row over 8257 4.6 + 4.4.
 // Slower: 64 rows a wavefront (275 and 320 us: two wavefronts a SIMD), exponentials one step behind the products (266, 283).
 #include <algorithm>
 

@@ -66,7 +66,11 @@ static inline WeightsPlan weights_plan(int n, int N, int Hq, int Hkv, int head_d
   // 64 rows a workgroup of the first pass in the place of 128 where there is little work (a wavefront's chain over a tile is half as
   // long, every K row is read twice as often): 28 / 4 heads of 128 (us, 128 rows and 64), 30 queries over 1103 16.0 and 14.1, 128 over
   // 8302 36.4 and 34.2, 128 over 16400 51.6 and 51.1, 251 84.9 and 87.8; over 65536 17 queries 37.8 and 40.2, but 8, which 64 rows
-  // hold, 33.8 and 28.9. 14 / 2 heads of 64, 251 over 16400 40.5 and 39.3, 500 over 32832 106 and 109.
+  // hold, 33.8 and 28.9. 14 / 2 heads of 64, 251 over 16400 40.5 and 39.3, 500 over 32832 106 and 109. The sides of the bound, in graph
+  // replays: with positions spread over the cache 64 rows lead to work = 14392 and past it (28 / 4 over 16400, 128 queries, work 7196, 42.8 and
+  // 40.4, 146, 8224, 50.1 and 49.4, 251, 14392, 64.2 and 63.6; 64 over 32832, 8208, 45.1 and 43.0); with query rows at the end of the
+  // cache up to it (128 52.4 and 51.4, 146 57.7 and 57.1, 64 over 32832 55.8 and 53.2) and not behind it (160 queries, 9252, 61.4 and 62.3;
+  // 91 over 32832, 10260, 69.2 and 71.2; 251 82.7 and 86.8).
   const int64_t work = (int64_t)((p.rows + 127) / 128) * tiles * Hkv;
   const bool short_rows = work <= 8300 && (int64_t)N * head_dim <= 5 << 20;
   p.qg = p.rows <= 64 || short_rows ? 1 : 2;
