@@ -692,8 +692,8 @@ def attention_quantized(
     split: bool = True,
 ) -> torch.Tensor:
     """attention_active over an 8-bit cache: the same function, with the same roundings, of the rows that its codes and
-    scales stand for. q, positions, scale, err and out as there; rows past the largest position may hold anything,
-    rows up to it are finite.
+    scales stand for. q, positions, scale, err and out as there (scale within fp32's normal range); rows past the largest
+    position may hold anything, rows up to it are finite.
     split: let launches use a workspace (allocated here): partial results where the cache range is split, and the cache as
     bf16 where many queries read it."""
     return _native.torch_ops().attention_quantized(q, cache.k, cache.v, cache.k_scale, cache.v_scale, cache.block_tokens,
@@ -715,7 +715,8 @@ def attention_weights(
 
     q: (1, Hq, n, D) bf16 with contiguous rows; K: (1, Hkv, N, D) bf16, a head's rows contiguous (e.g. a [:, :, :N] view of
     a longer cache), rows past the largest position anything, rows up to it finite. prior and out: float32 (1, Hkv, N) contiguous, and may be
-    one tensor (weights that grow over decode steps), else apart. Sums are fp32 in a fixed order.
+    one tensor (weights that grow over decode steps), else apart. scale is within fp32's normal range. Sums are fp32 in a fixed
+    order.
     """
     return _native.torch_ops().attention_weights(q, K, positions, scale, prior, out, err)
 
