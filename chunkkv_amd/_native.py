@@ -17,7 +17,7 @@ import torch  # noqa: F401  (must precede the CDLL load, see module docstring)
 
 LIB_PATH = Path(__file__).resolve().parent / "_lib" / "libchunkkv_amd.so"
 TORCH_OPS_PATH = LIB_PATH.with_name("_torch_ops.so")
-ABI_VERSION = 7
+ABI_VERSION = 8
 
 CKV_OK = 0
 CKV_ERR_INVALID_ARGUMENT = 1
@@ -44,6 +44,8 @@ POS_POOLED = 8
 
 SELECT_MAX_TOKENS = 131072
 DEVICE_ERR_RANGE = 1
+DEVICE_ERR_PAGES = 2  # fewer free pages than a sequence needs
+DEVICE_ERR_NO_TOKEN = 4  # every logit of a row is -infinity
 
 _p = ctypes.c_void_p
 _i32 = ctypes.c_int32
@@ -114,6 +116,34 @@ SIGNATURES = {
         _i32,
         [_p, _i64, _p, _i64, _p, _p, _p, _i64, _p, _i64, _p, _i64, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _p],
     ),
+    "ckv_extend_pages": (_i32, [_p, _p, _p, _i32, _p, _p, _p, _p, _i32, _i32, _i32, _i32, _p, _p]),
+    "ckv_fork_pages": (
+        _i32,
+        [_p, _p, _i64, _i64, _i32, _i32, _i32, _i32, _p, _p, _i32, _p, _p, _p, _i32, _i32, _i32, _i32, _p, _i64, _p, _p],
+    ),
+    "ckv_fork_pages_workspace_bytes": (_i64, [_i32]),
+    "ckv_free_pages": (_i32, [_p, _i32, _p, _p, _p, _i32, _i32, _i32, _i32, _p, _p]),
+    "ckv_compact_pages": (
+        _i32,
+        [_p, _p, _i64, _i64, _i32, _i32, _i32, _i32, _p, _p, _p, _p, _i32, _i32, _i32, _i32, _p, _i64, _p, _p],
+    ),
+    "ckv_compact_pages_workspace_bytes": (_i64, [_i32]),
+    "ckv_attention_paged": (
+        _i32,
+        [_p, _p, _i64, _i64, _p, _p, _i64, _p, _p, _p, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _f64, _p,
+         _i64, _p, _p],
+    ),
+    "ckv_attention_paged_workspace_bytes": (_i64, [_i32] * 8),
+    "ckv_adjust_logits": (
+        _i32,
+        [_p, _p, _i64, _i32, _i32, _i32, _p, _i64, _i32, _p, _i64, _i32, _p, _f32, _p, _f32, _p, _f32, _p, _i64, _p, _i64, _p],
+    ),
+    "ckv_next_tokens": (
+        _i32,
+        [_p, _p, _i64, _i32, _i32, _i32, _p, _i64, _i32, _p, _i64, _i32, _p, _f32, _p, _f32, _p, _f32, _p, _i64, _p, _i64, _p,
+         _i64, _p, _p],
+    ),
+    "ckv_next_tokens_workspace_bytes": (_i64, [_i32, _i32]),
     "ckv_add_rmsnorm": (_i32, [_p, _p, _p, _p, _p, _i64, _i32, _f32, _i32, _p]),
     "ckv_silu_mul": (_i32, [_p, _i64, _p, _i64, _p, _i64, _i64, _i32, _i32, _p]),
     "ckv_linear": (_i32, [_p, _p, _i64, _p, _p, _i32, _i32, _i32, _i32, _p, _i64, _p]),

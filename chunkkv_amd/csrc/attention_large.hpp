@@ -1,8 +1,9 @@
 // The attention of launches that 128-query workgroups fill (attention.hip describes it; attention_quantized.hip runs it over
-// 8-bit caches).
+// 8-bit caches, attention_paged.hip over paged ones).
 #pragma once
 
 #include "attention_common.hpp"
+#include "attention_paged.hpp"
 
 namespace ckv {
 
@@ -10,6 +11,8 @@ namespace ckv {
 // this one is worked on, and makes them bf16 on their way into the other buffer, once for the workgroup's 128 queries. The
 // same occupancy (230 and 144 registers at head_dim 128 and 64) and about a tenth more time (us, codes and bf16 rows: 28 / 4 heads
 // of 128, 128 queries over 28787 rows 67 and 62, 300 177 and 163; 14 / 2 heads of 64, 500 over 65536 136 and 126).
+// With a PagedRows argument a workgroup has 128 of the (token, query head) rows of a sequence's KV head (positions and the number of cached
+// rows are the sequence's), and a wavefront takes its part of a tile, which lies in one half of it, from the page that has those rows.
 // SPLIT: split z of the cache's tiles per workgroup, unnormalised rows with their max and sum to ws.
 template <int D, bool SPLIT, typename... Scales>
 __global__ __launch_bounds__(kAttnWaves * 64) void attn_active_kernel(
@@ -17,7 +20,8 @@ __global__ __launch_bounds__(kAttnWaves * 64) void attn_active_kernel(
     const int64_t* __restrict__ pos, int n, int N, const char* __restrict__ kc, const char* __restrict__ vc,
     int64_t kv_hs_b, const char* __restrict__ q, int64_t q_hs_b, int64_t q_ts_b, int Hq, int group, float scale_log2,
     char* __restrict__ out, int32_t* __restrict__ err, float* __restrict__ ws, int split_tiles, Scales... scales) {
-  constexpr bool CODES = sizeof...(Scales) == 1, GROUPED = (std::is_same_v<Scales, GroupedCacheScales> || ...);
+  constexpr bool PAGED = (std::is_same_v<Scales, PagedRows> || ...), CODES = sizeof...(Scales) == 1 && !PAGED;
+  constexpr bool GROUPED = PAGED || (std::is_same_v<Scales, GroupedCacheScales> || ...);
   constexpr int DS = D / 32;          // k-steps of S^T = K Q^T
   constexpr int DT = D / 16;          // 16-row tiles of O^T
   constexpr int CPR = D / 8;          // 16-byte chunks per cache row
@@ -39,6 +43,19 @@ __global__ __launch_bounds__(kAttnWaves * 64) void attn_active_kernel(
   int qb, hq, z;
   if (!attn_work_item(nqb, map_group, xpk_log, items, inv_group, inv_nqb, qb, hq, z)) return;
   const int hk = GROUPED ? hq : hq / group;
+  [[maybe_unused]] PagedItem it;
+  [[maybe_unused]] const int item = qb;
+  if constexpr (PAGED) {
+    if (!(paged_item<kAttnBM, kAttnBN>(scales, n, group, item, it), ...)) return;
+    qb = it.tile;
+    z = it.z;
+    n = it.count;
+    N = it.rows;
+    q += (int64_t)it.first * q_ts_b;
+    out += (int64_t)it.first * Hq * (D * 2);
+    split_tiles = it.split_units;
+  }
+  const bool part = SPLIT && (!PAGED || it.splits > 1);
   const int rows = GROUPED ? n * group : n;
   auto token_of = [&](int m) {  // of row m
     if constexpr (GROUPED) return div_by(m, group, (scales.inv_gqa, ...));
@@ -55,8 +72,10 @@ __global__ __launch_bounds__(kAttnWaves * 64) void attn_active_kernel(
     const int m = q0 + qg * 16 + lm;
     int p = -1;
     if (m < rows) {
-      const int64_t p64 = pos[token_of(m)];
-      if (p64 < 0 || p64 >= N) {
+      const int64_t p64 = PAGED ? N - n + token_of(m) : pos[token_of(m)];
+      if (PAGED) {
+        p = (int)max(p64, (int64_t)-1);  // -1: no row to see
+      } else if (p64 < 0 || p64 >= N) {
         flag_error(err, CKV_DEVICE_ERR_RANGE);
         p = p64 < 0 ? 0 : N - 1;
       } else {
@@ -76,8 +95,8 @@ __global__ __launch_bounds__(kAttnWaves * 64) void attn_active_kernel(
   for (int w = 1; w < kAttnWaves; ++w) bmax = max(bmax, blk_max_s[w]);
   bmax = __builtin_amdgcn_readfirstlane(bmax);
   int n_tiles = bmax < 0 ? 0 : bmax / kAttnBN + 1;
-  const int tile_begin = SPLIT ? z * split_tiles : 0;
-  if (SPLIT) n_tiles = min(n_tiles, tile_begin + split_tiles);
+  const int tile_begin = part ? z * split_tiles : 0;
+  if (part) n_tiles = min(n_tiles, tile_begin + split_tiles);
 
   // Q fragments (B operand of S^T): query q0 + 16 qg + lm, head-dim 32 s + 8 g .. + 8.
   bf16x8 qf[kAttnQG][DS];
@@ -130,15 +149,34 @@ __global__ __launch_bounds__(kAttnWaves * 64) void attn_active_kernel(
   for (int i = 0; i < KI; ++i) {
     const int P = (wave * KI + i) * 64 + lane;
     const int slot = P / CPR, pc = P % CPR;
-    off_k[i] = kslot_row(slot) * ROWB + (pc ^ swz_k<CPR>(slot)) * 16;
-    off_v[i] = slot * ROWB + (pc ^ swz_v<CPR>(slot)) * 16;
+    auto from = [](int row) { return PAGED ? row & 31 : row; };  // paged: row of its half of the tile
+    off_k[i] = from(kslot_row(slot)) * ROWB + (pc ^ swz_k<CPR>(slot)) * 16;
+    off_v[i] = from(slot) * ROWB + (pc ^ swz_v<CPR>(slot)) * 16;
   }
+  static_assert(KI * 64 * kAttnWaves / 2 == 32 * CPR, "two wavefronts load a half of a tile");
   typedef __attribute__((address_space(1))) void gvoid;
   typedef __attribute__((address_space(3))) void lvoid;
+  // Paged: the pages of this wavefront's halves of the next 64 tiles, a tile a lane.
+  [[maybe_unused]] int pages = 0, pages_from = tile_begin - 64;
+  [[maybe_unused]] auto page_row = [&](int tile, int at, const PagedRows& b) {  // where row `at` of the sequence is
+    if (tile - pages_from >= 64) {  // uniform
+      pages_from = tile;
+      const int r = (int)min((int64_t)(tile + lane) * kAttnBN + 32 * (wave / 2), (int64_t)bmax);
+      pages = paged_page(b, b.table + (int64_t)it.seq * b.M, r >> b.T_log);
+    }
+    return ((int64_t)__builtin_amdgcn_readlane(pages, tile - pages_from) << b.T_log) + (at & ((1 << b.T_log) - 1));
+  };
   auto issue = [&](int n0, char* kb, char* vb) {
     const char* kt = kh + (int64_t)n0 * ROWB;
     const char* vt = vh + (int64_t)n0 * ROWB;
-    const int last = bmax - n0;  // >= 0: only tiles that some query sees are issued
+    int last = bmax - n0;  // >= 0: only tiles that some query sees are issued
+    if constexpr (PAGED) {
+      const int first = n0 + 32 * (wave / 2), at = min(first, bmax);  // a half that no query sees loads the last row
+      const int64_t off = (page_row(n0 / kAttnBN, at, scales), ...) * ROWB;
+      kt = kh + off;
+      vt = vh + off;
+      last = bmax - at >= 31 ? kAttnBN - 1 : bmax - at;
+    }
     auto load = [&](const char* t, int off, char* to) {
       __builtin_amdgcn_global_load_lds((gvoid*)(t + (uint32_t)off), (lvoid*)to, 16, 0, 0);
     };
@@ -323,10 +361,11 @@ __global__ __launch_bounds__(kAttnWaves * 64) void attn_active_kernel(
     if (m >= rows) continue;
     const int t = token_of(m), h = head_of(m, t);
     if constexpr (GROUPED && SPLIT) {
-      if (my_pos[qg] < tile_begin * kAttnBN) continue;  // nothing of this split: its row is not read
+      if (part && my_pos[qg] < tile_begin * kAttnBN) continue;  // nothing of this split: its row is not read
     }
-    if (SPLIT) {
+    if (part) {
       float* prow = ws + (((int64_t)z * Hq + h) * n + t) * (D + 4);  // 16-byte aligned rows
+      if constexpr (PAGED) prow = ws + (((int64_t)hk * (scales.cap, ...) + item) * kAttnBM + m - qb * kAttnBM) * (D + 4);
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt) *(f32x4*)(prow + dt * 16 + 4 * g) = o[qg][dt];
       if (g == 0) {
@@ -335,7 +374,7 @@ __global__ __launch_bounds__(kAttnWaves * 64) void attn_active_kernel(
       }
       continue;
     }
-    const float inv = 1.f / l;
+    const float inv = PAGED && l == 0.f ? 0.f : 1.f / l;
     char* orow = out + ((int64_t)t * Hq + h) * (D * 2);
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) {

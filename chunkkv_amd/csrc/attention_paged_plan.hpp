@@ -1,0 +1,42 @@
+// How a launch of attention over a paged cache runs (attention_paged.hip). Host arithmetic only, without HIP, so that it
+// can be walked on a machine without a GPU.
+#pragma once
+
+#include "attention_plan.hpp"
+
+namespace ckv {
+
+constexpr int kPagedWaves = 4;                           // wavefronts of attn_paged_kernel
+constexpr int kPagedUnit = kPagedWaves * kWaveChunk;     // cache rows that a split is a multiple of there
+
+struct PagedPlan {
+  int rows = 0;    // (token, query head) rows of a tile: 16 or 32 (attn_paged_kernel), 128 (attn_active_kernel)
+  int target = 0;  // items of a KV head that splits aim at, beside the tiles; 0: the cache is not split
+  int min_units = 0;
+  int64_t items = 0;  // of a KV head, at most
+  int64_t ws_bytes = 0;
+  AttnMap map;
+};
+
+// n new tokens of S sequences, at most `most` of one, over at most `rows` cached rows each. Lengths are the device's: the items
+// are bounded by tiles (a sequence's last one may be partial) and by what splits add.
+static inline PagedPlan paged_plan(int64_t n, int64_t S, int64_t most, int64_t rows, int Hq, int Hkv, int head_dim, int64_t workspace_bytes) {
+  PagedPlan p;
+  const int64_t group = Hq / Hkv, one = std::min(most, n) * group;
+  p.rows = one <= 16 ? 16 : one <= 32 ? 32 : kAttnBM;
+  const int64_t tiles = n * group / p.rows + std::min(S, n);
+  const bool large = p.rows == kAttnBM;
+  const int unit = large ? kAttnBN : kPagedUnit;
+  // Workgroups that are resident at once.
+  const int64_t fill = 512 / Hkv;
+  p.min_units = large ? 4 : 2;
+  p.target = rows <= (int64_t)p.min_units * unit || (large && n * group / p.rows >= fill) ? 0 : (int)std::max<int64_t>(fill, 1);
+  const int64_t row_b = (int64_t)Hkv * p.rows * (head_dim + 4) * 4;
+  if (p.target > 0 && (tiles + p.target) * row_b > workspace_bytes) p.target = 0;
+  p.items = tiles + p.target;
+  p.ws_bytes = p.target > 0 ? p.items * row_b : 0;
+  if (p.items * Hkv < (1 << 30)) p.map = attn_map(p.items, Hkv, 1, 1);
+  return p;
+}
+
+}  // namespace ckv

@@ -783,7 +783,316 @@ PyObject* evict_rows(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
   CKV_PY_END
 }
 
+// The book of a paged cache: table (S, M), lengths (S,) and refs (P,), int32 on one device.
+struct PageBook {
+  const Tensor &table, &lengths, &refs;
+  int64_t S, M, P, T;
+  int32_t* at(const Tensor& t) const { return (int32_t*)ptr(t); }
+};
+PageBook page_book(PyObject* const* a) {
+  const Tensor &table = tensor(a[0]), &lengths = tensor(a[1]), &refs = tensor(a[2]);
+  const int64_t T = integer(a[3]);
+  same_device(table, lengths, refs);
+  if (T != 32 && T != 64 && T != 128) value_error("page_tokens must be 32, 64 or 128");
+  if (table.scalar_type() != at::kInt || lengths.scalar_type() != at::kInt || refs.scalar_type() != at::kInt)
+    type_error("table, lengths and refs must be int32");
+  if (table.dim() != 2 || lengths.dim() != 1 || refs.dim() != 1 || table.size(0) != lengths.size(0) || !table.is_contiguous() ||
+      !lengths.is_contiguous() || !refs.is_contiguous())
+    value_error("table must be (sequences, entries), lengths (sequences,) and refs (pages,), contiguous");
+  if (table.numel() == 0 || refs.numel() == 0) value_error("a paged cache has a sequence, an entry and a page at least");
+  if (table.size(0) > INT32_MAX || table.size(1) > INT32_MAX || refs.size(0) > INT32_MAX) value_error("too many pages");
+  return {table, lengths, refs, table.size(0), table.size(1), refs.size(0), T};
+}
+// Pools (L, 1, H, P * T, D) of K and V.
+struct PagePool {
+  const Tensor &k, &v;
+  int64_t L, H, D;
+};
+PagePool page_pool(const PageBook& b, PyObject* ko, PyObject* vo) {
+  const Tensor &k = tensor(ko), &v = tensor(vo);
+  same_device(b.table, k, v);
+  need_dims(k, 5, "a paged cache's k");
+  if (v.scalar_type() != k.scalar_type()) type_error("k and v must share a dtype");
+  if (k.size(1) != 1 || k.size(3) != b.P * b.T || v.sizes() != k.sizes() || !k.is_contiguous() || !v.is_contiguous() || k.numel() == 0)
+    value_error("a paged cache's k and v must be contiguous (layers, 1, Hkv, pages * page_tokens, D)");
+  if (k.size(0) > INT32_MAX || k.size(2) > INT32_MAX || k.size(4) > INT32_MAX) value_error("a paged cache's k is too large");
+  return {k, v, k.size(0), k.size(2), k.size(4)};
+}
+// An int32 vector on the book's device.
+Tensor int_vector(PyObject* o, const PageBook& b, const char* what) {
+  Tensor t = tensor(o);
+  same_device(b.table, t);
+  if (t.scalar_type() != at::kInt || t.dim() != 1) value_error(std::string(what) + " must be int32 of one dimension");
+  if (t.numel() > INT32_MAX) value_error(std::string(what) + " is too long");
+  return t.contiguous();
+}
+
+// extend_pages(table, lengths, refs, page_tokens, counts, n, err): (positions, rows, starts)
+PyObject* extend_pages(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
+  CKV_PY_BEGIN
+  need_args(n_args, 7);
+  const PageBook b = page_book(a);
+  const Tensor counts = int_vector(a[4], b, "counts"), err = optional_tensor(a[6]);
+  const int64_t n = integer(a[5]);
+  if (counts.numel() != b.S) value_error("counts must be (sequences,)");
+  if (n < 0 || n > INT32_MAX) value_error("n must be 0 to 2^31 - 1");
+  const Tensor positions = new_tensor({n}, at::kLong, b.table), rows = new_tensor({n}, at::kLong, b.table);
+  const Tensor starts = new_tensor({b.S + 1}, at::kInt, b.table);
+  int32_t* const e = status_word(err, b.table);
+  check(unlocked([&] {
+          const c10::DeviceGuard on(b.table.device());
+          return ckv_extend_pages((int64_t*)ptr(positions), (int64_t*)ptr(rows), (int32_t*)ptr(starts), int32(n), (const int32_t*)ptr(counts),
+                                  b.at(b.table), b.at(b.lengths), b.at(b.refs), int32(b.S), int32(b.M), int32(b.P), int32(b.T), e,
+                                  stream_of(b.table));
+        }),
+        "ckv_extend_pages");
+  return Py_BuildValue("(NNN)", THPVariable_Wrap(positions), THPVariable_Wrap(rows), THPVariable_Wrap(starts));
+  CKV_PY_END
+}
+
+// fork_pages(table, lengths, refs, page_tokens, k, v, sources, targets, err)
+PyObject* fork_pages(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
+  CKV_PY_BEGIN
+  need_args(n_args, 9);
+  const PageBook b = page_book(a);
+  const PagePool p = page_pool(b, a[4], a[5]);
+  const Tensor sources = int_vector(a[6], b, "sources"), targets = int_vector(a[7], b, "targets"), err = optional_tensor(a[8]);
+  const int64_t n = sources.numel();
+  if (targets.numel() != n) value_error("sources and targets must be of one length");
+  const int code = dtype_code(p.k);
+  const int64_t ws_bytes = ckv_fork_pages_workspace_bytes(int32(n));
+  Tensor ws;
+  if (ws_bytes > 0) ws = new_tensor({ws_bytes / 4}, at::kInt, b.table);
+  int32_t* const e = status_word(err, b.table);
+  check(unlocked([&] {
+          const c10::DeviceGuard on(b.table.device());
+          return ckv_fork_pages(ptr(p.k), ptr(p.v), p.k.stride(0), p.k.stride(2), int32(p.L), int32(p.H), int32(p.D), code,
+                                (const int32_t*)ptr(sources), (const int32_t*)ptr(targets), int32(n), b.at(b.table), b.at(b.lengths),
+                                b.at(b.refs), int32(b.S), int32(b.M), int32(b.P), int32(b.T), ptr(ws), ws_bytes, e, stream_of(b.table));
+        }),
+        "ckv_fork_pages");
+  Py_RETURN_NONE;
+  CKV_PY_END
+}
+
+// free_pages(table, lengths, refs, page_tokens, sequences, err)
+PyObject* free_pages(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
+  CKV_PY_BEGIN
+  need_args(n_args, 6);
+  const PageBook b = page_book(a);
+  const Tensor sequences = int_vector(a[4], b, "sequences"), err = optional_tensor(a[5]);
+  int32_t* const e = status_word(err, b.table);
+  check(unlocked([&] {
+          const c10::DeviceGuard on(b.table.device());
+          return ckv_free_pages((const int32_t*)ptr(sequences), int32(sequences.numel()), b.at(b.table), b.at(b.lengths), b.at(b.refs),
+                                int32(b.S), int32(b.M), int32(b.P), int32(b.T), e, stream_of(b.table));
+        }),
+        "ckv_free_pages");
+  Py_RETURN_NONE;
+  CKV_PY_END
+}
+
+// compact_pages(table, lengths, refs, page_tokens, k, v, err): used
+PyObject* compact_pages(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
+  CKV_PY_BEGIN
+  need_args(n_args, 7);
+  const PageBook b = page_book(a);
+  const PagePool p = page_pool(b, a[4], a[5]);
+  const Tensor err = optional_tensor(a[6]);
+  const int code = dtype_code(p.k);
+  const int64_t ws_bytes = ckv_compact_pages_workspace_bytes(int32(b.P));
+  const Tensor ws = new_tensor({ws_bytes / 4}, at::kInt, b.table), used = new_tensor({1}, at::kInt, b.table);
+  int32_t* const e = status_word(err, b.table);
+  check(unlocked([&] {
+          const c10::DeviceGuard on(b.table.device());
+          return ckv_compact_pages(ptr(p.k), ptr(p.v), p.k.stride(0), p.k.stride(2), int32(p.L), int32(p.H), int32(p.D), code,
+                                   (int32_t*)ptr(used), b.at(b.table), b.at(b.lengths), b.at(b.refs), int32(b.S), int32(b.M), int32(b.P),
+                                   int32(b.T), ptr(ws), ws_bytes, e, stream_of(b.table));
+        }),
+        "ckv_compact_pages");
+  return THPVariable_Wrap(used);
+  CKV_PY_END
+}
+
+// attention_paged(q, table, lengths, refs, page_tokens, k, v, layer, starts, most, scale, err, out, split)
+PyObject* attention_paged(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
+  CKV_PY_BEGIN
+  need_args(n_args, 14);
+  Tensor q = tensor(a[0]);
+  const PageBook b = page_book(a + 1);
+  const PagePool p = page_pool(b, a[5], a[6]);
+  const int64_t layer = integer(a[7]), most = a[9] == Py_None ? 0 : integer(a[9]);
+  const Tensor starts = int_vector(a[8], b, "starts"), err = optional_tensor(a[11]);
+  Tensor out = optional_tensor(a[12]);
+  same_device(q, p.k);
+  need_dims(q, 4, "q");
+  if (q.scalar_type() != at::kBFloat16 || p.k.scalar_type() != at::kBFloat16) type_error("attention_paged runs on bf16 q and cache");
+  const int64_t Hq = q.size(1), n = q.size(2);
+  if (q.size(0) != 1 || q.size(3) != p.D) value_error("q " + shape_of(q) + " must be (1, Hq, n, D) and match the cache's head_dim");
+  if (Hq <= 0 || Hq % p.H) value_error("the query heads must be a multiple of the KV heads");
+  if (n > INT32_MAX || Hq > INT32_MAX) value_error("too many query rows");
+  if (layer < 0 || layer >= p.L) value_error("layer " + std::to_string(layer) + " of a cache of " + std::to_string(p.L));
+  if (starts.numel() != b.S + 1) value_error("starts must be (sequences + 1,)");
+  if (a[9] != Py_None && (most < 1 || most > INT32_MAX)) value_error("most must be 1 to 2^31 - 1");
+  q = rows_view(q);
+  if (!out.defined()) {
+    out = new_tensor({1, n, Hq, p.D}, at::kBFloat16, q);
+  } else {
+    same_device(q, out);
+    if (out.sizes() != at::IntArrayRef({1, n, Hq, p.D}) || !out.is_contiguous() || out.scalar_type() != at::kBFloat16)
+      value_error("out must be contiguous (1, n, Hq, D) bf16");
+  }
+  const double scale = a[10] == Py_None ? 1.0 / std::sqrt((double)p.D) : real(a[10]);
+  const int split = PyObject_IsTrue(a[13]);
+  if (split < 0) throw python_error();
+  const int64_t ws_bytes = split ? ckv_attention_paged_workspace_bytes(int32(n), int32(b.S), int32(most ? most : n), int32(b.M), int32(b.T),
+                                                                       int32(Hq), int32(p.H), int32(p.D))
+                                 : 0;
+  Tensor ws;
+  if (ws_bytes > 0) ws = new_tensor({(ws_bytes + 3) / 4}, at::kFloat, q);
+  int32_t* const e = status_word(err, q);
+  check(unlocked([&] {
+          const c10::DeviceGuard on(q.device());
+          const int64_t at = layer * p.k.stride(0) * 2;
+          return ckv_attention_paged(ptr(out), ptr(q), step(q, 1, n * p.D), step(q, 2, p.D), (const char*)ptr(p.k) + at,
+                                     (const char*)ptr(p.v) + at, p.k.stride(2), b.at(b.table), b.at(b.lengths), (const int32_t*)ptr(starts),
+                                     int32(n), int32(most), int32(b.S), int32(b.M), int32(b.P), int32(b.T), int32(Hq), int32(p.H), int32(p.D),
+                                     CKV_DTYPE_BF16, scale, ptr(ws), ws_bytes, e, stream_of(q));
+        }),
+        "ckv_attention_paged");
+  return THPVariable_Wrap(out);
+  CKV_PY_END
+}
+
+// What adjust_logits and next_tokens share: (logits, prompt, generated, repetition, frequency, presence, bias, allowed).
+struct LogitArgs {
+  const Tensor& logits;
+  int64_t rows, vocab, row_stride;
+  int code;
+  Tensor prompt, generated, repetition, frequency, presence, bias, allowed;
+  float repetition_all = 1.f, frequency_all = 0.f, presence_all = 0.f;
+};
+LogitArgs logit_args(PyObject* const* a) {
+  const Tensor& x = tensor(a[0]);
+  same_device(x);
+  need_dims(x, 2, "logits");
+  if (x.scalar_type() != at::kBFloat16 && x.scalar_type() != at::kFloat) type_error("logits must be bfloat16 or float32");
+  LogitArgs r{x, x.size(0), x.size(1), 0, dtype_code(x), {}, {}, {}, {}, {}, {}, {}};
+  if (r.vocab < 1 || r.vocab > INT32_MAX || r.rows > INT32_MAX) value_error("logits must be (rows, vocab)");
+  if (r.vocab > 1 && x.stride(1) != 1) value_error("logits must have contiguous rows");
+  r.row_stride = step(x, 0, r.vocab);
+  if (r.row_stride < r.vocab) value_error("logits rows overlap");
+  auto tokens = [&](PyObject* o, const char* what) {
+    Tensor t = optional_tensor(o);
+    if (!t.defined()) return t;
+    same_device(x, t);
+    if (t.scalar_type() != at::kLong || t.dim() != 2 || t.size(0) != r.rows || t.size(1) > INT32_MAX)
+      value_error(std::string(what) + " must be int64 (rows, tokens)");
+    if (t.size(1) > 1 && t.stride(1) != 1) t = t.contiguous();
+    return t;
+  };
+  r.prompt = tokens(a[1], "prompt");
+  r.generated = tokens(a[2], "generated");
+  auto value = [&](PyObject* o, float& all, const char* what) {
+    Tensor t;
+    if (!THPVariable_Check(o)) {
+      all = (float)real(o);
+      return t;
+    }
+    t = tensor(o);
+    same_device(x, t);
+    if (t.scalar_type() != at::kFloat || t.dim() != 1 || t.size(0) != r.rows)
+      value_error(std::string(what) + " must be a number or float32 (rows,)");
+    return t.contiguous();
+  };
+  r.repetition = value(a[3], r.repetition_all, "repetition");
+  r.frequency = value(a[4], r.frequency_all, "frequency");
+  r.presence = value(a[5], r.presence_all, "presence");
+  if (!(r.repetition_all > 0.f)) value_error("repetition must be above 0");
+  auto per_row = [&](PyObject* o, at::ScalarType type, int64_t width, const char* what) {
+    Tensor t = optional_tensor(o);
+    if (!t.defined()) return t;
+    same_device(x, t);
+    if (t.dim() == 1) t = t.unsqueeze(0);
+    if (t.scalar_type() != type || t.dim() != 2 || (t.size(0) != 1 && t.size(0) != r.rows) || t.size(1) != width)
+      value_error(std::string(what) + " must be of " + std::to_string(width) + " for each row or for all, " + c10::toString(type));
+    if (width > 1 && t.stride(1) != 1) t = t.contiguous();
+    return t;
+  };
+  r.bias = per_row(a[6], at::kFloat, r.vocab, "bias");
+  r.allowed = per_row(a[7], at::kInt, (r.vocab + 31) / 32, "allowed");
+  return r;
+}
+int64_t rows_apart(const Tensor& t) { return t.defined() && t.size(0) > 1 ? t.stride(0) : 0; }
+#define CKV_LOGIT_ARGS(r)                                                                                                          \
+  ptr(r.logits), r.row_stride, int32(r.rows), int32(r.vocab), r.code, (const int64_t*)ptr(r.prompt), rows_apart(r.prompt),          \
+      int32(r.prompt.defined() ? r.prompt.size(1) : 0), (const int64_t*)ptr(r.generated), rows_apart(r.generated),                  \
+      int32(r.generated.defined() ? r.generated.size(1) : 0), (const float*)ptr(r.repetition), r.repetition_all,                    \
+      (const float*)ptr(r.frequency), r.frequency_all, (const float*)ptr(r.presence), r.presence_all, (const float*)ptr(r.bias),    \
+      rows_apart(r.bias), (const int32_t*)ptr(r.allowed), rows_apart(r.allowed)
+
+// adjust_logits(logits, prompt, generated, repetition, frequency, presence, bias, allowed, out)
+PyObject* adjust_logits(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
+  CKV_PY_BEGIN
+  need_args(n_args, 9);
+  const LogitArgs r = logit_args(a);
+  Tensor out = optional_tensor(a[8]);
+  if (!out.defined()) {
+    out = new_tensor({r.rows, r.vocab}, at::kFloat, r.logits);
+  } else {
+    same_device(r.logits, out);
+    if (out.sizes() != r.logits.sizes() || !out.is_contiguous() || out.scalar_type() != at::kFloat)
+      value_error("out must be contiguous (rows, vocab) float32");
+    // float32 logits may be adjusted in place: a thread reads what it writes
+    const uintptr_t o = (uintptr_t)out.data_ptr(), l = (uintptr_t)r.logits.data_ptr(), e = (uintptr_t)r.logits.element_size();
+    const uintptr_t o_end = o + (uintptr_t)out.numel() * 4, l_end = r.rows == 0 ? l : l + ((r.rows - 1) * r.row_stride + r.vocab) * e;
+    const bool in_place = o == l && r.code == CKV_DTYPE_F32 && (r.rows <= 1 || r.row_stride == r.vocab);
+    if (!in_place && o < l_end && l < o_end) value_error("out overlaps the logits without being them");
+  }
+  check(unlocked([&] {
+          const c10::DeviceGuard on(r.logits.device());
+          return ckv_adjust_logits((float*)ptr(out), CKV_LOGIT_ARGS(r), stream_of(r.logits));
+        }),
+        "ckv_adjust_logits");
+  return THPVariable_Wrap(out);
+  CKV_PY_END
+}
+
+// next_tokens(logits, prompt, generated, repetition, frequency, presence, bias, allowed, err, out)
+PyObject* next_tokens(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
+  CKV_PY_BEGIN
+  need_args(n_args, 10);
+  const LogitArgs r = logit_args(a);
+  const Tensor err = optional_tensor(a[8]);
+  Tensor out = optional_tensor(a[9]);
+  if (!out.defined()) {
+    out = new_tensor({r.rows}, at::kLong, r.logits);
+  } else {
+    same_device(r.logits, out);
+    if (out.sizes() != at::IntArrayRef({r.rows}) || !out.is_contiguous() || out.scalar_type() != at::kLong)
+      value_error("out must be contiguous (rows,) int64");
+  }
+  const int64_t ws_bytes = ckv_next_tokens_workspace_bytes(int32(r.rows), int32(r.vocab));
+  Tensor ws;
+  if (ws_bytes > 0) ws = new_tensor({ws_bytes / 8}, at::kLong, r.logits);
+  int32_t* const e = status_word(err, r.logits);
+  check(unlocked([&] {
+          const c10::DeviceGuard on(r.logits.device());
+          return ckv_next_tokens((int64_t*)ptr(out), CKV_LOGIT_ARGS(r), ptr(ws), ws_bytes, e, stream_of(r.logits));
+        }),
+        "ckv_next_tokens");
+  return THPVariable_Wrap(out);
+  CKV_PY_END
+}
+
 PyMethodDef kMethods[] = {
+    {"extend_pages", (PyCFunction)(void (*)(void))extend_pages, METH_FASTCALL, nullptr},
+    {"fork_pages", (PyCFunction)(void (*)(void))fork_pages, METH_FASTCALL, nullptr},
+    {"free_pages", (PyCFunction)(void (*)(void))free_pages, METH_FASTCALL, nullptr},
+    {"compact_pages", (PyCFunction)(void (*)(void))compact_pages, METH_FASTCALL, nullptr},
+    {"attention_paged", (PyCFunction)(void (*)(void))attention_paged, METH_FASTCALL, nullptr},
+    {"adjust_logits", (PyCFunction)(void (*)(void))adjust_logits, METH_FASTCALL, nullptr},
+    {"next_tokens", (PyCFunction)(void (*)(void))next_tokens, METH_FASTCALL, nullptr},
     {"quantize_rows", (PyCFunction)(void (*)(void))quantize_rows, METH_FASTCALL, nullptr},
     {"attention_quantized", (PyCFunction)(void (*)(void))attention_quantized, METH_FASTCALL, nullptr},
     {"attention_weights", (PyCFunction)(void (*)(void))attention_weights, METH_FASTCALL, nullptr},

@@ -751,6 +751,144 @@ def evict_rows(
     return Evicted(*_native.torch_ops().evict_rows(K, V, weights, int(n_keep), int(n_sink), int(n_recent), k_out, v_out))
 
 
+@dataclass
+class PagedCache:
+    """K/V caches of several sequences in pages of page_tokens rows. A layer's pool k[layer] is an ordinary cache: page p is its rows
+    [p * page_tokens, (p + 1) * page_tokens), of every head, so rope_qkv(rows=...) and scatter_rows write into it. The book
+    (table, lengths, refs) is the device's: extend_pages, fork_pages, free_pages and compact_pages change it without a read-back,
+    and may be captured. Calls on one cache are ordered, as on one stream."""
+
+    k: torch.Tensor  # (layers, 1, Hkv, pages * page_tokens, D), contiguous
+    v: torch.Tensor
+    table: torch.Tensor  # int32 (sequences, entries): the page of a sequence's rows j * page_tokens ..
+    lengths: torch.Tensor  # int32 (sequences,): its rows; 0: no sequence
+    refs: torch.Tensor  # int32 (pages,): how often the table names the page; 0: free
+    page_tokens: int = 64
+
+
+def paged_cache(n_layers: int, n_pages: int, n_kv_heads: int, head_dim: int, n_sequences: int, max_tokens: int, device,
+                page_tokens: int = 64, dtype: torch.dtype = torch.bfloat16) -> PagedCache:
+    """An empty cache of n_pages pages for up to n_sequences sequences of max_tokens rows each; rows are not initialised."""
+    T = int(page_tokens)
+    if T not in (32, 64, 128):
+        raise ValueError("page_tokens must be 32, 64 or 128")
+    if min(int(n_pages), int(n_sequences), int(max_tokens)) < 1:
+        raise ValueError("a paged cache has a sequence, an entry and a page at least")
+    dtype_code(dtype)
+    k = torch.empty((int(n_layers), 1, int(n_kv_heads), int(n_pages) * T, int(head_dim)), dtype=dtype, device=device)
+    book = lambda *shape, fill=0: torch.full(shape, fill, dtype=torch.int32, device=device)  # noqa: E731
+    return PagedCache(k, torch.empty_like(k), book(int(n_sequences), -(-int(max_tokens) // T), fill=-1), book(int(n_sequences)),
+                      book(int(n_pages)), T)
+
+
+@dataclass
+class PagedRows:
+    positions: torch.Tensor  # int64 (n,): each new token's row of its sequence
+    rows: torch.Tensor  # int64 (n,): the row of the pool that it takes
+    starts: torch.Tensor  # int32 (sequences + 1,): new tokens in front of each sequence's
+
+
+def extend_pages(cache: PagedCache, counts: torch.Tensor, n: int, err: torch.Tensor | None = None) -> PagedRows:
+    """Sequence s grows by counts[s] rows (int32 (sequences,); 0: not at all): the pages it needs are taken, lowest first, and each new
+    token, in the order of the sequences, gets its position and its row of the pool, which rope_qkv(positions, rows=rows) then writes
+    in every layer. n: the tokens, counts' sum, or room for more (behind the last one positions are 0 and rows -1, which writers skip
+    and flag). What does not fit its table, n or the free pages grows by nothing, nor does what comes behind it and needs such room,
+    and err is set (_native.DEVICE_ERR_RANGE, DEVICE_ERR_PAGES)."""
+    return PagedRows(*_native.torch_ops().extend_pages(cache.table, cache.lengths, cache.refs, cache.page_tokens, counts, n, err))
+
+
+def fork_pages(cache: PagedCache, sources: torch.Tensor, targets: torch.Tensor, err: torch.Tensor | None = None) -> None:
+    """Sequence targets[i] (int32, empty so far) continues sequence sources[i]: whole pages are shared, the partial last one is copied, in
+    every layer. Pairs that cannot be taken (a target with rows, named twice, no free page) are left out, and err is set."""
+    _native.torch_ops().fork_pages(cache.table, cache.lengths, cache.refs, cache.page_tokens, cache.k, cache.v, sources, targets, err)
+
+
+def free_pages(cache: PagedCache, sequences: torch.Tensor, err: torch.Tensor | None = None) -> None:
+    """The sequences (int32) end: pages that no other shares are free again."""
+    _native.torch_ops().free_pages(cache.table, cache.lengths, cache.refs, cache.page_tokens, sequences, err)
+
+
+def compact_pages(cache: PagedCache, err: torch.Tensor | None = None) -> torch.Tensor:
+    """Move the used pages, of every layer, to the front of the pool; returns how many there are, int32 (1,): the pool's rows from
+    used * page_tokens on hold nothing any more."""
+    return _native.torch_ops().compact_pages(cache.table, cache.lengths, cache.refs, cache.page_tokens, cache.k, cache.v, err)
+
+
+def attention_paged(
+    q: torch.Tensor,
+    cache: PagedCache,
+    layer: int,
+    starts: torch.Tensor,
+    scale: float | None = None,
+    *,
+    most: int | None = None,
+    err: torch.Tensor | None = None,
+    out: torch.Tensor | None = None,
+    split: bool = True,
+) -> torch.Tensor:
+    """Attention of new tokens over a layer of a paged cache that has their rows already: of sequence s, tokens starts[s] ..
+    starts[s + 1] (extend_pages' starts) are the last of its lengths[s] rows, and each sees its sequence's rows up to its own.
+
+    q: (1, Hq, n, D) bf16 with contiguous rows; the cache bf16, D 64 or 128. Returns (1, n, Hq, D) bf16, token-major; a token that sees no row
+    (more new tokens than rows) gives zeros, tokens outside [starts[0], starts[-1]) stay as they were in out (anything in a new tensor).
+    most: the most new tokens of one sequence, if known (1 in a decode step); it chooses the kernel's form, not the result.
+    split: let launches too small to fill the chip split the cache range (a workspace is allocated for the partial results).
+    """
+    return _native.torch_ops().attention_paged(q, cache.table, cache.lengths, cache.refs, cache.page_tokens, cache.k, cache.v, layer, starts,
+                                               most, scale, err, out, split)
+
+
+def adjust_logits(
+    logits: torch.Tensor,
+    *,
+    prompt: torch.Tensor | None = None,
+    generated: torch.Tensor | None = None,
+    repetition: float | torch.Tensor = 1.0,
+    frequency: float | torch.Tensor = 0.0,
+    presence: float | torch.Tensor = 0.0,
+    bias: torch.Tensor | None = None,
+    allowed: torch.Tensor | None = None,
+    out: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """Logits (rows, vocab), bf16 or float32, adjusted before a token is chosen; float32. In this order: the logit of a token that is in
+    the row's prompt or generated is divided by repetition where it is above 0 and multiplied by it elsewhere; one that was generated c
+    times loses frequency * c, then presence; bias is added; what allowed leaves out becomes -inf, whatever it was.
+
+    prompt, generated: int64 (rows, tokens); tokens outside the vocabulary (padding, -1) are passed over. repetition (> 0), frequency, presence: a number
+    or float32 (rows,). bias: float32 (vocab,) or (rows, vocab). allowed: int32 (ceil(vocab / 32),) for all rows or one each, bit v % 32 of
+    word v // 32 set where token v may come (token_bits). out may be the logits themselves, if they are float32.
+    """
+    return _native.torch_ops().adjust_logits(logits, prompt, generated, repetition, frequency, presence, bias, allowed, out)
+
+
+def next_tokens(
+    logits: torch.Tensor,
+    *,
+    prompt: torch.Tensor | None = None,
+    generated: torch.Tensor | None = None,
+    repetition: float | torch.Tensor = 1.0,
+    frequency: float | torch.Tensor = 0.0,
+    presence: float | torch.Tensor = 0.0,
+    bias: torch.Tensor | None = None,
+    allowed: torch.Tensor | None = None,
+    err: torch.Tensor | None = None,
+    out: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """adjust_logits(...).argmax(1), int64 (rows,), without writing the adjusted logits: the first of the largest, a NaN above every number.
+    A row of -inf alone gives 0 and sets err (_native.DEVICE_ERR_NO_TOKEN)."""
+    return _native.torch_ops().next_tokens(logits, prompt, generated, repetition, frequency, presence, bias, allowed, err, out)
+
+
+def token_bits(tokens, vocab: int, device) -> torch.Tensor:
+    """The mask of some tokens (any iterable of ints in [0, vocab)) for adjust_logits and next_tokens: int32 (ceil(vocab / 32),)."""
+    words = [0] * -(-int(vocab) // 32)
+    for t in tokens:
+        if not 0 <= t < vocab:
+            raise ValueError(f"token {t} outside the vocabulary of {vocab}")
+        words[t // 32] |= 1 << t % 32
+    return torch.tensor([w - (1 << 32) if w >> 31 else w for w in words], dtype=torch.int32).to(device)
+
+
 def rope_qkv(
     q_in: torch.Tensor | None,
     k_in: torch.Tensor,

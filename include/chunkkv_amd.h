@@ -30,7 +30,7 @@
 extern "C" {
 #endif
 
-#define CKV_ABI_VERSION 7
+#define CKV_ABI_VERSION 8
 
 typedef enum ckv_status {
   CKV_OK = 0,
@@ -47,6 +47,8 @@ typedef enum ckv_dtype {
 
 /* Bits a kernel ORs into the optional device status word `err`. */
 #define CKV_DEVICE_ERR_RANGE 1u
+#define CKV_DEVICE_ERR_PAGES 2u    /* fewer free pages than a sequence needs (ckv_extend_pages, ckv_fork_pages) */
+#define CKV_DEVICE_ERR_NO_TOKEN 4u /* every logit of a row is -infinity (ckv_next_tokens)                       */
 
 /* Per-position flags (one byte per token position), built by the host planner.
  * Mirrors the lists returned by plan_positions (src/chunkkv/engine/base.py:63-73). */
@@ -637,6 +639,125 @@ int32_t ckv_evict_rows(void* k_out, int64_t ko_head_stride, void* v_out, int64_t
                        int64_t v_head_stride, const float* weights, int64_t weights_head_stride, int32_t n_tokens,
                        int32_t n_keep, int32_t n_sink, int32_t n_recent, int32_t n_heads, int32_t head_dim,
                        int32_t dtype, void* stream);
+
+/*
+ * A cache that several sequences share, in pages (no counterpart in the reference). A pool of K or V is an ordinary cache of
+ * n_pages * page_tokens rows a head (bf16 or f32): page p is the rows [p * page_tokens, (p + 1) * page_tokens) of every layer and head, and
+ * the entry points that write rows of a cache write into pages as they are. The book, int32 on the device:
+ *   table    (n_sequences, n_entries)  entry j of a sequence: the page of its rows j * page_tokens ..; past its last one anything
+ *   lengths  (n_sequences)             its rows; 0: no sequence
+ *   refs     (n_pages)                 how often the table names the page; 0: free
+ * Pages are taken lowest first, sequences in order, so a call's result follows from the book alone. page_tokens 32, 64 or 128; at
+ * most 4096 sequences, and 2^31 - 1 rows of a sequence and of the pool (CKV_ERR_TOO_LARGE). Calls on one book go to one stream, or are ordered.
+ * A table that names a page outside the pool is flagged in *err and reads or writes nothing outside it.
+ *
+ * Sequence s grows by counts[s] rows (a whole prompt's, a chunk's, a token's, or 0): the pages it needs beyond those it has are
+ * taken, lengths[s] becomes lengths[s] + counts[s], and for new token i of all, in the order of the sequences,
+ *   positions[i]  its row of its sequence
+ *   rows[i]       that row's place in the pool: table entry * page_tokens + row % page_tokens
+ *   starts[s]     new tokens in front of sequence s's; starts[n_sequences]: all of them
+ * n_new is the room of positions and rows; behind the last token positions are 0 and rows -1. What does not fit grows by nothing and
+ * is flagged: a negative count or one past the table (CKV_DEVICE_ERR_RANGE), the first sequence whose tokens pass n_new and all behind it that have any
+ * (CKV_DEVICE_ERR_RANGE), the first whose pages pass the free ones and all behind it that need any (CKV_DEVICE_ERR_PAGES).
+ * Rows are written into the last page of a sequence, so a partial page has one sequence (ckv_fork_pages sees to it). One launch.
+ */
+int32_t ckv_extend_pages(int64_t* positions, int64_t* rows, int32_t* starts, int32_t n_new, const int32_t* counts,
+                         int32_t* table, int32_t* lengths, int32_t* refs, int32_t n_sequences, int32_t n_entries,
+                         int32_t n_pages, int32_t page_tokens, int32_t* err, void* stream);
+
+/*
+ * Sequence targets[i] continues sequence sources[i]: it shares its whole pages (refs + 1) and gets a copy of its partial last
+ * one, of every layer, in a free page. Pairs are taken in order; one whose target has rows, is its source, or was
+ * named before, or that names no sequence, is left out and flagged (CKV_DEVICE_ERR_RANGE), as is the first that finds no free page and all
+ * behind it that need one (CKV_DEVICE_ERR_PAGES). k_pool, v_pool: (n_layers, n_heads, n_pages * page_tokens, head_dim) with the given strides
+ * (elements, 16-byte multiples); head_dim 64, 128 or 256.
+ *   workspace  device buffer of workspace_bytes >= ckv_fork_pages_workspace_bytes(n_pairs)
+ * n_pairs at most 4096. Two launches.
+ */
+int32_t ckv_fork_pages(void* k_pool, void* v_pool, int64_t layer_stride, int64_t head_stride, int32_t n_layers, int32_t n_heads,
+                       int32_t head_dim, int32_t dtype, const int32_t* sources, const int32_t* targets, int32_t n_pairs,
+                       int32_t* table, int32_t* lengths, int32_t* refs, int32_t n_sequences, int32_t n_entries, int32_t n_pages,
+                       int32_t page_tokens, void* workspace, int64_t workspace_bytes, int32_t* err, void* stream);
+int64_t ckv_fork_pages_workspace_bytes(int32_t n_pairs); /* host-only */
+
+/*
+ * The sequences end: their pages' refs - 1, their table entries -1, their lengths 0. One named twice ends once, an empty one stays
+ * so, one that does not exist is flagged (CKV_DEVICE_ERR_RANGE). n at most 4096. One launch.
+ */
+int32_t ckv_free_pages(const int32_t* sequences, int32_t n, int32_t* table, int32_t* lengths, int32_t* refs, int32_t n_sequences,
+                       int32_t n_entries, int32_t n_pages, int32_t page_tokens, int32_t* err, void* stream);
+
+/*
+ * The used pages become pages 0 .. *used - 1: of U used ones, the i-th at U or above (ascending) moves to the i-th free one below U in
+ * every layer, and table and refs follow. The pages it left keep their bytes. Pools as for ckv_fork_pages.
+ *   workspace  device buffer of workspace_bytes >= ckv_compact_pages_workspace_bytes(n_pages)
+ * Two launches.
+ */
+int32_t ckv_compact_pages(void* k_pool, void* v_pool, int64_t layer_stride, int64_t head_stride, int32_t n_layers,
+                          int32_t n_heads, int32_t head_dim, int32_t dtype, int32_t* used, int32_t* table, int32_t* lengths,
+                          int32_t* refs, int32_t n_sequences, int32_t n_entries, int32_t n_pages, int32_t page_tokens,
+                          void* workspace, int64_t workspace_bytes, int32_t* err, void* stream);
+int64_t ckv_compact_pages_workspace_bytes(int32_t n_pages); /* host-only */
+
+/*
+ * Attention of new tokens over one layer of a paged cache: of sequence s's lengths[s] rows the last c = starts[s + 1] - starts[s] are new, and
+ * its query i (token starts[s] + i of q and out) sees its rows up to lengths[s] - c + i: ckv_attention_active's function on the rows that the
+ * table names, with its roundings. A query that sees no row (c above lengths[s]) gives zeros; tokens in front of starts[0] and from starts[n_sequences] on
+ * are not written. starts ascends (ckv_extend_pages gives it); whatever it holds, nothing outside the arrays is touched.
+ *   k_pool, v_pool  the layer's pool, (n_kv_heads, n_pages * page_tokens, head_dim), bf16, kv_head_stride elements between heads; rows of a
+ *                   page behind its sequence's last may hold anything
+ *   most_tokens     the most new tokens of a sequence, if known (0: not); it chooses the kernel's form, not the result
+ *   workspace       optional device buffer of workspace_bytes >= ckv_attention_paged_workspace_bytes(...) (16-byte aligned): partial rows
+ *                   of launches that split the cache; without it they run unsplit (slower; the same up to the order of fp32 sums)
+ * head_dim 64 or 128; scale within the normal fp32 numbers' range; lengths past n_entries * page_tokens count as that.
+ * No counterpart in the reference.
+ */
+int32_t ckv_attention_paged(void* out, const void* q, int64_t q_head_stride, int64_t q_token_stride, const void* k_pool,
+                            const void* v_pool, int64_t kv_head_stride, const int32_t* table, const int32_t* lengths,
+                            const int32_t* starts, int32_t n_tokens, int32_t most_tokens, int32_t n_sequences,
+                            int32_t n_entries, int32_t n_pages, int32_t page_tokens, int32_t n_q_heads, int32_t n_kv_heads,
+                            int32_t head_dim, int32_t dtype, double scale, void* workspace, int64_t workspace_bytes,
+                            int32_t* err, void* stream);
+
+/* Bytes of workspace that ckv_attention_paged uses for this shape (0: none). Host-only. */
+int64_t ckv_attention_paged_workspace_bytes(int32_t n_tokens, int32_t n_sequences, int32_t most_tokens, int32_t n_entries,
+                                            int32_t page_tokens, int32_t n_q_heads, int32_t n_kv_heads, int32_t head_dim);
+
+/*
+ * Logits (n_rows, vocab), bf16 or f32 with contiguous rows, adjusted before a token is chosen. With c = how often the row's `generated`
+ * holds token v, and seen = c > 0 or v in its `prompt`:
+ *   x = seen ? (x > 0 ? x / repetition : x * repetition) : x
+ *   x = x - frequency * c - presence                (c > 0)
+ *   x = x + bias[v]                                 (bias given)
+ *   x = -infinity, whatever x is                    (allowed given and bit v % 32 of its word v / 32 not set)
+ * in fp32, each step rounded once, from left to right; out is (n_rows, vocab) f32 contiguous.
+ *   prompt, generated   (n_rows, n_prompt or n_generated) int64 tokens; those outside [0, vocab) (padding) are passed over; counts 0: none
+ *   *_rows              a value for each row, or NULL: the value beside it for all
+ *   bias                (vocab) for each row, or one for all (row stride 0), f32; NULL: none
+ *   allowed             (ceil(vocab / 32)) words for each row or for all; NULL: every token is
+ * Row strides in elements. Nothing need be aligned beyond its elements. n_rows at most 65535. One launch.
+ * No counterpart in the reference, whose decode takes the argmax of the model's logits (torch_engine.py:197).
+ */
+int32_t ckv_adjust_logits(float* out, const void* logits, int64_t logits_row_stride, int32_t n_rows, int32_t vocab, int32_t dtype,
+                          const int64_t* prompt, int64_t prompt_row_stride, int32_t n_prompt, const int64_t* generated,
+                          int64_t generated_row_stride, int32_t n_generated, const float* repetition_rows, float repetition,
+                          const float* frequency_rows, float frequency, const float* presence_rows, float presence,
+                          const float* bias, int64_t bias_row_stride, const int32_t* allowed, int64_t allowed_row_stride,
+                          void* stream);
+
+/*
+ * The greedy token of the logits that ckv_adjust_logits gives, which are not written: tokens[row] = the first of the largest, a NaN above
+ * every number (torch.argmax). A row of -infinity alone gives 0 and is flagged (CKV_DEVICE_ERR_NO_TOKEN).
+ *   workspace  device buffer of workspace_bytes >= ckv_next_tokens_workspace_bytes(...) (8-byte aligned)
+ * Up to two launches.
+ */
+int32_t ckv_next_tokens(int64_t* tokens, const void* logits, int64_t logits_row_stride, int32_t n_rows, int32_t vocab, int32_t dtype,
+                        const int64_t* prompt, int64_t prompt_row_stride, int32_t n_prompt, const int64_t* generated,
+                        int64_t generated_row_stride, int32_t n_generated, const float* repetition_rows, float repetition,
+                        const float* frequency_rows, float frequency, const float* presence_rows, float presence,
+                        const float* bias, int64_t bias_row_stride, const int32_t* allowed, int64_t allowed_row_stride,
+                        void* workspace, int64_t workspace_bytes, int32_t* err, void* stream);
+int64_t ckv_next_tokens_workspace_bytes(int32_t n_rows, int32_t vocab); /* host-only */
 
 /*
  * Residual add and RMSNorm of each row, the elementwise steps around a decoder layer's GEMMs:
