@@ -66,6 +66,15 @@ __global__ __launch_bounds__(kPagedWaves * 64) void attn_paged_kernel(AttnMap ma
     pages = paged_page(b, table, (int)min(((int64_t)c + lane * W) * CH, (int64_t)wmax) >> b.T_log);
     asm volatile("" : "+v"(pages));  // waited for here, not at every use
   };
+  // Q operands: row lm of group qg, head-dim 32 ds + 8 g .. + 8.
+  bf16x8 qf[QG][DS];
+#pragma unroll
+  for (int qg = 0; qg < QG; ++qg) {
+    const int m = min(r0 + qg * 16 + lm, rows - 1), t = div_by(m, group, b.inv_gqa);
+    const char* qr = q + (int64_t)(hk * group + m - t * group) * q_hs_b + (int64_t)(it.first + t) * q_ts_b;
+#pragma unroll
+    for (int ds = 0; ds < DS; ++ds) qf[qg][ds] = __builtin_bit_cast(bf16x8, ld16(qr + (32 * ds + 8 * g) * 2));
+  }
   if (c < c_end) load_pages(c);
   typedef __attribute__((address_space(1))) void gvoid;
   typedef __attribute__((address_space(3))) void lvoid;
@@ -98,15 +107,6 @@ __global__ __launch_bounds__(kPagedWaves * 64) void attn_paged_kernel(AttnMap ma
       for (int i = 0; i < LI; ++i) load(vt, clamp(off_v[i]), wl + CH * ROWB + i * 1024);
     }
   };
-  // Q operands: row lm of group qg, head-dim 32 ds + 8 g .. + 8.
-  bf16x8 qf[QG][DS];
-#pragma unroll
-  for (int qg = 0; qg < QG; ++qg) {
-    const int m = min(r0 + qg * 16 + lm, rows - 1), t = div_by(m, group, b.inv_gqa);
-    const char* qr = q + (int64_t)(hk * group + m - t * group) * q_hs_b + (int64_t)(it.first + t) * q_ts_b;
-#pragma unroll
-    for (int ds = 0; ds < DS; ++ds) qf[qg][ds] = __builtin_bit_cast(bf16x8, ld16(qr + (32 * ds + 8 * g) * 2));
-  }
   if (c < c_end) issue(c, 0, lds0);
 
   f32x4 o[QG][DT], l_acc[QG];
@@ -244,65 +244,92 @@ __global__ __launch_bounds__(kPagedWaves * 64) void attn_paged_kernel(AttnMap ma
 }
 
 // ---- the splits joined -----------------------------------------------------------------------------------------
-// Row (token, query head) a wavefront: D / 4 lanes a partial row, 64 / (D / 4) partials side by side, four of each in
-// flight. Splits past the row's position were not written. Rows of sequences in one split are written already.
-template <int D, int ROWS, int UNIT>
+// D / 4 lanes have a (token, query head) row's columns, so a wavefront has JH = 64 / (D / 4) heads of a token side by side and nothing
+// crosses its lanes; it goes through their partial rows, JU in flight. Finding the token's items costs as many instructions as a few rows,
+// and instructions are what a launch of many rows waits for, so such launches (WPR = 1) give a wavefront kJoinTurns times JH heads; those of few rows
+// and more splits (WPR = 4) spread a row's partials over four wavefronts. Splits past the row's position were not written. Rows of
+// sequences in one split are written already.
+constexpr int kJoinTurns = 2, kJoinInFlight = 8;
+template <int D>
+constexpr int kJoinHeads = 256 / D;
+
+template <int D, int ROWS, int UNIT, int WPR>
 __global__ __launch_bounds__(256) void join_paged_kernel(char* __restrict__ out, const float* __restrict__ ws, PagedRows b, int n,
                                                          int Hq, int group) {
-  constexpr int LR = D / 4, P = 64 / LR, U = 4;
-  const int lane = threadIdx.x % 64, sub = lane / LR, col = lane % LR * 4;
-  const int64_t row = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
-  if (row >= (int64_t)n * Hq) return;
-  const int t = (int)(row / Hq), h = (int)(row - (int64_t)t * Hq), hk = h / group;
+  constexpr int LR = D / 4, JH = kJoinHeads<D>, U = kJoinInFlight, TURNS = WPR == 4 ? 1 : kJoinTurns;
+  static_assert(WPR == 1 || WPR == 4, "a wavefront or a workgroup a row");
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x % 64, sub = lane / LR, col = lane % LR * 4;
+  const int t = WPR == 4 ? (int)blockIdx.x : (int)blockIdx.x * 4 + wave;
+  if (t >= n) return;
   PagedItem it;
   if (!paged_find<ROWS, UNIT>(b, n, group, [&](int first, int count, int, int) { return t >= first && t - first < count; }, it)) return;
   if (it.splits == 1) return;
-  const int m = (t - it.first) * group + h - hk * group, p = it.rows - it.count + t - it.first;
-  const int live = p < 0 ? 0 : min(it.splits, p / (it.split_units * UNIT) + 1);
-  const int item = it.item0 + m / ROWS;  // of split 0
-  if (item + (int64_t)(live - 1) * it.tiles >= b.cap) return;  // starts that descend: no such items were run
-  const float* base = ws + (((int64_t)hk * b.cap + item) * ROWS + m % ROWS) * (D + 4);
+  const int p = it.rows - it.count + t - it.first;
+  const int live = p < 0 ? 0 : min(it.splits, (int)((uint32_t)p / (uint32_t)(it.split_units * UNIT)) + 1);
   const int64_t stride = (int64_t)it.tiles * ROWS * (D + 4);
-  float M = -INFINITY, L = 0.f;
-  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-  for (int z0 = 0; z0 < live; z0 += P * U) {
-    f32x4 o[U];
-    float2 ml[U];
+  __shared__ f32x4 s_o[WPR][64];
+  __shared__ float s_m[WPR][JH], s_l[WPR][JH];
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      o[u] = f32x4{0.f, 0.f, 0.f, 0.f};
-      ml[u] = make_float2(-INFINITY, 0.f);
-      if (z0 + u * P >= live) continue;  // uniform
-      const float* pz = base + (int64_t)min(z0 + u * P + sub, live - 1) * stride;
-      o[u] = *(const f32x4*)(pz + col);
-      ml[u] = *(const float2*)(pz + D);
-    }
+  for (int turn = 0; turn < TURNS; ++turn) {
+    const int h = ((int)blockIdx.y * TURNS + turn) * JH + sub, hc = min(h, Hq - 1), hk = div_by(hc, group, b.inv_gqa);
+    const int m = (t - it.first) * group + hc - hk * group, item = it.item0 + m / ROWS;  // of split 0
+    // items past cap: starts that descend; no such items were run
+    const int parts = item + (int64_t)(live - 1) * it.tiles < b.cap ? live : 0;
+    const float* base = ws + (((int64_t)hk * b.cap + item) * ROWS + m % ROWS) * (D + 4);
+    float M = -INFINITY, L = 0.f;
+    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+    const int begin = WPR == 4 ? wave * U : 0;
+    for (int z0 = begin; z0 < parts; z0 += WPR * U) {
+      f32x4 o[U];
+      float2 ml[U];
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const bool mine = z0 + u * P + sub < live;
-      const float mz = mine ? ml[u].x : -INFINITY, mn = fmaxf(M, mz), ref = mn == -INFINITY ? 0.f : mn;
-      const float a = __builtin_amdgcn_exp2f(M - ref), e = __builtin_amdgcn_exp2f(mz - ref);  // 0 of -inf
-      L = L * a + (mine ? ml[u].y : 0.f) * e;
-      acc = acc * a + o[u] * e;
+      for (int u = 0; u < U; ++u) {
+        o[u] = f32x4{0.f, 0.f, 0.f, 0.f};
+        ml[u] = make_float2(-INFINITY, 0.f);
+        if (z0 + u >= live) continue;  // uniform
+        const float* pz = base + (int64_t)min(z0 + u, parts - 1) * stride;
+        o[u] = *(const f32x4*)(pz + col);
+        ml[u] = *(const float2*)(pz + D);
+      }
+      float mn = M;
+#pragma unroll
+      for (int u = 0; u < U; ++u) mn = fmaxf(mn, ml[u].x);
+      const float ref = mn == -INFINITY ? 0.f : mn, a = __builtin_amdgcn_exp2f(M - ref);  // 0 of -inf
+      L *= a;
+      acc *= a;
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const float e = __builtin_amdgcn_exp2f(ml[u].x - ref);
+        L += ml[u].y * e;
+        acc += o[u] * e;
+      }
       M = mn;
     }
+    if constexpr (WPR == 4) {
+      s_o[wave][lane] = acc;
+      if (col == 0) {
+        s_m[wave][sub] = M;
+        s_l[wave][sub] = L;
+      }
+      __syncthreads();
+      if (wave != 0) return;
+      float mx = -INFINITY;
+#pragma unroll
+      for (int w = 0; w < 4; ++w) mx = fmaxf(mx, s_m[w][sub]);
+      L = 0.f;
+      acc = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        const float e = s_m[w][sub] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(s_m[w][sub] - mx);
+        L += s_l[w][sub] * e;
+        acc += s_o[w][lane] * e;
+      }
+    }
+    const float inv = L == 0.f ? 0.f : 1.f / L;
+    if (h < Hq)
+      *(uint2*)(out + ((int64_t)t * Hq + h) * (D * 2) + col * 2) =
+          uint2{f32x2_to_bf16x2_bits(acc[0] * inv, acc[1] * inv), f32x2_to_bf16x2_bits(acc[2] * inv, acc[3] * inv)};
   }
-  float mx = M;
-#pragma unroll
-  for (int d = LR; d < 64; d *= 2) mx = fmaxf(mx, __shfl_xor(mx, d));
-  const float s = M == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(M - mx);
-  L *= s;
-  acc *= s;
-#pragma unroll
-  for (int d = LR; d < 64; d *= 2) {
-    L += __shfl_xor(L, d);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) acc[e] += __shfl_xor(acc[e], d);
-  }
-  const float inv = L == 0.f ? 0.f : 1.f / L;
-  if (sub == 0)
-    *(uint2*)(out + row * (D * 2) + col * 2) =
-        uint2{f32x2_to_bf16x2_bits(acc[0] * inv, acc[1] * inv), f32x2_to_bf16x2_bits(acc[2] * inv, acc[3] * inv)};
 }
 
 }  // namespace ckv
@@ -343,7 +370,8 @@ extern "C" int32_t ckv_attention_paged(void* out, const void* q, int64_t q_head_
   if (plan.map.blocks == 0) return CKV_ERR_TOO_LARGE;
   float* ws = plan.target > 0 ? (float*)workspace : nullptr;
   const PagedRows b = {table, lengths, starts, n_sequences, n_entries, n_pages, page_tokens == 32 ? 5 : page_tokens == 64 ? 6 : 7,
-                       (int)plan.items, plan.target, plan.min_units, inverse_of((int64_t)n_tokens * group + kAttnBM, group), err};
+                       (int)plan.items, plan.target, plan.target > 0 ? 1.f / (float)plan.target : 0.f, plan.min_units,
+                       inverse_of(std::max((int64_t)n_tokens * group + kAttnBM, (int64_t)n_q_heads), group), err};
   const AttnMap& map = plan.map;
   const float scale_log2 = log2_scale(scale);
   hipStream_t st = (hipStream_t)stream;
@@ -366,18 +394,23 @@ extern "C" int32_t ckv_attention_paged(void* out, const void* q, int64_t q_head_
   }
   CKV_RETURN_IF_LAUNCH_FAILED();
   if (ws != nullptr) {
-    const dim3 grid((unsigned)(((int64_t)n_tokens * n_q_heads + 3) / 4));
-    auto join = [&](auto kernel) {
-      hipLaunchKernelGGL(kernel, grid, dim3(256), 0, st, (char*)out, (const float*)ws, b, n_tokens, n_q_heads, (int)group);
+    auto join = [&](auto kernel, int tokens, int heads) {
+      hipLaunchKernelGGL(kernel, dim3((unsigned)((n_tokens + tokens - 1) / tokens), (unsigned)((n_q_heads + heads - 1) / heads)), dim3(256), 0,
+                         st, (char*)out, (const float*)ws, b, n_tokens, n_q_heads, (int)group);
     };
-    if (head_dim == 128)
-      plan.rows == 16   ? join(join_paged_kernel<128, 16, kPagedUnit>)
-      : plan.rows == 32 ? join(join_paged_kernel<128, 32, kPagedUnit>)
-                        : join(join_paged_kernel<128, kAttnBM, kAttnBN>);
-    else
-      plan.rows == 16   ? join(join_paged_kernel<64, 16, kPagedUnit>)
-      : plan.rows == 32 ? join(join_paged_kernel<64, 32, kPagedUnit>)
-                        : join(join_paged_kernel<64, kAttnBM, kAttnBN>);
+#define CKV_JOIN(D, ROWS, UNIT)                                                       \
+  plan.spread_join ? join(join_paged_kernel<D, ROWS, UNIT, 4>, 1, kJoinHeads<D>)     \
+                   : join(join_paged_kernel<D, ROWS, UNIT, 1>, 4, kJoinTurns * kJoinHeads<D>)
+    if (head_dim == 128) {
+      if (plan.rows == 16) CKV_JOIN(128, 16, kPagedUnit);
+      else if (plan.rows == 32) CKV_JOIN(128, 32, kPagedUnit);
+      else CKV_JOIN(128, kAttnBM, kAttnBN);
+    } else {
+      if (plan.rows == 16) CKV_JOIN(64, 16, kPagedUnit);
+      else if (plan.rows == 32) CKV_JOIN(64, 32, kPagedUnit);
+      else CKV_JOIN(64, kAttnBM, kAttnBN);
+    }
+#undef CKV_JOIN
     CKV_RETURN_IF_LAUNCH_FAILED();
   }
   return CKV_OK;

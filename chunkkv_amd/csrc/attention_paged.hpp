@@ -20,10 +20,14 @@ struct PagedRows {
   int S, M, P, T_log;
   int cap;     // items of a KV head that the launch has room for
   int target;  // items that splits aim at, beside the tiles; 0: no splits
+  float inv_target;
   int min_units;
   uint32_t inv_gqa;
   int32_t* err;
 };
+
+// Units of all tiles up to which a split is one unit: as many partial rows as a join reads at once.
+constexpr float kPagedShort = 32.f;
 
 struct PagedItem {
   int seq, first, count, rows;  // the sequence, its first new token and their number, its rows
@@ -50,23 +54,25 @@ __device__ __forceinline__ bool paged_find(const PagedRows& b, int n, int group,
   auto tiles_of = [&](const Seq& q) { return (int)(((uint32_t)q.count * (uint32_t)group + ROWS - 1) / ROWS); };
   auto units_of = [&](const Seq& q) { return (int)(((uint32_t)q.rows + UNIT - 1) / UNIT); };
   const Seq head = seq(lane);
-  int split_units = INT32_MAX;
+  // The work's sum is off by less than 2^-17 of itself (64 additions in a lane, 6 across, roundings of 2^-24), so split_units, rounded up
+  // from more than that above it, is no less than work / target: splits add no more than target items. It is the same in every wavefront.
+  int split_units = 1 << 30;
   if (b.target > 0) {
-    uint64_t work = 0;
+    float work = 0.f;
     for (int s0 = 0; s0 < b.S; s0 += 64) {
       const Seq q = s0 == 0 ? head : seq(s0 + lane);
-      work += (uint64_t)tiles_of(q) * (uint64_t)units_of(q);
+      work += (float)tiles_of(q) * (float)units_of(q);
     }
-    work = wave_incl_scan(work);
-    const uint64_t all = (uint64_t)__builtin_amdgcn_readlane((uint32_t)(work >> 32), 63) << 32 | __builtin_amdgcn_readlane((uint32_t)work, 63);
-    const uint64_t each = all >> 32 ? (all + b.target - 1) / b.target : ((uint32_t)all + (uint64_t)b.target - 1) / (uint32_t)b.target;
-    split_units = (int)max((uint64_t)b.min_units, min(each, (uint64_t)INT32_MAX));
+    work = wave_butterfly_sum(work);
+    split_units = max(work <= kPagedShort ? 1 : b.min_units, (int)fminf(work * b.inv_target * (1.f + 0x1p-16f), 0x1p29f) + 1);
   }
+  const float inv_split = 1.f / (float)split_units;
   int before = 0;
   for (int s0 = 0; s0 < b.S; s0 += 64) {
     const Seq q = s0 == 0 ? head : seq(s0 + lane);
     const int tiles = tiles_of(q), units = units_of(q);
-    const int splits = units <= split_units ? 1 : (int)(((uint32_t)units + (uint32_t)split_units - 1) / (uint32_t)split_units);
+    int splits = max(1, (int)((float)units * inv_split));  // ceil(units / split_units), at most one off
+    if ((int64_t)splits * split_units < units) ++splits;
     const int items = tiles * splits;
     const int incl = before + (int)wave_incl_scan((uint32_t)items);
     const uint64_t hit = __builtin_amdgcn_ballot_w64(mine(q.first, q.count, incl - items, items));

@@ -13,6 +13,7 @@ struct PagedPlan {
   int rows = 0;    // (token, query head) rows of a tile: 16 or 32 (attn_paged_kernel), 128 (attn_active_kernel)
   int target = 0;  // items of a KV head that splits aim at, beside the tiles; 0: the cache is not split
   int min_units = 0;
+  bool spread_join = false;  // a row's partials are spread over four wavefronts
   int64_t items = 0;  // of a KV head, at most
   int64_t ws_bytes = 0;
   AttnMap map;
@@ -27,12 +28,12 @@ static inline PagedPlan paged_plan(int64_t n, int64_t S, int64_t most, int64_t r
   const int64_t tiles = n * group / p.rows + std::min(S, n);
   const bool large = p.rows == kAttnBM;
   const int unit = large ? kAttnBN : kPagedUnit;
-  // Workgroups that are resident at once.
-  const int64_t fill = 512 / Hkv;
+  const int64_t fill = (large ? 512 : 384) / Hkv;
   p.min_units = large ? 4 : 2;
   p.target = rows <= (int64_t)p.min_units * unit || (large && n * group / p.rows >= fill) ? 0 : (int)std::max<int64_t>(fill, 1);
   const int64_t row_b = (int64_t)Hkv * p.rows * (head_dim + 4) * 4;
   if (p.target > 0 && (tiles + p.target) * row_b > workspace_bytes) p.target = 0;
+  p.spread_join = p.target >= 8 * tiles || n * Hq <= 2048;
   p.items = tiles + p.target;
   p.ws_bytes = p.target > 0 ? p.items * row_b : 0;
   if (p.items * Hkv < (1 << 30)) p.map = attn_map(p.items, Hkv, 1, 1);

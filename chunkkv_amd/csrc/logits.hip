@@ -44,7 +44,8 @@ struct Adjust {
 constexpr int kLogitsEach = 8;  // logits of a thread
 constexpr uint32_t kInPrompt = 1u << 31;
 
-// f over the row's tokens that lie in [v0, v0 + count), as offsets.
+// f over the row's tokens that lie in [v0, v0 + count), as offsets. A batch's loads go out together, the last one's too
+// (past the row's end they read its last pair again, which is passed over).
 template <int NT, typename F>
 __device__ __forceinline__ void each_token(const Tokens& t, int row, int64_t v0, int count, F f) {
   const int64_t* p = t.at + row * t.stride;
@@ -53,21 +54,19 @@ __device__ __forceinline__ void each_token(const Tokens& t, int row, int64_t v0,
     const uint64_t o = (uint64_t)(v - v0);
     if (o < (uint64_t)count) f((int)o);
   };
-  int i = threadIdx.x * 2;
-  for (; i + 2 * NT * (U - 1) + 1 < t.n; i += 2 * NT * U) {
+  const int pairs = t.n / 2;
+  for (int i0 = 0; i0 < pairs; i0 += U * NT) {
     vec16 v[U];
 #pragma unroll
-    for (int u = 0; u < U; ++u) v[u] = ld16_any(p + i + 2 * NT * u);
+    for (int u = 0; u < U; ++u) v[u] = ld16_any(p + 2 * min(i0 + u * NT + (int)threadIdx.x, pairs - 1));
 #pragma unroll
     for (int u = 0; u < U; ++u) {
+      if (i0 + u * NT + (int)threadIdx.x >= pairs) continue;
       take((int64_t)((uint64_t)v[u][1] << 32 | v[u][0]));
       take((int64_t)((uint64_t)v[u][3] << 32 | v[u][2]));
     }
   }
-  for (; i < t.n; i += 2 * NT) {
-    take(p[i]);
-    if (i + 1 < t.n) take(p[i + 1]);
-  }
+  if ((t.n & 1) != 0 && threadIdx.x == 0) take(p[t.n - 1]);
 }
 
 // A logit as a key whose order is argmax's: larger logits first, a NaN above all, -0 as 0; then the lower index.

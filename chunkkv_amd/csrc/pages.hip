@@ -152,7 +152,7 @@ __global__ __launch_bounds__(kBookThreads) void extend_pages_kernel(int64_t* __r
     });
     __syncthreads();
   }
-  for (int i = tid; i < n; i += kBookThreads) {
+  for (int i = tid; positions != nullptr && i < n; i += kBookThreads) {
     int64_t pos = 0, row = -1;
     if (i < total) {
       const int s = interval_of(s_start, b.S, (uint32_t)i);
@@ -166,6 +166,29 @@ __global__ __launch_bounds__(kBookThreads) void extend_pages_kernel(int64_t* __r
   for (int s = tid; s <= b.S; s += kBookThreads) {
     starts[s] = (int32_t)s_start[s];
     if (s < b.S) b.lengths[s] = rows_of(b, s) + (int)(s_start[s + 1] - s_start[s]);
+  }
+}
+
+// The positions and rows of many tokens, after extend_pages_kernel without them (kRowsAlone).
+constexpr int kRowsThreads = 256, kRowsEach = 4;
+__global__ __launch_bounds__(kRowsThreads) void token_rows_kernel(int64_t* __restrict__ positions, int64_t* __restrict__ rows,
+                                                                  const int32_t* __restrict__ starts, int n, Book b) {
+  __shared__ uint32_t s_start[kMostSequences + 1];
+  for (int s = threadIdx.x; s <= b.S; s += kRowsThreads) s_start[s] = (uint32_t)starts[s];
+  __syncthreads();
+  const int total = (int)s_start[b.S];
+#pragma unroll
+  for (int e = 0; e < kRowsEach; ++e) {
+    const int64_t i = ((int64_t)blockIdx.x * kRowsEach + e) * kRowsThreads + threadIdx.x;
+    if (i >= n) return;
+    int64_t pos = 0, row = -1;
+    if (i < total) {
+      const int s = interval_of(s_start, b.S, (uint32_t)i);
+      pos = b.lengths[s] - (int64_t)s_start[s + 1] + i;
+      row = ((int64_t)b.table[(int64_t)s * b.M + (pos >> b.T_log)] << b.T_log) + (pos & ((1 << b.T_log) - 1));
+    }
+    positions[i] = pos;
+    rows[i] = row;
   }
 }
 
@@ -395,6 +418,9 @@ __global__ __launch_bounds__(kCopyThreads) void compact_copy_kernel(Moves m, Poo
   }
 }
 
+// New tokens from which their rows get a launch of their own: one workgroup writes 1024 in 0.7 us, a launch costs about three.
+constexpr int kRowsAlone = 4096;
+
 // ---- arguments -------------------------------------------------------------------------------------------------
 
 static int32_t make_book(Book& b, int32_t* table, int32_t* lengths, int32_t* refs, int32_t S, int32_t M, int32_t P, int32_t T) {
@@ -434,9 +460,16 @@ extern "C" int32_t ckv_extend_pages(int64_t* positions, int64_t* rows, int32_t* 
   CKV_RETURN_IF_BAD(make_book(b, table, lengths, refs, n_sequences, n_entries, n_pages, page_tokens));
   if (n_new < 0 || counts == nullptr || starts == nullptr || (n_new > 0 && (positions == nullptr || rows == nullptr)))
     return CKV_ERR_INVALID_ARGUMENT;
-  hipLaunchKernelGGL(extend_pages_kernel, dim3(1), dim3(kBookThreads), 0, (hipStream_t)stream, positions, rows, starts, n_new,
-                     counts, b, err);
+  const bool alone = n_new > kRowsAlone;
+  hipLaunchKernelGGL(extend_pages_kernel, dim3(1), dim3(kBookThreads), 0, (hipStream_t)stream, alone ? nullptr : positions, rows,
+                     starts, n_new, counts, b, err);
   CKV_RETURN_IF_LAUNCH_FAILED();
+  if (alone) {
+    constexpr int each = kRowsThreads * kRowsEach;
+    hipLaunchKernelGGL(token_rows_kernel, dim3((unsigned)(((int64_t)n_new + each - 1) / each)), dim3(kRowsThreads), 0,
+                       (hipStream_t)stream, positions, rows, starts, n_new, b);
+    CKV_RETURN_IF_LAUNCH_FAILED();
+  }
   return CKV_OK;
 }
 
