@@ -122,7 +122,7 @@ SIGNATURES = {
         [_p, _p, _i64, _i64, _i32, _i32, _i32, _i32, _p, _p, _i32, _p, _p, _p, _i32, _i32, _i32, _i32, _p, _i64, _p, _p],
     ),
     "ckv_fork_pages_workspace_bytes": (_i64, [_i32]),
-    "ckv_free_pages": (_i32, [_p, _i32, _p, _p, _p, _i32, _i32, _i32, _i32, _p, _p]),
+    "ckv_free_pages": (_i32, [_p, _p, _i32, _p, _p, _p, _i32, _i32, _i32, _i32, _p, _i64, _p, _p]),
     "ckv_compact_pages": (
         _i32,
         [_p, _p, _i64, _i64, _i32, _i32, _i32, _i32, _p, _p, _p, _p, _i32, _i32, _i32, _i32, _p, _i64, _p, _p],

@@ -9,7 +9,6 @@
 #include <algorithm>
 
 #include "attention_large.hpp"
-#include "attention_paged_plan.hpp"
 
 namespace ckv {
 

@@ -10,6 +10,7 @@
 #pragma once
 
 #include "attention_common.hpp"
+#include "attention_paged_plan.hpp"
 
 namespace ckv {
 
@@ -25,9 +26,6 @@ struct PagedRows {
   uint32_t inv_gqa;
   int32_t* err;
 };
-
-// Units of all tiles up to which a split is one unit: as many partial rows as a join reads at once.
-constexpr float kPagedShort = 32.f;
 
 struct PagedItem {
   int seq, first, count, rows;  // the sequence, its first new token and their number, its rows
@@ -54,8 +52,6 @@ __device__ __forceinline__ bool paged_find(const PagedRows& b, int n, int group,
   auto tiles_of = [&](const Seq& q) { return (int)(((uint32_t)q.count * (uint32_t)group + ROWS - 1) / ROWS); };
   auto units_of = [&](const Seq& q) { return (int)(((uint32_t)q.rows + UNIT - 1) / UNIT); };
   const Seq head = seq(lane);
-  // The work's sum is off by less than 2^-17 of itself (64 additions in a lane, 6 across, roundings of 2^-24), so split_units, rounded up
-  // from more than that above it, is no less than work / target: splits add no more than target items. It is the same in every wavefront.
   int split_units = 1 << 30;
   if (b.target > 0) {
     float work = 0.f;
@@ -64,15 +60,14 @@ __device__ __forceinline__ bool paged_find(const PagedRows& b, int n, int group,
       work += (float)tiles_of(q) * (float)units_of(q);
     }
     work = wave_butterfly_sum(work);
-    split_units = max(work <= kPagedShort ? 1 : b.min_units, (int)fminf(work * b.inv_target * (1.f + 0x1p-16f), 0x1p29f) + 1);
+    split_units = paged_split_units(work, b.inv_target, b.min_units);  // the same in every wavefront
   }
   const float inv_split = 1.f / (float)split_units;
   int before = 0;
   for (int s0 = 0; s0 < b.S; s0 += 64) {
     const Seq q = s0 == 0 ? head : seq(s0 + lane);
     const int tiles = tiles_of(q), units = units_of(q);
-    int splits = max(1, (int)((float)units * inv_split));  // ceil(units / split_units), at most one off
-    if ((int64_t)splits * split_units < units) ++splits;
+    const int splits = paged_splits(units, split_units, inv_split);
     const int items = tiles * splits;
     const int incl = before + (int)wave_incl_scan((uint32_t)items);
     const uint64_t hit = __builtin_amdgcn_ballot_w64(mine(q.first, q.count, incl - items, items));

@@ -2,12 +2,38 @@
 // can be walked on a machine without a GPU.
 #pragma once
 
+#include <cmath>
+
 #include "attention_plan.hpp"
+
+#ifdef __HIPCC__
+#define CKV_HOST_DEVICE __host__ __device__
+#else
+#define CKV_HOST_DEVICE
+#endif
 
 namespace ckv {
 
 constexpr int kPagedWaves = 4;                           // wavefronts of attn_paged_kernel
 constexpr int kPagedUnit = kPagedWaves * kWaveChunk;     // cache rows that a split is a multiple of there
+
+// Units of all tiles up to which a split is one unit: as many partial rows as a join reads at once.
+constexpr float kPagedShort = 32.f;
+
+// Units of a split, from a launch's work (tiles x units, summed in fp32) and 1 / target. The sum is off by less than 2^-17 of itself (64
+// additions in a lane, 6 across, roundings of 2^-24), so this, rounded up from more than that above it, is no less than work / target, and
+// splits add no more than target items.
+CKV_HOST_DEVICE static inline int paged_split_units(float work, float inv_target, int min_units) {
+  const int each = (int)fminf(work * inv_target * (1.f + 0x1p-16f), 0x1p29f) + 1;
+  const int least = work <= kPagedShort ? 1 : min_units;
+  return each > least ? each : least;
+}
+// ceil(units / split_units), at least 1; inv = 1.f / split_units. The product is at most one off: of a tile there are no more than
+// about target splits.
+CKV_HOST_DEVICE static inline int paged_splits(int units, int split_units, float inv) {
+  const int s = (int)((float)units * inv), some = s > 1 ? s : 1;
+  return (int64_t)some * split_units < units ? some + 1 : some;
+}
 
 struct PagedPlan {
   int rows = 0;    // (token, query head) rows of a tile: 16 or 32 (attn_paged_kernel), 128 (attn_active_kernel)

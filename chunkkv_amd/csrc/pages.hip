@@ -324,9 +324,31 @@ __global__ __launch_bounds__(kCopyThreads) void fork_copy_kernel(const Fork* __r
 
 // ---- ending sequences ------------------------------------------------------------------------------------------
 
-// A block a sequence; of two that are the same the first one's.
-__global__ __launch_bounds__(kCopyThreads) void free_pages_kernel(const int32_t* __restrict__ sequences, Book b,
-                                                                  int32_t* __restrict__ err) {
+// The rows that sequence sequences[i] keeps, into rows[i]: at most keep[i], all of them (flagged) where keep[i] is negative or its last row
+// would be one of several in a page that others share, which the next rows would then be written into.
+__global__ __launch_bounds__(kCopyThreads) void keep_rows_kernel(int32_t* __restrict__ rows, const int32_t* __restrict__ sequences,
+                                                                 const int32_t* __restrict__ keep, int n, Book b,
+                                                                 int32_t* __restrict__ err) {
+  const int i = blockIdx.x * kCopyThreads + threadIdx.x;
+  if (i >= n) return;
+  const int s = sequences[i];
+  if ((uint32_t)s >= (uint32_t)b.S) return;  // the next launch flags it
+  const int len = rows_of(b, s);
+  int left = min(keep[i], len);
+  if (left < len && (left & ((1 << b.T_log) - 1)) != 0) {
+    const int p = left < 0 ? -1 : b.table[(int64_t)s * b.M + (left >> b.T_log)];
+    if ((uint32_t)p >= (uint32_t)b.P || b.refs[p] > 1) left = -1;
+  }
+  if (left < 0) {
+    flag_error(err, CKV_DEVICE_ERR_RANGE);
+    left = len;
+  }
+  rows[i] = left;
+}
+
+// A block a sequence; of two that are the same the first one's. rows NULL: no row is kept.
+__global__ __launch_bounds__(kCopyThreads) void free_pages_kernel(const int32_t* __restrict__ sequences, const int32_t* __restrict__ rows,
+                                                                  Book b, int32_t* __restrict__ err) {
   const int s = sequences[blockIdx.x];
   if ((uint32_t)s >= (uint32_t)b.S) {
     if (threadIdx.x == 0) flag_error(err, CKV_DEVICE_ERR_RANGE);
@@ -335,16 +357,17 @@ __global__ __launch_bounds__(kCopyThreads) void free_pages_kernel(const int32_t*
   int before = 0;
   for (int i = threadIdx.x; i < (int)blockIdx.x; i += kCopyThreads) before |= sequences[i] == s;
   if (__syncthreads_or(before)) return;
-  const int pages = (rows_of(b, s) + (1 << b.T_log) - 1) >> b.T_log;
+  auto pages_of = [&](int r) { return (int)(((uint32_t)r + (1u << b.T_log) - 1) >> b.T_log); };
+  const int left = rows != nullptr ? rows[blockIdx.x] : 0, pages = pages_of(rows_of(b, s));
   int32_t* row = b.table + (int64_t)s * b.M;
-  for (int j = threadIdx.x; j < pages; j += kCopyThreads) {
+  for (int j = pages_of(left) + threadIdx.x; j < pages; j += kCopyThreads) {
     const int p = row[j];
     if ((uint32_t)p < (uint32_t)b.P) atomicSub(&b.refs[p], 1);
     else flag_error(err, CKV_DEVICE_ERR_RANGE);
     row[j] = -1;
   }
   __syncthreads();
-  if (threadIdx.x == 0) b.lengths[s] = 0;
+  if (threadIdx.x == 0) b.lengths[s] = left;
 }
 
 // ---- moving pages together -------------------------------------------------------------------------------------
@@ -502,9 +525,9 @@ extern "C" int32_t ckv_fork_pages(void* k_pool, void* v_pool, int64_t layer_stri
   return CKV_OK;
 }
 
-extern "C" int32_t ckv_free_pages(const int32_t* sequences, int32_t n, int32_t* table, int32_t* lengths, int32_t* refs,
-                                  int32_t n_sequences, int32_t n_entries, int32_t n_pages, int32_t page_tokens, int32_t* err,
-                                  void* stream) {
+extern "C" int32_t ckv_free_pages(const int32_t* sequences, const int32_t* keep, int32_t n, int32_t* table, int32_t* lengths,
+                                  int32_t* refs, int32_t n_sequences, int32_t n_entries, int32_t n_pages, int32_t page_tokens,
+                                  void* workspace, int64_t workspace_bytes, int32_t* err, void* stream) {
   using namespace ckv;
   Book b;
   CKV_RETURN_IF_BAD(make_book(b, table, lengths, refs, n_sequences, n_entries, n_pages, page_tokens));
@@ -512,7 +535,15 @@ extern "C" int32_t ckv_free_pages(const int32_t* sequences, int32_t n, int32_t* 
   if (n == 0) return CKV_OK;
   if (sequences == nullptr) return CKV_ERR_INVALID_ARGUMENT;
   if (n > kMostSequences) return CKV_ERR_TOO_LARGE;
-  hipLaunchKernelGGL(free_pages_kernel, dim3((unsigned)n), dim3(kCopyThreads), 0, (hipStream_t)stream, sequences, b, err);
+  int32_t* rows = nullptr;
+  if (keep != nullptr) {
+    if (workspace == nullptr || (uintptr_t)workspace % 4 || workspace_bytes < (int64_t)n * 4) return CKV_ERR_INVALID_ARGUMENT;
+    rows = (int32_t*)workspace;
+    hipLaunchKernelGGL(keep_rows_kernel, dim3((unsigned)((n + kCopyThreads - 1) / kCopyThreads)), dim3(kCopyThreads), 0,
+                       (hipStream_t)stream, rows, sequences, keep, n, b, err);
+    CKV_RETURN_IF_LAUNCH_FAILED();
+  }
+  hipLaunchKernelGGL(free_pages_kernel, dim3((unsigned)n), dim3(kCopyThreads), 0, (hipStream_t)stream, sequences, rows, b, err);
   CKV_RETURN_IF_LAUNCH_FAILED();
   return CKV_OK;
 }

@@ -833,12 +833,12 @@ PyObject* extend_pages(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
   need_args(n_args, 7);
   const PageBook b = page_book(a);
   const Tensor counts = int_vector(a[4], b, "counts"), err = optional_tensor(a[6]);
+  int32_t* const e = status_word(err, b.table);
   const int64_t n = integer(a[5]);
   if (counts.numel() != b.S) value_error("counts must be (sequences,)");
   if (n < 0 || n > INT32_MAX) value_error("n must be 0 to 2^31 - 1");
   const Tensor positions = new_tensor({n}, at::kLong, b.table), rows = new_tensor({n}, at::kLong, b.table);
   const Tensor starts = new_tensor({b.S + 1}, at::kInt, b.table);
-  int32_t* const e = status_word(err, b.table);
   check(unlocked([&] {
           const c10::DeviceGuard on(b.table.device());
           return ckv_extend_pages((int64_t*)ptr(positions), (int64_t*)ptr(rows), (int32_t*)ptr(starts), int32(n), (const int32_t*)ptr(counts),
@@ -857,13 +857,13 @@ PyObject* fork_pages(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
   const PageBook b = page_book(a);
   const PagePool p = page_pool(b, a[4], a[5]);
   const Tensor sources = int_vector(a[6], b, "sources"), targets = int_vector(a[7], b, "targets"), err = optional_tensor(a[8]);
+  int32_t* const e = status_word(err, b.table);
   const int64_t n = sources.numel();
   if (targets.numel() != n) value_error("sources and targets must be of one length");
   const int code = dtype_code(p.k);
   const int64_t ws_bytes = ckv_fork_pages_workspace_bytes(int32(n));
   Tensor ws;
   if (ws_bytes > 0) ws = new_tensor({ws_bytes / 4}, at::kInt, b.table);
-  int32_t* const e = status_word(err, b.table);
   check(unlocked([&] {
           const c10::DeviceGuard on(b.table.device());
           return ckv_fork_pages(ptr(p.k), ptr(p.v), p.k.stride(0), p.k.stride(2), int32(p.L), int32(p.H), int32(p.D), code,
@@ -875,17 +875,24 @@ PyObject* fork_pages(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
   CKV_PY_END
 }
 
-// free_pages(table, lengths, refs, page_tokens, sequences, err)
+// free_pages(table, lengths, refs, page_tokens, sequences, keep, err)
 PyObject* free_pages(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
   CKV_PY_BEGIN
-  need_args(n_args, 6);
+  need_args(n_args, 7);
   const PageBook b = page_book(a);
-  const Tensor sequences = int_vector(a[4], b, "sequences"), err = optional_tensor(a[5]);
+  const Tensor sequences = int_vector(a[4], b, "sequences"), err = optional_tensor(a[6]);
   int32_t* const e = status_word(err, b.table);
+  const int64_t n = sequences.numel();
+  Tensor keep, ws;
+  if (a[5] != Py_None) {
+    keep = int_vector(a[5], b, "keep");
+    if (keep.numel() != n) value_error("sequences and keep must be of one length");
+    ws = new_tensor({n}, at::kInt, b.table);
+  }
   check(unlocked([&] {
           const c10::DeviceGuard on(b.table.device());
-          return ckv_free_pages((const int32_t*)ptr(sequences), int32(sequences.numel()), b.at(b.table), b.at(b.lengths), b.at(b.refs),
-                                int32(b.S), int32(b.M), int32(b.P), int32(b.T), e, stream_of(b.table));
+          return ckv_free_pages((const int32_t*)ptr(sequences), (const int32_t*)ptr(keep), int32(n), b.at(b.table), b.at(b.lengths),
+                                b.at(b.refs), int32(b.S), int32(b.M), int32(b.P), int32(b.T), ptr(ws), n * 4, e, stream_of(b.table));
         }),
         "ckv_free_pages");
   Py_RETURN_NONE;
@@ -899,10 +906,10 @@ PyObject* compact_pages(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
   const PageBook b = page_book(a);
   const PagePool p = page_pool(b, a[4], a[5]);
   const Tensor err = optional_tensor(a[6]);
+  int32_t* const e = status_word(err, b.table);
   const int code = dtype_code(p.k);
   const int64_t ws_bytes = ckv_compact_pages_workspace_bytes(int32(b.P));
   const Tensor ws = new_tensor({ws_bytes / 4}, at::kInt, b.table), used = new_tensor({1}, at::kInt, b.table);
-  int32_t* const e = status_word(err, b.table);
   check(unlocked([&] {
           const c10::DeviceGuard on(b.table.device());
           return ckv_compact_pages(ptr(p.k), ptr(p.v), p.k.stride(0), p.k.stride(2), int32(p.L), int32(p.H), int32(p.D), code,
@@ -923,6 +930,7 @@ PyObject* attention_paged(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
   const PagePool p = page_pool(b, a[5], a[6]);
   const int64_t layer = integer(a[7]), most = a[9] == Py_None ? 0 : integer(a[9]);
   const Tensor starts = int_vector(a[8], b, "starts"), err = optional_tensor(a[11]);
+  int32_t* const e = status_word(err, q);
   Tensor out = optional_tensor(a[12]);
   same_device(q, p.k);
   need_dims(q, 4, "q");
@@ -950,7 +958,6 @@ PyObject* attention_paged(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
                                  : 0;
   Tensor ws;
   if (ws_bytes > 0) ws = new_tensor({(ws_bytes + 3) / 4}, at::kFloat, q);
-  int32_t* const e = status_word(err, q);
   check(unlocked([&] {
           const c10::DeviceGuard on(q.device());
           const int64_t at = layer * p.k.stride(0) * 2;
@@ -1064,6 +1071,7 @@ PyObject* next_tokens(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
   need_args(n_args, 10);
   const LogitArgs r = logit_args(a);
   const Tensor err = optional_tensor(a[8]);
+  int32_t* const e = status_word(err, r.logits);
   Tensor out = optional_tensor(a[9]);
   if (!out.defined()) {
     out = new_tensor({r.rows}, at::kLong, r.logits);
@@ -1075,7 +1083,6 @@ PyObject* next_tokens(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
   const int64_t ws_bytes = ckv_next_tokens_workspace_bytes(int32(r.rows), int32(r.vocab));
   Tensor ws;
   if (ws_bytes > 0) ws = new_tensor({ws_bytes / 8}, at::kLong, r.logits);
-  int32_t* const e = status_word(err, r.logits);
   check(unlocked([&] {
           const c10::DeviceGuard on(r.logits.device());
           return ckv_next_tokens((int64_t*)ptr(out), CKV_LOGIT_ARGS(r), ptr(ws), ws_bytes, e, stream_of(r.logits));

@@ -87,6 +87,7 @@ from torch.nn.modules.module import _has_any_global_hook
 
 from chunkkv_amd import _native, ops
 from chunkkv_amd.model import DecoderPieces
+from chunkkv_amd.paged import PagedSession
 from chunkkv_amd.planner import RequestPlan, local_index, plan_request, stats_dict
 from chunkkv_amd.types import BlendConfig, ChunkKV, Placement, PrefillResult, plan_positions  # noqa: F401
 
@@ -542,6 +543,11 @@ class HipEngine(DecoderPieces):
                                                enable_gqa=True)
             h, pending = self._mlp(li, layer, h, layer.self_attn.o_proj(o.transpose(1, 2).reshape(1, 1, -1)))
         tok.copy_(self._final_logits(h, pending)[0, -1].argmax().view(1, 1))
+
+    def paged(self, n_pages: int, n_sequences: int, max_tokens: int, page_tokens: int = 64) -> PagedSession:
+        """A cache of n_pages pages for up to n_sequences sequences of max_tokens rows each, decoded together: see PagedSession.
+        Needs the positions-masked attention kernel (bf16 caches with head_dim 64 or 128)."""
+        return PagedSession(self, n_pages, n_sequences, max_tokens, page_tokens)
 
     # -- main entry -----------------------------------------------------------------------
 

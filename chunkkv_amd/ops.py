@@ -803,9 +803,10 @@ def fork_pages(cache: PagedCache, sources: torch.Tensor, targets: torch.Tensor, 
     _native.torch_ops().fork_pages(cache.table, cache.lengths, cache.refs, cache.page_tokens, cache.k, cache.v, sources, targets, err)
 
 
-def free_pages(cache: PagedCache, sequences: torch.Tensor, err: torch.Tensor | None = None) -> None:
-    """The sequences (int32) end: pages that no other shares are free again."""
-    _native.torch_ops().free_pages(cache.table, cache.lengths, cache.refs, cache.page_tokens, sequences, err)
+def free_pages(cache: PagedCache, sequences: torch.Tensor, keep: torch.Tensor | None = None, err: torch.Tensor | None = None) -> None:
+    """The sequences (int32) end: pages that no other shares are free again. keep (int32, a number of rows each): they go back to their
+    first keep rows instead; one that would end inside a page that another shares stays as it is, and err is set."""
+    _native.torch_ops().free_pages(cache.table, cache.lengths, cache.refs, cache.page_tokens, sequences, keep, err)
 
 
 def compact_pages(cache: PagedCache, err: torch.Tensor | None = None) -> torch.Tensor:

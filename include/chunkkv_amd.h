@@ -681,11 +681,16 @@ int32_t ckv_fork_pages(void* k_pool, void* v_pool, int64_t layer_stride, int64_t
 int64_t ckv_fork_pages_workspace_bytes(int32_t n_pairs); /* host-only */
 
 /*
- * The sequences end: their pages' refs - 1, their table entries -1, their lengths 0. One named twice ends once, an empty one stays
- * so, one that does not exist is flagged (CKV_DEVICE_ERR_RANGE). n at most 4096. One launch.
+ * The sequences end: their pages' refs - 1, their table entries -1, their lengths 0. With keep they go back to their first keep[i] rows
+ * instead, where those are fewer (0: none), and give up the pages behind; one stays as it is and is flagged (CKV_DEVICE_ERR_RANGE) where keep[i] is negative or
+ * ends inside a page that another sequence shares. One named twice counts the first time, an empty one stays
+ * so, one that does not exist is flagged (CKV_DEVICE_ERR_RANGE). n at most 4096.
+ *   workspace  with keep: device buffer of workspace_bytes >= 4 n
+ * One launch, with keep two.
  */
-int32_t ckv_free_pages(const int32_t* sequences, int32_t n, int32_t* table, int32_t* lengths, int32_t* refs, int32_t n_sequences,
-                       int32_t n_entries, int32_t n_pages, int32_t page_tokens, int32_t* err, void* stream);
+int32_t ckv_free_pages(const int32_t* sequences, const int32_t* keep, int32_t n, int32_t* table, int32_t* lengths, int32_t* refs,
+                       int32_t n_sequences, int32_t n_entries, int32_t n_pages, int32_t page_tokens, void* workspace,
+                       int64_t workspace_bytes, int32_t* err, void* stream);
 
 /*
  * The used pages become pages 0 .. *used - 1: of U used ones, the i-th at U or above (ascending) moves to the i-th free one below U in

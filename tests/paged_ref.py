@@ -79,14 +79,22 @@ class Book:
                 self.moves.append((self.table[a][whole], self.table[b][whole]))
             self.lengths[b] = before[a]
 
-    def free(self, sequences):
-        for s in sequences:
+    def free(self, sequences, keep=None):
+        refs, done = list(self.refs), set()
+        for i, s in enumerate(sequences):
             if not 0 <= s < len(self.lengths):
                 self.err |= RANGE
                 continue
-            for p in self.table[s]:
+            left = 0 if keep is None else min(keep[i], self.lengths[s])
+            if s in done:
+                continue
+            done.add(s)
+            if left < 0 or left < self.lengths[s] and left % self.T and refs[self.table[s][left // self.T]] > 1:
+                self.err |= RANGE
+                continue
+            for p in self.table[s][self.pages_of(left):]:
                 self.refs[p] -= 1
-            self.table[s], self.lengths[s] = [], 0
+            self.table[s], self.lengths[s] = self.table[s][:self.pages_of(left)], left
 
     def compact(self):
         used = sum(r > 0 for r in self.refs)

@@ -67,7 +67,7 @@ def test_a_life_of_calls(T, S, max_tokens, P, dtype, D, seed):
     c, book, err = _cache(S, max_tokens, P, T, D=D, dtype=dtype)
     held = Held(c, book)
     for _ in range(25):
-        what = rng.choice(["extend", "extend", "extend", "fork", "free", "compact"])
+        what = rng.choice(["extend", "extend", "extend", "fork", "free", "keep", "compact"])
         if what == "extend":
             counts = [rng.choice([0, 0, 1, 1, rng.randint(0, max_tokens // 2), T, max_tokens + T, -1][:8 if rng.random() < 0.2 else 6]) for _ in range(S)]
             fits = [x for x in counts if x > 0]
@@ -88,10 +88,17 @@ def test_a_life_of_calls(T, S, max_tokens, P, dtype, D, seed):
         elif what == "free":
             ended = [rng.randrange(S) for _ in range(rng.randint(1, 3))] + ([S] if rng.random() < 0.1 else [])
             book.free(ended)
-            ops.free_pages(c, _ints(ended), err)
+            ops.free_pages(c, _ints(ended), err=err)
             for s in ended:
                 if s < S:
                     held.rows[s] = []
+        elif what == "keep":
+            at = rng.sample(range(S), min(S, 3))
+            left = [rng.choice([0, rng.randint(-1, max_tokens), T * rng.randint(0, 4)]) for _ in at]
+            book.free(at, left)
+            ops.free_pages(c, _ints(at), _ints(left), err)
+            for s in at:
+                held.rows[s] = held.rows[s][:book.lengths[s]]
         else:
             assert ops.compact_pages(c, err).tolist() == [book.compact()]
         book.check(c, err)
@@ -110,7 +117,7 @@ def test_pools_of_all_sizes(P):
         assert got.rows.tolist() == want[1]
         ended = rng.randrange(3)
         book.free([ended])
-        ops.free_pages(c, _ints([ended]), err)
+        ops.free_pages(c, _ints([ended]), err=err)
         book.check(c, err)
         assert ops.compact_pages(c, err).tolist() == [book.compact()]
         book.check(c, err)
@@ -128,7 +135,7 @@ def test_many_sequences(S):
         book.check(c, err)
     ended = rng.sample(range(S), S // 2) + [0, 0]
     book.free(ended)
-    ops.free_pages(c, _ints(ended), err)
+    ops.free_pages(c, _ints(ended), err=err)
     book.check(c, err)
     pairs = list(zip([rng.randrange(S) for _ in range(S)], rng.sample(range(S), S)))
     book.fork(*zip(*pairs))
@@ -154,7 +161,7 @@ def test_rows_of_other_pages_stay():
     book.extend(counts, 170)
     ops.extend_pages(c, _ints(counts), 170, err)
     book.free([0])
-    ops.free_pages(c, _ints([0]), err)
+    ops.free_pages(c, _ints([0]), err=err)
     for call in ("fork", "compact"):
         k, v = c.k.clone(), c.v.clone()
         if call == "fork":
@@ -176,7 +183,7 @@ def test_a_broken_table_is_flagged():
     c, book, err = _cache(3, 200, 8, 32)
     ops.extend_pages(c, _ints([70, 40, 0]), 110)
     c.table[0, 0], c.table[0, 2], c.table[1, 1] = 99, -5, 2**30
-    for call in (lambda: ops.fork_pages(c, _ints([0]), _ints([2]), err), lambda: ops.compact_pages(c, err), lambda: ops.free_pages(c, _ints([0, 1, 2]), err)):
+    for call in (lambda: ops.fork_pages(c, _ints([0]), _ints([2]), err), lambda: ops.compact_pages(c, err), lambda: ops.free_pages(c, _ints([0, 1, 2]), err=err)):
         err.zero_()
         call()
         assert int(err.item()) == 1
@@ -196,4 +203,19 @@ def test_captured_steps_take_pages():
         graph.replay()
         want = book.extend([1, 0, 40], 41)
         assert got.positions.tolist() == want[0] and got.rows.tolist() == want[1]
+        book.check(c, err)
+
+
+def test_going_back_inside_a_shared_page_is_refused():
+    """Two sequences share a page; one of them cannot go back into it, alone or together with the other, but to its end it can."""
+    c, book, err = _cache(3, 200, 12, 32)
+    book.extend([70, 0, 5], 75)
+    ops.extend_pages(c, _ints([70, 0, 5]), 75, err)
+    book.fork([0], [1])
+    ops.fork_pages(c, _ints([0]), _ints([1]), err)
+    for at, left in (([0], [40]), ([0, 1], [40, 50]), ([0, 1], [40, 0]), ([0], [64]), ([0, 0, 2], [32, 0, 3]), ([0, 2], [20, 9])):
+        book.err = 0
+        err.zero_()
+        book.free(at, left)
+        ops.free_pages(c, _ints(at), _ints(left), err)
         book.check(c, err)
