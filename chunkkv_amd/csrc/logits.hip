@@ -10,17 +10,17 @@
 // atomics: any order gives the same counts), while its logits are on their way, then reads each logit once.
 // No table of counts over the vocabulary exists in memory, so there is no state to keep, and a step reads the logits and
 // the tokens. Bound: latency up to a few rows, the logits' bytes (and the result's) beyond.
-#include "ckv_common.hpp"
+#include "attention_common.hpp"
 
 namespace ckv {
 
-// Loads and stores of 16 bytes wherever an element may lie: rows of an odd vocabulary start anywhere.
+// Sixteen bytes wherever an element may lie. Loads and stores here are of this kind: rows of an odd vocabulary start anywhere, and the
+// device takes 16 bytes at any address.
 __device__ __forceinline__ vec16 ld16_any(const void* p) {
   vec16 v;
   __builtin_memcpy(&v, p, 16);
   return v;
 }
-__device__ __forceinline__ void st16_any(void* p, const vec16& v) { __builtin_memcpy(p, &v, 16); }
 
 struct RowValue {  // of a row: rows[b], or one for all
   const float* rows;
@@ -41,39 +41,60 @@ struct Adjust {
   int64_t allowed_stride;
 };
 
-constexpr int kLogitsEach = 8;  // logits of a thread
+constexpr int kLogitsThreads = 512, kLogitsEach = 8;  // logits of a thread
+constexpr int kLogitsSlice = kLogitsThreads * kLogitsEach;
 constexpr uint32_t kInPrompt = 1u << 31;
 
-// f over the row's tokens that lie in [v0, v0 + count), as offsets. A batch's loads go out together, the last one's too
-// (past the row's end they read its last pair again, which is passed over).
-template <int NT, typename F>
-__device__ __forceinline__ void each_token(const Tokens& t, int row, int64_t v0, int count, F f) {
-  const int64_t* p = t.at + row * t.stride;
-  constexpr int U = 4;
-  auto take = [&](int64_t v) {
+// Counts the row's tokens that lie in [v0, v0 + kLogitsSlice) into count[]: occurrences in generated, kInPrompt where it is in the prompt. Both
+// lists are one of pairs, whose loads go out U at a time for each thread, the last of them too (past the end they read the last pair
+// again, which is passed over).
+__device__ __forceinline__ void count_tokens(const Tokens& prompt, const Tokens& generated, int row, int64_t v0, uint32_t* count) {
+  const int64_t* pt = prompt.at + row * prompt.stride;
+  const int64_t* gt = generated.at + row * generated.stride;
+  const int pp = prompt.n / 2, pairs = pp + generated.n / 2;
+  constexpr int NT = kLogitsThreads, U = 4;
+  auto take = [&](int64_t v, bool in_prompt) {
     const uint64_t o = (uint64_t)(v - v0);
-    if (o < (uint64_t)count) f((int)o);
+    if (o >= (uint64_t)kLogitsSlice) return;
+    if (in_prompt) atomicOr(&count[o], kInPrompt);
+    else atomicAdd(&count[o], 1u);
   };
-  const int pairs = t.n / 2;
   for (int i0 = 0; i0 < pairs; i0 += U * NT) {
     vec16 v[U];
 #pragma unroll
-    for (int u = 0; u < U; ++u) v[u] = ld16_any(p + 2 * min(i0 + u * NT + (int)threadIdx.x, pairs - 1));
+    for (int u = 0; u < U; ++u) {
+      if (i0 + u * NT >= pairs) continue;  // uniform
+      const int i = min(i0 + u * NT + (int)threadIdx.x, pairs - 1);
+      v[u] = ld16_any(i < pp ? pt + 2 * i : gt + 2 * (i - pp));
+    }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      if (i0 + u * NT + (int)threadIdx.x >= pairs) continue;
-      take((int64_t)((uint64_t)v[u][1] << 32 | v[u][0]));
-      take((int64_t)((uint64_t)v[u][3] << 32 | v[u][2]));
+      const int i = i0 + u * NT + (int)threadIdx.x;
+      if (i0 + u * NT >= pairs || i >= pairs) continue;
+      take((int64_t)((uint64_t)v[u][1] << 32 | v[u][0]), i < pp);
+      take((int64_t)((uint64_t)v[u][3] << 32 | v[u][2]), i < pp);
     }
   }
-  if ((t.n & 1) != 0 && threadIdx.x == 0) take(p[t.n - 1]);
+  if ((prompt.n & 1) != 0 && threadIdx.x == 0) take(pt[prompt.n - 1], true);
+  if ((generated.n & 1) != 0 && threadIdx.x == 64) take(gt[generated.n - 1], false);
 }
 
-// A logit as a key whose order is argmax's: larger logits first, a NaN above all, -0 as 0; then the lower index.
-__device__ __forceinline__ uint64_t logit_key(float x, int v) {
-  const uint32_t u = __float_as_uint(x == 0.f ? 0.f : x);
-  const uint32_t order = x != x ? UINT32_MAX : (u & 0x80000000u) ? ~u : u | 0x80000000u;
-  return (uint64_t)order << 32 | (uint32_t)(INT32_MAX - v);
+// A logit as a number whose order is argmax's: a NaN above all, -0 as 0.
+__device__ __forceinline__ uint32_t logit_order(float x) {
+  const uint32_t u = __float_as_uint(x + 0.f);  // -0 + 0 is 0
+  return x != x ? UINT32_MAX : u ^ ((uint32_t)((int32_t)u >> 31) | 0x80000000u);
+}
+// And with its place: of equal ones the first is the larger.
+__device__ __forceinline__ uint64_t logit_key(uint32_t order, int v) { return (uint64_t)order << 32 | (uint32_t)(INT32_MAX - v); }
+// The key of the wavefront's largest, for places that ascend with the lanes.
+__device__ __forceinline__ uint64_t wave_best(uint32_t order, int v) {
+  auto up = [](uint32_t a, uint32_t b) { return a > b ? a : b; };
+  uint32_t m = row16_reduce(order, up);
+  auto pair = [&](auto r) { return up(r[0], r[1]); };
+  m = pair(__builtin_amdgcn_permlane16_swap(m, m, false, false));
+  m = pair(__builtin_amdgcn_permlane32_swap(m, m, false, false));
+  const int first = __builtin_ctzll(__builtin_amdgcn_ballot_w64(order == m));
+  return logit_key(m, __builtin_amdgcn_readlane(v, first));
 }
 __device__ __forceinline__ uint64_t wave_max(uint64_t x) {
 #pragma unroll
@@ -89,109 +110,120 @@ __device__ __forceinline__ void store_token(int64_t* to, uint64_t key, int32_t* 
   if ((uint32_t)(key >> 32) == kNegInf) flag_error(err, CKV_DEVICE_ERR_NO_TOKEN);
 }
 
-// WRITE: the adjusted logits to out; else each slice's best key to keys, or the token where a row is one slice.
-template <typename E, int NT, bool WRITE>
-__global__ __launch_bounds__(NT) void adjust_logits_kernel(const char* __restrict__ logits, int64_t row_b, int V, Adjust a,
-                                                           float* __restrict__ out, uint64_t* __restrict__ keys,
-                                                           int64_t* __restrict__ tokens, int32_t* __restrict__ err) {
-  constexpr int N = kLogitsEach, SLICE = NT * N, VN = N / E::kVec;
-  __shared__ uint32_t s_count[SLICE];
-  const int row = blockIdx.y, v0 = blockIdx.x * SLICE, v = v0 + threadIdx.x * N;
-  const int here = min(N, V - v);  // <= 0: past the vocabulary
-  const char* p = logits + row * row_b + (int64_t)v * E::kBytes;
-  float x[N];
-  vec16 raw[VN];
-  if (here >= N) {
+// WRITE: the adjusted logits to out; else each slice's best key to keys, or the token where a row is one slice. A thread's logits are
+// vectors of W, a workgroup's threads side by side: 16 bytes of what is written, or else of what is read.
+template <typename E, bool WRITE>
+__global__ __launch_bounds__(kLogitsThreads) void adjust_logits_kernel(const char* __restrict__ logits, int64_t row_b, int V, Adjust a,
+                                                                       float* __restrict__ out, uint64_t* __restrict__ keys,
+                                                                       int64_t* __restrict__ tokens, int32_t* __restrict__ err) {
+  constexpr int NT = kLogitsThreads, W = WRITE ? 4 : E::kVec, NV = kLogitsEach / W;
+  __shared__ __attribute__((aligned(16))) uint32_t s_count[kLogitsSlice];
+  const int row = blockIdx.y, v0 = blockIdx.x * kLogitsSlice, tid = threadIdx.x;
+  const char* p = logits + row * row_b;
+  const float* bias = a.bias != nullptr ? a.bias + row * a.bias_stride : nullptr;
+  const uint32_t* allowed = a.allowed != nullptr ? a.allowed + row * a.allowed_stride : nullptr;
+  auto first = [&](int k) { return v0 + (k * NT + tid) * W; };
+  float x[NV][W], add[NV][W];
+  uint32_t bits[NV];
 #pragma unroll
-    for (int i = 0; i < VN; ++i) raw[i] = ld16_any(p + 16 * i);
-  }
-  const float* bias = a.bias != nullptr ? a.bias + row * a.bias_stride + v : nullptr;
-  vec16 b[N / 4];
-  if (bias != nullptr && here >= N) {
+  for (int k = 0; k < NV; ++k) {
+    const int v = first(k);
+    if (v + W <= V) {
+      uint32_t w[W * E::kBytes / 4];
+      __builtin_memcpy(w, p + (int64_t)v * E::kBytes, sizeof(w));
 #pragma unroll
-    for (int i = 0; i < N / 4; ++i) b[i] = ld16_any(bias + 4 * i);
-  }
-  uint32_t bits = ~0u;
-  if (a.allowed != nullptr && here > 0) bits = a.allowed[row * a.allowed_stride + v / 32] >> (v % 32);
-
-  const bool history = a.prompt.n > 0 || a.generated.n > 0;
-  if (history) {
+      for (int i = 0; i < W; ++i)
+        x[k][i] = E::kBytes == 4 ? __uint_as_float(w[i]) : __uint_as_float(i % 2 ? w[i / 2] & 0xffff0000u : w[i / 2] << 16);
+      if (bias != nullptr) __builtin_memcpy(add[k], bias + v, sizeof(add[k]));
+    } else {
 #pragma unroll
-    for (int i = 0; i < N; ++i) s_count[i * NT + threadIdx.x] = 0;
-    __syncthreads();
-    // a thread's N logits are N words NT apart, so that its reads below spread over the banks
-    auto word = [](int o) { return (o % N) * NT + o / N; };
-    if (a.prompt.n > 0) each_token<NT>(a.prompt, row, v0, SLICE, [&](int o) { atomicOr(&s_count[word(o)], kInPrompt); });
-    if (a.generated.n > 0) each_token<NT>(a.generated, row, v0, SLICE, [&](int o) { atomicAdd(&s_count[word(o)], 1u); });
-    __syncthreads();
-  }
-  if (here >= N) {
-#pragma unroll
-    for (int i = 0; i < VN; ++i) {
-      float f[E::kVec];
-      E::unpack(raw[i], f);
-#pragma unroll
-      for (int j = 0; j < E::kVec; ++j) x[i * E::kVec + j] = f[j];
+      for (int i = 0; i < W; ++i) {
+        x[k][i] = add[k][i] = 0.f;
+        if (v + i >= V) continue;
+        if constexpr (E::kBytes == 2) x[k][i] = bf16_bits_to_f32(((const uint16_t*)p)[v + i]);
+        else x[k][i] = ((const float*)p)[v + i];
+        if (bias != nullptr) add[k][i] = bias[v + i];
+      }
     }
-  } else {
+    bits[k] = ~0u;
+    if (allowed != nullptr && v < V) bits[k] = allowed[v / 32] >> (v % 32);
+  }
+
+  if (a.prompt.n > 0 || a.generated.n > 0) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      x[i] = 0.f;
-      if (i < here) {
-        if constexpr (E::kBytes == 2) x[i] = bf16_bits_to_f32(((const uint16_t*)p)[i]);
-        else x[i] = ((const float*)p)[i];
+    for (int i = 0; i < kLogitsEach / 4; ++i) ((vec16*)s_count)[i * NT + tid] = vec16{0, 0, 0, 0};
+    __syncthreads();
+    count_tokens(a.prompt, a.generated, row, v0, s_count);
+    __syncthreads();
+    const float r = a.repetition.at(row), f = a.frequency.at(row), pr = a.presence.at(row);
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      uint32_t s[W], any = 0;
+#pragma unroll
+      for (int i = 0; i < W / 4; ++i) *(vec16*)(s + 4 * i) = *(const vec16*)(s_count + (k * NT + tid) * W + 4 * i);
+#pragma unroll
+      for (int i = 0; i < W; ++i) any |= s[i];
+      if (__builtin_amdgcn_ballot_w64(any != 0) == 0) continue;  // uniform: most of a vocabulary
+#pragma unroll
+      for (int i = 0; i < W; ++i) {
+        if (__builtin_amdgcn_ballot_w64(s[i] != 0) == 0) continue;
+        const float y = x[k][i] > 0.f ? x[k][i] / r : x[k][i] * r;
+        const uint32_t c = s[i] & ~kInPrompt;
+        x[k][i] = s[i] == 0 ? x[k][i] : c == 0 ? y : y - f * (float)c - pr;
       }
     }
   }
-  if (history) {
-    const float r = a.repetition.at(row), f = a.frequency.at(row), pr = a.presence.at(row);
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const uint32_t s = s_count[i * NT + threadIdx.x];
-      if (s == 0) continue;
-      x[i] = x[i] > 0.f ? x[i] / r : x[i] * r;
-      const uint32_t c = s & ~kInPrompt;
-      if (c > 0) x[i] = x[i] - f * (float)c - pr;
-    }
-  }
   if (bias != nullptr) {
-    if (here >= N) {
 #pragma unroll
-      for (int i = 0; i < N; ++i) x[i] += __uint_as_float(b[i / 4][i % 4]);
-    } else {
+    for (int k = 0; k < NV; ++k)
 #pragma unroll
-      for (int i = 0; i < N; ++i)
-        if (i < here) x[i] += bias[i];
-    }
+      for (int i = 0; i < W; ++i) x[k][i] += add[k][i];
   }
+  if (allowed != nullptr) {
 #pragma unroll
-  for (int i = 0; i < N; ++i)
-    if (!(bits >> i & 1)) x[i] = -INFINITY;
+    for (int k = 0; k < NV; ++k)
+#pragma unroll
+      for (int i = 0; i < W; ++i)
+        if (!(bits[k] >> i & 1)) x[k][i] = -INFINITY;
+  }
 
   if constexpr (WRITE) {
-    float* to = out + (int64_t)row * V + v;
-    if (here >= N) {
+    // non-temporal: 64 rows of 152064, 61 MB, take 15.4 us in place of 18.2 (without a history 9.8 and 12.2)
 #pragma unroll
-      for (int i = 0; i < N / 4; ++i)
-        st16_any(to + 4 * i, vec16{__float_as_uint(x[4 * i]), __float_as_uint(x[4 * i + 1]), __float_as_uint(x[4 * i + 2]),
-                                   __float_as_uint(x[4 * i + 3])});
-    } else {
+    for (int k = 0; k < NV; ++k) {
+      const int v = first(k);
+      float* to = out + (int64_t)row * V + v;
+      if (v + W <= V) {
+        typedef float any4 __attribute__((ext_vector_type(4), aligned(4)));
+        static_assert(W == 4, "one store");
+        __builtin_nontemporal_store(any4{x[k][0], x[k][1], x[k][2], x[k][3]}, (any4*)to);
+      } else {
 #pragma unroll
-      for (int i = 0; i < N; ++i)
-        if (i < here) to[i] = x[i];
+        for (int i = 0; i < W; ++i)
+          if (v + i < V) to[i] = x[k][i];
+      }
     }
   } else {
-    uint64_t best = 0;  // below every logit's key
+    uint64_t best = 0;  // below every logit
 #pragma unroll
-    for (int i = 0; i < N; ++i)
-      if (i < here) best = max(best, logit_key(x[i], v + i));
+    for (int k = 0; k < NV; ++k) {
+      uint32_t top = 0;
+      int place = first(k);
+#pragma unroll
+      for (int i = 0; i < W; ++i) {
+        const uint32_t o = first(k) + i < V ? logit_order(x[k][i]) : 0;
+        place = o > top ? first(k) + i : place;
+        top = o > top ? o : top;
+      }
+      const uint64_t key = wave_best(top, place);
+      best = key > best ? key : best;
+    }
     __shared__ uint64_t s_best[NT / kWave];
-    best = wave_max(best);
-    if (threadIdx.x % kWave == 0) s_best[threadIdx.x / kWave] = best;
+    if (tid % kWave == 0) s_best[tid / kWave] = best;
     __syncthreads();
-    if (threadIdx.x >= kWave) return;
-    best = wave_max(threadIdx.x < NT / kWave ? s_best[threadIdx.x] : 0);
-    if (threadIdx.x != 0) return;
+    if (tid >= kWave) return;
+    best = wave_max(tid < NT / kWave ? s_best[tid] : 0);
+    if (tid != 0) return;
     if (gridDim.x == 1) store_token(tokens + row, best, err);
     else keys[(int64_t)row * gridDim.x + blockIdx.x] = best;
   }
@@ -207,8 +239,7 @@ __global__ __launch_bounds__(kWave) void best_token_kernel(const uint64_t* __res
   if (threadIdx.x == 0) store_token(tokens + row, best, err);
 }
 
-constexpr int kLogitsThreads = 512;
-static inline int64_t logits_slices(int64_t vocab) { return (vocab + kLogitsThreads * kLogitsEach - 1) / (kLogitsThreads * kLogitsEach); }
+static inline int64_t logits_slices(int64_t vocab) { return (vocab + kLogitsSlice - 1) / kLogitsSlice; }
 
 static int32_t check_adjust(const void* logits, int64_t row_stride, int32_t n_rows, int32_t vocab, int32_t dtype, const Adjust& a) {
   if (n_rows < 0 || vocab <= 0 || (dtype != CKV_DTYPE_BF16 && dtype != CKV_DTYPE_F32)) return CKV_ERR_INVALID_ARGUMENT;
@@ -221,7 +252,7 @@ static int32_t check_adjust(const void* logits, int64_t row_stride, int32_t n_ro
   }
   if ((uintptr_t)a.bias % 4 || (uintptr_t)a.allowed % 4) return CKV_ERR_INVALID_ARGUMENT;
   if (n_rows > 1 && (row_stride < vocab || a.bias_stride < 0 || a.allowed_stride < 0)) return CKV_ERR_OUT_OF_RANGE;
-  if (n_rows > 65535 || vocab > INT32_MAX - kLogitsThreads * kLogitsEach) return CKV_ERR_TOO_LARGE;
+  if (n_rows > 65535 || vocab > INT32_MAX - kLogitsSlice) return CKV_ERR_TOO_LARGE;
   return CKV_OK;
 }
 
@@ -233,8 +264,8 @@ static int32_t adjust_launch(const void* logits, int64_t row_stride, int32_t n_r
   auto launch = [&](auto kernel) {
     hipLaunchKernelGGL(kernel, grid, dim3(kLogitsThreads), 0, st, (const char*)logits, row_stride * e, vocab, a, out, keys, tokens, err);
   };
-  if (e == 2) launch(adjust_logits_kernel<Elem<CKV_DTYPE_BF16>, kLogitsThreads, WRITE>);
-  else launch(adjust_logits_kernel<Elem<CKV_DTYPE_F32>, kLogitsThreads, WRITE>);
+  if (e == 2) launch(adjust_logits_kernel<Elem<CKV_DTYPE_BF16>, WRITE>);
+  else launch(adjust_logits_kernel<Elem<CKV_DTYPE_F32>, WRITE>);
   CKV_RETURN_IF_LAUNCH_FAILED();
   return CKV_OK;
 }
