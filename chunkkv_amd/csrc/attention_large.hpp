@@ -44,7 +44,7 @@ __global__ __launch_bounds__(kAttnWaves * 64) void attn_active_kernel(
   if (!attn_work_item(nqb, map_group, xpk_log, items, inv_group, inv_nqb, qb, hq, z)) return;
   const int hk = GROUPED ? hq : hq / group;
   [[maybe_unused]] PagedItem it;
-  [[maybe_unused]] const int item = qb;
+  [[maybe_unused]] const int item = nqb - 1 - qb;  // paged: from the first
   if constexpr (PAGED) {
     if (!(paged_item<kAttnBM, kAttnBN>(scales, n, group, item, it), ...)) return;
     qb = it.tile;

@@ -34,6 +34,7 @@ __global__ __launch_bounds__(kPagedWaves * 64) void attn_paged_kernel(AttnMap ma
   const int g = lane / 16, lm = lane % 16;
   int item, hk, unused;
   if (!attn_work_item(map.nqb, map.group, map.xpk_log, map.items, map.inv_group, map.inv_nqb, item, hk, unused)) return;
+  item = map.nqb - 1 - item;
   PagedItem it;
   if (!paged_item<ROWS, kPagedUnit>(b, n, group, item, it)) return;
   const int rows = it.count * group, r0 = it.tile * ROWS;
@@ -271,7 +272,7 @@ __global__ __launch_bounds__(256) void join_paged_kernel(char* __restrict__ out,
 #pragma unroll
   for (int turn = 0; turn < TURNS; ++turn) {
     const int h = ((int)blockIdx.y * TURNS + turn) * JH + sub, hc = min(h, Hq - 1), hk = div_by(hc, group, b.inv_gqa);
-    const int m = (t - it.first) * group + hc - hk * group, item = it.item0 + m / ROWS;  // of split 0
+    const int m = (t - it.first) * group + hc - hk * group, item = it.item0 + it.tiles - 1 - m / ROWS;  // of split 0
     // items past cap: starts that descend; no such items were run
     const int parts = item + (int64_t)(live - 1) * it.tiles < b.cap ? live : 0;
     const float* base = ws + (((int64_t)hk * b.cap + item) * ROWS + m % ROWS) * (D + 4);

@@ -26,22 +26,30 @@ struct Book {
   int S, M, P, T_log;
 };
 
-// Inclusive prefix sum over the workgroup's threads of kBookThreads, and the total; s: kBookWaves words that no thread
-// reads any more.
-__device__ __forceinline__ uint64_t book_scan(uint64_t x, uint64_t* s, uint64_t& total) {
-  const int wave = threadIdx.x / kWave;
-  uint64_t incl = wave_incl_scan(x);
-  if (threadIdx.x % kWave == kWave - 1) s[wave] = incl;
-  __syncthreads();
-  total = 0;
-  uint64_t before = 0;
+// Inclusive prefix sums of K values over the workgroup's threads, in x, and the totals.
+template <int K>
+struct ScanRoom {
+  uint64_t of_wave[kBookWaves][K];
+};
+template <int K>
+__device__ __forceinline__ void book_scan(uint64_t (&x)[K], uint64_t (&total)[K], ScanRoom<K>& s) {
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), lane = threadIdx.x % kWave;
 #pragma unroll
-  for (int w = 0; w < kBookWaves; ++w) {
-    if (w == wave) before = total;
-    total += s[w];
+  for (int k = 0; k < K; ++k) {
+    x[k] = wave_incl_scan(x[k]);
+    if (lane == kWave - 1) s.of_wave[wave][k] = x[k];
   }
   __syncthreads();
-  return before + incl;
+  auto at = [](uint64_t v, int l) {
+    return (uint64_t)(uint32_t)__builtin_amdgcn_readlane((uint32_t)(v >> 32), l) << 32 | (uint32_t)__builtin_amdgcn_readlane((uint32_t)v, l);
+  };
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    const uint64_t w = wave_incl_scan(lane < kBookWaves ? s.of_wave[lane][k] : (uint64_t)0);
+    total[k] = at(w, kBookWaves - 1);
+    if (wave > 0) x[k] += at(w, wave - 1);
+  }
+  __syncthreads();
 }
 
 // The i with pre[i] <= x < pre[i + 1], for ascending pre[0 .. n] and pre[0] <= x < pre[n].
@@ -61,7 +69,15 @@ template <typename F>
 __device__ __forceinline__ void each_page(const Book& b, F f) {
   const int n = span_of(b.P);
   const int64_t first = (int64_t)threadIdx.x * n;
-  for (int64_t p = first; p < first + n && p < b.P; ++p) f((int)p, b.refs[p]);
+  const int end = (int)min((int64_t)n, b.P - first);  // <= 0: none
+  int i = 0;
+  for (; i + 4 <= end; i += 4) {
+    int r[4];  // 16 bytes at any word
+    __builtin_memcpy(r, b.refs + first + i, 16);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) f((int)first + i + j, r[j]);
+  }
+  for (; i < end; ++i) f((int)first + i, b.refs[first + i]);
 }
 
 __device__ __forceinline__ int rows_of(const Book& b, int s) { return min(max(b.lengths[s], 0), b.M << b.T_log); }
@@ -73,68 +89,73 @@ __global__ __launch_bounds__(kBookThreads) void extend_pages_kernel(int64_t* __r
                                                                     const int32_t* __restrict__ counts, Book b,
                                                                     int32_t* __restrict__ err) {
   __shared__ uint32_t s_need[kMostSequences + 1], s_start[kMostSequences + 1];  // pages and tokens of the sequences before
-  __shared__ uint64_t s_scan[kBookWaves];
+  __shared__ ScanRoom<2> s_scan2;
+  __shared__ ScanRoom<1> s_scan1;
   const int T = 1 << b.T_log, tid = threadIdx.x;
   auto pages_of = [&](int64_t r) { return (int)((r + T - 1) >> b.T_log); };
-
   auto count_of = [&](int s, int len) {
     const int c = counts[s];
     if (c >= 0 && c <= (b.M << b.T_log) - len) return c;
     flag_error(err, CKV_DEVICE_ERR_RANGE);
     return 0;
   };
-  uint64_t needed = 0;
+  uint64_t needed = 0, tokens = 0;
   for (int s0 = 0; s0 < b.S; s0 += kBookThreads) {
     const int s = s0 + tid;
-    uint64_t need = 0;
+    uint64_t x[2] = {0, 0}, total[2];
     if (s < b.S) {
-      const int len = rows_of(b, s);
-      need = pages_of(len + count_of(s, len)) - pages_of(len);
+      const int len = rows_of(b, s), c = count_of(s, len);
+      x[0] = pages_of(len + c) - pages_of(len);
+      x[1] = c;
     }
-    uint64_t total;
-    const uint64_t incl = needed + book_scan(need, s_scan, total);
-    if (s < b.S) s_need[s + 1] = (uint32_t)min(incl, (uint64_t)UINT32_MAX);
-    needed += total;
+    book_scan(x, total, s_scan2);
+    if (s < b.S) {
+      s_need[s + 1] = (uint32_t)min(needed + x[0], (uint64_t)UINT32_MAX);
+      s_start[s + 1] = (uint32_t)min(tokens + x[1], (uint64_t)UINT32_MAX);
+    }
+    needed += total[0];
+    tokens += total[1];
+  }
+  uint64_t free_pages = 0, free_before = 0;  // before this thread's own
+  if (needed > 0) {  // uniform; a decode step often needs none
+    uint64_t x[1] = {0}, total[1];
+    each_page(b, [&](int, int r) { x[0] += r <= 0; });
+    const uint64_t mine = x[0];
+    book_scan(x, total, s_scan1);
+    free_pages = total[0];
+    free_before = x[0] - mine;
   }
   if (tid == 0) s_need[0] = s_start[0] = 0;
-
-  uint64_t free_pages = 0, free_before = 0;  // before this thread's own
-  if (needed > 0) {  // uniform
-    uint64_t mine = 0;
-    each_page(b, [&](int, int r) { mine += r <= 0; });
-    free_before = book_scan(mine, s_scan, free_pages) - mine;
-  }
   __syncthreads();
-
-  uint64_t tokens = 0;
-  for (int s0 = 0; s0 < b.S; s0 += kBookThreads) {
-    const int s = s0 + tid;
-    uint64_t c = 0;
-    if (s < b.S) {
-      const int len = rows_of(b, s);
-      c = count_of(s, len);
-      if (s_need[s + 1] > s_need[s] && s_need[s + 1] > free_pages) {
-        c = 0;
-        flag_error(err, CKV_DEVICE_ERR_PAGES);
+  if (needed > free_pages || tokens > (uint64_t)n) {  // uniform: not all of them fit
+    tokens = 0;
+    for (int s0 = 0; s0 < b.S; s0 += kBookThreads) {
+      const int s = s0 + tid;
+      uint64_t x[1] = {0}, total[1];
+      if (s < b.S) {
+        x[0] = count_of(s, rows_of(b, s));
+        if (s_need[s + 1] > s_need[s] && s_need[s + 1] > free_pages) {
+          x[0] = 0;
+          flag_error(err, CKV_DEVICE_ERR_PAGES);
+        }
       }
+      const bool any = x[0] > 0;
+      book_scan(x, total, s_scan1);
+      if (s < b.S) {
+        if (any && tokens + x[0] > (uint64_t)n) flag_error(err, CKV_DEVICE_ERR_RANGE);
+        s_start[s + 1] = (uint32_t)min(tokens + x[0], (uint64_t)n + 1);
+      }
+      tokens += total[0];
     }
-    uint64_t total;
-    const uint64_t incl = tokens + book_scan(c, s_scan, total);
-    if (s < b.S) {
-      if (c > 0 && incl > (uint64_t)n) flag_error(err, CKV_DEVICE_ERR_RANGE);
-      s_start[s + 1] = (uint32_t)min(incl, (uint64_t)n + 1);
+    __syncthreads();
+    // Ends past n are n + 1, so of the sequences that reach there the first still has tokens before them: none of it stays.
+    if (tokens > (uint64_t)n) {
+      const int fit = interval_of(s_start, b.S, (uint32_t)n);  // uniform; s_start[fit] <= n < s_start[fit + 1]
+      const uint32_t end = s_start[fit];
+      __syncthreads();
+      for (int s = fit + 1 + tid; s <= b.S; s += kBookThreads) s_start[s] = end;
+      __syncthreads();
     }
-    tokens += total;
-  }
-  __syncthreads();
-  // Ends past n are n + 1, so of the sequences that reach there the first still has tokens before them: none of it stays.
-  int fit = b.S;  // sequences up to here end within n
-  if (tokens > (uint64_t)n) {
-    fit = interval_of(s_start, b.S, (uint32_t)n);  // uniform; s_start[fit] <= n < s_start[fit + 1]
-    const uint32_t end = s_start[fit];
-    __syncthreads();
-    for (int s = fit + 1 + tid; s <= b.S; s += kBookThreads) s_start[s] = end;
-    __syncthreads();
   }
   const int total = (int)s_start[b.S];
 
@@ -202,22 +223,25 @@ struct Pool {
 };
 constexpr int kCopyThreads = 256;
 
-// Part `part` of 2 * layers * heads (K's, then V's) of page src to page dst.
+// Part `part` of 2 * layers * heads (K's, then V's) of page src to page dst. ONCE: no other block reads it (non-temporal loads: 1.2 GB of
+// pages moved in 235 us, with ordinary ones 242); a page that 16 sequences get a copy of comes out of the L2 (118 MB 27 us, 34 without).
+template <bool ONCE>
 __device__ __forceinline__ void copy_page(const Pool& pool, int part, int src, int dst) {
   const int lh = pool.layers * pool.heads, at = part % lh;
   char* base = (part < lh ? pool.k : pool.v) + (int64_t)(at / pool.heads) * pool.layer_b + (int64_t)(at % pool.heads) * pool.head_b;
   const char* from = base + (int64_t)src * pool.page_b + threadIdx.x * 16;
   char* to = base + (int64_t)dst * pool.page_b + threadIdx.x * 16;
   constexpr int STEP = kCopyThreads * 16, U = 4;
+  auto load = [](const char* p) { return ONCE ? ld16_stream(p) : ld16(p); };
   int off = 0;
   for (; off + U * STEP <= pool.page_b; off += U * STEP) {
     vec16 v[U];
 #pragma unroll
-    for (int u = 0; u < U; ++u) v[u] = ld16_stream(from + off + u * STEP);
+    for (int u = 0; u < U; ++u) v[u] = load(from + off + u * STEP);
 #pragma unroll
     for (int u = 0; u < U; ++u) st16_stream(to + off + u * STEP, v[u]);
   }
-  for (; off < pool.page_b; off += STEP) st16_stream(to + off, ld16_stream(from + off));
+  for (; off < pool.page_b; off += STEP) st16_stream(to + off, load(from + off));
 }
 
 // ---- continuing sequences --------------------------------------------------------------------------------------
@@ -233,7 +257,7 @@ __global__ __launch_bounds__(kBookThreads) void fork_book_kernel(Fork* __restric
                                                                  int32_t* __restrict__ err) {
   __shared__ int s_first[kMostSequences];        // the first pair that names this target
   __shared__ uint32_t s_need[kMostSequences + 1];  // partial pages of the pairs before
-  __shared__ uint64_t s_scan[kBookWaves];
+  __shared__ ScanRoom<2> s_scan;
   const int T = 1 << b.T_log, tid = threadIdx.x;
   for (int s = tid; s < b.S; s += kBookThreads) s_first[s] = n;
   __syncthreads();
@@ -245,24 +269,23 @@ __global__ __launch_bounds__(kBookThreads) void fork_book_kernel(Fork* __restric
     const uint32_t s = (uint32_t)sources[i], t = (uint32_t)targets[i];
     return s < (uint32_t)b.S && t < (uint32_t)b.S && s != t && s_first[t] == i && b.lengths[t] == 0;
   };
-  uint64_t needed = 0;
+  uint64_t mine = 0;
+  each_page(b, [&](int, int r) { mine += r <= 0; });
+  uint64_t needed = 0, free_pages = 0, free_before = 0;  // before this thread's own
   for (int i0 = 0; i0 < n; i0 += kBookThreads) {
     const int i = i0 + tid;
-    uint64_t need = 0;
+    uint64_t x[2] = {0, i0 == 0 ? mine : 0}, total[2];
     if (i < n) {
-      if (taken(i)) need = rows_of(b, sources[i]) % T > 0;
+      if (taken(i)) x[0] = rows_of(b, sources[i]) % T > 0;
       else flag_error(err, CKV_DEVICE_ERR_RANGE);
     }
-    uint64_t total;
-    const uint64_t incl = needed + book_scan(need, s_scan, total);
-    if (i < n) s_need[i + 1] = (uint32_t)incl;
-    needed += total;
-  }
-  uint64_t free_pages = 0, free_before = 0;
-  if (needed > 0) {
-    uint64_t mine = 0;
-    each_page(b, [&](int, int r) { mine += r <= 0; });
-    free_before = book_scan(mine, s_scan, free_pages) - mine;
+    book_scan(x, total, s_scan);
+    if (i < n) s_need[i + 1] = (uint32_t)(needed + x[0]);
+    if (i0 == 0) {
+      free_pages = total[1];
+      free_before = x[1] - mine;
+    }
+    needed += total[0];
   }
   __syncthreads();
   for (int i = tid; i < n; i += kBookThreads) {
@@ -308,7 +331,7 @@ __global__ __launch_bounds__(kCopyThreads) void fork_copy_kernel(const Fork* __r
   const Fork f = forks[blockIdx.y];
   if (f.source < 0) return;
   if ((int)blockIdx.x < 2 * pool.layers * pool.heads) {
-    if (f.last >= 0) copy_page(pool, blockIdx.x, f.last, f.copy);
+    if (f.last >= 0) copy_page<false>(pool, blockIdx.x, f.last, f.copy);
     return;
   }
   const int32_t* from = b.table + (int64_t)f.source * b.M;
@@ -385,11 +408,13 @@ struct Moves {
 
 // Of U used pages the i-th at U or above moves to the i-th free one below U: targets and sources are apart, so the copies need no order.
 __global__ __launch_bounds__(kBookThreads) void compact_book_kernel(Moves m, int32_t* __restrict__ used_out, Book b) {
-  __shared__ uint64_t s_scan[kBookWaves];
+  __shared__ ScanRoom<1> s_scan;
   __shared__ int s_below;  // used pages below U
-  uint64_t mine = 0, total;
+  int mine = 0;
   each_page(b, [&](int, int r) { mine += r > 0; });
-  const int first = (int)(book_scan(mine, s_scan, total) - mine), U = (int)total;
+  uint64_t x[1] = {(uint64_t)mine}, total[1];
+  book_scan(x, total, s_scan);
+  const int first = (int)x[0] - mine, U = (int)total[0];
   if (threadIdx.x == 0) s_below = U;  // where all of them are, U = P among it
   __syncthreads();
   int used = first;
@@ -427,7 +452,7 @@ __global__ __launch_bounds__(kBookThreads) void compact_book_kernel(Moves m, int
 __global__ __launch_bounds__(kCopyThreads) void compact_copy_kernel(Moves m, Pool pool, Book b, int32_t* __restrict__ err) {
   if ((int)blockIdx.x < 2 * pool.layers * pool.heads) {
     const int count = m.count();
-    for (int i = blockIdx.y; i < count; i += gridDim.y) copy_page(pool, blockIdx.x, m.source(i), m.target(i));
+    for (int i = blockIdx.y; i < count; i += gridDim.y) copy_page<true>(pool, blockIdx.x, m.source(i), m.target(i));
     return;
   }
   for (int s = blockIdx.y; s < b.S; s += gridDim.y) {
@@ -567,7 +592,7 @@ extern "C" int32_t ckv_compact_pages(void* k_pool, void* v_pool, int64_t layer_s
   hipLaunchKernelGGL(compact_book_kernel, dim3(1), dim3(kBookThreads), 0, (hipStream_t)stream, m, used, b);
   CKV_RETURN_IF_LAUNCH_FAILED();
   const unsigned parts = 2u * n_layers * n_heads;
-  const unsigned per_part = std::max(1u, std::min((unsigned)(n_pages / 2 + 1), 4096 / parts + 1));
+  const unsigned per_part = std::max(1u, std::min((unsigned)(n_pages / 2 + 1), 32768 / parts + 1));
   hipLaunchKernelGGL(compact_copy_kernel, dim3(parts + 1, per_part), dim3(kCopyThreads), 0, (hipStream_t)stream, m, pool, b, err);
   CKV_RETURN_IF_LAUNCH_FAILED();
   return CKV_OK;
