@@ -20,16 +20,16 @@ constexpr int kPagedUnit = kPagedWaves * kWaveChunk;     // cache rows that a sp
 // Units of all tiles up to which a split is one unit: as many partial rows as a join reads at once.
 constexpr float kPagedShort = 32.f;
 
-// Units of a split, from a launch's work (tiles x units, summed in fp32) and 1 / target. The sum is off by less than 2^-17 of itself (64
-// additions in a lane, 6 across, roundings of 2^-24), so this, rounded up from more than that above it, is no less than work / target, and
-// splits add no more than target items.
+// Units of a split or share, from a launch's work (tiles x units, summed in fp32) and 1 / target. The sum is off by less than 2^-17 of itself
+// (64 additions in a lane, 6 across, roundings of 2^-24), so this, rounded up from more than that above it, is no less than work / target: splits
+// add no more than target items, and target shares are all of the work.
 CKV_HOST_DEVICE static inline int paged_split_units(float work, float inv_target, int min_units) {
   const int each = (int)fminf(work * inv_target * (1.f + 0x1p-16f), 0x1p29f) + 1;
   const int least = work <= kPagedShort ? 1 : min_units;
   return each > least ? each : least;
 }
-// ceil(units / split_units), at least 1; inv = 1.f / split_units. The product is at most one off: of a tile there are no more than
-// about target splits.
+// ceil(units / split_units), at least 1; inv = 1.f / split_units, within 2^-22. The product is at most one off: of a tile there are no more
+// than about target splits.
 CKV_HOST_DEVICE static inline int paged_splits(int units, int split_units, float inv) {
   const int s = (int)((float)units * inv), some = s > 1 ? s : 1;
   return (int64_t)some * split_units < units ? some + 1 : some;
@@ -37,10 +37,10 @@ CKV_HOST_DEVICE static inline int paged_splits(int units, int split_units, float
 
 struct PagedPlan {
   int rows = 0;    // (token, query head) rows of a tile: 16 or 32 (attn_paged_kernel), 128 (attn_active_kernel)
-  int target = 0;  // items of a KV head that splits aim at, beside the tiles; 0: the cache is not split
+  int target = 0;  // shares of the units of a KV head, or items that splits aim at, beside the tiles; 0: tiles are whole
   int min_units = 0;
   bool spread_join = false;  // a row's partials are spread over four wavefronts
-  int64_t items = 0;  // of a KV head, at most
+  int64_t items = 0;  // of a KV head, at most; or shares
   int64_t ws_bytes = 0;
   AttnMap map;
 };
@@ -50,18 +50,31 @@ struct PagedPlan {
 static inline PagedPlan paged_plan(int64_t n, int64_t S, int64_t most, int64_t rows, int Hq, int Hkv, int head_dim, int64_t workspace_bytes) {
   PagedPlan p;
   const int64_t group = Hq / Hkv, one = std::min(most, n) * group;
+  auto tiles_of = [&](int64_t r) { return n * group / r + std::min(S, n); };
+  auto units_of = [&](int64_t unit) { return (rows + unit - 1) / unit; };
   p.rows = one <= 16 ? 16 : one <= 32 ? 32 : kAttnBM;
-  const int64_t tiles = n * group / p.rows + std::min(S, n);
+  if (p.rows < kAttnBM && tiles_of(p.rows) * units_of(kPagedUnit) > INT32_MAX / 2) p.rows = kAttnBM;  // units are counted in 32 bits
   const bool large = p.rows == kAttnBM;
-  const int unit = large ? kAttnBN : kPagedUnit;
-  const int64_t fill = (large ? 512 : 384) / Hkv;
+  const int64_t tiles = tiles_of(p.rows), row_b = (int64_t)Hkv * p.rows * (head_dim + 4) * 4;
   p.min_units = large ? 4 : 2;
-  p.target = rows <= (int64_t)p.min_units * unit || (large && n * group / p.rows >= fill) ? 0 : (int)std::max<int64_t>(fill, 1);
-  const int64_t row_b = (int64_t)Hkv * p.rows * (head_dim + 4) * 4;
-  if (p.target > 0 && (tiles + p.target) * row_b > workspace_bytes) p.target = 0;
+  if (rows > p.min_units * (large ? kAttnBN : kPagedUnit)) {
+    if (!large) {
+      // A share for each workgroup that is resident: one of head size 128 on a CU, two of 64.
+      p.target = std::max(1, (head_dim == 128 ? 256 : 512) / Hkv);
+      p.items = p.target;
+      p.ws_bytes = 2 * p.target * row_b;  // of a share, its first and its last tile may be partial
+    } else if (n * group / p.rows < 512 / Hkv) {
+      p.target = std::max(1, 512 / Hkv);
+      p.items = tiles + p.target;
+      p.ws_bytes = p.items * row_b;
+    }
+  }
+  if (p.target == 0 || p.ws_bytes > workspace_bytes) {
+    p.target = 0;
+    p.items = tiles;
+    p.ws_bytes = 0;
+  }
   p.spread_join = p.target >= 8 * tiles || n * Hq <= 2048;
-  p.items = tiles + p.target;
-  p.ws_bytes = p.target > 0 ? p.items * row_b : 0;
   if (p.items * Hkv < (1 << 30)) p.map = attn_map(p.items, Hkv, 1, 1);
   return p;
 }

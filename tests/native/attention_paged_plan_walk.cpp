@@ -1,5 +1,6 @@
 // Walks the launch plans of attention over a paged cache (attention_paged_plan.hpp) and shares out the work of random batches as the
 // kernels do: the items fit the launch, and a sequence's splits cover its rows.
+#include <algorithm>
 #include <cstdio>
 #include <random>
 #include <vector>
@@ -34,24 +35,36 @@ int main() {
         ++checked;
         split += p.target > 0;
         bool ok = (p.rows == 16 || p.rows == 32 || large) && p.map.blocks > 0 && (p.target == 0) == (p.ws_bytes == 0);
-        ok = ok && p.ws_bytes == (p.target > 0 ? p.items * h[1] * p.rows * (h[2] + 4) * 4 : 0);
+        ok = ok && p.ws_bytes == (p.target > 0 ? (large ? p.items : 2 * p.items) * h[1] * p.rows * (h[2] + 4) * 4 : 0);
         const int64_t group = h[0] / h[1], unit = large ? kAttnBN : kPagedUnit;
         float work = 0.f;
+        int64_t all_tiles = 0, all_units = 0;
         std::vector<int64_t> tiles(S), units(S);
         for (int64_t s = 0; s < S; ++s) {
           tiles[s] = (count[s] * group + p.rows - 1) / p.rows;
-          units[s] = (rows[s] + unit - 1) / unit;
+          units[s] = std::max<int64_t>(1, (rows[s] + unit - 1) / unit);
           work += (float)tiles[s] * (float)units[s];
+          all_tiles += tiles[s];
+          all_units += tiles[s] * units[s];
         }
-        const int su = p.target > 0 ? paged_split_units(work, 1.f / (float)p.target, p.min_units) : 1 << 30;
-        const float inv = 1.f / (float)su;
         int64_t items = 0;
-        for (int64_t s = 0; s < S; ++s) {
-          const int z = paged_splits((int)units[s], su, inv);
-          ok = ok && z >= 1 && (tiles[s] == 0 || ((int64_t)z * su >= units[s] && (p.target > 0 || z == 1)));
-          items += tiles[s] * z;
+        if (large) {
+          const int su = p.target > 0 ? paged_split_units(work, 1.f / (float)p.target, p.min_units) : 1 << 30;
+          const float inv = 1.f / (float)su;
+          for (int64_t s = 0; s < S; ++s) {
+            const int z = paged_splits((int)units[s], su, inv);
+            ok = ok && z >= 1 && (tiles[s] == 0 || ((int64_t)z * su >= units[s] && (p.target > 0 || z == 1)));
+            items += tiles[s] * z;
+          }
+          ok = ok && items <= p.items;
+        } else if (p.target > 0) {  // equal shares: they are all of the units, which are counted in 32 bits
+          const int64_t share = paged_split_units((float)(uint32_t)all_units, 1.f / (float)p.target, p.min_units);
+          ok = ok && p.items == p.target && share * p.items >= all_units && all_units <= INT32_MAX / 2 && share * (p.items + 1) < (1ll << 32);
+          items = (all_units + share - 1) / share;
+        } else {
+          items = all_tiles;
+          ok = ok && items <= p.items;
         }
-        ok = ok && items <= p.items;
         // less workspace than asked for: no splits, and never more than there is
         const PagedPlan q = paged_plan(n, S, hint, M * T, h[0], h[1], h[2], p.ws_bytes - 1);
         ok = ok && (p.target == 0 || (q.target == 0 && q.ws_bytes == 0));
