@@ -52,15 +52,25 @@ static inline PagedPlan paged_plan(int64_t n, int64_t S, int64_t most, int64_t r
   const int64_t group = Hq / Hkv, one = std::min(most, n) * group;
   auto tiles_of = [&](int64_t r) { return n * group / r + std::min(S, n); };
   auto units_of = [&](int64_t unit) { return (rows + unit - 1) / unit; };
-  p.rows = one <= 16 ? 16 : one <= 32 ? 32 : kAttnBM;
+  const int64_t places = std::max(1, (head_dim == 128 ? 256 : 512) / Hkv);  // workgroups of attn_paged_kernel that are resident, a KV head
+  // Units that each has to read, of tiles of r rows over sequences as long as they may be.
+  auto share_of = [&](int64_t r) { return (double)tiles_of(r) * (double)units_of(kPagedUnit) / (double)places; };
+  // Few rows of a sequence are read by attn_paged_kernel whatever their number, and more of them where its tiles are few: a step of it is short,
+  // though for a row it costs up to three times what the 128-row tiles take, which need splits and a longer start. us, tiles of 16, 32 and 128:
+  // 28 / 4 heads of 128 over 8302 rows, 9 tokens (4 units) 15.2, 15.8 and 17.2, 18 (9 and 4) 18.2, 18.7, 20.3, 36 (17 and 8) 26.2, 23.6,
+  // 23.0; 8 sequences of 500 rows, 40 tokens each (9 and 5), 17.4, 15.2, 17.2; 16 of up to 4000 rows, 9 each (36 and 24), 23.4, 20.9, 20.6; 14 / 2 heads of 64,
+  // 16 of 500, 18 each (2 and 1) 9.3, 10.2, 12.2, 16 of up to 4000, 9 each (10 and 6) 12.5, 11.9, 12.5; 8 / 8 of 64 over 8302, 64 (5) 13.1, 13.2, 15.4.
+  const bool d128 = head_dim == 128;
+  if (one <= 16 || (one > 32 && share_of(16) <= (d128 ? 8 : 5))) p.rows = 16;
+  else if (one <= 32 || share_of(32) <= (d128 ? 5 : 6)) p.rows = 32;
+  else p.rows = kAttnBM;
   if (p.rows < kAttnBM && tiles_of(p.rows) * units_of(kPagedUnit) > INT32_MAX / 2) p.rows = kAttnBM;  // units are counted in 32 bits
   const bool large = p.rows == kAttnBM;
   const int64_t tiles = tiles_of(p.rows), row_b = (int64_t)Hkv * p.rows * (head_dim + 4) * 4;
   p.min_units = large ? 4 : 2;
   if (rows > p.min_units * (large ? kAttnBN : kPagedUnit)) {
     if (!large) {
-      // A share for each workgroup that is resident: one of head size 128 on a CU, two of 64.
-      p.target = std::max(1, (head_dim == 128 ? 256 : 512) / Hkv);
+      p.target = (int)places;
       p.items = p.target;
       p.ws_bytes = 2 * p.target * row_b;  // of a share, its first and its last tile may be partial
     } else if (n * group / p.rows < 512 / Hkv) {

@@ -169,3 +169,20 @@ def adjusted(logits, prompt=None, generated=None, repetition=1.0, frequency=0.0,
             at = torch.arange(n)
             x[i, ((w[at // 32] >> (at % 32)) & 1) == 0] = -math.inf
     return x
+
+
+# Launches of attention over a paged cache that reach every kernel form: (heads, sequences (rows, new tokens), most, split).
+_7B, _05B = (28, 4, 128), (14, 2, 64)
+FORMS = [(h, seqs, most, split) for h, cases in (
+    (_7B, [
+        ([(100, 1)], 1, True), ([(100, 4)], 4, True), ([(64, 1)] * 70, 1, True), ([(64, 3)] * 70, 3, True),
+        ([(3000, 1)], 1, True), ([(3000, 4)], 4, True), ([(3000, 2), (5, 1)] + [(300, 2)] * 58, 2, True), ([(2500, 4)] + [(300, 4)] * 29, 4, True),
+        ([(3000, 1)] + [(40, 1)] * 69, 1, True), ([(3000, 1)] + [(40, 1)] * 79, 1, True), ([(3000, 4)] + [(40, 1)] * 65, 4, True), ([(3000, 4)] + [(40, 4)] * 69, 4, True),
+        ([(9000, 40)], 40, True), ([(6000, 300)], 300, True), ([(1500, 1200), (33, 20)], 1200, False),
+    ]),
+    (_05B, [
+        ([(100, 1)], 1, True), ([(100, 4)], 4, True), ([(64, 1)] * 70, 1, True), ([(64, 3)] * 70, 3, True),
+        ([(3000, 1)], 1, True), ([(3000, 4)], 4, True), ([(2000, 20)] + [(100, 20)] * 9, 1, True), ([(2500, 4)] + [(100, 4)] * 49, 4, True),
+        ([(3000, 1)] + [(40, 1)] * 69, 1, True), ([(3000, 2)] + [(40, 2)] * 79, 2, True), ([(3000, 4)] + [(40, 1)] * 65, 4, True), ([(3000, 4)] + [(40, 4)] * 69, 4, True),
+        ([(20000, 60)], 60, True), ([(6000, 600)], 600, True), ([(1500, 1200), (33, 20)], 1200, False),
+    ])) for seqs, most, split in cases]

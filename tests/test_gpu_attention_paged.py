@@ -80,6 +80,13 @@ def test_matches_the_64_bit_form(heads, T, seqs):
     assert int(err.item()) == 0
 
 
+@pytest.mark.parametrize("form", range(len(R.FORMS)))
+def test_every_kernel_form(form):
+    heads, seqs, most, split = R.FORMS[form]
+    q, cache, starts = _batch(heads, 64, seqs, seed=form)
+    _check(ops.attention_paged(q, cache, 0, starts, most=most, split=split), _want(q, cache, seqs))
+
+
 @pytest.mark.parametrize("heads", [(28, 4, 128), (14, 2, 64)])
 @pytest.mark.parametrize("seqs", [[(9000, 1)], [(9000, 3), (100, 1)], [(6000, 20)], [(5000, 1)] * 3 + [(17, 1)] * 40, [(20000, 4)]])
 def test_long_caches(heads, seqs):

@@ -11,7 +11,7 @@ import pytest
 import torch
 
 from chunkkv_amd import _native, ops
-from tests.paged_ref import Book, adjusted, attention
+from tests.paged_ref import FORMS, Book, adjusted, attention
 
 ROOT = Path(__file__).resolve().parents[1]
 INVALID, RANGE, LARGE, OK = (_native.CKV_ERR_INVALID_ARGUMENT, _native.CKV_ERR_OUT_OF_RANGE, _native.CKV_ERR_TOO_LARGE, _native.CKV_OK)
@@ -95,6 +95,23 @@ def test_every_paged_plan_can_be_launched(tmp_path):
     out = subprocess.run([str(exe)], check=True, capture_output=True, text=True, timeout=300).stdout
     checked, split, bad = map(int, out.splitlines()[-1].split())
     assert checked > 40_000 and split > 10_000 and bad == 0, out
+
+
+def test_every_kernel_form_is_tested(tmp_path):
+    """The launches that tests/test_gpu_attention_paged.py compares reach every form that a plan can name."""
+    gxx = shutil.which("g++")
+    if gxx is None:
+        pytest.skip("g++ not available")
+    exe = tmp_path / "attention_paged_forms"
+    subprocess.run([gxx, "-O2", "-std=c++17", f"-I{ROOT / 'chunkkv_amd' / 'csrc'}", str(ROOT / "tests" / "native" / "attention_paged_forms.cpp"), "-o", str(exe)], check=True)
+    lines = []
+    for (hq, hkv, d), seqs, most, split in FORMS:
+        entries = max(-(-r // 64) for r, _ in seqs) + 1  # as the GPU test's batches have them
+        lines.append(f"{sum(c for _, c in seqs)} {len(seqs)} {most} {entries * 64} {hq} {hkv} {d} {int(split)}")
+    out = subprocess.run([str(exe)], check=True, capture_output=True, text=True, input="\n".join(lines), timeout=60).stdout
+    got = {tuple(map(int, line.split())) for line in out.splitlines()}
+    want = {(d, r, split, spread, many) for d in (64, 128) for r in (16, 32, 128) for split, spread in ((0, 0), (1, 0), (1, 1)) for many in ((0, 1) if r < 128 else (0,))}
+    assert got == want, (want - got, got - want)
 
 
 def test_host_tensors_and_page_sizes_are_refused():
