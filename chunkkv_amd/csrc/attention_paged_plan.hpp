@@ -68,7 +68,10 @@ static inline PagedPlan paged_plan(int64_t n, int64_t S, int64_t most, int64_t r
   const bool large = p.rows == kAttnBM;
   const int64_t tiles = tiles_of(p.rows), row_b = (int64_t)Hkv * p.rows * (head_dim + 4) * 4;
   p.min_units = large ? 4 : 2;
-  if (rows > p.min_units * (large ? kAttnBN : kPagedUnit)) {
+  // Tiles over few rows are whole, without the second launch of a join. us, split and whole: tiles of few rows, one token a sequence, 28 / 4 heads
+  // of 128 over 512 rows 9.3 and 8.5, 768 rows 9.4 and 9.8, 64 sequences of 512 14.0 and 9.4; 14 / 2 of 64 over 1024 8.5 and 7.9, 2048 8.6 and
+  // 11.2, 32 sequences of 1024 9.0 and 7.9; tiles of 128, 28 / 4 of 128, 4 sequences of 500 rows and tokens 19.8 and 17.7, of 1000 26.5 and 28.0.
+  if (rows > (large || d128 ? 512 : 1024)) {
     if (!large) {
       p.target = (int)places;
       p.items = p.target;
