@@ -793,7 +793,7 @@ def extend_pages(cache: PagedCache, counts: torch.Tensor, n: int, err: torch.Ten
     token, in the order of the sequences, gets its position and its row of the pool, which rope_qkv(positions, rows=rows) then writes
     in every layer. n: the tokens, counts' sum, or room for more (behind the last one positions are 0 and rows -1, which writers skip
     and flag). What does not fit its table, n or the free pages grows by nothing, nor does what comes behind it and needs such room,
-    and err is set (_native.DEVICE_ERR_RANGE, DEVICE_ERR_PAGES)."""
+    and err is set (_native.DEVICE_ERR_RANGE, DEVICE_ERR_PAGES); starts then counts the tokens of those that grew alone."""
     return PagedRows(*_native.torch_ops().extend_pages(cache.table, cache.lengths, cache.refs, cache.page_tokens, counts, n, err))
 
 

@@ -103,13 +103,15 @@ class PagedSession:
         self._check_err()
         self.tokens[s] = tokens
         if result.logits.shape[0]:
-            self._logits[s] = result.logits[-1:]
+            self._logits[s] = result.logits[-1:].clone()  # not the prefill's other rows
         return s
 
     @torch.inference_mode()
     def fork(self, sequence: int, n: int = 1) -> list[int]:
         """n new sequences that continue this one; its whole pages are shared."""
         (source,) = self._known([sequence])
+        if n < 0:
+            raise ValueError("a number of new sequences is 0 or more")
         targets = self._slots(n)
         if len(self.tokens[source]) % self.cache.page_tokens and n > self.free_pages:
             raise ValueError(f"{n} more pages are needed, {self.free_pages} are free")

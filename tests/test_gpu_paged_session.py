@@ -197,6 +197,30 @@ def test_what_does_not_fit_is_refused_before_anything_is_done():
     assert s.generate([], 5) == [] and s.generate([0], 0) == [[]] and s.feed({}) == {}
 
 
+def test_a_number_of_forks_below_zero_is_refused():
+    eng = _engine()
+    s, _, _ = _session(eng, (40,))
+    with pytest.raises(ValueError, match="0 or more"):
+        s.fork(0, -1)
+    assert s.fork(0, 0) == [] and list(s.tokens) == [0] and s.free_pages == 58
+
+
+def test_a_prefill_of_many_logits_is_not_kept():
+    eng = _engine()
+    s = eng.paged(n_pages=8, n_sequences=2, max_tokens=64, page_tokens=32)
+    p = _tokens(40)
+    result = eng.prefill(p, logits_from=0)
+    s.add(result, p)
+    assert s._logits[0].untyped_storage().nbytes() == VOCAB * result.logits.element_size() < result.logits.untyped_storage().nbytes()
+
+
+def test_the_library_attention_of_prefills_may_fill_the_cache():
+    eng = _engine(attention="sdpa")
+    s, ids, prompts = _session(eng, (40, 129))
+    for p, tokens in zip(prompts, s.generate(ids, 12)):
+        _greedy_run(eng, p, tokens, 12)
+
+
 def test_models_without_the_kernel_are_refused():
     eng = _engine(attention="reference")
     with pytest.raises(ValueError, match="bf16"):

@@ -219,3 +219,38 @@ def test_going_back_inside_a_shared_page_is_refused():
         book.free(at, left)
         ops.free_pages(c, _ints(at), _ints(left), err)
         book.check(c, err)
+
+
+def test_pages_past_4_gb():
+    """Rows whose offsets in a head pass 32 bits: taken, copied, read by every form of the attention and moved, as in a small pool."""
+    T, H, D, small = 64, 2, 128, 40
+    big = 2 ** 32 // (T * D * 2) + small  # pages; the last `small` lie past 4 GB
+    a, b = ops.paged_cache(1, small, H, D, 4, 1024, DEV, T), ops.paged_cache(1, big, H, D, 4, 1024, DEV, T)
+    far = big - small
+    b.refs[:far] = 1
+    for t, u in ((a.k, b.k), (a.v, b.v)):
+        t.normal_()
+        u[:, :, :, far * T:] = t
+    err = torch.zeros(1, dtype=I32, device=DEV)
+    g = torch.Generator().manual_seed(3)
+    for counts in ([700, 33, 0, 0], [3, 1, 0, 0], [1, 150, 0, 0]):
+        n = sum(counts)
+        news = [ops.extend_pages(c, _ints(counts), n, err) for c in (a, b)]
+        assert torch.equal(news[0].rows + far * T, news[1].rows) and torch.equal(news[0].positions, news[1].positions)
+        q = torch.randn((1, n, 14, D), generator=g).to(torch.bfloat16).to(DEV).transpose(1, 2)
+        for most in (1, 16, n):
+            x, y = (ops.attention_paged(q, c, 0, w.starts, most=most, err=err) for c, w in zip((a, b), news))
+            assert torch.equal(x, y)
+    for c in (a, b):
+        ops.fork_pages(c, _ints([0, 1]), _ints([2, 3]), err)
+        ops.free_pages(c, _ints([0]), err=err)
+    for t, u in ((a.k, b.k), (a.v, b.v)):
+        assert torch.equal(t, u[:, :, :, far * T:])
+    b.refs[:far] = 0  # from there to the front
+    assert int(ops.compact_pages(b, err).item()) == int((a.refs > 0).sum()) and int(err.item()) == 0
+    for s in (1, 2, 3):
+        at = torch.arange(int(a.lengths[s]), device=DEV)
+        rows = [c.table[s].long()[at // T] * T + at % T for c in (a, b)]
+        assert int(rows[1].max()) < small * T
+        for t, u in ((a.k, b.k), (a.v, b.v)):
+            assert torch.equal(t[:, :, :, rows[0]], u[:, :, :, rows[1]])
