@@ -257,18 +257,19 @@ __global__ __launch_bounds__(kPagedWaves * 64) void attn_paged_kernel(AttnMap ma
 
 // ---- the partial rows joined -----------------------------------------------------------------------------------
 // D / 4 lanes have a (token, query head) row's columns, so a wavefront has JH = 64 / (D / 4) heads of a token side by side and nothing
-// crosses its lanes; it goes through their partial rows, JU in flight. Finding the token's items costs as many instructions as a few rows,
+// crosses its lanes; it goes through their partial rows, some in flight. Finding the token's items costs as many instructions as a few rows,
 // and instructions are what a launch of many rows waits for, so such launches (WPR = 1) give a wavefront kJoinTurns times JH heads; those of few rows
 // and more splits (WPR = 4) spread a row's partials over four wavefronts. Partials past the row's position are not read. Rows of
-// tiles that were whole are written already.
-constexpr int kJoinTurns = 2, kJoinInFlight = 8;
+// tiles that were whole are written already. kJoinSpread: 40 partials at once; one round fewer of a sequence of 8302 rows, which has 33 (one token, 28 / 4
+// heads of 128, 11.6 us in place of 12.0 with 32 at once, 14 / 2 of 64 9.2 and 9.7; 48 cost those with fewer partials 0.1, 64 0.3).
+constexpr int kJoinTurns = 2, kJoinInFlight = 8, kJoinSpread = 10;
 template <int D>
 constexpr int kJoinHeads = 256 / D;
 
 template <int D, int ROWS, int UNIT, int WPR, bool MANY>
 __global__ __launch_bounds__(256) void join_paged_kernel(char* __restrict__ out, const float* __restrict__ ws, PagedRows b, int n,
                                                          int Hq, int group) {
-  constexpr int LR = D / 4, JH = kJoinHeads<D>, U = kJoinInFlight, TURNS = WPR == 4 ? 1 : kJoinTurns;
+  constexpr int LR = D / 4, JH = kJoinHeads<D>, U = WPR == 4 ? kJoinSpread : kJoinInFlight, TURNS = WPR == 4 ? 1 : kJoinTurns;
   constexpr bool SHARES = ROWS < kAttnBM;
   static_assert(WPR == 1 || WPR == 4, "a wavefront or a workgroup a row");
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x % 64, sub = lane / LR, col = lane % LR * 4;
