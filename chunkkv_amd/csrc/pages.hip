@@ -8,8 +8,11 @@
 // often the table names page p (free: 0). Pages are taken lowest first, so a book's next state follows from its last.
 //
 // Bookkeeping runs in one workgroup: which page is the r-th free one is a prefix sum over all of them, a few microseconds for
-// tens of thousands of pages, and a second launch would cost as much. Bound: latency, of dependent loads and barriers.
-// Copies of pages run in a launch of their own over (layer, head, K or V) x page; bound: their bytes.
+// tens of thousands of pages, and a second launch would cost as much. Bound: latency, of dependent loads and barriers. Traced: a decode
+// step of 32 sequences over 1704 pages 3.6 us, 63255 tokens of 16 prompts that take about 2000 pages 6.8 (and 4.8 for the launch that writes their
+// rows), 16 forks among 197 pages 6.3, 634 pages moved together 4.6.
+// Copies of pages run in a launch of their own over (layer, head, K or V) x page; bound: their bytes (1.17 GB read and written in 235 us,
+// 5.0 TB/s, what a large torch copy reaches; the 117 MB of 16 forks 17.5).
 #include <algorithm>
 
 #include "ckv_common.hpp"

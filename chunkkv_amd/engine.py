@@ -44,7 +44,8 @@ kernels:
                                                        cut by the attention weights of prefill(observe=...)
                                                        and held in 8 bits (ckv_attention_weights,
                                                        ckv_evict_rows, ckv_quantize_rows,
-                                                       ckv_attention_quantized)
+                                                       ckv_attention_quantized); paged(...): several
+                                                       sequences over one cache in pages (PagedSession)
 All layers' caches live in one (L, 1, H, N, D) slab; PrefillResult.keys/values are its views.
 
 Attention: the reference calls SDPA with enable_gqa and an explicit boolean (n_active x N) mask,
