@@ -130,10 +130,10 @@ SIGNATURES = {
     "ckv_compact_pages_workspace_bytes": (_i64, [_i32]),
     "ckv_attention_paged": (
         _i32,
-        [_p, _p, _i64, _i64, _p, _p, _i64, _p, _p, _p, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _f64, _p,
+        [_p, _p, _i64, _i64, _p, _p, _i64, _p, _p, _p, _i32, _i32, _i32, _i64, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _f64, _p,
          _i64, _p, _p],
     ),
-    "ckv_attention_paged_workspace_bytes": (_i64, [_i32] * 8),
+    "ckv_attention_paged_workspace_bytes": (_i64, [_i32] * 4 + [_i64] + [_i32] * 5),
     "ckv_adjust_logits": (
         _i32,
         [_p, _p, _i64, _i32, _i32, _i32, _p, _i64, _i32, _p, _i64, _i32, _p, _f32, _p, _f32, _p, _f32, _p, _i64, _p, _i64, _p],

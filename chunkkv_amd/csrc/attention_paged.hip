@@ -3,8 +3,8 @@
 //   out = sum_j w_j V[row(j)] / sum_j w_j,  w_j = exp(scale q . K[row(j)]),  row(j) = table[j / T] T + j % T
 // in attention.hip's manner (scores, softmax and sums in fp32, weights rounded to bf16 for the second product).
 //
-//  - Sequences of up to 32 (token, query head) rows of a KV head, decode among them: attn_paged_kernel below.
-//  - More: attention_large.hpp's workgroups of 128 rows, with splits of the cache where they are few. 4096 tokens over 32832 rows, 28 / 4 heads of
+//  - Tiles of 16 or 32 (token, query head) rows of a sequence's KV head, decode among them: attn_paged_kernel below.
+//  - Of 128, where many tokens fill the card: attention_large.hpp's workgroups, with splits of the cache where they are few. 4096 tokens over 32832 rows, 28 / 4 heads of
 //    128, 1.67 ms: 1.08 PFLOP/s, as fast as that kernel over one contiguous cache (1.83 on the card where this took 1.78).
 // attention_paged.hpp says how the work is shared out, attention_paged_plan.hpp by which rule.
 #include <algorithm>
@@ -389,24 +389,26 @@ __global__ __launch_bounds__(256) void join_paged_kernel(char* __restrict__ out,
 
 }  // namespace ckv
 
-extern "C" int64_t ckv_attention_paged_workspace_bytes(int32_t n_tokens, int32_t n_sequences, int32_t most_tokens, int32_t n_entries,
-                                                       int32_t page_tokens, int32_t n_q_heads, int32_t n_kv_heads, int32_t head_dim) {
-  if (n_tokens <= 0 || n_sequences <= 0 || most_tokens <= 0 || n_entries <= 0 || page_tokens <= 0 || n_q_heads <= 0 || n_kv_heads <= 0 ||
+extern "C" int64_t ckv_attention_paged_workspace_bytes(int32_t n_tokens, int32_t n_sequences, int32_t most_tokens, int32_t most_rows, int64_t total_rows,
+                                                       int32_t n_entries, int32_t page_tokens, int32_t n_q_heads, int32_t n_kv_heads, int32_t head_dim) {
+  if (n_tokens <= 0 || n_sequences <= 0 || most_tokens < 0 || most_rows < 0 || total_rows < 0 || n_entries <= 0 || page_tokens <= 0 || n_q_heads <= 0 || n_kv_heads <= 0 ||
       head_dim <= 0 || n_q_heads % n_kv_heads)
     return 0;
-  return ckv::paged_plan(n_tokens, n_sequences, most_tokens, (int64_t)n_entries * page_tokens, n_q_heads, n_kv_heads, head_dim, INT64_MAX).ws_bytes;
+  const int64_t rows = (int64_t)n_entries * page_tokens;
+  return ckv::paged_plan(n_tokens, n_sequences, most_tokens == 0 ? n_tokens : most_tokens, most_rows == 0 ? rows : most_rows, total_rows, rows,
+                         n_q_heads, n_kv_heads, head_dim, INT64_MAX).ws_bytes;
 }
 
 extern "C" int32_t ckv_attention_paged(void* out, const void* q, int64_t q_head_stride, int64_t q_token_stride, const void* k_pool,
                                        const void* v_pool, int64_t kv_head_stride, const int32_t* table, const int32_t* lengths,
-                                       const int32_t* starts, int32_t n_tokens, int32_t most_tokens, int32_t n_sequences,
+                                       const int32_t* starts, int32_t n_tokens, int32_t most_tokens, int32_t most_rows, int64_t total_rows, int32_t n_sequences,
                                        int32_t n_entries, int32_t n_pages, int32_t page_tokens, int32_t n_q_heads,
                                        int32_t n_kv_heads, int32_t head_dim, int32_t dtype, double scale, void* workspace,
                                        int64_t workspace_bytes, int32_t* err, void* stream) {
   using namespace ckv;
   if (dtype != CKV_DTYPE_BF16 || (head_dim != 64 && head_dim != 128)) return CKV_ERR_INVALID_ARGUMENT;
   if (page_tokens != 32 && page_tokens != 64 && page_tokens != 128) return CKV_ERR_INVALID_ARGUMENT;
-  if (n_tokens < 0 || most_tokens < 0 || n_sequences <= 0 || n_entries <= 0 || n_pages <= 0 || n_q_heads <= 0 || n_kv_heads <= 0 ||
+  if (n_tokens < 0 || most_tokens < 0 || most_rows < 0 || total_rows < 0 || n_sequences <= 0 || n_entries <= 0 || n_pages <= 0 || n_q_heads <= 0 || n_kv_heads <= 0 ||
       n_q_heads % n_kv_heads != 0 || log2_scale(scale) == 0.f)
     return CKV_ERR_INVALID_ARGUMENT;
   if (n_tokens == 0) return CKV_OK;
@@ -420,7 +422,8 @@ extern "C" int32_t ckv_attention_paged(void* out, const void* q, int64_t q_head_
       n_tokens * group > (1 << 30))
     return CKV_ERR_TOO_LARGE;
   if (workspace == nullptr || (uintptr_t)workspace % 16) workspace_bytes = 0;
-  const PagedPlan plan = paged_plan(n_tokens, n_sequences, most_tokens == 0 ? n_tokens : most_tokens, (int64_t)n_entries * page_tokens,
+  const int64_t rows = (int64_t)n_entries * page_tokens;
+  const PagedPlan plan = paged_plan(n_tokens, n_sequences, most_tokens == 0 ? n_tokens : most_tokens, most_rows == 0 ? rows : most_rows, total_rows, rows,
                                     n_q_heads, n_kv_heads, head_dim, workspace_bytes);
   if (plan.map.blocks == 0) return CKV_ERR_TOO_LARGE;
   float* ws = plan.target > 0 ? (float*)workspace : nullptr;

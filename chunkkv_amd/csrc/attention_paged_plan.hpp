@@ -45,49 +45,68 @@ struct PagedPlan {
   AttnMap map;
 };
 
-// n new tokens of S sequences, at most `most` of one, over at most `rows` cached rows each. Lengths are the device's: the items
-// are bounded by tiles (a sequence's last one may be partial) and by what splits add.
-static inline PagedPlan paged_plan(int64_t n, int64_t S, int64_t most, int64_t rows, int Hq, int Hkv, int head_dim, int64_t workspace_bytes) {
+// A kernel form's time in a graph replay, us at one load: `start` and a `step` for each 128 rows that its workgroups read one after the other, of head
+// sizes 64 and 128; `places`: workgroups that the card holds of it. From 285 shapes (28 / 4 heads of 128, 14 / 2 and 8 / 8 of 64; 1 to 100 sequences of 200 to 8302 rows, equal,
+// ragged and one long among short ones, 1 to 500 new tokens each), every form timed: the one with the least estimate takes 1.6 % more than the fastest on average, at
+// most 31 %, and 1.7 and 66 % where the rows of all are not told (tiles by a launch's load alone and splits from 512 or 1024 rows on took 4.1 % more, at most 79 %).
+struct PagedForm {
+  int rows;
+  double start, step[2];
+  int places[2];
+};
+constexpr PagedForm kPagedForms[] = {{16, 5.5, {0.55, 0.75}, {512, 256}}, {32, 5.7, {0.6, 1.1}, {512, 256}}, {kAttnBM, 5.0, {1.5, 2.4}, {768, 512}}};
+constexpr double kPagedJoin = 5.0, kPagedJoinByte = 1.5e-6;  // us that splitting adds, and for each byte of the result in fp32
+constexpr double kPagedMean = 0.6;  // of the longest sequence's rows, where the sum is not known
+
+// n new tokens of S sequences; `most` of one, `longest` cached rows of one and `total` of all that have tokens (0: not known) are estimates, `rows` is the most that
+// a sequence can have. Lengths are the device's: the items are bounded by tiles (a sequence's last one may be partial) and by what splits add. Of a sequence whose (token, query head) rows fit 16 or 32
+// larger tiles read the cache as often for nothing. us, whole and split, and other tiles:
+//   28 / 4 heads of 128, one token over 512 rows 8.5 and 9.3, 768 9.8 and 9.4, 31 sequences of 683 12.6 and 15.9, 69 of up to 576, 1 to 3 tokens, 13.7 and 24.4
+//   4 sequences of 500 rows and tokens 17.7 (128), 19.8 split; 2 of 832 rows, 57 tokens, 11.1 (16), 18.5 split
+//   14 / 2 of 64, 9 sequences of up to 2000 rows, 1280 tokens, 16.5 (32), 18.1 (16), 21.8 (128, split), 32.9 (128)
+//   8 / 8 of 64, 22 of up to 1976 rows, 1314 tokens, 15.8 (16), 16.6 (32), 19.4 (128, split), 26.8 (16, split)
+static inline PagedPlan paged_plan(int64_t n, int64_t S, int64_t most, int64_t longest, int64_t total, int64_t rows, int Hq, int Hkv, int head_dim, int64_t workspace_bytes) {
   PagedPlan p;
-  const int64_t group = Hq / Hkv, one = std::min(most, n) * group;
-  auto tiles_of = [&](int64_t r) { return n * group / r + std::min(S, n); };
-  auto units_of = [&](int64_t unit) { return (rows + unit - 1) / unit; };
-  const int64_t places = std::max(1, (head_dim == 128 ? 256 : 512) / Hkv);  // workgroups of attn_paged_kernel that are resident, a KV head
-  // Units that each has to read, of tiles of r rows over sequences as long as they may be.
-  auto share_of = [&](int64_t r) { return (double)tiles_of(r) * (double)units_of(kPagedUnit) / (double)places; };
-  // Few rows of a sequence are read by attn_paged_kernel whatever their number, and more of them where its tiles are few: a step of it is short,
-  // though for a row it costs up to three times what the 128-row tiles take, which need splits and a longer start. us, tiles of 16, 32 and 128:
-  // 28 / 4 heads of 128 over 8302 rows, 9 tokens (4 units) 15.2, 15.8 and 17.2, 18 (9 and 4) 18.2, 18.7, 20.3, 36 (17 and 8) 26.2, 23.6,
-  // 23.0; 8 sequences of 500 rows, 40 tokens each (9 and 5), 17.4, 15.2, 17.2; 16 of up to 4000 rows, 9 each (36 and 24), 23.4, 20.9, 20.6; 14 / 2 heads of 64,
-  // 16 of 500, 18 each (2 and 1) 9.3, 10.2, 12.2, 16 of up to 4000, 9 each (10 and 6) 12.5, 11.9, 12.5; 8 / 8 of 64 over 8302, 64 (5) 13.1, 13.2, 15.4.
-  const bool d128 = head_dim == 128;
-  if (one <= 16 || (one > 32 && share_of(16) <= (d128 ? 8 : 5))) p.rows = 16;
-  else if (one <= 32 || share_of(32) <= (d128 ? 5 : 6)) p.rows = 32;
-  else p.rows = kAttnBM;
-  if (p.rows < kAttnBM && tiles_of(p.rows) * units_of(kPagedUnit) > INT32_MAX / 2) p.rows = kAttnBM;  // units are counted in 32 bits
-  const bool large = p.rows == kAttnBM;
-  const int64_t tiles = tiles_of(p.rows), row_b = (int64_t)Hkv * p.rows * (head_dim + 4) * 4;
-  p.min_units = large ? 4 : 2;
-  // Tiles over few rows are whole, without the second launch of a join. us, split and whole: tiles of few rows, one token a sequence, 28 / 4 heads
-  // of 128 over 512 rows 9.3 and 8.5, 768 rows 9.4 and 9.8, 64 sequences of 512 14.0 and 9.4; 14 / 2 of 64 over 1024 8.5 and 7.9, 2048 8.6 and
-  // 11.2, 32 sequences of 1024 9.0 and 7.9; tiles of 128, 28 / 4 of 128, 4 sequences of 500 rows and tokens 19.8 and 17.7, of 1000 26.5 and 28.0.
-  if (rows > (large || d128 ? 512 : 1024)) {
-    if (!large) {
-      p.target = (int)places;
-      p.items = p.target;
-      p.ws_bytes = 2 * p.target * row_b;  // of a share, its first and its last tile may be partial
-    } else if (n * group / p.rows < 512 / Hkv) {
-      p.target = std::max(1, 512 / Hkv);
-      p.items = tiles + p.target;
-      p.ws_bytes = p.items * row_b;
+  const int64_t group = Hq / Hkv, used = std::min(S, n), one = std::min(most, n) * group;
+  const int d128 = head_dim == 128;
+  const double longer = (double)std::min(longest, rows), mean = total > 0 ? std::min((double)total / (double)used, longer) : kPagedMean * longer;
+  double least = INFINITY;
+  for (const PagedForm& f : kPagedForms) {
+    if ((f.rows > 16 && one <= 16) || (f.rows > 32 && one <= 32)) continue;
+    const bool large = f.rows == kAttnBM;
+    const int64_t unit = large ? kAttnBN : kPagedUnit, tiles = n * group / f.rows + used;
+    const double half = (double)unit / 2.0, units = std::ceil(longer / (double)unit) * (double)unit / 128.0;
+    const double likely = (double)std::min(tiles, used * ((one + f.rows - 1) / f.rows));
+    const double load = 1.3 * std::min((mean + half) / 128.0, units) * likely * Hkv / f.places[d128];  // of a workgroup, if three of four are busy
+    const double whole = f.start + f.step[d128] * std::max(units, load);
+    if (whole < least) {
+      least = whole;
+      p = {};
+      p.rows = f.rows;
+      p.items = tiles;
+    }
+    PagedPlan s;
+    s.rows = f.rows;
+    s.min_units = large ? 4 : 2;
+    const int64_t row_b = (int64_t)Hkv * f.rows * (head_dim + 4) * 4;
+    if (large) {
+      s.target = std::max(1, 512 / Hkv);
+      s.items = tiles + s.target;
+      s.ws_bytes = s.items * row_b;
+      if (n * group / f.rows >= s.target) continue;  // enough tiles
+    } else {
+      s.target = std::max(1, f.places[d128] / Hkv);
+      s.items = s.target;
+      s.ws_bytes = 2 * s.items * row_b;  // of a share, its first and its last tile may be partial
+      if (tiles * ((rows + unit - 1) / unit) > INT32_MAX / 2) continue;  // units are counted in 32 bits
+    }
+    const double split = f.start + kPagedJoin + kPagedJoinByte * 4.0 * (double)(n * Hq * head_dim) + f.step[d128] * std::max(2.0, load);
+    if (split < least && s.ws_bytes <= workspace_bytes) {
+      least = split;
+      s.spread_join = s.target >= 8 * tiles || n * Hq <= 2048;
+      p = s;
     }
   }
-  if (p.target == 0 || p.ws_bytes > workspace_bytes) {
-    p.target = 0;
-    p.items = tiles;
-    p.ws_bytes = 0;
-  }
-  p.spread_join = p.target >= 8 * tiles || n * Hq <= 2048;
   if (p.items * Hkv < (1 << 30)) p.map = attn_map(p.items, Hkv, 1, 1);
   return p;
 }

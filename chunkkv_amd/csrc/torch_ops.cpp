@@ -921,17 +921,18 @@ PyObject* compact_pages(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
   CKV_PY_END
 }
 
-// attention_paged(q, table, lengths, refs, page_tokens, k, v, layer, starts, most, scale, err, out, split)
+// attention_paged(q, table, lengths, refs, page_tokens, k, v, layer, starts, most, longest, total, scale, err, out, split)
 PyObject* attention_paged(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
   CKV_PY_BEGIN
-  need_args(n_args, 14);
+  need_args(n_args, 16);
   Tensor q = tensor(a[0]);
   const PageBook b = page_book(a + 1);
   const PagePool p = page_pool(b, a[5], a[6]);
-  const int64_t layer = integer(a[7]), most = a[9] == Py_None ? 0 : integer(a[9]);
-  const Tensor starts = int_vector(a[8], b, "starts"), err = optional_tensor(a[11]);
+  const int64_t layer = integer(a[7]), most = a[9] == Py_None ? 0 : integer(a[9]), longest = a[10] == Py_None ? 0 : integer(a[10]),
+                total = a[11] == Py_None ? 0 : integer(a[11]);
+  const Tensor starts = int_vector(a[8], b, "starts"), err = optional_tensor(a[13]);
   int32_t* const e = status_word(err, q);
-  Tensor out = optional_tensor(a[12]);
+  Tensor out = optional_tensor(a[14]);
   same_device(q, p.k);
   need_dims(q, 4, "q");
   if (q.scalar_type() != at::kBFloat16 || p.k.scalar_type() != at::kBFloat16) type_error("attention_paged runs on bf16 q and cache");
@@ -942,6 +943,8 @@ PyObject* attention_paged(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
   if (layer < 0 || layer >= p.L) value_error("layer " + std::to_string(layer) + " of a cache of " + std::to_string(p.L));
   if (starts.numel() != b.S + 1) value_error("starts must be (sequences + 1,)");
   if (a[9] != Py_None && (most < 1 || most > INT32_MAX)) value_error("most must be 1 to 2^31 - 1");
+  if (a[10] != Py_None && (longest < 1 || longest > INT32_MAX)) value_error("longest must be 1 to 2^31 - 1");
+  if (a[11] != Py_None && total < 1) value_error("total must be 1 or more");
   q = rows_view(q);
   if (!out.defined()) {
     out = new_tensor({1, n, Hq, p.D}, at::kBFloat16, q);
@@ -950,10 +953,10 @@ PyObject* attention_paged(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
     if (out.sizes() != at::IntArrayRef({1, n, Hq, p.D}) || !out.is_contiguous() || out.scalar_type() != at::kBFloat16)
       value_error("out must be contiguous (1, n, Hq, D) bf16");
   }
-  const double scale = a[10] == Py_None ? 1.0 / std::sqrt((double)p.D) : real(a[10]);
-  const int split = PyObject_IsTrue(a[13]);
+  const double scale = a[12] == Py_None ? 1.0 / std::sqrt((double)p.D) : real(a[12]);
+  const int split = PyObject_IsTrue(a[15]);
   if (split < 0) throw python_error();
-  const int64_t ws_bytes = split ? ckv_attention_paged_workspace_bytes(int32(n), int32(b.S), int32(most ? most : n), int32(b.M), int32(b.T),
+  const int64_t ws_bytes = split ? ckv_attention_paged_workspace_bytes(int32(n), int32(b.S), int32(most), int32(longest), total, int32(b.M), int32(b.T),
                                                                        int32(Hq), int32(p.H), int32(p.D))
                                  : 0;
   Tensor ws;
@@ -963,7 +966,7 @@ PyObject* attention_paged(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
           const int64_t at = layer * p.k.stride(0) * 2;
           return ckv_attention_paged(ptr(out), ptr(q), step(q, 1, n * p.D), step(q, 2, p.D), (const char*)ptr(p.k) + at,
                                      (const char*)ptr(p.v) + at, p.k.stride(2), b.at(b.table), b.at(b.lengths), (const int32_t*)ptr(starts),
-                                     int32(n), int32(most), int32(b.S), int32(b.M), int32(b.P), int32(b.T), int32(Hq), int32(p.H), int32(p.D),
+                                     int32(n), int32(most), int32(longest), total, int32(b.S), int32(b.M), int32(b.P), int32(b.T), int32(Hq), int32(p.H), int32(p.D),
                                      CKV_DTYPE_BF16, scale, ptr(ws), ws_bytes, e, stream_of(q));
         }),
         "ckv_attention_paged");

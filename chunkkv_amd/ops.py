@@ -823,6 +823,8 @@ def attention_paged(
     scale: float | None = None,
     *,
     most: int | None = None,
+    longest: int | None = None,
+    total: int | None = None,
     err: torch.Tensor | None = None,
     out: torch.Tensor | None = None,
     split: bool = True,
@@ -832,11 +834,13 @@ def attention_paged(
 
     q: (1, Hq, n, D) bf16 with contiguous rows; the cache bf16, D 64 or 128. Returns (1, n, Hq, D) bf16, token-major; a token that sees no row
     (more new tokens than rows) gives zeros, tokens outside [starts[0], starts[-1]) stay as they were in out (anything in a new tensor).
-    most: the most new tokens of one sequence, if known (1 in a decode step); it chooses the kernel's form, not the result.
+    most, longest, total: the most new tokens of one sequence (1 in a decode step), the most rows of one that has any, and those of all that have any
+    together, if known, or about: they choose the kernel's form, not the result. Without longest the table's width counts, which makes short
+    sequences in a wide table slower.
     split: let launches too small to fill the chip split the cache range (a workspace is allocated for the partial results).
     """
     return _native.torch_ops().attention_paged(q, cache.table, cache.lengths, cache.refs, cache.page_tokens, cache.k, cache.v, layer, starts,
-                                               most, scale, err, out, split)
+                                               most, longest, total, scale, err, out, split)
 
 
 def adjust_logits(

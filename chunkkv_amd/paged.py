@@ -141,10 +141,11 @@ class PagedSession:
 
     # -- the model ------------------------------------------------------------------------
 
-    def _forward(self, tok: torch.Tensor, counts: torch.Tensor, most: int):
-        """New tokens tok (n,), in the order of the sequences, counts[s] of each and most of one at most: their rows are taken and
-        written, layer by layer. (h, pending, starts), for the engine's _final_logits."""
+    def _forward(self, tok: torch.Tensor, counts: torch.Tensor, most: int, rows: list[int]):
+        """New tokens tok (n,), in the order of the sequences, counts[s] of each, most of one at most; rows: of each with them. The new rows
+        are taken and written, layer by layer. (h, pending, starts), for the engine's _final_logits."""
         e, c = self.engine, self.cache
+        known = dict(most=most, longest=max(rows), total=sum(rows))
         H, D, n = e.n_kv, e.head_dim, tok.shape[0]
         new = ops.extend_pages(c, counts, n, self._err)
         h, pending = e.inner.embed_tokens(tok[None]), None
@@ -153,7 +154,7 @@ class PagedSession:
             q_in, k_in, v_in = e._project(li, x)
             q, _ = ops.rope_qkv(q_in, k_in, v_in, new.positions, e.n_heads, H, D, e.theta, k_out=c.k[li], v_out=c.v[li], rows=new.rows,
                                 err=self._err)
-            o = ops.attention_paged(q.transpose(1, 2), c, li, new.starts, most=most, err=self._err)
+            o = ops.attention_paged(q.transpose(1, 2), c, li, new.starts, err=self._err, **known)
             h, pending = e._mlp(li, layer, h, layer.self_attn.o_proj(o.view(1, n, -1)))
         return h, pending, new.starts
 
@@ -168,7 +169,7 @@ class PagedSession:
         more = {s: len(chunk) for s, chunk in chunks.items()}
         self._check_room(more)
         tok = torch.tensor([t for chunk in chunks.values() for t in chunk], dtype=torch.int64).to(self.engine.device)
-        h, pending, starts = self._forward(tok, self._counts(more), max(more.values()))
+        h, pending, starts = self._forward(tok, self._counts(more), max(more.values()), [len(self.tokens[s]) + n for s, n in more.items()])
         last = starts[1:].long()[torch.tensor(list(chunks)).to(starts.device)] - 1
         logits = self.engine._final_logits(h[:, last], None if pending is None else pending[:, last])[0]
         self._check_err()
@@ -223,7 +224,7 @@ class PagedSession:
             ops.next_tokens(logits, prompt=prompt, generated=generated, allowed=masks, err=self._err, out=tok, **fixed)
             generated.scatter_(1, at, tok[:, None])
             at.add_(1)
-            h, pending, _ = self._forward(tok, counts, 1)
+            h, pending, _ = self._forward(tok, counts, 1, [len(self.tokens[s]) + max_tokens for s in slots])
             logits.copy_(self.engine._final_logits(h, pending)[0])
 
         before = [len(self.tokens[s]) for s in slots]

@@ -711,7 +711,9 @@ int64_t ckv_compact_pages_workspace_bytes(int32_t n_pages); /* host-only */
  * are not written. starts ascends (ckv_extend_pages gives it); whatever it holds, nothing outside the arrays is touched.
  *   k_pool, v_pool  the layer's pool, (n_kv_heads, n_pages * page_tokens, head_dim), bf16, kv_head_stride elements between heads; rows of a
  *                   page behind its sequence's last may hold anything
- *   most_tokens     the most new tokens of a sequence, if known (0: not); it chooses the kernel's form, not the result
+ *   most_tokens, most_rows, total_rows  of the sequences with new tokens, if known, or about: the most tokens of one, the most rows of one, and
+ *                   all of their rows (0: not known; n_tokens, n_entries * page_tokens and a part of that for each then); they choose the
+ *                   kernel's form, not the result
  *   workspace       optional device buffer of workspace_bytes >= ckv_attention_paged_workspace_bytes(...) (16-byte aligned): partial rows
  *                   of launches that split the cache; without it they run unsplit (slower; the same up to the order of fp32 sums)
  * head_dim 64 or 128; scale within the normal fp32 numbers' range; lengths past n_entries * page_tokens count as that.
@@ -719,14 +721,14 @@ int64_t ckv_compact_pages_workspace_bytes(int32_t n_pages); /* host-only */
  */
 int32_t ckv_attention_paged(void* out, const void* q, int64_t q_head_stride, int64_t q_token_stride, const void* k_pool,
                             const void* v_pool, int64_t kv_head_stride, const int32_t* table, const int32_t* lengths,
-                            const int32_t* starts, int32_t n_tokens, int32_t most_tokens, int32_t n_sequences,
-                            int32_t n_entries, int32_t n_pages, int32_t page_tokens, int32_t n_q_heads, int32_t n_kv_heads,
+                            const int32_t* starts, int32_t n_tokens, int32_t most_tokens, int32_t most_rows,
+                            int64_t total_rows, int32_t n_sequences, int32_t n_entries, int32_t n_pages, int32_t page_tokens, int32_t n_q_heads, int32_t n_kv_heads,
                             int32_t head_dim, int32_t dtype, double scale, void* workspace, int64_t workspace_bytes,
                             int32_t* err, void* stream);
 
 /* Bytes of workspace that ckv_attention_paged uses for this shape (0: none). Host-only. */
-int64_t ckv_attention_paged_workspace_bytes(int32_t n_tokens, int32_t n_sequences, int32_t most_tokens, int32_t n_entries,
-                                            int32_t page_tokens, int32_t n_q_heads, int32_t n_kv_heads, int32_t head_dim);
+int64_t ckv_attention_paged_workspace_bytes(int32_t n_tokens, int32_t n_sequences, int32_t most_tokens, int32_t most_rows,
+                                            int64_t total_rows, int32_t n_entries, int32_t page_tokens, int32_t n_q_heads, int32_t n_kv_heads, int32_t head_dim);
 
 /*
  * Logits (n_rows, vocab), bf16 or f32 with contiguous rows, adjusted before a token is chosen. With c = how often the row's `generated`

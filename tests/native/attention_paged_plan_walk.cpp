@@ -30,7 +30,9 @@ int main() {
       }
       if (n == 0) continue;
       for (int64_t hint : {most, n, (int64_t)1}) {  // a hint below the truth too
-        const PagedPlan p = paged_plan(n, S, hint, M * T, h[0], h[1], h[2], INT64_MAX);
+        const int64_t longest = rng() % 2 ? M * T : log_int(1, M * T);  // and of the rows
+        const int64_t total = rng() % 2 ? 0 : log_int(1, S * M * T);
+        const PagedPlan p = paged_plan(n, S, hint, longest, total, M * T, h[0], h[1], h[2], INT64_MAX);
         const bool large = p.rows == kAttnBM;
         ++checked;
         split += p.target > 0;
@@ -65,9 +67,9 @@ int main() {
           items = all_tiles;
           ok = ok && items <= p.items;
         }
-        // less workspace than asked for: no splits, and never more than there is
-        const PagedPlan q = paged_plan(n, S, hint, M * T, h[0], h[1], h[2], p.ws_bytes - 1);
-        ok = ok && (p.target == 0 || (q.target == 0 && q.ws_bytes == 0));
+        // less workspace than asked for: a form that needs none or less
+        const PagedPlan q = paged_plan(n, S, hint, longest, total, M * T, h[0], h[1], h[2], p.ws_bytes - 1);
+        ok = ok && (p.target == 0 || q.ws_bytes < p.ws_bytes) && (q.target == 0) == (q.ws_bytes == 0);
         if (!ok) {
           ++bad;
           if (bad < 10) std::printf("S %ld n %ld most %ld rows %ld heads %d/%d: items %ld of %ld\n", (long)S, (long)n, (long)hint, (long)(M * T), h[0], h[1], (long)items, (long)p.items);

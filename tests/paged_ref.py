@@ -171,18 +171,38 @@ def adjusted(logits, prompt=None, generated=None, repetition=1.0, frequency=0.0,
     return x
 
 
-# Launches of attention over a paged cache that reach every kernel form: (heads, sequences (rows, new tokens), most, split).
+# Launches of attention over a paged cache that reach every kernel form: heads, sequences (rows, new tokens), most, whether all rows together are told
+# (and then the rows of a tile, whether they are split, their joins spread, the sequences more than 64).
 _7B, _05B = (28, 4, 128), (14, 2, 64)
-FORMS = [(h, seqs, most, split) for h, cases in (
-    (_7B, [
-        ([(100, 1)], 1, True), ([(100, 4)], 4, True), ([(64, 1)] * 70, 1, True), ([(64, 3)] * 70, 3, True),
-        ([(3000, 1)], 1, True), ([(3000, 4)], 4, True), ([(3000, 2), (5, 1)] + [(300, 2)] * 58, 2, True), ([(2500, 4)] + [(300, 4)] * 29, 4, True),
-        ([(3000, 1)] + [(40, 1)] * 69, 1, True), ([(3000, 1)] + [(40, 1)] * 79, 1, True), ([(3000, 4)] + [(40, 1)] * 65, 4, True), ([(3000, 4)] + [(40, 4)] * 69, 4, True),
-        ([(9000, 40)], 40, True), ([(6000, 300)], 300, True), ([(1500, 1200), (33, 20)], 1200, False),
-    ]),
-    (_05B, [
-        ([(100, 1)], 1, True), ([(100, 4)], 4, True), ([(64, 1)] * 70, 1, True), ([(64, 3)] * 70, 3, True),
-        ([(3000, 1)], 1, True), ([(3000, 4)], 4, True), ([(2000, 20)] + [(100, 20)] * 9, 1, True), ([(2500, 4)] + [(100, 4)] * 49, 4, True),
-        ([(3000, 1)] + [(40, 1)] * 69, 1, True), ([(3000, 2)] + [(40, 2)] * 79, 2, True), ([(3000, 4)] + [(40, 1)] * 65, 4, True), ([(3000, 4)] + [(40, 4)] * 69, 4, True),
-        ([(20000, 60)], 60, True), ([(6000, 600)], 600, True), ([(1500, 1200), (33, 20)], 1200, False),
-    ])) for seqs, most, split in cases]
+FORMS = [
+    (_05B, [(64, 1)], 1, False),  # 16, 0, 0, 0
+    (_05B, [(64, 1)] + [(40, 1)] * 64, 1, False),  # 16, 0, 0, 1
+    (_05B, [(1500, 8)] + [(40, 8)] * 19, 8, True),  # 16, 1, 0, 0
+    (_05B, [(1500, 3)] + [(40, 3)] * 64, 3, True),  # 16, 1, 0, 1
+    (_05B, [(1500, 1)], 1, False),  # 16, 1, 1, 0
+    (_05B, [(1500, 1)] + [(40, 1)] * 65, 1, False),  # 16, 1, 1, 1
+    (_05B, [(100, 60)] + [(40, 40)] * 19, 60, False),  # 32, 0, 0, 0
+    (_05B, [(100, 12)] + [(40, 12)] * 65, 12, False),  # 32, 0, 0, 1
+    (_05B, [(2000, 8)] + [(40, 8)] * 19, 8, False),  # 32, 1, 0, 0
+    (_05B, [(2000, 3)] + [(40, 3)] * 64, 3, False),  # 32, 1, 0, 1
+    (_05B, [(2000, 5)] + [(40, 5)] * 19, 5, False),  # 32, 1, 1, 0
+    (_05B, [(1500, 3)] + [(40, 1)] * 64, 3, False),  # 32, 1, 1, 1
+    (_05B, [(64, 60)] * 2 + [(64, 60)] * 18, 60, True),  # 128, 0, 0, 0
+    (_05B, [(2500, 8)] + [(40, 8)] * 29, 8, False),  # 128, 1, 0, 0
+    (_05B, [(2500, 40)] + [(40, 40)] * 9, 40, False),  # 128, 1, 1, 0
+    (_7B, [(64, 1)], 1, False),  # 16, 0, 0, 0
+    (_7B, [(64, 1)] + [(40, 1)] * 64, 1, False),  # 16, 0, 0, 1
+    (_7B, [(1500, 12)] + [(40, 12)] * 9, 12, True),  # 16, 1, 0, 0
+    (_7B, [(1500, 2)] + [(40, 2)] * 65, 2, True),  # 16, 1, 0, 1
+    (_7B, [(1500, 1)], 1, False),  # 16, 1, 1, 0
+    (_7B, [(1500, 1)] + [(40, 1)] * 64, 1, True),  # 16, 1, 1, 1
+    (_7B, [(100, 40)] + [(40, 40)] * 9, 40, False),  # 32, 0, 0, 0
+    (_7B, [(64, 3)] * 2 + [(40, 3)] * 63, 3, False),  # 32, 0, 0, 1
+    (_7B, [(1500, 40)] + [(64, 40)], 40, True),  # 32, 1, 0, 0
+    (_7B, [(2000, 3)] + [(40, 3)] * 79, 3, True),  # 32, 1, 0, 1
+    (_7B, [(1500, 3)] + [(40, 3)] * 9, 3, False),  # 32, 1, 1, 0
+    ((3, 1, 128), [(1500, 8)] + [(40, 8)] * 64, 8, False),  # 32, 1, 1, 1
+    (_7B, [(64, 40)] + [(40, 40)] * 9, 40, False),  # 128, 0, 0, 0
+    (_7B, [(2000, 5)] + [(40, 5)] * 19, 5, False),  # 128, 1, 0, 0
+    (_7B, [(2000, 12)] + [(40, 12)] * 9, 12, False),  # 128, 1, 1, 0
+]

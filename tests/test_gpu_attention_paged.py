@@ -82,9 +82,22 @@ def test_matches_the_64_bit_form(heads, T, seqs):
 
 @pytest.mark.parametrize("form", range(len(R.FORMS)))
 def test_every_kernel_form(form):
-    heads, seqs, most, split = R.FORMS[form]
+    heads, seqs, most, known = R.FORMS[form]
     q, cache, starts = _batch(heads, 64, seqs, seed=form)
-    _check(ops.attention_paged(q, cache, 0, starts, most=most, split=split), _want(q, cache, seqs))
+    total = sum(r for r, _ in seqs) if known else None
+    _check(ops.attention_paged(q, cache, 0, starts, most=most, total=total), _want(q, cache, seqs))
+
+
+@pytest.mark.parametrize("seqs", [[(1, 1)], [(700, 1), (0, 0), (64, 30), (3000, 2)], [(900, 300), (40, 1)], [(60, 1)] * 70 + [(4000, 9)]])
+@pytest.mark.parametrize("heads", [(28, 4, 128), (14, 2, 64)])
+def test_estimates_choose_the_form_only(heads, seqs):
+    """Whatever most, longest and total say, far too little or too much."""
+    q, cache, starts = _batch(heads, 32, seqs, seed=11)
+    want = _want(q, cache, seqs)
+    for most in (1, 5, 10**6):
+        for longest in (1, 600, 2**31 - 1):
+            for total in (None, 1, 10**12):
+                _check(ops.attention_paged(q, cache, 0, starts, most=most, longest=longest, total=total), want)
 
 
 @pytest.mark.parametrize("heads", [(28, 4, 128), (14, 2, 64)])

@@ -23,7 +23,7 @@ FORK = [*POOL, ("sources", 16), ("targets", 16), ("n", 2), *BOOK, ("ws", 16), ("
 FREE = [("sequences", 16), ("keep", None), ("n", 2), *BOOK, ("ws", 16), ("wsb", 8), ("err", None), ("stream", None)]
 COMPACT = [*POOL, ("used", 16), *BOOK, ("ws", 16), ("wsb", 1 << 20), ("err", None), ("stream", None)]
 ATTN = [("out", 16), ("q", 16), ("q_hs", 64), ("q_ts", 256), ("k", 16), ("v", 16), ("hs", 640 * 64), ("table", 16), ("lengths", 16), ("starts", 16),
-        ("n", 5), ("most", 0), ("S", 4), ("M", 8), ("P", 20), ("T", 32), ("Hq", 4), ("Hkv", 2), ("D", 64), ("dtype", 1), ("scale", 0.125), ("ws", None),
+        ("n", 5), ("most", 0), ("longest", 0), ("total", 0), ("S", 4), ("M", 8), ("P", 20), ("T", 32), ("Hq", 4), ("Hkv", 2), ("D", 64), ("dtype", 1), ("scale", 0.125), ("ws", None),
         ("wsb", 0), ("err", None), ("stream", None)]
 LOGITS = [("logits", 16), ("row", 100), ("n", 2), ("vocab", 100), ("dtype", 1), ("prompt", 16), ("p_row", 7), ("np", 7), ("gen", 16), ("g_row", 3), ("ng", 3),
           ("rep_rows", None), ("rep", 1.0), ("freq_rows", None), ("freq", 0.0), ("pres_rows", None), ("pres", 0.0), ("bias", 16), ("b_row", 0),
@@ -58,7 +58,7 @@ def _with(base, **kw):
     ("ckv_attention_paged", ATTN, [
         (dict(out=None), INVALID), (dict(q=None), INVALID), (dict(k=None), INVALID), (dict(table=None), INVALID), (dict(lengths=None), INVALID),
         (dict(starts=None), INVALID), (dict(q=8), INVALID), (dict(v=8), INVALID), (dict(out=8), INVALID), (dict(D=256), INVALID), (dict(dtype=0), INVALID),
-        (dict(T=16), INVALID), (dict(Hq=3), INVALID), (dict(Hkv=0), INVALID), (dict(n=-1), INVALID), (dict(most=-1), INVALID), (dict(S=0), INVALID), (dict(M=0), INVALID),
+        (dict(T=16), INVALID), (dict(Hq=3), INVALID), (dict(Hkv=0), INVALID), (dict(n=-1), INVALID), (dict(most=-1), INVALID), (dict(longest=-1), INVALID), (dict(total=-1), INVALID), (dict(S=0), INVALID), (dict(M=0), INVALID),
         (dict(P=0), INVALID), (dict(scale=0.0), INVALID), (dict(scale=float("inf")), INVALID), (dict(scale=1e-40), INVALID), (dict(q_hs=68), INVALID),
         (dict(q_ts=56), RANGE), (dict(hs=639 * 64), RANGE), (dict(S=4097), LARGE), (dict(M=1 << 26), LARGE), (dict(P=1 << 26, hs=1 << 40), LARGE), (dict(n=1 << 30), LARGE),
         (dict(n=0, q=None, out=None), OK)]),
@@ -79,10 +79,11 @@ def test_workspace_sizes_are_host_only():
     assert lib.ckv_next_tokens_workspace_bytes(3, 100) == 0 and lib.ckv_next_tokens_workspace_bytes(0, 152064) == 0
     assert lib.ckv_next_tokens_workspace_bytes(3, 152064) % 24 == 0 and lib.ckv_next_tokens_workspace_bytes(3, 152064) > 0
     w = lib.ckv_attention_paged_workspace_bytes
-    assert w(1, 1, 1, 2, 64, 28, 4, 128) == 0  # a table of one split's rows
-    assert w(1, 1, 1, 200, 64, 28, 4, 128) > 0 and w(1, 1, 1, 200, 64, 28, 4, 128) % (4 * 16 * 132 * 4) == 0
-    assert w(8000, 2, 4000, 200, 64, 28, 4, 128) == 0  # tiles enough
-    assert w(0, 1, 1, 200, 64, 28, 4, 128) == w(1, 1, 1, 200, 64, 28, 3, 128) == w(1, 0, 1, 200, 64, 28, 4, 128) == 0
+    assert w(1, 1, 1, 0, 0, 2, 64, 28, 4, 128) == 0  # a table of one split's rows
+    assert w(1, 1, 1, 0, 0, 200, 64, 28, 4, 128) > 0 and w(1, 1, 1, 0, 0, 200, 64, 28, 4, 128) % (4 * 16 * 132 * 4) == 0
+    assert w(1, 1, 1, 500, 0, 200, 64, 28, 4, 128) == 0  # short rows, if they are known to be
+    assert w(8000, 2, 4000, 0, 0, 200, 64, 28, 4, 128) == 0  # tiles enough
+    assert w(0, 1, 1, 0, 0, 200, 64, 28, 4, 128) == w(1, 1, 1, 0, 0, 200, 64, 28, 3, 128) == w(1, 0, 1, 0, 0, 200, 64, 28, 4, 128) == 0
 
 
 def test_every_paged_plan_can_be_launched(tmp_path):
@@ -105,9 +106,10 @@ def test_every_kernel_form_is_tested(tmp_path):
     exe = tmp_path / "attention_paged_forms"
     subprocess.run([gxx, "-O2", "-std=c++17", f"-I{ROOT / 'chunkkv_amd' / 'csrc'}", str(ROOT / "tests" / "native" / "attention_paged_forms.cpp"), "-o", str(exe)], check=True)
     lines = []
-    for (hq, hkv, d), seqs, most, split in FORMS:
+    for (hq, hkv, d), seqs, most, known in FORMS:
         entries = max(-(-r // 64) for r, _ in seqs) + 1  # as the GPU test's batches have them
-        lines.append(f"{sum(c for _, c in seqs)} {len(seqs)} {most} {entries * 64} {hq} {hkv} {d} {int(split)}")
+        total = sum(r for r, _ in seqs) if known else 0
+        lines.append(f"{sum(c for _, c in seqs)} {len(seqs)} {most} {entries * 64} {total} {hq} {hkv} {d} 1")
     out = subprocess.run([str(exe)], check=True, capture_output=True, text=True, input="\n".join(lines), timeout=60).stdout
     got = {tuple(map(int, line.split())) for line in out.splitlines()}
     want = {(d, r, split, spread, many) for d in (64, 128) for r in (16, 32, 128) for split, spread in ((0, 0), (1, 0), (1, 1)) for many in ((0, 1) if r < 128 else (0,))}
@@ -239,6 +241,8 @@ with FakeTensorMode():
     bad("negative layer", ValueError, lambda: A(q, cache(), -1, t(4)))
     bad("starts", ValueError, lambda: A(q, cache(), 0, t(3)))
     bad("most", ValueError, lambda: A(q, cache(), 0, t(4), most=0))
+    bad("longest", ValueError, lambda: A(q, cache(), 0, t(4), longest=0))
+    bad("total", ValueError, lambda: A(q, cache(), 0, t(4), total=0))
     bad("out", ValueError, lambda: A(q, cache(), 0, t(4), out=t(1, 8, 4, 32, dtype=BF)))
     bad("f32 cache", TypeError, lambda: A(q, book(k=t(2, 1, 2, 128, 64, dtype=F32), v=t(2, 1, 2, 128, 64, dtype=F32)), 0, t(4)))
     x = t(2, 100, dtype=BF)
