@@ -109,7 +109,7 @@ def test_long_caches(heads, seqs):
         _check(ops.attention_paged(q, cache, 0, starts, **kw), want)
 
 
-@pytest.mark.parametrize("S", [64, 65, 200, 1000])
+@pytest.mark.parametrize("S", [64, 65, 200, 1000, 4096])
 def test_many_sequences(S):
     rng = random.Random(S)
     seqs = [(rng.choice([1, 5, 33, 64, 200]), 1) if rng.random() < 0.8 else (rng.choice([0, 9]), 0) for _ in range(S)]

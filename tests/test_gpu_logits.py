@@ -139,3 +139,24 @@ def test_graph_replays_follow_the_tokens():
         graph.replay()
     want = expect(torch.full((3, 16), -1, dtype=torch.int64), 6)
     assert torch.equal(seen.cpu(), want)
+
+
+def test_as_many_rows_as_there_may_be():
+    """65535 rows, one more is refused; rows past 4 GB have the results that they have alone."""
+    logits, kw = _case(3, 40, F32, 1, 5, 5)
+    logits = logits[torch.arange(65535) % 3].contiguous()
+    kw = {k: v[torch.arange(65535) % 3] if isinstance(v, torch.Tensor) and v.dim() and v.shape[0] == 3 else v for k, v in kw.items()}
+    got, tokens = ops.adjust_logits(logits, **kw), ops.next_tokens(logits, **kw)
+    assert torch.equal(got, got[:3][torch.arange(65535) % 3]) and torch.equal(tokens, got.argmax(1))
+    more = torch.zeros((65536, 40), device=DEV)
+    for call in (ops.adjust_logits, ops.next_tokens):
+        with pytest.raises(ValueError):
+            call(more)
+    big = torch.zeros((16000, 152064), dtype=BF, device=DEV)
+    big[-3:] = torch.randn((3, 152064), device=DEV).to(BF)
+    history = torch.randint(0, 152064, (16000, 9), device=DEV)
+    got = ops.adjust_logits(big, generated=history, repetition=1.5, frequency=0.25)
+    want = ops.adjust_logits(big[-3:].clone(), generated=history[-3:], repetition=1.5, frequency=0.25)
+    assert torch.equal(got[-3:], want)
+    del got
+    assert torch.equal(ops.next_tokens(big, generated=history, repetition=1.5, frequency=0.25)[-3:], want.argmax(1))

@@ -254,3 +254,27 @@ def test_pages_past_4_gb():
         assert int(rows[1].max()) < small * T
         for t, u in ((a.k, b.k), (a.v, b.v)):
             assert torch.equal(t[:, :, :, rows[0]], u[:, :, :, rows[1]])
+
+
+def test_as_many_pairs_as_there_may_be():
+    """4095 continuations of one sequence in a call, all 4096 ended in another."""
+    S, T = 4096, 32
+    c, b, err = _cache(S, 128, 4200, T, layers=1, H=1)
+    held = Held(c, b)
+    counts = [70] + [0] * (S - 1)
+    new = ops.extend_pages(c, _ints(counts), 70, err)
+    held.write(b.extend(counts, 70)[1], new.starts.tolist())
+    ops.fork_pages(c, _ints([0] * (S - 1)), _ints(list(range(1, S))), err)
+    b.fork([0] * (S - 1), list(range(1, S)))
+    b.check(c, err)
+    assert int(c.refs.max()) == S
+    for s in (0, 1, 2047, 4095):
+        i = b.rows(s).to(DEV)
+        assert torch.equal(c.k[0, 0, 0, i], c.k[0, 0, 0, b.rows(0).to(DEV)]) and torch.equal(c.v[0, 0, 0, i], c.v[0, 0, 0, b.rows(0).to(DEV)])
+    ends = list(range(S - 1, -1, -1))
+    ops.free_pages(c, _ints(ends), err=err)
+    b.free(ends)
+    b.check(c, err)
+    assert not c.refs.any()
+    with pytest.raises(ValueError):
+        ops.free_pages(c, _ints(list(range(S)) + [0]), err=err)
