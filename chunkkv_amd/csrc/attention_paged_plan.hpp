@@ -46,17 +46,18 @@ struct PagedPlan {
 };
 
 // A kernel form's time in a graph replay, us at one load: `start` and a `step` for each 128 rows that its workgroups read one after the other, of head
-// sizes 64 and 128; `places`: workgroups that the card holds of it. From 285 shapes (28 / 4 heads of 128, 14 / 2 and 8 / 8 of 64; 1 to 100 sequences of 200 to 8302 rows, equal,
-// ragged and one long among short ones, 1 to 500 new tokens each), every form timed: the one with the least estimate takes 1.6 % more than the fastest on average, at
-// most 31 %, and 1.7 and 66 % where the rows of all are not told (tiles by a launch's load alone and splits from 512 or 1024 rows on took 4.1 % more, at most 79 %).
+// sizes 64 and 128; `places`: workgroups that the card holds of it; `tile`: steps that a tile's beginning and end cost where a place has several. From 357 shapes (28 / 4, 32 / 8,
+// 8 / 2 and 16 / 16 heads of 128, 14 / 2, 8 / 8 and 32 / 1 of 64; 1 to 100 sequences of 200 to 8302 rows, equal, ragged and one long among short ones, 1 to 500 new
+// tokens each), every form timed: the one with the least estimate takes 1.1 % more than the fastest on average and 29 % at most, where the rows of all are not told
+// 1.7 and 124 % (40 sequences, one of 2992 rows, the others 187: 66.9 for 29.8); tiles by a launch's load alone and splits from 512 or 1024 rows on 4.1 and 79 %.
 struct PagedForm {
   int rows;
-  double start, step[2];
+  double start, step[2], tile;
   int places[2];
 };
-constexpr PagedForm kPagedForms[] = {{16, 5.5, {0.55, 0.75}, {512, 256}}, {32, 5.7, {0.6, 1.1}, {512, 256}}, {kAttnBM, 5.0, {1.5, 2.4}, {768, 512}}};
-constexpr double kPagedJoin = 5.0, kPagedJoinByte = 1.5e-6;  // us that splitting adds, and for each byte of the result in fp32
-constexpr double kPagedMean = 0.6;  // of the longest sequence's rows, where the sum is not known
+constexpr PagedForm kPagedForms[] = {{16, 5.5, {0.5, 0.8}, 1.5, {512, 256}}, {32, 6.0, {0.55, 1.1}, 1.5, {512, 256}}, {kAttnBM, 5.0, {1.5, 2.4}, 0.5, {768, 512}}};
+constexpr double kPagedJoin = 4.5, kPagedJoinByte = 1.5e-6;  // us that splitting adds, and for each byte in fp32 of the results that are split
+constexpr double kPagedMean = 0.5;  // of the longest sequence's rows, where the sum is not known
 
 // n new tokens of S sequences; `most` of one, `longest` cached rows of one and `total` of all that have tokens (0: not known) are estimates, `rows` is the most that
 // a sequence can have. Lengths are the device's: the items are bounded by tiles (a sequence's last one may be partial) and by what splits add. Of a sequence whose (token, query head) rows fit 16 or 32
@@ -75,9 +76,10 @@ static inline PagedPlan paged_plan(int64_t n, int64_t S, int64_t most, int64_t l
     if ((f.rows > 16 && one <= 16) || (f.rows > 32 && one <= 32)) continue;
     const bool large = f.rows == kAttnBM;
     const int64_t unit = large ? kAttnBN : kPagedUnit, tiles = n * group / f.rows + used;
-    const double half = (double)unit / 2.0, units = std::ceil(longer / (double)unit) * (double)unit / 128.0;
+    const double least_units = (double)unit / 128.0, units = std::ceil(longer / (double)unit) * least_units;
+    const double mean_units = std::min(std::max(mean / 128.0 + least_units / 2.0, least_units), units);
     const double likely = (double)std::min(tiles, used * ((one + f.rows - 1) / f.rows));
-    const double load = 1.3 * std::min((mean + half) / 128.0, units) * likely * Hkv / f.places[d128];  // of a workgroup, if three of four are busy
+    const double load = 1.3 * (mean_units + f.tile) * likely * Hkv / f.places[d128];  // of a workgroup, if three of four are busy
     const double whole = f.start + f.step[d128] * std::max(units, load);
     if (whole < least) {
       least = whole;
@@ -100,7 +102,8 @@ static inline PagedPlan paged_plan(int64_t n, int64_t S, int64_t most, int64_t l
       s.ws_bytes = 2 * s.items * row_b;  // of a share, its first and its last tile may be partial
       if (tiles * ((rows + unit - 1) / unit) > INT32_MAX / 2) continue;  // units are counted in 32 bits
     }
-    const double split = f.start + kPagedJoin + kPagedJoinByte * 4.0 * (double)(n * Hq * head_dim) + f.step[d128] * std::max(2.0, load);
+    const double joined = 4.0 * (double)(n * Hq * head_dim) * (total > 0 ? mean_units / units : 1.0);  // tiles of short sequences are mostly whole
+    const double split = f.start + kPagedJoin + kPagedJoinByte * joined + f.step[d128] * std::max(2.0, load);
     if (split < least && s.ws_bytes <= workspace_bytes) {
       least = split;
       s.spread_join = s.target >= 8 * tiles || n * Hq <= 2048;

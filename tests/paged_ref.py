@@ -177,32 +177,32 @@ _7B, _05B = (28, 4, 128), (14, 2, 64)
 FORMS = [
     (_05B, [(64, 1)], 1, False),  # 16, 0, 0, 0
     (_05B, [(64, 1)] + [(40, 1)] * 64, 1, False),  # 16, 0, 0, 1
-    (_05B, [(1500, 8)] + [(40, 8)] * 19, 8, True),  # 16, 1, 0, 0
+    (_05B, [(1500, 20)] + [(40, 20)] * 9, 20, True),  # 16, 1, 0, 0
     (_05B, [(1500, 3)] + [(40, 3)] * 64, 3, True),  # 16, 1, 0, 1
     (_05B, [(1500, 1)], 1, False),  # 16, 1, 1, 0
     (_05B, [(1500, 1)] + [(40, 1)] * 65, 1, False),  # 16, 1, 1, 1
-    (_05B, [(100, 60)] + [(40, 40)] * 19, 60, False),  # 32, 0, 0, 0
-    (_05B, [(100, 12)] + [(40, 12)] * 65, 12, False),  # 32, 0, 0, 1
+    (_05B, [(300, 60)] + [(64, 60)] * 9, 60, False),  # 32, 0, 0, 0
+    (_05B, [(100, 8)] * 2 + [(40, 8)] * 64, 8, False),  # 32, 0, 0, 1
     (_05B, [(2000, 8)] + [(40, 8)] * 19, 8, False),  # 32, 1, 0, 0
     (_05B, [(2000, 3)] + [(40, 3)] * 64, 3, False),  # 32, 1, 0, 1
-    (_05B, [(2000, 5)] + [(40, 5)] * 19, 5, False),  # 32, 1, 1, 0
-    (_05B, [(1500, 3)] + [(40, 1)] * 64, 3, False),  # 32, 1, 1, 1
-    (_05B, [(64, 60)] * 2 + [(64, 60)] * 18, 60, True),  # 128, 0, 0, 0
+    (_05B, [(2000, 60)] + [(40, 40)] * 2, 60, False),  # 32, 1, 1, 0
+    (_05B, [(2000, 4)] + [(40, 1)] * 64, 4, False),  # 32, 1, 1, 1
+    (_05B, [(64, 40)] + [(64, 40)] * 9, 40, False),  # 128, 0, 0, 0
     (_05B, [(2500, 8)] + [(40, 8)] * 29, 8, False),  # 128, 1, 0, 0
     (_05B, [(2500, 40)] + [(40, 40)] * 9, 40, False),  # 128, 1, 1, 0
     (_7B, [(64, 1)], 1, False),  # 16, 0, 0, 0
     (_7B, [(64, 1)] + [(40, 1)] * 64, 1, False),  # 16, 0, 0, 1
-    (_7B, [(1500, 12)] + [(40, 12)] * 9, 12, True),  # 16, 1, 0, 0
+    (_7B, [(1500, 8)] + [(100, 8)] * 9, 8, True),  # 16, 1, 0, 0
     (_7B, [(1500, 2)] + [(40, 2)] * 65, 2, True),  # 16, 1, 0, 1
-    (_7B, [(1500, 1)], 1, False),  # 16, 1, 1, 0
-    (_7B, [(1500, 1)] + [(40, 1)] * 64, 1, True),  # 16, 1, 1, 1
-    (_7B, [(100, 40)] + [(40, 40)] * 9, 40, False),  # 32, 0, 0, 0
+    (_7B, [(900, 1)], 1, False),  # 16, 1, 1, 0
+    ((3, 1, 128), [(900, 1)] + [(40, 1)] * 64, 1, False),  # 16, 1, 1, 1
+    (_7B, [(100, 100)] + [(40, 40)], 100, False),  # 32, 0, 0, 0
     (_7B, [(64, 3)] * 2 + [(40, 3)] * 63, 3, False),  # 32, 0, 0, 1
-    (_7B, [(1500, 40)] + [(64, 40)], 40, True),  # 32, 1, 0, 0
-    (_7B, [(2000, 3)] + [(40, 3)] * 79, 3, True),  # 32, 1, 0, 1
-    (_7B, [(1500, 3)] + [(40, 3)] * 9, 3, False),  # 32, 1, 1, 0
+    (_7B, [(1500, 12)] + [(40, 12)] * 9, 12, True),  # 32, 1, 0, 0
+    (_7B, [(1500, 3)] + [(40, 3)] * 64, 3, True),  # 32, 1, 0, 1
+    (_7B, [(1500, 12)] + [(40, 12)] * 4, 12, False),  # 32, 1, 1, 0
     ((3, 1, 128), [(1500, 8)] + [(40, 8)] * 64, 8, False),  # 32, 1, 1, 1
-    (_7B, [(64, 40)] + [(40, 40)] * 9, 40, False),  # 128, 0, 0, 0
+    (_7B, [(64, 60)] * 2, 60, False),  # 128, 0, 0, 0
     (_7B, [(2000, 5)] + [(40, 5)] * 19, 5, False),  # 128, 1, 0, 0
     (_7B, [(2000, 12)] + [(40, 12)] * 9, 12, False),  # 128, 1, 1, 0
 ]
