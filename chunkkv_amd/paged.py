@@ -142,7 +142,7 @@ class PagedSession:
     # -- the model ------------------------------------------------------------------------
 
     def _forward(self, tok: torch.Tensor, counts: torch.Tensor, most: int, rows: list[int]):
-        """New tokens tok (n,), in the order of the sequences, counts[s] of each, most of one at most; rows: of each with them. The new rows
+        """New tokens tok (n,), in the order of the sequences, counts[s] of each, most of one at most; rows: of each with them, or about. The new rows
         are taken and written, layer by layer. (h, pending, starts), for the engine's _final_logits."""
         e, c = self.engine, self.cache
         known = dict(most=most, longest=max(rows), total=sum(rows))
@@ -224,7 +224,7 @@ class PagedSession:
             ops.next_tokens(logits, prompt=prompt, generated=generated, allowed=masks, err=self._err, out=tok, **fixed)
             generated.scatter_(1, at, tok[:, None])
             at.add_(1)
-            h, pending, _ = self._forward(tok, counts, 1, [len(self.tokens[s]) + max_tokens for s in slots])
+            h, pending, _ = self._forward(tok, counts, 1, [len(self.tokens[s]) + (max_tokens + 1) // 2 for s in slots])
             logits.copy_(self.engine._final_logits(h, pending)[0])
 
         before = [len(self.tokens[s]) for s in slots]
