@@ -15,6 +15,8 @@ graph; the host keeps each sequence's tokens, which say how many rows and pages 
 
 from __future__ import annotations
 
+from contextlib import contextmanager
+
 import torch
 
 from chunkkv_amd import _native, ops
@@ -68,6 +70,19 @@ class PagedSession:
                 raise ValueError("a mask left no token to choose")
             raise RuntimeError(f"a paged cache kernel reported an error ({bits})")
 
+    @contextmanager
+    def _or_back(self, rows: dict[int, int]):
+        """Where this block raises, an interrupt among it, sequences s go back to rows[s] rows, which the device may have left; else the next rows
+        would come behind ones that were never written."""
+        try:
+            yield
+        except BaseException:
+            self._go_back(rows)
+            raise
+
+    def _go_back(self, rows: dict[int, int]) -> None:
+        ops.free_pages(self.cache, self._ints(rows), self._ints(rows.values()), self._err)
+
     def _token_list(self, tokens) -> list[int]:
         tokens = [int(t) for t in tokens]
         vocab = self.engine.inner.embed_tokens.weight.shape[0]
@@ -93,17 +108,24 @@ class PagedSession:
     def add(self, result, tokens) -> int:
         """A new sequence of a prefill's rows (PrefillResult, its logits' last row the last token's); its number."""
         tokens = self._token_list(tokens)
-        if len(result.keys) != self.cache.k.shape[0] or len(tokens) != result.keys[0].shape[2]:
-            raise ValueError(f"{len(tokens)} tokens of {self.cache.k.shape[0]} layers for {result.keys[0].shape[2]} rows of {len(result.keys)}")
+        c = self.cache
+        if len(result.keys) != c.k.shape[0] or len(tokens) != result.keys[0].shape[2]:
+            raise ValueError(f"{len(tokens)} tokens of {c.k.shape[0]} layers for {result.keys[0].shape[2]} rows of {len(result.keys)}")
+        shape = (1, c.k.shape[2], len(tokens), c.k.shape[4])
+        for layers in (result.keys, result.values):
+            if len(layers) != c.k.shape[0] or any(t.shape != shape or t.dtype != c.k.dtype or t.device != c.k.device for t in layers):
+                raise ValueError(f"a prefill's keys and values are {tuple(shape)} {c.k.dtype} on {c.k.device} in each of {c.k.shape[0]} layers here")
         (s,) = self._slots(1)
         self._check_room({s: len(tokens)})
-        new = ops.extend_pages(self.cache, self._counts({s: len(tokens)}), len(tokens), self._err)
-        for li in range(self.cache.k.shape[0]):
-            ops.scatter_rows(self.cache.k[li], self.cache.v[li], result.keys[li], result.values[li], new.rows, self._err)
-        self._check_err()
+        with self._or_back({s: 0}):
+            new = ops.extend_pages(c, self._counts({s: len(tokens)}), len(tokens), self._err)
+            for li in range(c.k.shape[0]):
+                ops.scatter_rows(c.k[li], c.v[li], result.keys[li], result.values[li], new.rows, self._err)
+            logits = result.logits[-1:].clone()  # not the prefill's other rows
+            self._check_err()
         self.tokens[s] = tokens
-        if result.logits.shape[0]:
-            self._logits[s] = result.logits[-1:].clone()  # not the prefill's other rows
+        if logits.shape[0]:
+            self._logits[s] = logits
         return s
 
     @torch.inference_mode()
@@ -115,8 +137,9 @@ class PagedSession:
         targets = self._slots(n)
         if len(self.tokens[source]) % self.cache.page_tokens and n > self.free_pages:
             raise ValueError(f"{n} more pages are needed, {self.free_pages} are free")
-        ops.fork_pages(self.cache, self._ints([source] * n), self._ints(targets), self._err)
-        self._check_err()
+        with self._or_back(dict.fromkeys(targets, 0)):
+            ops.fork_pages(self.cache, self._ints([source] * n), self._ints(targets), self._err)
+            self._check_err()
         for t in targets:
             self.tokens[t] = list(self.tokens[source])
             if source in self._logits:
@@ -169,10 +192,11 @@ class PagedSession:
         more = {s: len(chunk) for s, chunk in chunks.items()}
         self._check_room(more)
         tok = torch.tensor([t for chunk in chunks.values() for t in chunk], dtype=torch.int64).to(self.engine.device)
-        h, pending, starts = self._forward(tok, self._counts(more), max(more.values()), [len(self.tokens[s]) + n for s, n in more.items()])
-        last = starts[1:].long()[torch.tensor(list(chunks)).to(starts.device)] - 1
-        logits = self.engine._final_logits(h[:, last], None if pending is None else pending[:, last])[0]
-        self._check_err()
+        with self._or_back({s: len(self.tokens[s]) for s in chunks}):
+            h, pending, starts = self._forward(tok, self._counts(more), max(more.values()), [len(self.tokens[s]) + n for s, n in more.items()])
+            last = starts[1:].long()[torch.tensor(list(chunks)).to(starts.device)] - 1
+            logits = self.engine._final_logits(h[:, last], None if pending is None else pending[:, last])[0]
+            self._check_err()
         for i, (s, chunk) in enumerate(chunks.items()):
             self.tokens[s] += chunk
             self._logits[s] = logits[i:i + 1]
@@ -227,13 +251,9 @@ class PagedSession:
             h, pending, _ = self._forward(tok, counts, 1, [len(self.tokens[s]) + (max_tokens + 1) // 2 for s in slots])
             logits.copy_(self.engine._final_logits(h, pending)[0])
 
-        before = [len(self.tokens[s]) for s in slots]
-
-        def go_back(rows):  # every sequence of the batch took a row a step
-            ops.free_pages(self.cache, self._ints(slots), self._ints(rows), self._err)
-
+        before = {s: len(self.tokens[s]) for s in slots}
         live, graph, steps = set(range(B)), None, 0
-        try:
+        with self._or_back(before):
             while live and steps < max_tokens:
                 if steps and callable(allowed):
                     masks.copy_(mask())
@@ -253,10 +273,7 @@ class PagedSession:
                         else:
                             out[i].append(t)
             self._check_err()
-        except BaseException:  # the sequences are what they were
-            go_back(before)
-            raise
-        go_back(before[i] + len(out[i]) for i in range(B))
+        self._go_back({s: before[s] + len(out[i]) for i, s in enumerate(slots)})  # every one took a row a step
         for i, s in enumerate(slots):
             self.tokens[s] = self.tokens[s] + out[i]
             if i in live:

@@ -1,0 +1,106 @@
+"""HipEngine.paged where a call fails: the sequences are what they were, and the next call is right."""
+
+import pytest
+import torch
+
+from chunkkv_amd import ops
+from tests.test_gpu_paged_session import DEV, VOCAB, _close, _engine, _greedy_run, _session, _tokens
+
+pytestmark = pytest.mark.gpu
+
+
+class Stop(BaseException):
+    """As an interrupt: no Exception."""
+
+
+def _state(s):
+    return s.free_pages, s.cache.lengths.tolist(), s.cache.refs.tolist(), {k: list(v) for k, v in s.tokens.items()}, sorted(s._logits), int(s._err.item())
+
+
+def _fails_at(monkeypatch, name, call, error):
+    """ops.<name> raises at its call-th call from now on, once."""
+    real, calls = getattr(ops, name), []
+
+    def broken(*args, **kw):
+        calls.append(0)
+        if len(calls) == call:
+            raise error("broken")
+        return real(*args, **kw)
+
+    monkeypatch.setattr(ops, name, broken)
+
+
+@pytest.mark.parametrize("error", [RuntimeError, Stop])
+@pytest.mark.parametrize("name,call", [("rope_qkv", 1), ("attention_paged", 1), ("attention_paged", 3)])
+def test_a_feed_that_fails_takes_nothing(monkeypatch, name, call, error):
+    eng = _engine()
+    s, (a, b), prompts = _session(eng, (70, 33))
+    (c,) = s.fork(a)
+    before = _state(s)
+    chunks = {c: _tokens(41, 1), a: _tokens(1, 2), b: _tokens(170, 3)}
+    with monkeypatch.context() as m:
+        _fails_at(m, name, call, error)
+        with pytest.raises(error):
+            s.feed(chunks)
+    assert _state(s) == before
+    got = s.feed(chunks)
+    for i, prompt in ((a, prompts[0]), (b, prompts[1]), (c, prompts[0])):
+        _close(got[i][0], eng.prefill(prompt + chunks[i]).logits[-1])
+        assert int(s.cache.lengths[i]) == len(prompt) + len(chunks[i])
+
+
+@pytest.mark.parametrize("error", [RuntimeError, Stop])
+def test_an_addition_that_fails_takes_nothing(monkeypatch, error):
+    eng = _engine()
+    s, (a,), _ = _session(eng, (40,))
+    before, p = _state(s), _tokens(90, 4)
+    result = eng.prefill(p)
+    with monkeypatch.context() as m:
+        _fails_at(m, "scatter_rows", 2, error)
+        with pytest.raises(error):
+            s.add(result, p)
+    assert _state(s) == before
+    q = _tokens(50, 5)
+    assert s.add(eng.prefill(q), q) == 1 and int(s.cache.lengths[1]) == 50
+    _greedy_run(eng, q, s.generate([1], 12)[0], 12)
+
+
+def test_prefills_of_another_shape_are_refused_before_anything_is_done():
+    eng = _engine()
+    s, _, _ = _session(eng, (40,))
+    before, p = _state(s), _tokens(90, 4)
+    result = eng.prefill(p)
+
+    def changed(**kw):
+        r = eng.prefill(p)
+        for name, (layer, value) in kw.items():
+            getattr(r, name)[layer] = value
+        return r
+
+    K = result.keys[0]
+    for bad in (_engine(4, 4).prefill(p), changed(keys=(1, K[:, :, :80])), changed(values=(2, K[:, :1])), changed(keys=(2, K.float())),
+                changed(values=(0, K[..., :32])), changed(values=(1, K.cpu()))):
+        with pytest.raises((ValueError, TypeError)):
+            s.add(bad, p)
+        assert _state(s) == before
+    short = eng.prefill(p)
+    short.values.pop()
+    with pytest.raises(ValueError):
+        s.add(short, p)
+    assert _state(s) == before and s.add(result, p) == 1
+
+
+def test_a_fork_that_fails_takes_nothing(monkeypatch):
+    eng = _engine()
+    s, (a,), (prompt,) = _session(eng, (70,))
+    before = _state(s)
+    with monkeypatch.context() as m:
+        def interrupted():
+            raise Stop("broken")
+
+        m.setattr(s, "_check_err", interrupted)  # behind the device's part
+        with pytest.raises(Stop):
+            s.fork(a, 3)
+    assert _state(s) == before
+    b = s.fork(a)[0]
+    _greedy_run(eng, prompt, s.generate([b], 9)[0], 9)
