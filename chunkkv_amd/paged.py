@@ -78,6 +78,7 @@ class PagedSession:
             yield
         except BaseException:
             self._go_back(rows)
+            self._err.zero_()  # what this call flagged is not the next one's
             raise
 
     def _go_back(self, rows: dict[int, int]) -> None:
@@ -154,6 +155,7 @@ class PagedSession:
         for s in sequences:
             del self.tokens[s]
             self._logits.pop(s, None)
+        self._check_err()
 
     @torch.inference_mode()
     def compact(self) -> int:

@@ -104,3 +104,37 @@ def test_a_fork_that_fails_takes_nothing(monkeypatch):
     assert _state(s) == before
     b = s.fork(a)[0]
     _greedy_run(eng, prompt, s.generate([b], 9)[0], 9)
+
+
+@pytest.mark.parametrize("then", ["feed", "add", "fork", "generate"])
+def test_what_a_failed_call_flagged_is_not_the_next_ones(monkeypatch, then):
+    """A mask leaves nothing, and before that is read something else fails."""
+    eng = _engine()
+    s, (a, b), prompts = _session(eng, (40, 65))
+    before = _state(s)
+    with monkeypatch.context() as m:
+        _fails_at(m, "attention_paged", 2, RuntimeError)
+        with pytest.raises(RuntimeError, match="broken"):
+            s.generate([a, b], 9, allowed=ops.token_bits([], VOCAB, DEV))
+    assert _state(s) == before
+    chunk = _tokens(9, 5)
+    if then == "feed":
+        _close(s.feed({b: chunk})[b][0], eng.prefill(prompts[1] + chunk).logits[-1])
+    elif then == "add":
+        assert s.add(eng.prefill(chunk), chunk) == 2
+        _greedy_run(eng, chunk, s.generate([2], 5)[0], 5)
+    elif then == "fork":
+        (c,) = s.fork(b)
+        _greedy_run(eng, prompts[1], s.generate([c], 5)[0], 5)
+    else:
+        _greedy_run(eng, prompts[0], s.generate([a], 5)[0], 5)
+
+
+def test_ending_sequences_reads_its_own_flags():
+    eng = _engine()
+    s, (a, b), prompts = _session(eng, (40, 65))
+    s.cache.table[a, 1] = 10**6  # a broken book
+    with pytest.raises(RuntimeError, match="reported an error"):
+        s.free([a])
+    assert list(s.tokens) == [b] and s.cache.lengths.tolist()[:2] == [0, 65] and int(s._err.item()) == 0
+    _greedy_run(eng, prompts[1], s.generate([b], 5)[0], 5)
