@@ -211,7 +211,8 @@ class PagedSession:
 
         repetition, frequency, presence, bias, allowed: as ops.next_tokens takes them, rows in the order of `sequences`; a
         sequence's tokens before this call are its prompt, those of this call its generated ones. allowed may be a function of the
-        new tokens so far (a list for each sequence), called before each step, that returns the step's mask."""
+        new tokens so far (a list for each sequence), called before each step, that returns the step's mask; what that leaves a sequence
+        that ended is passed over."""
         order = self._known(sequences)
         if not order or max_tokens <= 0:
             return [[] for _ in order]
@@ -234,7 +235,8 @@ class PagedSession:
 
         def mask():
             m = allowed([out[by_slot.index(i)] for i in range(B)]) if callable(allowed) else allowed
-            return rows_of(m) if m.dim() == 2 else m
+            m = rows_of(m) if m.dim() == 2 else m
+            return m.expand(B, m.shape[-1]) if callable(allowed) else m  # one for all, or one each at another step
 
         if allowed is not None:
             masks = mask().clone()
@@ -259,6 +261,8 @@ class PagedSession:
             while live and steps < max_tokens:
                 if steps and callable(allowed):
                     masks.copy_(mask())
+                    if len(live) < B:  # what a mask leaves an ended sequence is no matter
+                        masks[[i for i in range(B) if i not in live]] = -1
                 if graph is not None:
                     graph.replay()
                 else:

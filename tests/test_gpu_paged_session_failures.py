@@ -138,3 +138,35 @@ def test_ending_sequences_reads_its_own_flags():
         s.free([a])
     assert list(s.tokens) == [b] and s.cache.lengths.tolist()[:2] == [0, 65] and int(s._err.item()) == 0
     _greedy_run(eng, prompts[1], s.generate([b], 5)[0], 5)
+
+
+@pytest.mark.parametrize("graphs", [True, False])
+@pytest.mark.parametrize("order", [(0, 1), (1, 0)])
+def test_a_mask_that_leaves_an_ended_sequence_nothing(graphs, order):
+    """The one sequence ends at its third token and its mask is empty from then on; the other's tokens are those it has where it is not."""
+    eng = _engine()
+    eng.decode_graphs = graphs
+    some, end, none = (ops.token_bits(t, VOCAB, DEV) for t in (range(7, 100), [0], []))
+    got = []
+    for behind in (none, some):
+        s, ids, _ = _session(eng, (20, 50))
+        calls = []
+
+        def allowed(outs):
+            calls.append(0)
+            return torch.stack([some if len(calls) < 3 else end if len(calls) == 3 else behind, some])
+
+        got.append(s.generate([ids[i] for i in order], 9, allowed=allowed))
+        assert len(got[-1][0]) == 2 and len(got[-1][1]) == 9 and len(calls) == 9
+    assert got[0] == got[1] and all(7 <= t < 100 for tokens in got[0] for t in tokens)
+
+
+def test_one_mask_for_all_may_become_one_each():
+    eng = _engine()
+    s, ids, _ = _session(eng, (20, 50))
+    some, end = ops.token_bits(range(7, 100), VOCAB, DEV), ops.token_bits([0], VOCAB, DEV)
+
+    def allowed(outs):
+        return some if len(outs[1]) < 2 else torch.stack([end, some]) if len(outs[1]) == 2 else some[None]
+
+    assert [len(t) for t in s.generate(ids, 6, allowed=allowed)] == [2, 6]
