@@ -212,7 +212,7 @@ class PagedSession:
         repetition, frequency, presence, bias, allowed: as ops.next_tokens takes them, rows in the order of `sequences`; a
         sequence's tokens before this call are its prompt, those of this call its generated ones. allowed may be a function of the
         new tokens so far (a list for each sequence), called before each step, that returns the step's mask; what that leaves a sequence
-        that ended is passed over."""
+        that ended is passed over. Where a mask leaves another nothing, the call raises at that step, and the sequences are what they were."""
         order = self._known(sequences)
         if not order or max_tokens <= 0:
             return [[] for _ in order]
@@ -246,7 +246,8 @@ class PagedSession:
         at = torch.zeros((B, 1), dtype=torch.int64, device=dev)
         counts = self._counts({s: 1 for s in slots})
         logits = torch.cat([self._logits[s] for s in slots])
-        tok = torch.empty(B, dtype=torch.int64, device=dev)
+        read = torch.zeros(B + 1, dtype=torch.int64, device=dev)  # what the host reads of a step: its tokens, and what it flagged
+        tok = read[:B]
 
         def step():
             ops.next_tokens(logits, prompt=prompt, generated=generated, allowed=masks, err=self._err, out=tok, **fixed)
@@ -254,6 +255,7 @@ class PagedSession:
             at.add_(1)
             h, pending, _ = self._forward(tok, counts, 1, [len(self.tokens[s]) + (max_tokens + 1) // 2 for s in slots])
             logits.copy_(self.engine._final_logits(h, pending)[0])
+            read[B:].copy_(self._err)
 
         before = {s: len(self.tokens[s]) for s in slots}
         live, graph, steps = set(range(B)), None, 0
@@ -272,13 +274,15 @@ class PagedSession:
                         with torch.cuda.graph(graph):
                             step()
                 steps += 1
-                for i, t in enumerate(tok.tolist()):
+                *new, flagged = read.tolist()
+                if flagged:
+                    self._check_err()
+                for i, t in enumerate(new):
                     if i in live:
                         if t in self.engine.eos:
                             live.discard(i)
                         else:
                             out[i].append(t)
-            self._check_err()
         self._go_back({s: before[s] + len(out[i]) for i, s in enumerate(slots)})  # every one took a row a step
         for i, s in enumerate(slots):
             self.tokens[s] = self.tokens[s] + out[i]

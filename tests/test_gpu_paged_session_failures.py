@@ -170,3 +170,21 @@ def test_one_mask_for_all_may_become_one_each():
         return some if len(outs[1]) < 2 else torch.stack([end, some]) if len(outs[1]) == 2 else some[None]
 
     assert [len(t) for t in s.generate(ids, 6, allowed=allowed)] == [2, 6]
+
+
+@pytest.mark.parametrize("graphs", [True, False])
+def test_a_mask_that_leaves_nothing_ends_the_call_at_its_step(graphs):
+    eng = _engine()
+    eng.decode_graphs = graphs
+    s, ids, prompts = _session(eng, (33, 50))
+    before, asked = _state(s), []
+
+    def allowed(outs):
+        asked.append([list(o) for o in outs])
+        return torch.stack([ops.token_bits(range(7, 100), VOCAB, DEV), ops.token_bits(range(7, 100) if len(asked) != 4 else [], VOCAB, DEV)])
+
+    with pytest.raises(ValueError, match="mask"):
+        s.generate(ids, 40, allowed=allowed)
+    assert _state(s) == before and len(asked) == 4
+    for p, tokens in zip(prompts, s.generate(ids, 8)):
+        _greedy_run(eng, p, tokens, 8)
