@@ -136,8 +136,9 @@ __global__ __launch_bounds__(kBookThreads) void extend_pages_kernel(int64_t* __r
       const int s = s0 + tid;
       uint64_t x[1] = {0}, total[1];
       if (s < b.S) {
-        x[0] = count_of(s, rows_of(b, s));
-        if (s_need[s + 1] > s_need[s] && s_need[s + 1] > free_pages) {
+        const int len = rows_of(b, s), c = count_of(s, len);
+        x[0] = c;
+        if (pages_of(len + c) > pages_of(len) && s_need[s + 1] > free_pages) {  // its own need, not s_need's step: that saturates
           x[0] = 0;
           flag_error(err, CKV_DEVICE_ERR_PAGES);
         }

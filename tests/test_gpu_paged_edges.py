@@ -1,0 +1,28 @@
+"""The paged cache's and the logits' operators at requests past what they count in, broken tables, infinities, and buffers that overlap."""
+
+import pytest
+import torch
+
+from chunkkv_amd import _native, ops
+from tests import paged_ref as R
+from tests.test_gpu_attention_paged import _batch, _check, _want
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+BF, I32, F32 = torch.bfloat16, torch.int32, torch.float32
+
+
+def _ints(v):
+    return torch.tensor(v, dtype=I32, device=DEV)
+
+
+def test_more_pages_asked_for_than_32_bits_count():
+    """65 sequences ask for 2^26 - 2 pages each, 2^32 and some together, of a pool of four; the one behind them for one: none grows."""
+    M, T, S = 2**26 - 1, 32, 66
+    k = torch.zeros((1, 1, 1, 4 * T, 64), dtype=BF, device=DEV)
+    c = ops.PagedCache(k, k.clone(), torch.empty((S, M), dtype=I32, device=DEV), torch.zeros(S, dtype=I32, device=DEV), torch.zeros(4, dtype=I32, device=DEV), T)
+    c.table[:, 0] = 3  # an entry from before
+    err = torch.zeros(1, dtype=I32, device=DEV)
+    got = ops.extend_pages(c, _ints([2**31 - 64] * 65 + [1]), 1, err)
+    assert int(err.item()) == _native.DEVICE_ERR_PAGES
+    assert got.rows.tolist() == [-1] and got.positions.tolist() == [0] and not got.starts.any() and not c.lengths.any() and not c.refs.any()
