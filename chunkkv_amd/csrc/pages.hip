@@ -85,6 +85,14 @@ __device__ __forceinline__ void each_page(const Book& b, F f) {
 
 __device__ __forceinline__ int rows_of(const Book& b, int s) { return min(max(b.lengths[s], 0), b.M << b.T_log); }
 
+// The pool's row of row `pos` of sequence s; -1, flagged, where the table names no page of the pool.
+__device__ __forceinline__ int64_t pool_row(const Book& b, int s, int64_t pos, int32_t* err) {
+  const int p = b.table[(int64_t)s * b.M + (pos >> b.T_log)];
+  if ((uint32_t)p < (uint32_t)b.P) return ((int64_t)p << b.T_log) + (pos & ((1 << b.T_log) - 1));
+  flag_error(err, CKV_DEVICE_ERR_RANGE);
+  return -1;
+}
+
 // Sequence s grows by counts[s] rows, or not at all (flagged): where the count is negative or past its table, the tokens
 // past n, or its pages past the free ones.
 __global__ __launch_bounds__(kBookThreads) void extend_pages_kernel(int64_t* __restrict__ positions, int64_t* __restrict__ rows,
@@ -182,7 +190,7 @@ __global__ __launch_bounds__(kBookThreads) void extend_pages_kernel(int64_t* __r
     if (i < total) {
       const int s = interval_of(s_start, b.S, (uint32_t)i);
       pos = rows_of(b, s) + i - (int)s_start[s];
-      row = ((int64_t)b.table[(int64_t)s * b.M + (pos >> b.T_log)] << b.T_log) + (pos & (T - 1));
+      row = pool_row(b, s, pos, err);
     }
     positions[i] = pos;
     rows[i] = row;
@@ -197,7 +205,8 @@ __global__ __launch_bounds__(kBookThreads) void extend_pages_kernel(int64_t* __r
 // The positions and rows of many tokens, after extend_pages_kernel without them (kRowsAlone).
 constexpr int kRowsThreads = 256, kRowsEach = 4;
 __global__ __launch_bounds__(kRowsThreads) void token_rows_kernel(int64_t* __restrict__ positions, int64_t* __restrict__ rows,
-                                                                  const int32_t* __restrict__ starts, int n, Book b) {
+                                                                  const int32_t* __restrict__ starts, int n, Book b,
+                                                                  int32_t* __restrict__ err) {
   __shared__ uint32_t s_start[kMostSequences + 1];
   for (int s = threadIdx.x; s <= b.S; s += kRowsThreads) s_start[s] = (uint32_t)starts[s];
   __syncthreads();
@@ -210,7 +219,7 @@ __global__ __launch_bounds__(kRowsThreads) void token_rows_kernel(int64_t* __res
     if (i < total) {
       const int s = interval_of(s_start, b.S, (uint32_t)i);
       pos = b.lengths[s] - (int64_t)s_start[s + 1] + i;
-      row = ((int64_t)b.table[(int64_t)s * b.M + (pos >> b.T_log)] << b.T_log) + (pos & ((1 << b.T_log) - 1));
+      row = pool_row(b, s, pos, err);
     }
     positions[i] = pos;
     rows[i] = row;
@@ -519,7 +528,7 @@ extern "C" int32_t ckv_extend_pages(int64_t* positions, int64_t* rows, int32_t* 
   if (alone) {
     constexpr int each = kRowsThreads * kRowsEach;
     hipLaunchKernelGGL(token_rows_kernel, dim3((unsigned)(((int64_t)n_new + each - 1) / each)), dim3(kRowsThreads), 0,
-                       (hipStream_t)stream, positions, rows, starts, n_new, b);
+                       (hipStream_t)stream, positions, rows, starts, n_new, b, err);
     CKV_RETURN_IF_LAUNCH_FAILED();
   }
   return CKV_OK;

@@ -654,7 +654,7 @@ int32_t ckv_evict_rows(void* k_out, int64_t ko_head_stride, void* v_out, int64_t
  * Sequence s grows by counts[s] rows (a whole prompt's, a chunk's, a token's, or 0): the pages it needs beyond those it has are
  * taken, lengths[s] becomes lengths[s] + counts[s], and for new token i of all, in the order of the sequences,
  *   positions[i]  its row of its sequence
- *   rows[i]       that row's place in the pool: table entry * page_tokens + row % page_tokens
+ *   rows[i]       that row's place in the pool: table entry * page_tokens + row % page_tokens (-1, flagged, where the table names no page)
  *   starts[s]     new tokens in front of sequence s's; starts[n_sequences]: all of them
  * n_new is the room of positions and rows; behind the last token positions are 0 and rows -1. What does not fit grows by nothing and
  * is flagged: a negative count or one past the table (CKV_DEVICE_ERR_RANGE), the first sequence whose tokens pass n_new and all behind it that have any

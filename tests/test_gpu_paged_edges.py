@@ -26,3 +26,22 @@ def test_more_pages_asked_for_than_32_bits_count():
     got = ops.extend_pages(c, _ints([2**31 - 64] * 65 + [1]), 1, err)
     assert int(err.item()) == _native.DEVICE_ERR_PAGES
     assert got.rows.tolist() == [-1] and got.positions.tolist() == [0] and not got.starts.any() and not c.lengths.any() and not c.refs.any()
+
+
+@pytest.mark.parametrize("page", [400, 999, -5, 2**31 - 1, -2**31])
+@pytest.mark.parametrize("more", [1, 5000])  # rows by the one launch, and by one of their own
+def test_rows_of_a_page_that_the_pool_does_not_have(page, more):
+    """A partial last page outside the pool: its new rows are -1 and flagged, the other sequences' are theirs."""
+    T, P = 32, 400
+    c = ops.paged_cache(1, P, 1, 64, 3, 6000, DEV, T)
+    err = torch.zeros(1, dtype=I32, device=DEV)
+    ops.extend_pages(c, _ints([70, 40, 0]), 110, err)
+    c.table[0, 2] = page
+    got = ops.extend_pages(c, _ints([30, more, 0]), 30 + more, err)
+    assert int(err.item()) == _native.DEVICE_ERR_RANGE
+    assert got.positions.tolist() == [*range(70, 100), *range(40, 40 + more)]
+    rows = got.rows.tolist()
+    assert rows[:26] == [-1] * 26
+    at = got.positions[26:]
+    of = torch.tensor([0] * 4 + [1] * more, device=DEV)
+    assert rows[26:] == (c.table[of, at // T].long() * T + at % T).tolist() and min(rows[26:]) >= 0
