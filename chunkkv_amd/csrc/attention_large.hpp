@@ -374,7 +374,7 @@ __global__ __launch_bounds__(kAttnWaves * 64) void attn_active_kernel(
       }
       continue;
     }
-    const float inv = PAGED && l == 0.f ? 0.f : 1.f / l;
+    const float inv = PAGED && my_pos[qg] < 0 ? 0.f : 1.f / l;
     char* orow = out + ((int64_t)t * Hq + h) * (D * 2);
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) {

@@ -244,10 +244,10 @@ __global__ __launch_bounds__(kPagedWaves * 64) void attn_paged_kernel(AttnMap ma
           prow[D + 1] = l;
         }
       } else {
-        const float inv = l == 0.f ? 0.f : 1.f / l;  // a row that sees nothing
+        const int t = div_by(m, group, b.inv_gqa);
+        const float inv = it.rows - it.count + t < 0 ? 0.f : 1.f / l;  // a row that sees nothing; scores of -inf alone give NaN
         x *= inv;
         y *= inv;
-        const int t = div_by(m, group, b.inv_gqa);
         *(vec16*)(out + ((int64_t)(it.first + t) * Hq + hk * group + m - t * group) * ROWB + col * 2) =
             vec16{f32x2_to_bf16x2_bits(x[0], x[1]), f32x2_to_bf16x2_bits(x[2], x[3]), f32x2_to_bf16x2_bits(y[0], y[1]),
                   f32x2_to_bf16x2_bits(y[2], y[3])};
@@ -380,7 +380,7 @@ __global__ __launch_bounds__(256) void join_paged_kernel(char* __restrict__ out,
         acc += s_o[w][lane] * e;
       }
     }
-    const float inv = L == 0.f ? 0.f : 1.f / L;
+    const float inv = parts <= 0 ? 0.f : 1.f / L;  // sees nothing
     if (!done)
       *(uint2*)(out + ((int64_t)t * Hq + h) * (D * 2) + col * 2) =
           uint2{f32x2_to_bf16x2_bits(acc[0] * inv, acc[1] * inv), f32x2_to_bf16x2_bits(acc[2] * inv, acc[3] * inv)};

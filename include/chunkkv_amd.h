@@ -707,10 +707,12 @@ int64_t ckv_compact_pages_workspace_bytes(int32_t n_pages); /* host-only */
 /*
  * Attention of new tokens over one layer of a paged cache: of sequence s's lengths[s] rows the last c = starts[s + 1] - starts[s] are new, and
  * its query i (token starts[s] + i of q and out) sees its rows up to lengths[s] - c + i: ckv_attention_active's function on the rows that the
- * table names, with its roundings. A query that sees no row (c above lengths[s]) gives zeros; tokens in front of starts[0] and from starts[n_sequences] on
+ * table names, with its roundings. A query that sees no row (c above lengths[s]) gives zeros, one whose scores are all
+ * -infinity NaN; tokens in front of starts[0] and from starts[n_sequences] on
  * are not written. starts ascends (ckv_extend_pages gives it); whatever it holds, nothing outside the arrays is touched.
  *   k_pool, v_pool  the layer's pool, (n_kv_heads, n_pages * page_tokens, head_dim), bf16, kv_head_stride elements between heads; rows of a
- *                   page behind its sequence's last may hold anything
+ *                   page behind its sequence's last may hold anything. Infinite values of its own rows may give NaN, as there: zero
+ *                   weights meet rows that a query does not see
  *   most_tokens, most_rows, total_rows  of the sequences with new tokens, if known, or about: the most tokens of one, the most rows of one, and
  *                   all of their rows (0: not known; n_tokens, n_entries * page_tokens and a part of that for each then); they choose the
  *                   kernel's form, not the result

@@ -45,3 +45,29 @@ def test_rows_of_a_page_that_the_pool_does_not_have(page, more):
     at = got.positions[26:]
     of = torch.tensor([0] * 4 + [1] * more, device=DEV)
     assert rows[26:] == (c.table[of, at // T].long() * T + at % T).tolist() and min(rows[26:]) >= 0
+
+
+@pytest.mark.parametrize("form", range(len(R.FORMS)))
+def test_rows_whose_scores_are_all_minus_infinity(form):
+    """They are NaN, as the softmax of -infinities is and as over a contiguous cache; a token that sees no row is zeros; others as ever."""
+    heads, seqs, most, known = R.FORMS[form]
+    q, cache, starts = _batch(heads, 64, seqs, seed=form)
+    q = q.clone(memory_format=torch.preserve_format)
+    q[..., 0] = 1.0
+    c, last = seqs[0][1], len(seqs) - 1
+    at = torch.arange(seqs[0][0], device=DEV)
+    rows = cache.table[0, at // 64].long() * 64 + at % 64
+    cache.k[0, 0, :, rows, 0] = float("-inf")
+    if last > 0:
+        cache.lengths[last] = 0  # its new tokens see no row
+    total = sum(r for r, _ in seqs) if known else None
+    got = ops.attention_paged(q, cache, 0, starts, most=most, total=total)
+    assert got[0, :c].isnan().all()
+    if last > 0:
+        assert not got[0, -seqs[-1][1]:].any()
+        middle = slice(c, got.shape[1] - seqs[-1][1])
+        if middle.stop > middle.start:
+            part = ops.PagedCache(cache.k, cache.v, cache.table[1:-1], cache.lengths[1:-1], cache.refs, 64)
+            _check(got[:, middle], _want(q[:, :, middle], part, seqs[1:-1]))
+    K, V = (x[0][:, :, rows].contiguous() for x in (cache.k, cache.v))
+    assert ops.attention_active(q[:, :, :c], K, V, at[-c:].contiguous()).isnan().all()
