@@ -921,6 +921,28 @@ PyObject* compact_pages(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
   CKV_PY_END
 }
 
+// Whether `out`, contiguous, and t have a byte in common: of t, what dimensions d and behind it have from address `at` on.
+bool meets(uintptr_t lo, uintptr_t hi, const Tensor& t, int64_t d, uintptr_t at) {
+  const int64_t e = t.element_size();
+  int64_t span = e, held = e;
+  for (int64_t i = d; i < t.dim(); ++i) {
+    if (t.stride(i) == 0) continue;  // the same bytes again
+    span += (t.size(i) - 1) * t.stride(i) * e;
+    held *= t.size(i);
+  }
+  if (at >= hi || at + (uintptr_t)span <= lo) return false;
+  if (held >= span || at >= lo) return true;  // no gaps, or its first element
+  const int64_t n = t.stride(d) == 0 ? 1 : t.size(d);
+  for (int64_t i = 0; i < n; ++i)
+    if (meets(lo, hi, t, d + 1, at + (uintptr_t)(i * t.stride(d) * e))) return true;
+  return false;
+}
+bool meets(const Tensor& out, const Tensor& t) {
+  if (!t.defined() || t.numel() == 0 || out.numel() == 0) return false;
+  const uintptr_t lo = (uintptr_t)out.data_ptr();
+  return meets(lo, lo + (uintptr_t)(out.numel() * out.element_size()), t, 0, (uintptr_t)t.data_ptr());
+}
+
 // attention_paged(q, table, lengths, refs, page_tokens, k, v, layer, starts, most, longest, total, scale, err, out, split)
 PyObject* attention_paged(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
   CKV_PY_BEGIN
@@ -952,6 +974,10 @@ PyObject* attention_paged(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
     same_device(q, out);
     if (out.sizes() != at::IntArrayRef({1, n, Hq, p.D}) || !out.is_contiguous() || out.scalar_type() != at::kBFloat16)
       value_error("out must be contiguous (1, n, Hq, D) bf16");
+    // token-major queries may be written over: the workgroup that writes a row has read it, and no other reads it
+    const bool in_place = out.data_ptr() == q.data_ptr() && step(q, 1, p.D) == p.D && step(q, 2, Hq * p.D) == Hq * p.D;
+    if ((!in_place && meets(out, q)) || meets(out, p.k) || meets(out, p.v) || meets(out, b.table) || meets(out, b.lengths) || meets(out, starts))
+      value_error("out overlaps q without being it, or the cache");
   }
   const double scale = a[12] == Py_None ? 1.0 / std::sqrt((double)p.D) : real(a[12]);
   const int split = PyObject_IsTrue(a[15]);

@@ -834,6 +834,7 @@ def attention_paged(
 
     q: (1, Hq, n, D) bf16 with contiguous rows; the cache bf16, D 64 or 128. Returns (1, n, Hq, D) bf16, token-major; a token that sees no row
     (more new tokens than rows) gives zeros, tokens outside [starts[0], starts[-1]) stay as they were in out (anything in a new tensor).
+    out overlaps neither the cache nor q, but may be q itself where a token's heads lie together.
     most, longest, total: the most new tokens of one sequence (1 in a decode step), the most rows of one that has any, and those of all that have any
     together, if known, or about: they choose the kernel's form, not the result. Without longest the table's width counts, which makes short
     sequences in a wide table slower.

@@ -709,7 +709,8 @@ int64_t ckv_compact_pages_workspace_bytes(int32_t n_pages); /* host-only */
  * its query i (token starts[s] + i of q and out) sees its rows up to lengths[s] - c + i: ckv_attention_active's function on the rows that the
  * table names, with its roundings. A query that sees no row (c above lengths[s]) gives zeros, one whose scores are all
  * -infinity NaN; tokens in front of starts[0] and from starts[n_sequences] on
- * are not written. starts ascends (ckv_extend_pages gives it); whatever it holds, nothing outside the arrays is touched.
+ * are not written. starts ascends (ckv_extend_pages gives it); whatever it holds, nothing outside the arrays is touched. out (n_tokens,
+ * n_q_heads, head_dim) overlaps no input, but may be q where that lies alike.
  *   k_pool, v_pool  the layer's pool, (n_kv_heads, n_pages * page_tokens, head_dim), bf16, kv_head_stride elements between heads; rows of a
  *                   page behind its sequence's last may hold anything. Infinite values of its own rows may give NaN, as there: zero
  *                   weights meet rows that a query does not see

@@ -71,3 +71,45 @@ def test_rows_whose_scores_are_all_minus_infinity(form):
             _check(got[:, middle], _want(q[:, :, middle], part, seqs[1:-1]))
     K, V = (x[0][:, :, rows].contiguous() for x in (cache.k, cache.v))
     assert ops.attention_active(q[:, :, :c], K, V, at[-c:].contiguous()).isnan().all()
+
+
+@pytest.mark.parametrize("most", [1, 40])
+@pytest.mark.parametrize("seqs", [[(700, 1), (40, 1)], [(900, 40), (2000, 3)], [(3000, 300)]])
+def test_attention_into_a_buffer_that_it_reads_is_refused(seqs, most):
+    """Its queries alone may be written over, where each is."""
+    hq, _, d = heads = (14, 2, 64)
+    q, cache, starts = _batch(heads, 64, seqs, seed=2)
+    n = q.shape[2]
+    want = ops.attention_paged(q, cache, 0, starts, most=most)
+    size = n * hq * d
+    for t in (cache.k, cache.v):
+        for at in (0, t.numel() - size):
+            if 0 <= at:
+                with pytest.raises(ValueError, match="overlap"):
+                    ops.attention_paged(q, cache, 0, starts, most=most, out=t.view(-1)[at:at + size].view(1, n, hq, d))
+    room = torch.zeros(3 * size, dtype=BF, device=DEV)
+    held = room[size:2 * size].view(1, n, hq, d)
+    held.copy_(q.transpose(1, 2))
+    for at in (size - 8, size + 8, 2 * size - 8, 8):
+        with pytest.raises(ValueError, match="overlap"):
+            ops.attention_paged(held.transpose(1, 2), cache, 0, starts, most=most, out=room[at:at + size].view(1, n, hq, d))
+    for at in (0, 2 * size):
+        out = room[at:at + size].view(1, n, hq, d)
+        assert torch.equal(ops.attention_paged(held.transpose(1, 2), cache, 0, starts, most=most, out=out), want)
+    assert ops.attention_paged(held.transpose(1, 2), cache, 0, starts, most=most, out=held).data_ptr() == held.data_ptr() and torch.equal(held, want)
+    held.copy_(q.transpose(1, 2))
+    if n > 1:
+        with pytest.raises(ValueError, match="overlap"):  # heads first: another query is where a result goes
+            ops.attention_paged(held.view(1, hq, n, d), cache, 0, starts, most=most, out=held)
+
+
+def test_attention_beside_its_queries_in_one_buffer_is_accepted():
+    """Queries in a wider buffer's columns, the results in what lies between two of its rows: no byte is shared."""
+    heads = (4, 2, 64)
+    q, cache, starts = _batch(heads, 64, [(300, 2)], seed=2)
+    want = ops.attention_paged(q, cache, 0, starts)
+    room = torch.zeros((2, 6 * 64 * 4), dtype=BF, device=DEV)
+    view = room[:, :256].view(1, 2, 4, 64).transpose(1, 2)
+    view.copy_(q)
+    out = room[0, 512:1024].view(1, 2, 4, 64)
+    assert torch.equal(ops.attention_paged(view, cache, 0, starts, out=out), want)
