@@ -1079,11 +1079,14 @@ PyObject* adjust_logits(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
     same_device(r.logits, out);
     if (out.sizes() != r.logits.sizes() || !out.is_contiguous() || out.scalar_type() != at::kFloat)
       value_error("out must be contiguous (rows, vocab) float32");
-    // float32 logits may be adjusted in place: a thread reads what it writes
-    const uintptr_t o = (uintptr_t)out.data_ptr(), l = (uintptr_t)r.logits.data_ptr(), e = (uintptr_t)r.logits.element_size();
-    const uintptr_t o_end = o + (uintptr_t)out.numel() * 4, l_end = r.rows == 0 ? l : l + ((r.rows - 1) * r.row_stride + r.vocab) * e;
-    const bool in_place = o == l && r.code == CKV_DTYPE_F32 && (r.rows <= 1 || r.row_stride == r.vocab);
-    if (!in_place && o < l_end && l < o_end) value_error("out overlaps the logits without being them");
+    // float32 logits, or a bias of each row, may be where the result goes: a thread reads what it writes
+    auto there = [&](const Tensor& t) {
+      return t.data_ptr() == out.data_ptr() && t.scalar_type() == at::kFloat && t.size(0) == r.rows && step(t, 0, r.vocab) == r.vocab;
+    };
+    if (!there(r.logits) && meets(out, r.logits)) value_error("out overlaps the logits without being them");
+    if (r.bias.defined() && !there(r.bias) && meets(out, r.bias)) value_error("out overlaps the bias without being it");
+    for (const Tensor* t : {&r.prompt, &r.generated, &r.repetition, &r.frequency, &r.presence, &r.allowed})
+      if (meets(out, *t)) value_error("out overlaps what the logits are adjusted by");
   }
   check(unlocked([&] {
           const c10::DeviceGuard on(r.logits.device());
@@ -1101,6 +1104,7 @@ PyObject* next_tokens(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
   const LogitArgs r = logit_args(a);
   const Tensor err = optional_tensor(a[8]);
   int32_t* const e = status_word(err, r.logits);
+  const int64_t ws_bytes = ckv_next_tokens_workspace_bytes(int32(r.rows), int32(r.vocab));
   Tensor out = optional_tensor(a[9]);
   if (!out.defined()) {
     out = new_tensor({r.rows}, at::kLong, r.logits);
@@ -1108,8 +1112,11 @@ PyObject* next_tokens(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
     same_device(r.logits, out);
     if (out.sizes() != at::IntArrayRef({r.rows}) || !out.is_contiguous() || out.scalar_type() != at::kLong)
       value_error("out must be contiguous (rows,) int64");
+    // with a workspace a second launch writes the tokens; without it a row's workgroup does, when it has read all of its row
+    if (ws_bytes == 0 && r.rows > 1)
+      for (const Tensor* t : {&r.logits, &r.prompt, &r.generated, &r.repetition, &r.frequency, &r.presence, &r.bias, &r.allowed})
+        if (meets(out, *t)) value_error("out overlaps what the tokens are chosen from");
   }
-  const int64_t ws_bytes = ckv_next_tokens_workspace_bytes(int32(r.rows), int32(r.vocab));
   Tensor ws;
   if (ws_bytes > 0) ws = new_tensor({ws_bytes / 8}, at::kLong, r.logits);
   check(unlocked([&] {

@@ -862,7 +862,8 @@ def adjust_logits(
 
     prompt, generated: int64 (rows, tokens); tokens outside the vocabulary (padding, -1) are passed over. repetition (> 0), frequency, presence: a number
     or float32 (rows,). bias: float32 (vocab,) or (rows, vocab). allowed: int32 (ceil(vocab / 32),) for all rows or one each, bit v % 32 of
-    word v // 32 set where token v may come (token_bits). out may be the logits themselves, if they are float32.
+    word v // 32 set where token v may come (token_bits). out overlaps no input, but may be the logits themselves, if they are float32, or a bias of
+    each row.
     """
     return _native.torch_ops().adjust_logits(logits, prompt, generated, repetition, frequency, presence, bias, allowed, out)
 
@@ -881,7 +882,8 @@ def next_tokens(
     out: torch.Tensor | None = None,
 ) -> torch.Tensor:
     """adjust_logits(...).argmax(1), int64 (rows,), without writing the adjusted logits: the first of the largest, a NaN above every number.
-    A row of -inf alone gives 0 and sets err (_native.DEVICE_ERR_NO_TOKEN)."""
+    A row of -inf alone gives 0 and sets err (_native.DEVICE_ERR_NO_TOKEN). out overlaps no input, unless there is one row or a vocabulary
+    above 4096 (a row's token may go behind its own history)."""
     return _native.torch_ops().next_tokens(logits, prompt, generated, repetition, frequency, presence, bias, allowed, err, out)
 
 

@@ -740,7 +740,8 @@ int64_t ckv_attention_paged_workspace_bytes(int32_t n_tokens, int32_t n_sequence
  *   x = x - frequency * c - presence                (c > 0)
  *   x = x + bias[v]                                 (bias given)
  *   x = -infinity, whatever x is                    (allowed given and bit v % 32 of its word v / 32 not set)
- * in fp32, each step rounded once, from left to right; out is (n_rows, vocab) f32 contiguous.
+ * in fp32, each step rounded once, from left to right; out is (n_rows, vocab) f32 contiguous and overlaps no input, but may be f32
+ * logits, or a bias of each row, that lie alike.
  *   prompt, generated   (n_rows, n_prompt or n_generated) int64 tokens; those outside [0, vocab) (padding) are passed over; counts 0: none
  *   *_rows              a value for each row, or NULL: the value beside it for all
  *   bias                (vocab) for each row, or one for all (row stride 0), f32; NULL: none
@@ -758,6 +759,7 @@ int32_t ckv_adjust_logits(float* out, const void* logits, int64_t logits_row_str
 /*
  * The greedy token of the logits that ckv_adjust_logits gives, which are not written: tokens[row] = the first of the largest, a NaN above
  * every number (torch.argmax). A row of -infinity alone gives 0 and is flagged (CKV_DEVICE_ERR_NO_TOKEN).
+ * tokens overlaps no input where n_rows is above 1 and no workspace is needed (a row's workgroup writes its token then).
  *   workspace  device buffer of workspace_bytes >= ckv_next_tokens_workspace_bytes(...) (8-byte aligned)
  * Up to two launches.
  */

@@ -113,3 +113,64 @@ def test_attention_beside_its_queries_in_one_buffer_is_accepted():
     view.copy_(q)
     out = room[0, 512:1024].view(1, 2, 4, 64)
     assert torch.equal(ops.attention_paged(view, cache, 0, starts, out=out), want)
+
+
+@pytest.mark.parametrize("vocab", [1000, 5000])
+def test_logits_into_a_buffer_that_they_are_made_from_are_refused(vocab):
+    g = torch.Generator().manual_seed(1)
+    logits = torch.randn((3, vocab), generator=g).to(BF).to(DEV)
+    room = torch.zeros(8 * vocab, device=DEV)
+    out = room[vocab:4 * vocab].view(3, vocab)
+    ids = torch.randint(0, vocab, (3, 10), generator=g).to(DEV)
+
+    def inside(at, x):
+        """x's values in the room, `at` elements of fp32 from its front."""
+        view = room[at:at + x.numel() * x.element_size() // 4].view(x.dtype).view(x.shape)
+        view.copy_(x)
+        return view
+
+    bias = torch.randn((3, vocab), generator=g).to(DEV)
+    words = -(-vocab // 32)
+    bits = torch.randint(-2**31, 2**31, (3, words), generator=g).to(I32).to(DEV)
+    rows = torch.rand(3, generator=g).to(DEV)
+    for at in (vocab, 2 * vocab + 4, 4 * vocab - 2):
+        for kw in (dict(prompt=ids), dict(generated=ids), dict(repetition=rows + 1, prompt=ids), dict(frequency=rows, generated=ids), dict(presence=rows, generated=ids),
+                   dict(bias=bias[0]), dict(bias=bias), dict(allowed=bits[0]), dict(allowed=bits)):
+            name = next(iter(kw))
+            if name == "bias" and kw[name].dim() == 2 and at == vocab:
+                continue  # where the result goes: below
+            with pytest.raises(ValueError, match="overlap"):
+                ops.adjust_logits(logits, out=out, **dict(kw, **{name: inside(at, kw[name])}))
+    # a bias of each row where that row's result goes is read first, as float32 logits are; one row's for one row too
+    want = ops.adjust_logits(logits, bias=bias)
+    assert torch.equal(ops.adjust_logits(logits, bias=inside(vocab, bias), out=out), want)
+    want = ops.adjust_logits(logits[:1], bias=bias[0])
+    assert torch.equal(ops.adjust_logits(logits[:1], bias=inside(vocab, bias[0]), out=out[:1]), want)
+    # beside it
+    want = ops.adjust_logits(logits, bias=bias[0], prompt=ids, repetition=2.0)
+    assert torch.equal(ops.adjust_logits(logits, bias=inside(0, bias[0]), prompt=inside(4 * vocab, ids), repetition=2.0, out=out), want)
+
+
+@pytest.mark.parametrize("vocab", [1000, 5000])
+def test_tokens_into_a_buffer_that_they_are_chosen_from(vocab):
+    """A row's token may go behind its own history; rows of one slice of the vocabulary end in any order, so over others' histories only where a second
+    launch writes the tokens."""
+    g = torch.Generator().manual_seed(1)
+    logits = torch.randn((3, vocab), generator=g).to(BF).to(DEV)
+    logits[:, 7] = 9.0
+    ids = torch.randint(0, vocab, (3, 10), generator=g).to(DEV)
+    ids[:, 4] = 7
+    want = ops.next_tokens(logits, generated=ids, presence=20.0)
+    for i in range(3):
+        one = ids[i:i + 1].clone()
+        assert ops.next_tokens(logits[i:i + 1], generated=one, presence=20.0, out=one[0, 4:5]).item() == want[i] == one[0, 4]
+    for at in (0, 9, 27):
+        held = ids.clone()
+        call = lambda: ops.next_tokens(logits, generated=held, presence=20.0, out=held.view(-1)[at:at + 3])  # noqa: E731
+        if vocab > 4096:
+            assert torch.equal(call(), want)
+        else:
+            with pytest.raises(ValueError, match="overlap"):
+                call()
+    wide = ids.t().contiguous()  # tokens first: a step's tokens lie together
+    assert torch.equal(ops.next_tokens(logits, generated=wide.t(), presence=20.0, out=wide[4]), want) and torch.equal(wide[4], want)
