@@ -45,6 +45,7 @@ struct Adjust {
 constexpr int kLogitsThreads = 512, kLogitsEach = 8;  // logits of a thread
 constexpr int kLogitsSlice = kLogitsThreads * kLogitsEach;
 constexpr uint32_t kInPrompt = 1u << 31;
+constexpr int kPairsEach = 4, kPairsStep = kPairsEach * kLogitsThreads;  // pairs of tokens that a thread, a workgroup, has in flight
 
 // Counts the row's tokens that lie in [v0, v0 + kLogitsSlice) into count[]: occurrences in generated, kInPrompt where it is in the prompt. Both
 // lists are one of pairs, whose loads go out U at a time for each thread, the last of them too (past the end they read the last pair
@@ -53,14 +54,14 @@ __device__ __forceinline__ void count_tokens(const Tokens& prompt, const Tokens&
   const int64_t* pt = prompt.at + row * prompt.stride;
   const int64_t* gt = generated.at + row * generated.stride;
   const int pp = prompt.n / 2, pairs = pp + generated.n / 2;
-  constexpr int NT = kLogitsThreads, U = 4;
+  constexpr int NT = kLogitsThreads, U = kPairsEach;
   auto take = [&](int64_t v, bool in_prompt) {
     const uint64_t o = (uint64_t)v - (uint64_t)v0;  // any token
     if (o >= (uint64_t)kLogitsSlice) return;
     if (in_prompt) atomicOr(&count[o], kInPrompt);
     else atomicAdd(&count[o], 1u);
   };
-  for (int i0 = 0; i0 < pairs; i0 += U * NT) {
+  for (int i0 = 0; i0 < pairs; i0 += kPairsStep) {
     vec16 v[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
@@ -254,6 +255,7 @@ static int32_t check_adjust(const void* logits, int64_t row_stride, int32_t n_ro
   if ((uintptr_t)a.bias % 4 || (uintptr_t)a.allowed % 4) return CKV_ERR_INVALID_ARGUMENT;
   if (n_rows > 1 && (row_stride < vocab || a.bias_stride < 0 || a.allowed_stride < 0)) return CKV_ERR_OUT_OF_RANGE;
   if (n_rows > 65535 || vocab > INT32_MAX - kLogitsSlice) return CKV_ERR_TOO_LARGE;
+  if ((int64_t)a.prompt.n / 2 + a.generated.n / 2 > INT32_MAX - kPairsStep) return CKV_ERR_TOO_LARGE;  // count_tokens' numbers
   return CKV_OK;
 }
 

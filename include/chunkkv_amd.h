@@ -746,7 +746,8 @@ int64_t ckv_attention_paged_workspace_bytes(int32_t n_tokens, int32_t n_sequence
  *   *_rows              a value for each row, or NULL: the value beside it for all
  *   bias                (vocab) for each row, or one for all (row stride 0), f32; NULL: none
  *   allowed             (ceil(vocab / 32)) words for each row or for all; NULL: every token is
- * Row strides in elements. Nothing need be aligned beyond its elements. n_rows at most 65535. One launch.
+ * Row strides in elements. Nothing need be aligned beyond its elements. n_rows at most 65535, n_prompt + n_generated at most 2^32 - 4098
+ * (CKV_ERR_TOO_LARGE). One launch.
  * No counterpart in the reference, whose decode takes the argmax of the model's logits (torch_engine.py:197).
  */
 int32_t ckv_adjust_logits(float* out, const void* logits, int64_t logits_row_stride, int32_t n_rows, int32_t vocab, int32_t dtype,
