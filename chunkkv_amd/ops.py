@@ -799,7 +799,8 @@ def extend_pages(cache: PagedCache, counts: torch.Tensor, n: int, err: torch.Ten
 
 def fork_pages(cache: PagedCache, sources: torch.Tensor, targets: torch.Tensor, err: torch.Tensor | None = None) -> None:
     """Sequence targets[i] (int32, empty so far) continues sequence sources[i]: whole pages are shared, the partial last one is copied, in
-    every layer. Pairs that cannot be taken (a target with rows, named twice, no free page) are left out, and err is set."""
+    every layer. Sources are read as they were when the call began: a target of the same call is an empty one. Pairs that cannot be taken (a
+    target with rows, named twice, no free page) are left out, and err is set."""
     _native.torch_ops().fork_pages(cache.table, cache.lengths, cache.refs, cache.page_tokens, cache.k, cache.v, sources, targets, err)
 
 

@@ -667,7 +667,8 @@ int32_t ckv_extend_pages(int64_t* positions, int64_t* rows, int32_t* starts, int
 
 /*
  * Sequence targets[i] continues sequence sources[i]: it shares its whole pages (refs + 1) and gets a copy of its partial last
- * one, of every layer, in a free page. Pairs are taken in order; one whose target has rows, is its source, or was
+ * one, of every layer, in a free page. Free pages go to the pairs in order; sequences are read as they were when the call began, so a
+ * source that is another pair's target is an empty one, and its own target stays empty. A pair whose target has rows, is its source, or was
  * named before, or that names no sequence, is left out and flagged (CKV_DEVICE_ERR_RANGE), as is the first that finds no free page and all
  * behind it that need one (CKV_DEVICE_ERR_PAGES). k_pool, v_pool: (n_layers, n_heads, n_pages * page_tokens, head_dim) with the given strides
  * (elements, 16-byte multiples); head_dim 64, 128 or 256.
