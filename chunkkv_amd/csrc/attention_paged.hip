@@ -1,11 +1,12 @@
-// Attention of new tokens, one or a chunk a sequence, over a paged cache (pages.hip): query i of a sequence's c new tokens,
-// of its `rows` cached ones the last c, sees its rows j <= p = rows - c + i:
+// Attention of new tokens, one or a chunk a sequence, over a paged cache (pages.hip): query i of a sequence's c new
+// tokens, of its `rows` cached ones the last c, sees its rows j <= p = rows - c + i:
 //   out = sum_j w_j V[row(j)] / sum_j w_j,  w_j = exp(scale q . K[row(j)]),  row(j) = table[j / T] T + j % T
 // in attention.hip's manner (scores, softmax and sums in fp32, weights rounded to bf16 for the second product).
 //
 //  - Tiles of 16 or 32 (token, query head) rows of a sequence's KV head, decode among them: attn_paged_kernel below.
-//  - Of 128, where many tokens fill the card: attention_large.hpp's workgroups, with splits of the cache where they are few. 4096 tokens over 32832 rows, 28 / 4 heads of
-//    128, 1.67 ms: 1.08 PFLOP/s, as fast as that kernel over one contiguous cache (1.83 on the card where this took 1.78).
+//  - Of 128, where many tokens fill the card: attention_large.hpp's workgroups, with splits of the cache where they are
+//    few. 4096 tokens over 32832 rows, 28 / 4 heads of 128, 1.67 ms: 1.08 PFLOP/s, as fast as that kernel over one
+//    contiguous cache (1.83 on the card where this took 1.78).
 // attention_paged.hpp says how the work is shared out, attention_paged_plan.hpp by which rule.
 #include <algorithm>
 
@@ -14,12 +15,14 @@
 namespace ckv {
 
 // ---- few rows of a sequence ------------------------------------------------------------------------------------
-// A workgroup streams its share of the units, a unit of 128 cached rows a step of its four wavefronts, for one tile of 16 QG
-// (token, query head) rows after the other: mostly a part of one sequence, or the end of one and the beginning of the next. Each wavefront takes
-// every fourth chunk of 32 rows with a softmax of its own (no barrier in the loop), loads it straight into LDS, two stages, and the four
-// results meet in LDS behind a tile's last chunk. A chunk lies within a page; the pages of a wavefront's next 64 chunks are held
-// a chunk a lane. Bound: the cache's bytes; for one short sequence the chain of its loads. Traced, 28 / 4 heads of 128: one token over 8302 rows
-// 7.1 us (17 MB; the join 3.9), 28 sequences' over 97000 rows together 33.0 (199 MB, 6.0 TB/s, part of them in the memory-side cache; the join 4.7).
+// A workgroup streams its share of the units, a unit of 128 cached rows a step of its four wavefronts, for one tile of
+// 16 QG (token, query head) rows after the other: mostly a part of one sequence, or the end of one and the beginning of
+// the next. Each wavefront takes every fourth chunk of 32 rows with a softmax of its own (no barrier in the loop),
+// loads it straight into LDS, two stages, and the four results meet in LDS behind a tile's last chunk. A chunk lies
+// within a page; the pages of a wavefront's next 64 chunks are held a chunk a lane. Bound: the cache's bytes; for one
+// short sequence the chain of its loads. Traced, 28 / 4 heads of 128: one token over 8302 rows 7.1 us (17 MB; the join
+// 3.9), 28 sequences' over 97000 rows together 33.0 (199 MB, 6.0 TB/s, part of them in the memory-side cache; the join
+// 4.7).
 template <int D, int QG, bool MANY>
 __global__ __launch_bounds__(kPagedWaves * 64) void attn_paged_kernel(AttnMap map, PagedRows b, int n, const char* __restrict__ kc,
                                                                       const char* __restrict__ vc, int64_t kv_hs_b,
@@ -203,8 +206,8 @@ __global__ __launch_bounds__(kPagedWaves * 64) void attn_paged_kernel(AttnMap ma
       if (c < c_end) body(lds1, lds0);
     }
 
-    // Join the wavefronts: each scales its rows to the common maximum and leaves them in the first stage's place, column
-    // group j of row r at j ^ r % 8 of its eighths.
+    // Join the wavefronts: each scales its rows to the common maximum and leaves them in the first stage's place,
+    // column group j of row r at j ^ r % 8 of its eighths.
 #pragma unroll
     for (int qg = 0; qg < QG; ++qg)
       if (g == 0) s_m[wave][qg * 16 + lm] = m_run[qg];
@@ -258,12 +261,15 @@ __global__ __launch_bounds__(kPagedWaves * 64) void attn_paged_kernel(AttnMap ma
 }
 
 // ---- the partial rows joined -----------------------------------------------------------------------------------
-// D / 4 lanes have a (token, query head) row's columns, so a wavefront has JH = 64 / (D / 4) heads of a token side by side and nothing
-// crosses its lanes; it goes through their partial rows, some in flight. Finding the token's items costs as many instructions as a few rows,
-// and instructions are what a launch of many rows waits for, so such launches (WPR = 1) give a wavefront kJoinTurns times JH heads; those of few rows
-// and more splits (WPR = 4) spread a row's partials over four wavefronts. Partials past the row's position are not read. Rows of
-// tiles that were whole are written already. kJoinSpread: 40 partials at once; one round fewer of a sequence of 8302 rows, which has 33 (one token, 28 / 4
-// heads of 128, 11.6 us in place of 12.0 with 32 at once, 14 / 2 of 64 9.2 and 9.7; 48 cost those with fewer partials 0.1, 64 0.3).
+// D / 4 lanes have a (token, query head) row's columns, so a wavefront has JH = 64 / (D / 4) heads of a token side by
+// side and nothing crosses its lanes; it goes through their partial rows, some in flight. Finding the token's items
+// costs as many instructions as a few rows, and instructions are what a launch of many rows waits for, so such launches
+// (WPR = 1) give a wavefront kJoinTurns times JH heads; those of few rows and more splits (WPR = 4) spread a row's
+// partials over four wavefronts. Partials past the row's position are not read. Rows of tiles that were whole are
+// written already. kJoinSpread: 40 partials at once. 32 in its place take a round more of 33 to 40 of them: one token
+// over 8302 rows, 28 / 4 heads of 128, 11.95 us for 11.45, over 10000 12.6 for 11.9 (14 / 2 of 64 9.7 for 9.2, 9.9 for
+// 9.3); with fewer or more of them they take 0.0-0.15 less (2000 rows 9.7 and 9.75, 5000 10.75 and 10.85, 12000 12.9
+// and 13.05, 32000 20.1 and 20.2).
 constexpr int kJoinTurns = 2, kJoinInFlight = 8, kJoinSpread = 10;
 template <int D>
 constexpr int kJoinHeads = 256 / D;
@@ -296,7 +302,8 @@ __global__ __launch_bounds__(256) void join_paged_kernel(char* __restrict__ out,
   for (int turn = 0; turn < TURNS; ++turn) {
     const int h = ((int)blockIdx.y * TURNS + turn) * JH + sub, hc = min(h, Hq - 1), hk = div_by(hc, group, b.inv_gqa);
     const int m = (t - it.first) * group + hc - hk * group, tile = m / ROWS;
-    // Partial z of the row is at slot + (z > 0 ? later + z * step : 0), for z < parts; done: the row is written already.
+    // Partial z of the row is at slot + (z > 0 ? later + z * step : 0), for z < parts; done: the row is written
+    // already.
     int64_t slot, later = 0, step;
     int parts, most;  // most: of the wavefront's rows
     bool done = h >= Hq;

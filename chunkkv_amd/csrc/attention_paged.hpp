@@ -4,11 +4,11 @@
 // New tokens are ragged over the sequences and only the device knows the lengths, so a launch is sized by what the host
 // knows (tokens, sequences) and shared out on the device. The rows of a KV head are the (token, query head) pairs of a
 // sequence, cut into tiles of ROWS; a tile's part of the cache is its units of UNIT rows. Two ways of sharing:
-//  - Tiles of 16 or 32 rows: all units of all tiles in a row, in equal shares (PagedShare), so that every workgroup reads as much of the
-//    cache whatever the lengths are. A tile that lies in several shares has a partial row in each.
-//  - Tiles of 128: items of a tile and a split of its units (paged_item), as long as all the work over the workgroups that the launch aims
-//    at, numbered by (sequence, split, tile), tiles from a sequence's last. Workgroups without an item come last in the grid: in front they
-//    held CUs that the others waited for.
+//  - Tiles of 16 or 32 rows: all units of all tiles in a row, in equal shares (PagedShare), so that every workgroup
+//    reads as much of the cache whatever the lengths are. A tile that lies in several shares has a partial row in each.
+//  - Tiles of 128: items of a tile and a split of its units (paged_item), as long as all the work over the workgroups
+//    that the launch aims at, numbered by (sequence, split, tile), tiles from a sequence's last. Workgroups without an
+//    item come last in the grid: in front they held CUs that the others waited for.
 // Each wavefront finds its own part by a prefix sum over the sequences.
 #pragma once
 
@@ -86,9 +86,9 @@ struct PagedWalk {
 };
 
 // ---- equal shares of units -------------------------------------------------------------------------------------
-// Where shares that keep tiles apart would be hardly longer (one unit, of which a launch of little work has few), they do: ending a tile and
-// beginning the next costs a workgroup more than a microsecond. A launch without splits takes whole tiles. Counts fit 32 bits (the plan
-// sees to it).
+// Where shares that keep tiles apart would be hardly longer (one unit, of which a launch of little work has few), they
+// do: ending a tile and beginning the next costs a workgroup more than a microsecond. A launch without splits takes
+// whole tiles. Counts fit 32 bits (the plan sees to it).
 template <int ROWS, int UNIT, bool MANY>
 struct PagedShare {
   const PagedWalk<ROWS, UNIT, MANY> walk;

@@ -7,16 +7,17 @@
 // in fp32, each step rounded once. The token is the first of the largest (a NaN above every number, as torch's argmax).
 //
 // A workgroup has a slice of a row's vocabulary: it counts the row's tokens that fall into the slice in LDS (integer
-// atomics: any order gives the same counts), while its logits are on their way, then reads each logit once.
-// No table of counts over the vocabulary exists in memory, so there is no state to keep, and a step reads the logits and
-// the tokens. Bound: latency up to a few rows (one row of 152064 behind 8302 + 256 tokens 6.0 us traced and 1.4 for the joined slices: 8.4 in a graph),
-// the logits' bytes and the result's beyond (64 rows under a grammar with a bias, 61 MB, 15.4 us: 4.0 TB/s).
+// atomics: any order gives the same counts), while its logits are on their way, then reads each logit once. No table of
+// counts over the vocabulary exists in memory, so there is no state to keep, and a step reads the logits and the
+// tokens. Bound: latency up to a few rows (one row of 152064 behind 8302 + 256 tokens 6.0 us traced and 1.4 for the
+// joined slices: 8.4 in a graph), the logits' bytes and the result's beyond (64 rows under a grammar with a bias, 61
+// MB, 15.4 us: 4.0 TB/s).
 #include "attention_common.hpp"
 
 namespace ckv {
 
-// Sixteen bytes wherever an element may lie. Loads and stores here are of this kind: rows of an odd vocabulary start anywhere, and the
-// device takes 16 bytes at any address.
+// Sixteen bytes wherever an element may lie. Loads and stores here are of this kind: rows of an odd vocabulary start
+// anywhere, and the device takes 16 bytes at any address.
 __device__ __forceinline__ vec16 ld16_any(const void* p) {
   vec16 v;
   __builtin_memcpy(&v, p, 16);
@@ -47,9 +48,9 @@ constexpr int kLogitsSlice = kLogitsThreads * kLogitsEach;
 constexpr uint32_t kInPrompt = 1u << 31;
 constexpr int kPairsEach = 4, kPairsStep = kPairsEach * kLogitsThreads;  // pairs of tokens that a thread, a workgroup, has in flight
 
-// Counts the row's tokens that lie in [v0, v0 + kLogitsSlice) into count[]: occurrences in generated, kInPrompt where it is in the prompt. Both
-// lists are one of pairs, whose loads go out U at a time for each thread, the last of them too (past the end they read the last pair
-// again, which is passed over).
+// Counts the row's tokens that lie in [v0, v0 + kLogitsSlice) into count[]: occurrences in generated, kInPrompt where
+// it is in the prompt. Both lists are one of pairs, whose loads go out U at a time for each thread, the last of them
+// too (past the end they read the last pair again, which is passed over).
 __device__ __forceinline__ void count_tokens(const Tokens& prompt, const Tokens& generated, int row, int64_t v0, uint32_t* count) {
   const int64_t* pt = prompt.at + row * prompt.stride;
   const int64_t* gt = generated.at + row * generated.stride;
@@ -112,8 +113,9 @@ __device__ __forceinline__ void store_token(int64_t* to, uint64_t key, int32_t* 
   if ((uint32_t)(key >> 32) == kNegInf) flag_error(err, CKV_DEVICE_ERR_NO_TOKEN);
 }
 
-// WRITE: the adjusted logits to out; else each slice's best key to keys, or the token where a row is one slice. A thread's logits are
-// vectors of W, a workgroup's threads side by side: 16 bytes of what is written, or else of what is read.
+// WRITE: the adjusted logits to out; else each slice's best key to keys, or the token where a row is one slice. A
+// thread's logits are vectors of W, a workgroup's threads side by side: 16 bytes of what is written, or else of what is
+// read.
 template <typename E, bool WRITE>
 __global__ __launch_bounds__(kLogitsThreads) void adjust_logits_kernel(const char* __restrict__ logits, int64_t row_b, int V, Adjust a,
                                                                        float* __restrict__ out, uint64_t* __restrict__ keys,

@@ -1,18 +1,19 @@
 // The pages of a cache that several sequences share (no counterpart in the reference): sequences grow, continue one
-// another, end, and the pages that stay move together, all on the device, so that a captured decode step takes its pages
-// itself and nothing is read back.
+// another, end, and the pages that stay move together, all on the device, so that a captured decode step takes its
+// pages itself and nothing is read back.
 //
-// A pool is an ordinary cache (layers, heads, pages * page_tokens, head_dim): page p is the rows [p * page_tokens,
-// (p + 1) * page_tokens) of every layer and head, so the kernels that write rows of a cache write into pages as they are.
+// A pool is an ordinary cache (layers, heads, pages * page_tokens, head_dim): page p is the rows [p * page_tokens, (p +
+// 1) * page_tokens) of every layer and head, so the kernels that write rows of a cache write into pages as they are.
 // The book beside it: table[s][j], the page of sequence s's rows j * page_tokens ..; lengths[s], its rows; refs[p], how
 // often the table names page p (free: 0). Pages are taken lowest first, so a book's next state follows from its last.
 //
-// Bookkeeping runs in one workgroup: which page is the r-th free one is a prefix sum over all of them, a few microseconds for
-// tens of thousands of pages, and a second launch would cost as much. Bound: latency, of dependent loads and barriers. Traced: a decode
-// step of 32 sequences over 1704 pages 3.6 us, 63255 tokens of 16 prompts that take about 2000 pages 6.8 (and 4.8 for the launch that writes their
-// rows), 16 forks among 197 pages 6.3, 634 pages moved together 4.6.
-// Copies of pages run in a launch of their own over (layer, head, K or V) x page; bound: their bytes (1.17 GB read and written in 235 us,
-// 5.0 TB/s, what a large torch copy reaches; the 117 MB of 16 forks 17.5).
+// Bookkeeping runs in one workgroup: which page is the r-th free one is a prefix sum over all of them, a few
+// microseconds for tens of thousands of pages, and a second launch would cost as much. Bound: latency, of dependent
+// loads and barriers. Traced: a decode step of 32 sequences over 1704 pages 3.6-3.7 us, 63255 tokens of 16 prompts that
+// take about 2000 pages 6.7-7.0 (and 4.8 for the launch that writes their rows), 16 forks among 197 pages 6.3, 634
+// pages moved together 4.6. Copies of pages run in a launch of their own over (layer, head, K or V) x page; bound:
+// their bytes (1.17 GB read and written in 235 us, 5.0 TB/s, what a large torch copy reaches; the 117 MB of 16 forks
+// 17.5).
 #include <algorithm>
 
 #include "ckv_common.hpp"
@@ -93,8 +94,8 @@ __device__ __forceinline__ int64_t pool_row(const Book& b, int s, int64_t pos, i
   return -1;
 }
 
-// Sequence s grows by counts[s] rows, or not at all (flagged): where the count is negative or past its table, the tokens
-// past n, or its pages past the free ones.
+// Sequence s grows by counts[s] rows, or not at all (flagged): where the count is negative or past its table, the
+// tokens past n, or its pages past the free ones.
 __global__ __launch_bounds__(kBookThreads) void extend_pages_kernel(int64_t* __restrict__ positions, int64_t* __restrict__ rows,
                                                                     int32_t* __restrict__ starts, int n,
                                                                     const int32_t* __restrict__ counts, Book b,
@@ -160,7 +161,8 @@ __global__ __launch_bounds__(kBookThreads) void extend_pages_kernel(int64_t* __r
       tokens += total[0];
     }
     __syncthreads();
-    // Ends past n are n + 1, so of the sequences that reach there the first still has tokens before them: none of it stays.
+    // Ends past n are n + 1, so of the sequences that reach there the first still has tokens before them: none of it
+    // stays.
     if (tokens > (uint64_t)n) {
       const int fit = interval_of(s_start, b.S, (uint32_t)n);  // uniform; s_start[fit] <= n < s_start[fit + 1]
       const uint32_t end = s_start[fit];
@@ -236,8 +238,9 @@ struct Pool {
 };
 constexpr int kCopyThreads = 256;
 
-// Part `part` of 2 * layers * heads (K's, then V's) of page src to page dst. ONCE: no other block reads it (non-temporal loads: 1.2 GB of
-// pages moved in 235 us, with ordinary ones 242); a page that 16 sequences get a copy of comes out of the L2 (118 MB 27 us, 34 without).
+// Part `part` of 2 * layers * heads (K's, then V's) of page src to page dst. ONCE: no other block reads it
+// (non-temporal loads: 1.2 GB of pages moved in 235 us, with ordinary ones 242); a page that 16 sequences get a copy of
+// comes out of the L2 (118 MB 27 us, 34 without).
 template <bool ONCE>
 __device__ __forceinline__ void copy_page(const Pool& pool, int part, int src, int dst) {
   const int lh = pool.layers * pool.heads, at = part % lh;
@@ -360,8 +363,9 @@ __global__ __launch_bounds__(kCopyThreads) void fork_copy_kernel(const Fork* __r
 
 // ---- ending sequences ------------------------------------------------------------------------------------------
 
-// The rows that sequence sequences[i] keeps, into rows[i]: at most keep[i], all of them (flagged) where keep[i] is negative or its last row
-// would be one of several in a page that others share, which the next rows would then be written into.
+// The rows that sequence sequences[i] keeps, into rows[i]: at most keep[i], all of them (flagged) where keep[i] is
+// negative or its last row would be one of several in a page that others share, which the next rows would then be
+// written into.
 __global__ __launch_bounds__(kCopyThreads) void keep_rows_kernel(int32_t* __restrict__ rows, const int32_t* __restrict__ sequences,
                                                                  const int32_t* __restrict__ keep, int n, Book b,
                                                                  int32_t* __restrict__ err) {
@@ -419,7 +423,8 @@ struct Moves {
   __device__ int32_t& name(int p) const { return words[1 + P / 2 * 2 + p]; }
 };
 
-// Of U used pages the i-th at U or above moves to the i-th free one below U: targets and sources are apart, so the copies need no order.
+// Of U used pages the i-th at U or above moves to the i-th free one below U: targets and sources are apart, so the
+// copies need no order.
 __global__ __launch_bounds__(kBookThreads) void compact_book_kernel(Moves m, int32_t* __restrict__ used_out, Book b) {
   __shared__ ScanRoom<1> s_scan;
   __shared__ int s_below;  // used pages below U
@@ -479,7 +484,8 @@ __global__ __launch_bounds__(kCopyThreads) void compact_copy_kernel(Moves m, Poo
   }
 }
 
-// New tokens from which their rows get a launch of their own: one workgroup writes 1024 in 0.7 us, a launch costs about three.
+// New tokens from which their rows get a launch of their own: one workgroup writes 1024 in 0.7 us, a launch costs about
+// three.
 constexpr int kRowsAlone = 4096;
 
 // ---- arguments -------------------------------------------------------------------------------------------------
