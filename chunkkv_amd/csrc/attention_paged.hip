@@ -57,7 +57,8 @@ __global__ __launch_bounds__(kPagedWaves * 64) void attn_paged_kernel(AttnMap ma
   }
   PagedSeq it;
   for (uint32_t at = begin_at; at < end_at && shares.part(at, it);) {  // uniform
-    const uint32_t parts = shares.parts_of(it), local = at - it.before, tile = parts == 1 ? local : it.tiles == 1 ? 0 : local / parts, from = local - tile * parts;
+    const uint32_t parts = shares.parts_of(it), local = at - it.before;
+    const uint32_t tile = parts == 1 ? local : it.tiles == 1 ? 0 : local / parts, from = local - tile * parts;
     // units [u0, u1) of the tile
     const uint32_t u0 = shares.apart ? from * share : from;
     const uint32_t u1 = min((uint32_t)it.units, shares.apart ? u0 + share : u0 + (end_at - at));
@@ -292,7 +293,8 @@ __global__ __launch_bounds__(256) void join_paged_kernel(char* __restrict__ out,
     splits = shares.apart ? shares.splits_of(it) : 0;
     if (splits == 1) return;
   } else {
-    if (!paged_find<ROWS, UNIT>(b, n, group, [&](const PagedSeq& q, uint32_t, uint32_t) { return t >= q.first && t - q.first < q.count; }, it)) return;
+    const auto mine = [&](const PagedSeq& q, uint32_t, uint32_t) { return t >= q.first && t - q.first < q.count; };
+    if (!paged_find<ROWS, UNIT>(b, n, group, mine, it)) return;
     if (it.splits == 1) return;
   }
   const int p = it.rows - it.count + t - it.first;  // the row's position
@@ -396,30 +398,33 @@ __global__ __launch_bounds__(256) void join_paged_kernel(char* __restrict__ out,
 
 }  // namespace ckv
 
-extern "C" int64_t ckv_attention_paged_workspace_bytes(int32_t n_tokens, int32_t n_sequences, int32_t most_tokens, int32_t most_rows, int64_t total_rows,
-                                                       int32_t n_entries, int32_t page_tokens, int32_t n_q_heads, int32_t n_kv_heads, int32_t head_dim) {
-  if (n_tokens <= 0 || n_sequences <= 0 || most_tokens < 0 || most_rows < 0 || total_rows < 0 || n_entries <= 0 || page_tokens <= 0 || n_q_heads <= 0 || n_kv_heads <= 0 ||
-      head_dim <= 0 || n_q_heads % n_kv_heads)
+extern "C" int64_t ckv_attention_paged_workspace_bytes(int32_t n_tokens, int32_t n_sequences, int32_t most_tokens,
+                                                       int32_t most_rows, int64_t total_rows, int32_t n_entries,
+                                                       int32_t page_tokens, int32_t n_q_heads, int32_t n_kv_heads,
+                                                       int32_t head_dim) {
+  if (n_tokens <= 0 || n_sequences <= 0 || most_tokens < 0 || most_rows < 0 || total_rows < 0 || n_entries <= 0 ||
+      page_tokens <= 0 || n_q_heads <= 0 || n_kv_heads <= 0 || head_dim <= 0 || n_q_heads % n_kv_heads)
     return 0;
   const int64_t rows = (int64_t)n_entries * page_tokens;
-  return ckv::paged_plan(n_tokens, n_sequences, most_tokens == 0 ? n_tokens : most_tokens, most_rows == 0 ? rows : most_rows, total_rows, rows,
-                         n_q_heads, n_kv_heads, head_dim, INT64_MAX).ws_bytes;
+  return ckv::paged_plan(n_tokens, n_sequences, most_tokens == 0 ? n_tokens : most_tokens, most_rows == 0 ? rows : most_rows,
+                         total_rows, rows, n_q_heads, n_kv_heads, head_dim, INT64_MAX).ws_bytes;
 }
 
 extern "C" int32_t ckv_attention_paged(void* out, const void* q, int64_t q_head_stride, int64_t q_token_stride, const void* k_pool,
                                        const void* v_pool, int64_t kv_head_stride, const int32_t* table, const int32_t* lengths,
-                                       const int32_t* starts, int32_t n_tokens, int32_t most_tokens, int32_t most_rows, int64_t total_rows, int32_t n_sequences,
-                                       int32_t n_entries, int32_t n_pages, int32_t page_tokens, int32_t n_q_heads,
-                                       int32_t n_kv_heads, int32_t head_dim, int32_t dtype, double scale, void* workspace,
-                                       int64_t workspace_bytes, int32_t* err, void* stream) {
+                                       const int32_t* starts, int32_t n_tokens, int32_t most_tokens, int32_t most_rows,
+                                       int64_t total_rows, int32_t n_sequences, int32_t n_entries, int32_t n_pages,
+                                       int32_t page_tokens, int32_t n_q_heads, int32_t n_kv_heads, int32_t head_dim,
+                                       int32_t dtype, double scale, void* workspace, int64_t workspace_bytes, int32_t* err, void* stream) {
   using namespace ckv;
   if (dtype != CKV_DTYPE_BF16 || (head_dim != 64 && head_dim != 128)) return CKV_ERR_INVALID_ARGUMENT;
   if (page_tokens != 32 && page_tokens != 64 && page_tokens != 128) return CKV_ERR_INVALID_ARGUMENT;
-  if (n_tokens < 0 || most_tokens < 0 || most_rows < 0 || total_rows < 0 || n_sequences <= 0 || n_entries <= 0 || n_pages <= 0 || n_q_heads <= 0 || n_kv_heads <= 0 ||
-      n_q_heads % n_kv_heads != 0 || log2_scale(scale) == 0.f)
+  if (n_tokens < 0 || most_tokens < 0 || most_rows < 0 || total_rows < 0 || n_sequences <= 0 || n_entries <= 0 || n_pages <= 0 ||
+      n_q_heads <= 0 || n_kv_heads <= 0 || n_q_heads % n_kv_heads != 0 || log2_scale(scale) == 0.f)
     return CKV_ERR_INVALID_ARGUMENT;
   if (n_tokens == 0) return CKV_OK;
-  if (out == nullptr || q == nullptr || k_pool == nullptr || v_pool == nullptr || table == nullptr || lengths == nullptr || starts == nullptr)
+  if (out == nullptr || q == nullptr || k_pool == nullptr || v_pool == nullptr || table == nullptr || lengths == nullptr ||
+      starts == nullptr)
     return CKV_ERR_INVALID_ARGUMENT;
   if (q_token_stride % 8 || q_head_stride % 8 || kv_head_stride % 8) return CKV_ERR_INVALID_ARGUMENT;  // 16-byte rows
   if (((uintptr_t)out | (uintptr_t)q | (uintptr_t)k_pool | (uintptr_t)v_pool) % 16) return CKV_ERR_INVALID_ARGUMENT;
@@ -430,8 +435,9 @@ extern "C" int32_t ckv_attention_paged(void* out, const void* q, int64_t q_head_
     return CKV_ERR_TOO_LARGE;
   if (workspace == nullptr || (uintptr_t)workspace % 16) workspace_bytes = 0;
   const int64_t rows = (int64_t)n_entries * page_tokens;
-  const PagedPlan plan = paged_plan(n_tokens, n_sequences, most_tokens == 0 ? n_tokens : most_tokens, most_rows == 0 ? rows : most_rows, total_rows, rows,
-                                    n_q_heads, n_kv_heads, head_dim, workspace_bytes);
+  const PagedPlan plan = paged_plan(n_tokens, n_sequences, most_tokens == 0 ? n_tokens : most_tokens,
+                                    most_rows == 0 ? rows : most_rows, total_rows, rows, n_q_heads, n_kv_heads, head_dim,
+                                    workspace_bytes);
   if (plan.map.blocks == 0) return CKV_ERR_TOO_LARGE;
   float* ws = plan.target > 0 ? (float*)workspace : nullptr;
   const bool many = n_sequences > 64;
@@ -443,9 +449,9 @@ extern "C" int32_t ckv_attention_paged(void* out, const void* q, int64_t q_head_
   hipStream_t st = (hipStream_t)stream;
   if (plan.rows < kAttnBM) {
     auto launch = [&](auto kernel) {
-      hipLaunchKernelGGL(kernel, dim3(map.blocks), dim3(kPagedWaves * 64), 0, st, map, b, n_tokens, (const char*)k_pool, (const char*)v_pool,
-                         kv_head_stride * 2, (const char*)q, q_head_stride * 2, q_token_stride * 2, n_q_heads, (int)group, scale_log2,
-                         (char*)out, ws);
+      hipLaunchKernelGGL(kernel, dim3(map.blocks), dim3(kPagedWaves * 64), 0, st, map, b, n_tokens, (const char*)k_pool,
+                         (const char*)v_pool, kv_head_stride * 2, (const char*)q, q_head_stride * 2, q_token_stride * 2, n_q_heads,
+                         (int)group, scale_log2, (char*)out, ws);
     };
 #define CKV_ROWS(D, QG) many ? launch(attn_paged_kernel<D, QG, true>) : launch(attn_paged_kernel<D, QG, false>)
     if (head_dim == 128) {
@@ -458,18 +464,22 @@ extern "C" int32_t ckv_attention_paged(void* out, const void* q, int64_t q_head_
 #undef CKV_ROWS
   } else {
     auto launch = [&](auto kernel) {
-      hipLaunchKernelGGL(kernel, dim3(map.blocks), dim3(kAttnWaves * 64), 0, st, map.nqb, map.group, map.xpk_log, map.items, map.inv_group,
-                         map.inv_nqb, (const int64_t*)nullptr, n_tokens, 0, (const char*)k_pool, (const char*)v_pool, kv_head_stride * 2,
-                         (const char*)q, q_head_stride * 2, q_token_stride * 2, n_q_heads, (int)group, scale_log2, (char*)out, err, ws, 0, b);
+      hipLaunchKernelGGL(kernel, dim3(map.blocks), dim3(kAttnWaves * 64), 0, st, map.nqb, map.group, map.xpk_log, map.items,
+                         map.inv_group, map.inv_nqb, (const int64_t*)nullptr, n_tokens, 0, (const char*)k_pool,
+                         (const char*)v_pool, kv_head_stride * 2, (const char*)q, q_head_stride * 2, q_token_stride * 2, n_q_heads,
+                         (int)group, scale_log2, (char*)out, err, ws, 0, b);
     };
-    if (head_dim == 128) ws != nullptr ? launch(attn_active_kernel<128, true, PagedRows>) : launch(attn_active_kernel<128, false, PagedRows>);
-    else ws != nullptr ? launch(attn_active_kernel<64, true, PagedRows>) : launch(attn_active_kernel<64, false, PagedRows>);
+#define CKV_LARGE(D) \
+  ws != nullptr ? launch(attn_active_kernel<D, true, PagedRows>) : launch(attn_active_kernel<D, false, PagedRows>)
+    if (head_dim == 128) CKV_LARGE(128);
+    else CKV_LARGE(64);
+#undef CKV_LARGE
   }
   CKV_RETURN_IF_LAUNCH_FAILED();
   if (ws != nullptr) {
     auto join = [&](auto kernel, int tokens, int heads) {
-      hipLaunchKernelGGL(kernel, dim3((unsigned)((n_tokens + tokens - 1) / tokens), (unsigned)((n_q_heads + heads - 1) / heads)), dim3(256), 0,
-                         st, (char*)out, (const float*)ws, b, n_tokens, n_q_heads, (int)group);
+      const dim3 grid((unsigned)((n_tokens + tokens - 1) / tokens), (unsigned)((n_q_heads + heads - 1) / heads));
+      hipLaunchKernelGGL(kernel, grid, dim3(256), 0, st, (char*)out, (const float*)ws, b, n_tokens, n_q_heads, (int)group);
     };
 #define CKV_JOIN(D, ROWS, UNIT, MANY)                                                       \
   plan.spread_join ? join(join_paged_kernel<D, ROWS, UNIT, 4, MANY>, 1, kJoinHeads<D>)     \

@@ -107,13 +107,16 @@ struct PagedShare {
     share = (uint32_t)paged_split_units((float)units, b.inv_target, b.min_units);
     apart = false;
     if (tiles < (uint32_t)b.target) {  // then no more than units / longer + tiles shares
-      const uint32_t longer = (uint32_t)paged_split_units((float)units, __builtin_amdgcn_rcpf((float)(b.target - (int)tiles)), b.min_units);
+      const float inv_left = __builtin_amdgcn_rcpf((float)(b.target - (int)tiles));
+      const uint32_t longer = (uint32_t)paged_split_units((float)units, inv_left, b.min_units);
       apart = longer <= share + 1;
       if (apart) share = longer;
     }
   }
   // Shares of each of a sequence's tiles, where they are apart.
-  __device__ uint32_t splits_of(const PagedSeq& q) const { return (uint32_t)paged_splits(q.units, (int)share, __builtin_amdgcn_rcpf((float)(int)share)); }
+  __device__ uint32_t splits_of(const PagedSeq& q) const {
+    return (uint32_t)paged_splits(q.units, (int)share, __builtin_amdgcn_rcpf((float)(int)share));
+  }
   // What shares are counted in: shares, where they are apart, or units.
   __device__ uint32_t parts_of(const PagedSeq& q) const { return apart ? splits_of(q) : (uint32_t)q.units; }
   __device__ auto counter() const {
@@ -121,7 +124,8 @@ struct PagedShare {
   }
   // The sequence that has part `at`.
   __device__ bool part(uint32_t at, PagedSeq& it) const {
-    return walk.find(counter(), [at](const PagedSeq&, uint32_t before, uint32_t own) { return at >= before && at - before < own; }, it);
+    const auto mine = [at](const PagedSeq&, uint32_t before, uint32_t own) { return at >= before && at - before < own; };
+    return walk.find(counter(), mine, it);
   }
   // The sequence that has token t.
   __device__ bool token(int t, PagedSeq& it) const {
@@ -145,7 +149,8 @@ __device__ __forceinline__ bool paged_find(const PagedRows& b, int n, int group,
     split_units = paged_split_units(wave_butterfly_sum(work), b.inv_target, b.min_units);  // the same in every wavefront
   }
   const float inv_split = __builtin_amdgcn_rcpf((float)split_units);
-  if (!walk.find([&](const PagedSeq& q) { return (uint32_t)(q.tiles * paged_splits(q.units, split_units, inv_split)); }, mine, it)) return false;
+  const auto items = [&](const PagedSeq& q) { return (uint32_t)(q.tiles * paged_splits(q.units, split_units, inv_split)); };
+  if (!walk.find(items, mine, it)) return false;
   it.split_units = split_units;
   it.splits = paged_splits(it.units, split_units, inv_split);
   return true;
@@ -154,7 +159,9 @@ __device__ __forceinline__ bool paged_find(const PagedRows& b, int n, int group,
 // Item `item` of a KV head; false: the launch has no such item.
 template <int ROWS, int UNIT>
 __device__ __forceinline__ bool paged_item(const PagedRows& b, int n, int group, int item, PagedItem& it) {
-  const auto mine = [item](const PagedSeq&, uint32_t before, uint32_t own) { return (uint32_t)item >= before && (uint32_t)item - before < own; };
+  const auto mine = [item](const PagedSeq&, uint32_t before, uint32_t own) {
+    return (uint32_t)item >= before && (uint32_t)item - before < own;
+  };
   if (!paged_find<ROWS, UNIT>(b, n, group, mine, it)) return false;
   const int local = item - (int)it.before;
   it.z = it.splits == 1 ? 0 : (int)((uint32_t)local / (uint32_t)it.tiles);

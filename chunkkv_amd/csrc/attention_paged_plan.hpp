@@ -63,8 +63,11 @@ struct PagedForm {
   double start, step[2], tile;
   int places[2];
 };
-constexpr PagedForm kPagedForms[] = {{16, 5.5, {0.5, 0.8}, 1.5, {512, 256}}, {32, 6.0, {0.55, 1.1}, 1.5, {512, 256}}, {kAttnBM, 5.0, {1.5, 2.4}, 0.5, {768, 512}}};
-constexpr double kPagedJoin = 4.5, kPagedJoinByte = 1.5e-6;  // us that splitting adds, and for each byte in fp32 of the results that are split
+constexpr PagedForm kPagedForms[] = {{16, 5.5, {0.5, 0.8}, 1.5, {512, 256}},
+                                     {32, 6.0, {0.55, 1.1}, 1.5, {512, 256}},
+                                     {kAttnBM, 5.0, {1.5, 2.4}, 0.5, {768, 512}}};
+// us that splitting adds, and for each byte in fp32 of the results that are split
+constexpr double kPagedJoin = 4.5, kPagedJoinByte = 1.5e-6;
 constexpr double kPagedMean = 0.5;  // of the longest sequence's rows, where the sum is not known
 
 // n new tokens of S sequences; `most` of one, `longest` cached rows of one and `total` of all that have tokens (0: not
@@ -76,11 +79,13 @@ constexpr double kPagedMean = 0.5;  // of the longest sequence's rows, where the
 //   4 sequences of 500 rows and tokens 17.7 (128), 19.8 split; 2 of 832 rows, 57 tokens, 11.1 (16), 18.5 split
 //   14 / 2 of 64, 9 sequences of up to 2000 rows, 1280 tokens, 16.5 (32), 18.1 (16), 21.8 (128, split), 32.9 (128)
 //   8 / 8 of 64, 22 of up to 1976 rows, 1314 tokens, 15.8 (16), 16.6 (32), 19.4 (128, split), 26.8 (16, split)
-static inline PagedPlan paged_plan(int64_t n, int64_t S, int64_t most, int64_t longest, int64_t total, int64_t rows, int Hq, int Hkv, int head_dim, int64_t workspace_bytes) {
+static inline PagedPlan paged_plan(int64_t n, int64_t S, int64_t most, int64_t longest, int64_t total, int64_t rows, int Hq,
+                                   int Hkv, int head_dim, int64_t workspace_bytes) {
   PagedPlan p;
   const int64_t group = Hq / Hkv, used = std::min(S, n), one = std::min(most, n) * group;
   const int d128 = head_dim == 128;
-  const double longer = (double)std::min(longest, rows), mean = total > 0 ? std::min((double)total / (double)used, longer) : kPagedMean * longer;
+  const double longer = (double)std::min(longest, rows);
+  const double mean = total > 0 ? std::min((double)total / (double)used, longer) : kPagedMean * longer;
   double least = INFINITY;
   for (const PagedForm& f : kPagedForms) {
     if ((f.rows > 16 && one <= 16) || (f.rows > 32 && one <= 32)) continue;
@@ -112,7 +117,8 @@ static inline PagedPlan paged_plan(int64_t n, int64_t S, int64_t most, int64_t l
       s.ws_bytes = 2 * s.items * row_b;  // of a share, its first and its last tile may be partial
       if (tiles * ((rows + unit - 1) / unit) > INT32_MAX / 2) continue;  // units are counted in 32 bits
     }
-    const double joined = 4.0 * (double)(n * Hq * head_dim) * (total > 0 ? mean_units / units : 1.0);  // tiles of short sequences are mostly whole
+    // tiles of short sequences are mostly whole
+    const double joined = 4.0 * (double)(n * Hq * head_dim) * (total > 0 ? mean_units / units : 1.0);
     const double split = f.start + kPagedJoin + kPagedJoinByte * joined + f.step[d128] * std::max(2.0, load);
     if (split < least && s.ws_bytes <= workspace_bytes) {
       least = split;

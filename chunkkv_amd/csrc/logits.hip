@@ -46,7 +46,8 @@ struct Adjust {
 constexpr int kLogitsThreads = 512, kLogitsEach = 8;  // logits of a thread
 constexpr int kLogitsSlice = kLogitsThreads * kLogitsEach;
 constexpr uint32_t kInPrompt = 1u << 31;
-constexpr int kPairsEach = 4, kPairsStep = kPairsEach * kLogitsThreads;  // pairs of tokens that a thread, a workgroup, has in flight
+// Pairs of tokens that a thread, and a workgroup, has in flight.
+constexpr int kPairsEach = 4, kPairsStep = kPairsEach * kLogitsThreads;
 
 // Counts the row's tokens that lie in [v0, v0 + kLogitsSlice) into count[]: occurrences in generated, kInPrompt where
 // it is in the prompt. Both lists are one of pairs, whose loads go out U at a time for each thread, the last of them

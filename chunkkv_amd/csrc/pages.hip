@@ -45,7 +45,8 @@ __device__ __forceinline__ void book_scan(uint64_t (&x)[K], uint64_t (&total)[K]
   }
   __syncthreads();
   auto at = [](uint64_t v, int l) {
-    return (uint64_t)(uint32_t)__builtin_amdgcn_readlane((uint32_t)(v >> 32), l) << 32 | (uint32_t)__builtin_amdgcn_readlane((uint32_t)v, l);
+    const uint32_t hi = __builtin_amdgcn_readlane((uint32_t)(v >> 32), l), lo = __builtin_amdgcn_readlane((uint32_t)v, l);
+    return (uint64_t)hi << 32 | lo;
   };
 #pragma unroll
   for (int k = 0; k < K; ++k) {

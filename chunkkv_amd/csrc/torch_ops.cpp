@@ -841,9 +841,9 @@ PyObject* extend_pages(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
   const Tensor starts = new_tensor({b.S + 1}, at::kInt, b.table);
   check(unlocked([&] {
           const c10::DeviceGuard on(b.table.device());
-          return ckv_extend_pages((int64_t*)ptr(positions), (int64_t*)ptr(rows), (int32_t*)ptr(starts), int32(n), (const int32_t*)ptr(counts),
-                                  b.at(b.table), b.at(b.lengths), b.at(b.refs), int32(b.S), int32(b.M), int32(b.P), int32(b.T), e,
-                                  stream_of(b.table));
+          return ckv_extend_pages((int64_t*)ptr(positions), (int64_t*)ptr(rows), (int32_t*)ptr(starts), int32(n),
+                                  (const int32_t*)ptr(counts), b.at(b.table), b.at(b.lengths), b.at(b.refs), int32(b.S), int32(b.M),
+                                  int32(b.P), int32(b.T), e, stream_of(b.table));
         }),
         "ckv_extend_pages");
   return Py_BuildValue("(NNN)", THPVariable_Wrap(positions), THPVariable_Wrap(rows), THPVariable_Wrap(starts));
@@ -976,15 +976,17 @@ PyObject* attention_paged(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
       value_error("out must be contiguous (1, n, Hq, D) bf16");
     // token-major queries may be written over: the workgroup that writes a row has read it, and no other reads it
     const bool in_place = out.data_ptr() == q.data_ptr() && step(q, 1, p.D) == p.D && step(q, 2, Hq * p.D) == Hq * p.D;
-    if ((!in_place && meets(out, q)) || meets(out, p.k) || meets(out, p.v) || meets(out, b.table) || meets(out, b.lengths) || meets(out, starts))
-      value_error("out overlaps q without being it, or the cache");
+    if (!in_place && meets(out, q)) value_error("out overlaps q without being it");
+    for (const Tensor* t : {&p.k, &p.v, &b.table, &b.lengths, &starts})
+      if (meets(out, *t)) value_error("out overlaps the cache or starts");
   }
   const double scale = a[12] == Py_None ? 1.0 / std::sqrt((double)p.D) : real(a[12]);
   const int split = PyObject_IsTrue(a[15]);
   if (split < 0) throw python_error();
-  const int64_t ws_bytes = split ? ckv_attention_paged_workspace_bytes(int32(n), int32(b.S), int32(most), int32(longest), total, int32(b.M), int32(b.T),
-                                                                       int32(Hq), int32(p.H), int32(p.D))
-                                 : 0;
+  const int64_t ws_bytes =
+      split ? ckv_attention_paged_workspace_bytes(int32(n), int32(b.S), int32(most), int32(longest), total, int32(b.M), int32(b.T),
+                                                  int32(Hq), int32(p.H), int32(p.D))
+            : 0;
   Tensor ws;
   if (ws_bytes > 0) ws = new_tensor({(ws_bytes + 3) / 4}, at::kFloat, q);
   check(unlocked([&] {
@@ -992,8 +994,8 @@ PyObject* attention_paged(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
           const int64_t at = layer * p.k.stride(0) * 2;
           return ckv_attention_paged(ptr(out), ptr(q), step(q, 1, n * p.D), step(q, 2, p.D), (const char*)ptr(p.k) + at,
                                      (const char*)ptr(p.v) + at, p.k.stride(2), b.at(b.table), b.at(b.lengths), (const int32_t*)ptr(starts),
-                                     int32(n), int32(most), int32(longest), total, int32(b.S), int32(b.M), int32(b.P), int32(b.T), int32(Hq), int32(p.H), int32(p.D),
-                                     CKV_DTYPE_BF16, scale, ptr(ws), ws_bytes, e, stream_of(q));
+                                     int32(n), int32(most), int32(longest), total, int32(b.S), int32(b.M), int32(b.P), int32(b.T),
+                                     int32(Hq), int32(p.H), int32(p.D), CKV_DTYPE_BF16, scale, ptr(ws), ws_bytes, e, stream_of(q));
         }),
         "ckv_attention_paged");
   return THPVariable_Wrap(out);

@@ -29,7 +29,8 @@ class PagedSession:
         if not (engine._native_attention and engine.attention in ("fused", "sdpa")):
             raise ValueError("a paged cache needs the attention kernel: bf16, head_dim 64 or 128, attention 'fused' or 'sdpa'")
         self.engine = engine
-        self.cache = ops.paged_cache(len(engine.layers), n_pages, engine.n_kv, engine.head_dim, n_sequences, max_tokens, engine.device, page_tokens)
+        self.cache = ops.paged_cache(len(engine.layers), n_pages, engine.n_kv, engine.head_dim, n_sequences, max_tokens,
+                                     engine.device, page_tokens)
         self.tokens: dict[int, list[int]] = {}  # of each sequence, one for each of its rows
         self._logits: dict[int, torch.Tensor] = {}  # (1, vocab) behind a sequence's last row
         self._err = torch.zeros(1, dtype=torch.int32, device=engine.device)
@@ -72,8 +73,8 @@ class PagedSession:
 
     @contextmanager
     def _or_back(self, rows: dict[int, int]):
-        """Where this block raises, an interrupt among it, sequences s go back to rows[s] rows, which the device may have left; else the next rows
-        would come behind ones that were never written."""
+        """Where this block raises, an interrupt among it, sequences s go back to rows[s] rows, which the device may have left; else
+        the next rows would come behind ones that were never written."""
         try:
             yield
         except BaseException:
@@ -115,7 +116,7 @@ class PagedSession:
         shape = (1, c.k.shape[2], len(tokens), c.k.shape[4])
         for layers in (result.keys, result.values):
             if len(layers) != c.k.shape[0] or any(t.shape != shape or t.dtype != c.k.dtype or t.device != c.k.device for t in layers):
-                raise ValueError(f"a prefill's keys and values are {tuple(shape)} {c.k.dtype} on {c.k.device} in each of {c.k.shape[0]} layers here")
+                raise ValueError(f"a prefill's keys and values are {shape} {c.k.dtype} on {c.k.device} in each of {c.k.shape[0]} layers here")
         (s,) = self._slots(1)
         self._check_room({s: len(tokens)})
         with self._or_back({s: 0}):
@@ -167,8 +168,8 @@ class PagedSession:
     # -- the model ------------------------------------------------------------------------
 
     def _forward(self, tok: torch.Tensor, counts: torch.Tensor, most: int, rows: list[int]):
-        """New tokens tok (n,), in the order of the sequences, counts[s] of each, most of one at most; rows: of each with them, or about. The new rows
-        are taken and written, layer by layer. (h, pending, starts), for the engine's _final_logits."""
+        """New tokens tok (n,), in the order of the sequences, counts[s] of each, most of one at most; rows: of each with them, or
+        about. The new rows are taken and written, layer by layer. (h, pending, starts), for the engine's _final_logits."""
         e, c = self.engine, self.cache
         known = dict(most=most, longest=max(rows), total=sum(rows))
         H, D, n = e.n_kv, e.head_dim, tok.shape[0]
@@ -195,7 +196,8 @@ class PagedSession:
         self._check_room(more)
         tok = torch.tensor([t for chunk in chunks.values() for t in chunk], dtype=torch.int64).to(self.engine.device)
         with self._or_back({s: len(self.tokens[s]) for s in chunks}):
-            h, pending, starts = self._forward(tok, self._counts(more), max(more.values()), [len(self.tokens[s]) + n for s, n in more.items()])
+            rows = [len(self.tokens[s]) + n for s, n in more.items()]
+            h, pending, starts = self._forward(tok, self._counts(more), max(more.values()), rows)
             last = starts[1:].long()[torch.tensor(list(chunks)).to(starts.device)] - 1
             logits = self.engine._final_logits(h[:, last], None if pending is None else pending[:, last])[0]
             self._check_err()
@@ -205,7 +207,8 @@ class PagedSession:
         return {s: self._logits[s] for s in chunks}
 
     @torch.inference_mode()
-    def generate(self, sequences, max_tokens: int = 32, *, repetition=1.0, frequency=0.0, presence=0.0, bias=None, allowed=None) -> list[list[int]]:
+    def generate(self, sequences, max_tokens: int = 32, *, repetition=1.0, frequency=0.0, presence=0.0, bias=None,
+                 allowed=None) -> list[list[int]]:
         """Greedy decode of these sequences together, each up to max_tokens tokens or its end-of-sequence token (not among those returned);
         the new tokens of each, in the order they were named. They stay in the cache, and a sequence that did not end can go on.
 

@@ -642,23 +642,26 @@ int32_t ckv_evict_rows(void* k_out, int64_t ko_head_stride, void* v_out, int64_t
 
 /*
  * A cache that several sequences share, in pages (no counterpart in the reference). A pool of K or V is an ordinary cache of
- * n_pages * page_tokens rows a head (bf16 or f32): page p is the rows [p * page_tokens, (p + 1) * page_tokens) of every layer and head, and
- * the entry points that write rows of a cache write into pages as they are. The book, int32 on the device:
+ * n_pages * page_tokens rows a head (bf16 or f32): page p is the rows [p * page_tokens, (p + 1) * page_tokens) of every layer
+ * and head, and the entry points that write rows of a cache write into pages as they are. The book, int32 on the device:
  *   table    (n_sequences, n_entries)  entry j of a sequence: the page of its rows j * page_tokens ..; past its last one anything
  *   lengths  (n_sequences)             its rows; 0: no sequence
  *   refs     (n_pages)                 how often the table names the page; 0: free
- * Pages are taken lowest first, sequences in order, so a call's result follows from the book alone. page_tokens 32, 64 or 128; at
- * most 4096 sequences, and 2^31 - 1 rows of a sequence and of the pool (CKV_ERR_TOO_LARGE). Calls on one book go to one stream, or are ordered.
- * A table that names a page outside the pool is flagged in *err and reads or writes nothing outside it.
+ * Pages are taken lowest first, sequences in order, so a call's result follows from the book alone. page_tokens 32, 64 or
+ * 128; at most 4096 sequences, and 2^31 - 1 rows of a sequence and of the pool (CKV_ERR_TOO_LARGE). Calls on one book go to
+ * one stream, or are ordered. A table that names a page outside the pool is flagged in *err and reads or writes nothing
+ * outside it.
  *
  * Sequence s grows by counts[s] rows (a whole prompt's, a chunk's, a token's, or 0): the pages it needs beyond those it has are
  * taken, lengths[s] becomes lengths[s] + counts[s], and for new token i of all, in the order of the sequences,
  *   positions[i]  its row of its sequence
- *   rows[i]       that row's place in the pool: table entry * page_tokens + row % page_tokens (-1, flagged, where the table names no page)
+ *   rows[i]       that row's place in the pool: table entry * page_tokens + row % page_tokens (-1, flagged, where the table
+ *                 names no page)
  *   starts[s]     new tokens in front of sequence s's; starts[n_sequences]: all of them
- * n_new is the room of positions and rows; behind the last token positions are 0 and rows -1. What does not fit grows by nothing and
- * is flagged: a negative count or one past the table (CKV_DEVICE_ERR_RANGE), the first sequence whose tokens pass n_new and all behind it that have any
- * (CKV_DEVICE_ERR_RANGE), the first whose pages pass the free ones and all behind it that need any (CKV_DEVICE_ERR_PAGES).
+ * n_new is the room of positions and rows; behind the last token positions are 0 and rows -1. What does not fit grows by
+ * nothing and is flagged: a negative count or one past the table (CKV_DEVICE_ERR_RANGE), the first sequence whose tokens pass
+ * n_new and all behind it that have any (CKV_DEVICE_ERR_RANGE), the first whose pages pass the free ones and all behind it
+ * that need any (CKV_DEVICE_ERR_PAGES).
  * Rows are written into the last page of a sequence, so a partial page has one sequence (ckv_fork_pages sees to it). One launch.
  */
 int32_t ckv_extend_pages(int64_t* positions, int64_t* rows, int32_t* starts, int32_t n_new, const int32_t* counts,
@@ -667,11 +670,11 @@ int32_t ckv_extend_pages(int64_t* positions, int64_t* rows, int32_t* starts, int
 
 /*
  * Sequence targets[i] continues sequence sources[i]: it shares its whole pages (refs + 1) and gets a copy of its partial last
- * one, of every layer, in a free page. Free pages go to the pairs in order; sequences are read as they were when the call began, so a
- * source that is another pair's target is an empty one, and its own target stays empty. A pair whose target has rows, is its source, or was
- * named before, or that names no sequence, is left out and flagged (CKV_DEVICE_ERR_RANGE), as is the first that finds no free page and all
- * behind it that need one (CKV_DEVICE_ERR_PAGES). k_pool, v_pool: (n_layers, n_heads, n_pages * page_tokens, head_dim) with the given strides
- * (elements, 16-byte multiples); head_dim 64, 128 or 256.
+ * one, of every layer, in a free page. Free pages go to the pairs in order; sequences are read as they were when the call
+ * began, so a source that is another pair's target is an empty one, and its own target stays empty. A pair whose target has
+ * rows, is its source, or was named before, or that names no sequence, is left out and flagged (CKV_DEVICE_ERR_RANGE), as is
+ * the first that finds no free page and all behind it that need one (CKV_DEVICE_ERR_PAGES). k_pool, v_pool: (n_layers,
+ * n_heads, n_pages * page_tokens, head_dim) with the given strides (elements, 16-byte multiples); head_dim 64, 128 or 256.
  *   workspace  device buffer of workspace_bytes >= ckv_fork_pages_workspace_bytes(n_pairs)
  * n_pairs at most 4096. Two launches.
  */
@@ -682,10 +685,10 @@ int32_t ckv_fork_pages(void* k_pool, void* v_pool, int64_t layer_stride, int64_t
 int64_t ckv_fork_pages_workspace_bytes(int32_t n_pairs); /* host-only */
 
 /*
- * The sequences end: their pages' refs - 1, their table entries -1, their lengths 0. With keep they go back to their first keep[i] rows
- * instead, where those are fewer (0: none), and give up the pages behind; one stays as it is and is flagged (CKV_DEVICE_ERR_RANGE) where keep[i] is negative or
- * ends inside a page that another sequence shares. One named twice counts the first time, an empty one stays
- * so, one that does not exist is flagged (CKV_DEVICE_ERR_RANGE). n at most 4096.
+ * The sequences end: their pages' refs - 1, their table entries -1, their lengths 0. With keep they go back to their first
+ * keep[i] rows instead, where those are fewer (0: none), and give up the pages behind; one stays as it is and is flagged
+ * (CKV_DEVICE_ERR_RANGE) where keep[i] is negative or ends inside a page that another sequence shares. One named twice counts
+ * the first time, an empty one stays so, one that does not exist is flagged (CKV_DEVICE_ERR_RANGE). n at most 4096.
  *   workspace  with keep: device buffer of workspace_bytes >= 4 n
  * One launch, with keep two.
  */
@@ -706,33 +709,35 @@ int32_t ckv_compact_pages(void* k_pool, void* v_pool, int64_t layer_stride, int6
 int64_t ckv_compact_pages_workspace_bytes(int32_t n_pages); /* host-only */
 
 /*
- * Attention of new tokens over one layer of a paged cache: of sequence s's lengths[s] rows the last c = starts[s + 1] - starts[s] are new, and
- * its query i (token starts[s] + i of q and out) sees its rows up to lengths[s] - c + i: ckv_attention_active's function on the rows that the
- * table names, with its roundings. A query that sees no row (c above lengths[s]) gives zeros, one whose scores are all
- * -infinity NaN; tokens in front of starts[0] and from starts[n_sequences] on
- * are not written. starts ascends (ckv_extend_pages gives it); whatever it holds, nothing outside the arrays is touched. out (n_tokens,
- * n_q_heads, head_dim) overlaps no input, but may be q where that lies alike.
- *   k_pool, v_pool  the layer's pool, (n_kv_heads, n_pages * page_tokens, head_dim), bf16, kv_head_stride elements between heads; rows of a
- *                   page behind its sequence's last may hold anything. Infinite values of its own rows may give NaN, as there: zero
- *                   weights meet rows that a query does not see
- *   most_tokens, most_rows, total_rows  of the sequences with new tokens, if known, or about: the most tokens of one, the most rows of one, and
- *                   all of their rows (0: not known; n_tokens, n_entries * page_tokens and a part of that for each then); they choose the
- *                   kernel's form, not the result
- *   workspace       optional device buffer of workspace_bytes >= ckv_attention_paged_workspace_bytes(...) (16-byte aligned): partial rows
- *                   of launches that split the cache; without it they run unsplit (slower; the same up to the order of fp32 sums)
+ * Attention of new tokens over one layer of a paged cache: of sequence s's lengths[s] rows the last c = starts[s + 1] -
+ * starts[s] are new, and its query i (token starts[s] + i of q and out) sees its rows up to lengths[s] - c + i:
+ * ckv_attention_active's function on the rows that the table names, with its roundings. A query that sees no row (c above
+ * lengths[s]) gives zeros, one whose scores are all -infinity NaN; tokens in front of starts[0] and from starts[n_sequences] on
+ * are not written. starts ascends (ckv_extend_pages gives it); whatever it holds, nothing outside the arrays is touched. out
+ * (n_tokens, n_q_heads, head_dim) overlaps no input, but may be q where that lies alike.
+ *   k_pool, v_pool  the layer's pool, (n_kv_heads, n_pages * page_tokens, head_dim), bf16, kv_head_stride elements between
+ *                   heads; rows of a page behind its sequence's last may hold anything. Infinite values of its own rows may
+ *                   give NaN, as there: zero weights meet rows that a query does not see
+ *   most_tokens, most_rows, total_rows  of the sequences with new tokens, if known, or about: the most tokens of one, the most
+ *                   rows of one, and all of their rows (0: not known; n_tokens, n_entries * page_tokens and a part of that for
+ *                   each then); they choose the kernel's form, not the result
+ *   workspace       optional device buffer of workspace_bytes >= ckv_attention_paged_workspace_bytes(...) (16-byte aligned):
+ *                   partial rows of launches that split the cache; without it they run unsplit (slower; the same up to the
+ *                   order of fp32 sums)
  * head_dim 64 or 128; scale within the normal fp32 numbers' range; lengths past n_entries * page_tokens count as that.
  * No counterpart in the reference.
  */
 int32_t ckv_attention_paged(void* out, const void* q, int64_t q_head_stride, int64_t q_token_stride, const void* k_pool,
                             const void* v_pool, int64_t kv_head_stride, const int32_t* table, const int32_t* lengths,
                             const int32_t* starts, int32_t n_tokens, int32_t most_tokens, int32_t most_rows,
-                            int64_t total_rows, int32_t n_sequences, int32_t n_entries, int32_t n_pages, int32_t page_tokens, int32_t n_q_heads, int32_t n_kv_heads,
-                            int32_t head_dim, int32_t dtype, double scale, void* workspace, int64_t workspace_bytes,
-                            int32_t* err, void* stream);
+                            int64_t total_rows, int32_t n_sequences, int32_t n_entries, int32_t n_pages, int32_t page_tokens,
+                            int32_t n_q_heads, int32_t n_kv_heads, int32_t head_dim, int32_t dtype, double scale,
+                            void* workspace, int64_t workspace_bytes, int32_t* err, void* stream);
 
 /* Bytes of workspace that ckv_attention_paged uses for this shape (0: none). Host-only. */
 int64_t ckv_attention_paged_workspace_bytes(int32_t n_tokens, int32_t n_sequences, int32_t most_tokens, int32_t most_rows,
-                                            int64_t total_rows, int32_t n_entries, int32_t page_tokens, int32_t n_q_heads, int32_t n_kv_heads, int32_t head_dim);
+                                            int64_t total_rows, int32_t n_entries, int32_t page_tokens, int32_t n_q_heads,
+                                            int32_t n_kv_heads, int32_t head_dim);
 
 /*
  * Logits (n_rows, vocab), bf16 or f32 with contiguous rows, adjusted before a token is chosen. With c = how often the row's `generated`
