@@ -364,27 +364,22 @@ __global__ __launch_bounds__(kCopyThreads) void fork_copy_kernel(const Fork* __r
 
 // ---- ending sequences ------------------------------------------------------------------------------------------
 
-// The rows that sequence sequences[i] keeps, into rows[i]: at most keep[i], all of them (flagged) where keep[i] is
-// negative or its last row would be one of several in a page that others share, which the next rows would then be
-// written into.
+// The rows that sequence sequences[i] keeps, into rows[i]: at most keep[i], -1 (all of them, flagged by the next launch,
+// which knows whether the sequence was named before) where keep[i] is negative or its last row would be one of several
+// in a page that others share, which the next rows would then be written into.
 __global__ __launch_bounds__(kCopyThreads) void keep_rows_kernel(int32_t* __restrict__ rows, const int32_t* __restrict__ sequences,
-                                                                 const int32_t* __restrict__ keep, int n, Book b,
-                                                                 int32_t* __restrict__ err) {
+                                                                 const int32_t* __restrict__ keep, int n, Book b) {
   const int i = blockIdx.x * kCopyThreads + threadIdx.x;
   if (i >= n) return;
   const int s = sequences[i];
-  if ((uint32_t)s >= (uint32_t)b.S) return;  // the next launch flags it
+  if ((uint32_t)s >= (uint32_t)b.S) return;  // flagged there too
   const int len = rows_of(b, s);
   int left = min(keep[i], len);
   if (left < len && (left & ((1 << b.T_log) - 1)) != 0) {
     const int p = left < 0 ? -1 : b.table[(int64_t)s * b.M + (left >> b.T_log)];
     if ((uint32_t)p >= (uint32_t)b.P || b.refs[p] > 1) left = -1;
   }
-  if (left < 0) {
-    flag_error(err, CKV_DEVICE_ERR_RANGE);
-    left = len;
-  }
-  rows[i] = left;
+  rows[i] = max(left, -1);
 }
 
 // A block a sequence; of two that are the same the first one's. rows NULL: no row is kept.
@@ -399,7 +394,12 @@ __global__ __launch_bounds__(kCopyThreads) void free_pages_kernel(const int32_t*
   for (int i = threadIdx.x; i < (int)blockIdx.x; i += kCopyThreads) before |= sequences[i] == s;
   if (__syncthreads_or(before)) return;
   auto pages_of = [&](int r) { return (int)(((uint32_t)r + (1u << b.T_log) - 1) >> b.T_log); };
-  const int left = rows != nullptr ? rows[blockIdx.x] : 0, pages = pages_of(rows_of(b, s));
+  const int len = rows_of(b, s), pages = pages_of(len);
+  int left = rows != nullptr ? rows[blockIdx.x] : 0;
+  if (left < 0) {
+    if (threadIdx.x == 0) flag_error(err, CKV_DEVICE_ERR_RANGE);
+    left = len;
+  }
   int32_t* row = b.table + (int64_t)s * b.M;
   for (int j = pages_of(left) + threadIdx.x; j < pages; j += kCopyThreads) {
     const int p = row[j];
@@ -585,7 +585,7 @@ extern "C" int32_t ckv_free_pages(const int32_t* sequences, const int32_t* keep,
     if (workspace == nullptr || (uintptr_t)workspace % 4 || workspace_bytes < (int64_t)n * 4) return CKV_ERR_INVALID_ARGUMENT;
     rows = (int32_t*)workspace;
     hipLaunchKernelGGL(keep_rows_kernel, dim3((unsigned)((n + kCopyThreads - 1) / kCopyThreads)), dim3(kCopyThreads), 0,
-                       (hipStream_t)stream, rows, sequences, keep, n, b, err);
+                       (hipStream_t)stream, rows, sequences, keep, n, b);
     CKV_RETURN_IF_LAUNCH_FAILED();
   }
   hipLaunchKernelGGL(free_pages_kernel, dim3((unsigned)n), dim3(kCopyThreads), 0, (hipStream_t)stream, sequences, rows, b, err);

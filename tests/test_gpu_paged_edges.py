@@ -174,3 +174,19 @@ def test_tokens_into_a_buffer_that_they_are_chosen_from(vocab):
                 call()
     wide = ids.t().contiguous()  # tokens first: a step's tokens lie together
     assert torch.equal(ops.next_tokens(logits, generated=wide.t(), presence=20.0, out=wide[4]), want) and torch.equal(wide[4], want)
+
+
+def test_a_sequence_named_twice_going_back_counts_the_first_time():
+    """What is asked for it the second time is no error, whatever it is."""
+    c = ops.paged_cache(1, 12, 1, 64, 3, 200, DEV, 32)
+    book, err = R.Book(3, c.table.shape[1], 12, 32), torch.zeros(1, dtype=I32, device=DEV)
+    for call in (lambda x: x.extend([70, 0, 40], 110), lambda x: x.fork([0], [1])):
+        call(book)
+    ops.extend_pages(c, _ints([70, 0, 40]), 110, err)
+    ops.fork_pages(c, _ints([0]), _ints([1]), err)
+    for at, left in (([0, 0], [66, -1]), ([0, 2, 0, 2], [64, 39, 40, -7]), ([1, 1], [70, 33]), ([2, 2], [-1, 5]), ([0, 0], [40, 32])):
+        book.err = 0
+        err.zero_()
+        book.free(at, left)
+        ops.free_pages(c, _ints(at), _ints(left), err)
+        book.check(c, err)
