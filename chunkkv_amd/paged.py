@@ -286,12 +286,12 @@ class PagedSession:
                             live.discard(i)
                         else:
                             out[i].append(t)
-        self._go_back({s: before[s] + len(out[i]) for i, s in enumerate(slots)})  # every one took a row a step
+            self._go_back({s: before[s] + len(out[i]) for i, s in enumerate(slots)})  # every one took a row a step
+            self._check_err()
         for i, s in enumerate(slots):
             self.tokens[s] = self.tokens[s] + out[i]
             if i in live:
                 self._logits[s] = logits[i:i + 1]
             else:
                 del self._logits[s]
-        self._check_err()
         return [out[by_slot.index(i)] for i in range(B)]

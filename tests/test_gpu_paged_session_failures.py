@@ -188,3 +188,17 @@ def test_a_mask_that_leaves_nothing_ends_the_call_at_its_step(graphs):
     assert _state(s) == before and len(asked) == 4
     for p, tokens in zip(prompts, s.generate(ids, 8)):
         _greedy_run(eng, p, tokens, 8)
+
+
+@pytest.mark.parametrize("error", [RuntimeError, Stop])
+def test_a_generate_that_fails_behind_its_last_step_takes_nothing(monkeypatch, error):
+    eng = _engine()
+    s, ids, prompts = _session(eng, (33, 50))
+    before = _state(s)
+    with monkeypatch.context() as m:
+        _fails_at(m, "free_pages", 1, error)  # going back to what was generated
+        with pytest.raises(error):
+            s.generate(ids, 8)
+    assert _state(s) == before
+    for p, tokens in zip(prompts, s.generate(ids, 8)):
+        _greedy_run(eng, p, tokens, 8)
