@@ -152,11 +152,12 @@ class PagedSession:
     def free(self, sequences) -> None:
         """These sequences end; pages that no other shares are free again."""
         sequences = self._known(sequences)
-        ops.free_pages(self.cache, self._ints(sequences), err=self._err)
-        for s in sequences:
-            del self.tokens[s]
-            self._logits.pop(s, None)
-        self._check_err()
+        with self._or_back(dict.fromkeys(sequences, 0)):  # ended is what they are then, too
+            for s in sequences:
+                del self.tokens[s]
+                self._logits.pop(s, None)
+            ops.free_pages(self.cache, self._ints(sequences), err=self._err)
+            self._check_err()
 
     @torch.inference_mode()
     def compact(self) -> int:

@@ -202,3 +202,25 @@ def test_a_generate_that_fails_behind_its_last_step_takes_nothing(monkeypatch, e
     assert _state(s) == before
     for p, tokens in zip(prompts, s.generate(ids, 8)):
         _greedy_run(eng, p, tokens, 8)
+
+
+@pytest.mark.parametrize("where", ["before", "behind"])
+def test_sequences_whose_end_fails_have_ended(monkeypatch, where):
+    """On the device and on the host alike, so that the next sequence begins with no rows."""
+    eng = _engine()
+    s, (a, b), prompts = _session(eng, (40, 65))
+    with monkeypatch.context() as m:
+        if where == "before":
+            _fails_at(m, "free_pages", 1, Stop)
+        else:
+            def interrupted():
+                raise Stop("broken")
+
+            m.setattr(s, "_check_err", interrupted)
+        with pytest.raises(Stop):
+            s.free([a])
+    assert list(s.tokens) == [b] and s.cache.lengths.tolist()[:2] == [0, 65] and s.free_pages == 60 - 3
+    p = _tokens(50, 5)
+    assert s.add(eng.prefill(p), p) == a
+    _greedy_run(eng, p, s.generate([a], 9)[0], 9)
+    _greedy_run(eng, prompts[1], s.generate([b], 9)[0], 9)
