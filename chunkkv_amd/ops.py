@@ -833,12 +833,12 @@ def attention_paged(
     """Attention of new tokens over a layer of a paged cache that has their rows already: of sequence s, tokens starts[s] ..
     starts[s + 1] (extend_pages' starts) are the last of its lengths[s] rows, and each sees its sequence's rows up to its own.
 
-    q: (1, Hq, n, D) bf16 with contiguous rows; the cache bf16, D 64 or 128. Returns (1, n, Hq, D) bf16, token-major; a token that sees no row
-    (more new tokens than rows) gives zeros, tokens outside [starts[0], starts[-1]) stay as they were in out (anything in a new tensor).
-    out overlaps neither the cache nor q, but may be q itself where a token's heads lie together.
-    most, longest, total: the most new tokens of one sequence (1 in a decode step), the most rows of one that has any, and those of all that have any
-    together, if known, or about: they choose the kernel's form, not the result. Without longest the table's width counts, which makes short
-    sequences in a wide table slower.
+    q: (1, Hq, n, D) bf16 with contiguous rows; the cache bf16, D 64 or 128. Returns (1, n, Hq, D) bf16, token-major; a token that
+    sees no row (more new tokens than rows) gives zeros, tokens outside [starts[0], starts[-1]) stay as they were in out (anything in
+    a new tensor). out overlaps neither the cache nor q, but may be q itself where a token's heads lie together.
+    most, longest, total: the most new tokens of one sequence (1 in a decode step), the most rows of one that has any, and those of
+    all that have any together, if known, or about: they choose the kernel's form, not the result. Without longest the table's width
+    counts, which makes short sequences in a wide table slower.
     split: let launches too small to fill the chip split the cache range (a workspace is allocated for the partial results).
     """
     return _native.torch_ops().attention_paged(q, cache.table, cache.lengths, cache.refs, cache.page_tokens, cache.k, cache.v, layer, starts,
@@ -861,10 +861,10 @@ def adjust_logits(
     the row's prompt or generated is divided by repetition where it is above 0 and multiplied by it elsewhere; one that was generated c
     times loses frequency * c, then presence; bias is added; what allowed leaves out becomes -inf, whatever it was.
 
-    prompt, generated: int64 (rows, tokens); tokens outside the vocabulary (padding, -1) are passed over. repetition (> 0), frequency, presence: a number
-    or float32 (rows,). bias: float32 (vocab,) or (rows, vocab). allowed: int32 (ceil(vocab / 32),) for all rows or one each, bit v % 32 of
-    word v // 32 set where token v may come (token_bits). out overlaps no input, but may be the logits themselves, if they are float32, or a bias of
-    each row.
+    prompt, generated: int64 (rows, tokens); tokens outside the vocabulary (padding, -1) are passed over. repetition (> 0),
+    frequency, presence: a number or float32 (rows,). bias: float32 (vocab,) or (rows, vocab). allowed: int32 (ceil(vocab / 32),) for
+    all rows or one each, bit v % 32 of word v // 32 set where token v may come (token_bits). out overlaps no input, but may be the
+    logits themselves, if they are float32, or a bias of each row.
     """
     return _native.torch_ops().adjust_logits(logits, prompt, generated, repetition, frequency, presence, bias, allowed, out)
 
